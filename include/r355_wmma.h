@@ -261,6 +261,123 @@ int r355_decompress_24(const uint8_t* values, const uint8_t* meta, uint32_t m, u
 int r355_compress_24_16(const uint16_t* dense, uint32_t m, uint32_t k, uint16_t* values, uint8_t* meta);
 int r355_decompress_24_16(const uint16_t* values, const uint8_t* meta, uint32_t m, uint32_t k, uint16_t* dense);
 
+/*
+ * ---- A decoding step: products with 4-bit weights, rotary positions, attention of drafted tokens over a paged cache.
+ * No counterpart in the reference.
+ */
+
+/*
+ * y[t][r] = alpha * sum_k x[t][k] (q[r][k] - z[k / group][r]) s[k / group][r] + beta * c[t][r]
+ * for `tokens` rows of x (in_type R355_F16 or R355_BF16) and n rows of 4-bit weights q = 0..15, in the storage that r355_w4_pack writes:
+ *   [ceil(n / 16)][ceil(k / 128)][4][16][4] dwords; dword i of lane group g and row r of a block holds k = 32 i + 8 g + 0..7 of the block,
+ *   element e in bits 4 (e / 2 + 4 (e % 2)) + 0..3; zeros past n and k.  r355_w4_packed_bytes: its size.
+ * scales: [ceil(k / group)][n] of in_type; zeros: the same shape in bytes of 0..15, or NULL for 8 everywhere.  group: 32, 64 or a multiple
+ * of 128.  out_type: in_type or R355_F32 (c and y).  Sums and scaling are f32; y is rounded once.  c may be y; it is not read, and may
+ * be NULL, where beta is 0.  Any n, k and tokens (0: nothing is done); x, c and y of any leading dimension and alignment of an element, fastest
+ * with rows of x on 16-byte boundaries and n, ldc and ldy multiples of 4.
+ * Inside, a sum over a group is the difference of two that are about five times as large: where x (16 + q) summed over a group passes the
+ * range of f32, or x holds an infinity, the result is a NaN.
+ */
+typedef struct
+{
+    int32_t        in_type;  /* r355_dtype of x and scales */
+    int32_t        out_type; /* r355_dtype of c and y */
+    uint32_t       tokens, n, k, group;
+    const void*    x;
+    const void*    w; /* packed; 16-byte aligned */
+    const void*    scales;
+    const uint8_t* zeros; /* or NULL */
+    const void*    c;
+    void*          y;
+    uint32_t       ldx, ldc, ldy; /* elements */
+    double         alpha, beta;
+} r355_w4_args;
+int    r355_w4_matmul(const r355_w4_args* args, void* stream);
+size_t r355_w4_packed_bytes(uint32_t n, uint32_t k);
+/* q: [n] rows of ldq bytes, two weights a byte, the even k in the low half; device memory, as is `packed`. */
+int r355_w4_pack(const uint8_t* q, uint32_t n, uint32_t k, uint32_t ldq, void* packed, void* stream);
+
+/*
+ * Rotary positions: (a, b) -> scale (a cos t - b sin t, a sin t + b cos t) with t = 2 pi position turns[i], over the pairs of the
+ * first rotary_dim elements of every head; the rest of the head is copied.  inverse: rotation by -t (the gradient with respect to x).
+ * turns: what pair i turns per position, as a 64-bit fraction of a turn (device memory); r355_rope_turns fills a host array.
+ * Up to three parts go out in one launch (queries, keys, values), each with its own strides; a part with rotate = 0 is copied, one with
+ * to_slots writes token t to row slots[t] of y (the cache) and leaves out tokens whose slot is not in [0, slot_count).  Tokens must not
+ * share a slot.  y may be x with the same strides.  type: R355_F16, R355_BF16, R355_F32; any strides and alignment of an element, fastest in
+ * multiples of 16 bytes.
+ */
+typedef enum
+{
+    R355_ROPE_HALF        = 0, /* pairs (i, i + rotary_dim / 2) */
+    R355_ROPE_INTERLEAVED = 1  /* pairs (2 i, 2 i + 1) */
+} r355_rope_layout;
+#define R355_ROPE_MAX_PARTS 3u
+typedef struct
+{
+    const void* x; /* [tokens][heads][head_dim] by strides in elements */
+    void*       y;
+    uint32_t    heads;
+    int32_t     rotate, to_slots;
+    int64_t     x_token_stride, x_head_stride, y_token_stride, y_head_stride;
+} r355_rope_part;
+typedef struct
+{
+    int32_t         type, layout; /* r355_dtype, r355_rope_layout */
+    uint32_t        tokens, head_dim, rotary_dim, parts;
+    r355_rope_part  part[R355_ROPE_MAX_PARTS];
+    const int32_t*  positions; /* [tokens] */
+    const uint64_t* turns;     /* [rotary_dim / 2] */
+    const int32_t*  slots;     /* [tokens], or NULL where no part writes to slots */
+    uint32_t        slot_count;
+    int32_t         inverse;
+    double          scale;
+} r355_rope_args;
+int r355_rope(const r355_rope_args* args, void* stream);
+/* turns[i] = f_i / (2 pi) as a fraction of 2^64, f_i = base^(-2 i / rotary_dim).  factor lengthens the wavelengths: all of them with
+ * original_length 0; otherwise those that turn at most `slow` times in original_length positions, not those that turn `fast` times or
+ * more, and those between in proportion.  Host memory. */
+int r355_rope_turns(uint32_t rotary_dim, double base, double factor, uint32_t original_length, double slow, double fast, uint64_t* turns);
+
+/*
+ * Attention of drafted tokens over a paged cache: out_i = sum_j p_ij v_j, p_ij = exp(scale q_i . k_j - lse_i), over the positions j that row i sees.
+ * Sequence b has the rows q_start[b] .. q_start[b + 1] of q (its drafted tokens, their keys and values being the last rows of its cache) and
+ * kv_len[b] cached positions, the drafted among them.  A row sees every position before the drafted ones and, of those, the tokens whose bit is
+ * set in its row of `mask` (bit j % 64 of word j / 64: token j of the same sequence; as a rule its ancestors and itself); with mask = NULL those
+ * up to itself: one token, or a chunk of a prompt.  What a row does not see does not count, whatever the cache holds there.  A row that sees
+ * nothing gives zeros, and lse = -infinity.
+ * k, v: [pages * page_size slots][kv_heads][head_dim] by strides; position p of sequence b lies in slot
+ * table[b * table_stride + p / page_size] * page_size + p % page_size.  A page outside [0, pages) reads as zeros.
+ * Query head h uses key head h / (heads / kv_heads).  head_dim: a multiple of 8 up to 256; page_size: a multiple of 16; type: R355_F16 or R355_BF16
+ * for q, k, v and out.  Scores, softmax and sums are f32; the weights are rounded to `type` for the product with v.
+ * max_tokens and max_kv: bounds of what q_start and kv_len hold (device memory, not read by the host): what lies beyond is left out.
+ * workspace (16-byte aligned, contents irrelevant): with it the positions of a sequence are split over workgroups where there are few,
+ * up to what r355_tree_attention_workspace_bytes asks for; with less, fewer.  Calls that overlap need one each.  The result depends on
+ * the sizes and the workspace offered, not on scheduling.
+ */
+typedef struct
+{
+    int32_t         type;
+    uint32_t        batch, total_tokens, heads, kv_heads, head_dim;
+    uint32_t        max_tokens, max_kv;
+    const void*     q; /* [total_tokens][heads][head_dim] by strides in elements */
+    const void*     k;
+    const void*     v;
+    void*           out;
+    float*          lse; /* [total_tokens][heads], or NULL */
+    int64_t         q_token_stride, q_head_stride, k_slot_stride, k_head_stride, v_slot_stride, v_head_stride, out_token_stride, out_head_stride;
+    const int32_t*  table;
+    uint32_t        table_stride, page_size, pages;
+    const int32_t*  q_start; /* [batch + 1] */
+    const int32_t*  kv_len;  /* [batch] */
+    const uint64_t* mask;    /* [total_tokens][mask_words], or NULL */
+    uint32_t        mask_words;
+    double          scale;
+    void*           workspace;
+    uint64_t        workspace_bytes;
+} r355_tree_attention_args;
+int    r355_tree_attention(const r355_tree_attention_args* args, void* stream);
+size_t r355_tree_attention_workspace_bytes(const r355_tree_attention_args* args);
+
 /* Device facts used by the roofline report (test/hip_device.hpp:101-119 in the reference). */
 typedef struct
 {

@@ -1,4 +1,4 @@
-"""rocwmma_amd: MI355X (gfx950) matrix-fragment hot path -- GEMM, DLRM dot interaction, GEMV.
+"""rocwmma_amd: MI355X (gfx950) matrix-fragment hot path -- GEMM, DLRM dot interaction, GEMV, and the operators of a decoding step.
 
 The device code lives in csrc/ (hand-written HIP) and include/rocwmma/ (the header-only
 fragment API, same names as the reference's rocwmma.hpp).  This module is the thin host
@@ -24,11 +24,15 @@ KERNEL_TILED_64 = 7
 # r355_dlrm_kernel_id
 DLRM_KERNEL_SPECIALISED, DLRM_KERNEL_BLOCK_PER_WAVE, DLRM_KERNEL_REGISTER_BLOCKED, DLRM_KERNEL_TILED_64, DLRM_KERNEL_TILED_128 = 1, 2, 3, 64, 128
 
+# r355_rope_layout
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+
 DTYPE_BYTES = {F16: 2, BF16: 2, E4M3: 1, I8: 1, F32: 4, I32: 4, F64: 8, E5M2: 1}
 
 EXPORTS = [
     "r355_gemm", "r355_gemm_noalloc", "r355_gemm_query", "r355_gemm_launch_plan", "r355_gemm_timed", "r355_dlrm_fwd", "r355_dlrm_fwd_timed",
     "r355_dlrm_bwd", "r355_dlrm_kernel", "r355_gemv", "r355_gemv_timed", "r355_dgemv", "r355_gemv_workspace_bytes", "r355_gemv_ws", "r355_dgemv_ws", "r355_compress_24", "r355_decompress_24", "r355_compress_24_16", "r355_decompress_24_16",
+    "r355_w4_matmul", "r355_w4_packed_bytes", "r355_w4_pack", "r355_rope", "r355_rope_turns", "r355_tree_attention", "r355_tree_attention_workspace_bytes",
     "r355_get_device_info", "r355_last_error", "r355_version",
 ]
 
@@ -62,6 +66,52 @@ class GemmPlan(ctypes.Structure):
         ("block_x", ctypes.c_uint32), ("block_y", ctypes.c_uint32),
         ("lds_bytes", ctypes.c_uint32),
         ("split_k", ctypes.c_uint32), ("workspace_bytes", ctypes.c_uint64),
+    ]
+
+
+class W4Args(ctypes.Structure):
+    _fields_ = [
+        ("in_type", ctypes.c_int32), ("out_type", ctypes.c_int32),
+        ("tokens", ctypes.c_uint32), ("n", ctypes.c_uint32), ("k", ctypes.c_uint32), ("group", ctypes.c_uint32),
+        ("x", ctypes.c_void_p), ("w", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("zeros", ctypes.c_void_p),
+        ("c", ctypes.c_void_p), ("y", ctypes.c_void_p),
+        ("ldx", ctypes.c_uint32), ("ldc", ctypes.c_uint32), ("ldy", ctypes.c_uint32),
+        ("alpha", ctypes.c_double), ("beta", ctypes.c_double),
+    ]
+
+
+class RopePart(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("y", ctypes.c_void_p), ("heads", ctypes.c_uint32),
+        ("rotate", ctypes.c_int32), ("to_slots", ctypes.c_int32),
+        ("x_token_stride", ctypes.c_int64), ("x_head_stride", ctypes.c_int64),
+        ("y_token_stride", ctypes.c_int64), ("y_head_stride", ctypes.c_int64),
+    ]
+
+
+class RopeArgs(ctypes.Structure):
+    _fields_ = [
+        ("type", ctypes.c_int32), ("layout", ctypes.c_int32),
+        ("tokens", ctypes.c_uint32), ("head_dim", ctypes.c_uint32), ("rotary_dim", ctypes.c_uint32), ("parts", ctypes.c_uint32),
+        ("part", RopePart * 3),
+        ("positions", ctypes.c_void_p), ("turns", ctypes.c_void_p), ("slots", ctypes.c_void_p),
+        ("slot_count", ctypes.c_uint32), ("inverse", ctypes.c_int32), ("scale", ctypes.c_double),
+    ]
+
+
+class TreeAttentionArgs(ctypes.Structure):
+    _fields_ = [
+        ("type", ctypes.c_int32), ("batch", ctypes.c_uint32), ("total_tokens", ctypes.c_uint32),
+        ("heads", ctypes.c_uint32), ("kv_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
+        ("max_tokens", ctypes.c_uint32), ("max_kv", ctypes.c_uint32),
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("out", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+        ("q_token_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
+        ("k_slot_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64),
+        ("v_slot_stride", ctypes.c_int64), ("v_head_stride", ctypes.c_int64),
+        ("out_token_stride", ctypes.c_int64), ("out_head_stride", ctypes.c_int64),
+        ("table", ctypes.c_void_p), ("table_stride", ctypes.c_uint32), ("page_size", ctypes.c_uint32), ("pages", ctypes.c_uint32),
+        ("q_start", ctypes.c_void_p), ("kv_len", ctypes.c_void_p), ("mask", ctypes.c_void_p), ("mask_words", ctypes.c_uint32),
+        ("scale", ctypes.c_double), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64),
     ]
 
 
@@ -107,6 +157,13 @@ def lib():
         L.r355_decompress_24.argtypes = [vp, vp, u32, u32, vp]
         L.r355_compress_24_16.argtypes = [vp, u32, u32, vp, vp]
         L.r355_decompress_24_16.argtypes = [vp, vp, u32, u32, vp]
+        L.r355_w4_matmul.argtypes = [ctypes.POINTER(W4Args), vp]
+        L.r355_w4_packed_bytes.argtypes = [u32, u32]
+        L.r355_w4_pack.argtypes = [vp, u32, u32, u32, vp, vp]
+        L.r355_rope.argtypes = [ctypes.POINTER(RopeArgs), vp]
+        L.r355_rope_turns.argtypes = [u32, ctypes.c_double, ctypes.c_double, u32, ctypes.c_double, ctypes.c_double, vp]
+        L.r355_tree_attention.argtypes = [ctypes.POINTER(TreeAttentionArgs), vp]
+        L.r355_tree_attention_workspace_bytes.argtypes = [ctypes.POINTER(TreeAttentionArgs)]
         L.r355_get_device_info.argtypes = [ctypes.POINTER(DeviceInfo)]
         L.r355_last_error.argtypes = []
         L.r355_version.argtypes = []
@@ -115,6 +172,8 @@ def lib():
         for name in EXPORTS:
             if name not in ("r355_last_error", "r355_version"):
                 getattr(L, name).restype = ctypes.c_int
+        for name in ("r355_w4_packed_bytes", "r355_tree_attention_workspace_bytes"):
+            getattr(L, name).restype = ctypes.c_size_t
         _lib = L
     return _lib
 
@@ -314,6 +373,78 @@ def decompress_24(values, meta):
     fn = {1: lib().r355_decompress_24, 2: lib().r355_decompress_24_16}[es]
     _check(fn(_ptr(values), _ptr(meta), m, k, _ptr(dense)))
     return dense
+
+
+def w4_packed_bytes(n, k):
+    """Bytes of the packed storage of n x k 4-bit weights."""
+    return lib().r355_w4_packed_bytes(n, k)
+
+
+def w4_pack(q, n, k, packed, ldq=None, stream=None):
+    """Device-side: n rows of ldq bytes (default: ceil(k / 2)), two weights a byte, the even k in the low half, into the storage
+    that w4_matmul reads (include/r355_wmma.h)."""
+    _check(lib().r355_w4_pack(_ptr(q), n, k, ldq if ldq is not None else (k + 1) // 2, _ptr(packed), _stream_handle(stream)))
+
+
+def w4_matmul(in_type, out_type, tokens, n, k, group, x, w, scales, y, zeros=None, c=None, alpha=1.0, beta=0.0, ldx=None, ldc=None,
+              ldy=None, stream=None):
+    """y = alpha * x W^T + beta * c for packed 4-bit W (n x k) with scales (and zero points; default 8) per `group` of k."""
+    a = W4Args(in_type, out_type, tokens, n, k, group, _ptr(x), _ptr(w), _ptr(scales), _ptr(zeros), _ptr(c), _ptr(y),
+               k if ldx is None else ldx, n if ldc is None else ldc, n if ldy is None else ldy, alpha, beta)
+    _check(lib().r355_w4_matmul(ctypes.byref(a), _stream_handle(stream)))
+
+
+def rope_turns(rotary_dim, base=10000.0, factor=1.0, original_length=0, slow=1.0, fast=4.0):
+    """What each pair turns per position, as 64-bit fractions of a turn (numpy uint64; the kernels read it in device memory).  factor
+    lengthens the wavelengths: all of them, or with original_length those that turn less than `fast` times in it (by `slow`: fully)."""
+    import numpy as np
+
+    turns = np.zeros(max(rotary_dim // 2, 1), dtype=np.uint64)
+    _check(lib().r355_rope_turns(rotary_dim, base, factor, original_length, slow, fast, _ptr(turns)))
+    return turns
+
+
+def rope_part(x, y, heads, x_strides, y_strides, rotate=True, to_slots=False):
+    """One of up to three tensors of a rope() call; strides: (token, head) in elements."""
+    return RopePart(_ptr(x), _ptr(y), heads, rotate, to_slots, x_strides[0], x_strides[1], y_strides[0], y_strides[1])
+
+
+def rope(dtype, layout, tokens, head_dim, rotary_dim, parts, positions, turns, scale=1.0, inverse=False, slots=None, slot_count=0, stream=None):
+    """Rotates (inverse: back) the first rotary_dim elements of every head of the parts by their token's position, in one launch; parts with
+    to_slots go to rows slots[token] of a cache."""
+    if not 1 <= len(parts) <= 3:
+        raise ValueError("rope: 1 to 3 parts, got %d" % len(parts))
+    a = RopeArgs(dtype, layout, tokens, head_dim, rotary_dim, len(parts), tuple(parts), _ptr(positions), _ptr(turns), _ptr(slots), slot_count,
+                 inverse, scale)
+    _check(lib().r355_rope(ctypes.byref(a), _stream_handle(stream)))
+
+
+def tree_attention_args(dtype, batch, total_tokens, heads, kv_heads, head_dim, q, k, v, out, table, page_size, pages, q_start, kv_len, max_tokens,
+                        max_kv, mask=None, mask_words=0, lse=None, scale=None, workspace=None, workspace_bytes=None, q_strides=None,
+                        k_strides=None, v_strides=None, out_strides=None, table_stride=None):
+    row, slot = (heads * head_dim, head_dim), (kv_heads * head_dim, head_dim)
+    qs, ks, vs, os_ = q_strides or row, k_strides or slot, v_strides or slot, out_strides or row
+    if workspace_bytes is None:
+        workspace_bytes = workspace.numel() * workspace.element_size() if hasattr(workspace, "numel") else 0
+    return TreeAttentionArgs(
+        dtype, batch, total_tokens, heads, kv_heads, head_dim, max_tokens, max_kv, _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse),
+        qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os_[0], os_[1], _ptr(table), table.shape[1] if table_stride is None else table_stride,
+        page_size, pages, _ptr(q_start), _ptr(kv_len), _ptr(mask), mask_words, head_dim ** -0.5 if scale is None else scale,
+        _ptr(workspace), workspace_bytes)
+
+
+def tree_attention(dtype, batch, total_tokens, heads, kv_heads, head_dim, q, k, v, out, table, page_size, pages, q_start, kv_len, max_tokens,
+                   max_kv, mask=None, mask_words=0, lse=None, scale=None, workspace=None, stream=None, **strides):
+    """Attention of the drafted tokens of `batch` sequences over a paged cache (include/r355_wmma.h).  scale: default
+    1 / sqrt(head_dim); strides: q_strides, k_strides, v_strides, out_strides as (token or slot, head) in elements, table_stride."""
+    a = tree_attention_args(dtype, batch, total_tokens, heads, kv_heads, head_dim, q, k, v, out, table, page_size, pages, q_start, kv_len,
+                            max_tokens, max_kv, mask, mask_words, lse, scale, workspace, **strides)
+    _check(lib().r355_tree_attention(ctypes.byref(a), _stream_handle(stream)))
+
+
+def tree_attention_workspace_bytes(a):
+    """Bytes of workspace that r355_tree_attention makes use of for TreeAttentionArgs (0: none)."""
+    return lib().r355_tree_attention_workspace_bytes(ctypes.byref(a))
 
 
 def device_info():
