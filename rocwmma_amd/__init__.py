@@ -212,11 +212,10 @@ def _ptr(t):
     """Device (or host) address of a torch tensor / numpy array / raw int / None."""
     if t is None:
         return None
-    if isinstance(t, int):
-        return t
-    if hasattr(t, "data_ptr"):
-        return t.data_ptr()
-    return t.ctypes.data
+    try:
+        return t.data_ptr()  # (first: the small calls take about as long as what is done here)
+    except AttributeError:
+        return t if isinstance(t, int) else t.ctypes.data
 
 
 def _stream_handle(stream):

@@ -32,6 +32,8 @@ namespace
 
     constexpr uint32_t WAVES = 4;
     constexpr uint32_t LEAST_CHUNK = 256; // positions of a workgroup at least
+    constexpr uint32_t ABSENT = 0xFFFFFFFFu; // no such block of the cache
+    constexpr uint32_t OUTSIDE = 0x7FFFFFF0u; // a lane's offset past the end of any buffer
 
     struct TreeParams
     {
@@ -49,7 +51,8 @@ namespace
         uint32_t        batch, heads, kvHeads, group, dim, totalTokens, maxTokens, maxKv;
         uint32_t        pageSize, pages, tableStride, maskWords;
         uint32_t        splits, columns; // columns: (sequence, key head, split) triples
-        float           scale2; // scale * log2(e)
+        float           scale2; // |scale| * log2(e), at least the smallest normal number (times minus infinity it is minus infinity)
+        uint32_t        signs; // what turns the signs of two elements of q: the scale's
     };
 
     // the positions of one sequence that a workgroup takes
@@ -66,9 +69,8 @@ namespace
     };
 
     // what the arrays say of a sequence, held to what the host was told
-    __device__ __forceinline__ Sequence sequenceOf(const TreeParams& p, uint32_t b)
+    __device__ __forceinline__ Sequence sequenceOf(const TreeParams& p, int32_t from, int32_t to, int32_t len)
     {
-        const int32_t from = p.qStart[b], to = p.qStart[b + 1u], len = p.kvLen[b];
         Sequence      s;
         s.first  = from < 0 ? 0u : static_cast<uint32_t>(from);
         s.first  = s.first < p.totalTokens ? s.first : p.totalTokens;
@@ -80,6 +82,36 @@ namespace
         return s;
     }
 
+    // where block `inChunk` (of 16 positions) of the chunk that begins at block `first` of sequence b lies, in blocks of the cache
+    __device__ __forceinline__ uint32_t placeOf(const TreeParams& p, uint32_t b, uint32_t first, uint32_t inChunk, uint32_t blocks, uint32_t pageBlocks)
+    {
+        if(inChunk >= blocks)
+            return ABSENT;
+        const uint32_t page = (first + inChunk) / pageBlocks, to = static_cast<uint32_t>(p.table[(uint64_t)b * p.tableStride + page]);
+        return to < p.pages ? to * pageBlocks + (first + inChunk - page * pageBlocks) : ABSENT;
+    }
+
+    // which of 32 positions a row sees: bit i the one that holds drafted token past + i of the sequence (negative: of the prefix, seen by all);
+    // past is less than the number of drafted tokens
+    __device__ __forceinline__ uint32_t seenOf(const TreeParams& p, uint32_t row, uint32_t token, int64_t past)
+    {
+        if(past <= -32)
+            return 0xFFFFFFFFu;
+        const uint32_t before = past < 0 ? static_cast<uint32_t>(-past) : 0u, from = past < 0 ? 0u : static_cast<uint32_t>(past);
+        uint32_t       bits; // of the drafted tokens from .. from + 31
+        if(p.mask)
+        {
+            const uint64_t* words = p.mask + (uint64_t)row * p.maskWords + from / 64u;
+            uint64_t        w     = words[0] >> (from % 64u);
+            if(from % 64u > 32u && from / 64u + 1u < p.maskWords)
+                w |= words[1] << (64u - from % 64u);
+            bits = static_cast<uint32_t>(w);
+        }
+        else
+            bits = token < from ? 0u : token - from >= 31u ? 0xFFFFFFFFu : (2u << (token - from)) - 1u;
+        return (bits << before) | ((1u << before) - 1u);
+    }
+
     template <uint32_t D>
     __device__ __forceinline__ uint32_t swizzleK(uint32_t row)
     {
@@ -89,6 +121,22 @@ namespace
     __device__ __forceinline__ uint32_t swizzleV(uint32_t row)
     {
         return D == 64u ? ((row >> 1) & 3u) << 1 : (row & 7u) << 1;
+    }
+
+    // of two 16-bit numbers: 1 in each half that holds an infinity or a NaN
+    template <typename T>
+    __device__ __forceinline__ uint32_t unfitHalves(uint32_t v)
+    {
+        constexpr uint32_t EXPONENT = std::is_same_v<T, __bf16> ? 0x7F807F80u : 0x7C007C00u, ULP = std::is_same_v<T, __bf16> ? 0x00800080u : 0x04000400u;
+        return (((v & EXPONENT) + ULP) >> 15) & 0x00010001u;
+    }
+    // 1.0 in each half that holds a NaN or the infinity of the given sign, otherwise zero
+    template <typename T>
+    __device__ __forceinline__ uint32_t unfitOnes(uint32_t v, bool negative)
+    {
+        constexpr uint32_t INF = std::is_same_v<T, __bf16> ? 0x7F80u : 0x7C00u, ONE = std::is_same_v<T, __bf16> ? 0x3F80u : 0x3C00u;
+        const uint32_t     lo = v & 0xFFFFu, hi = v >> 16, want = negative ? INF | 0x8000u : INF;
+        return (lo == want || (lo & 0x7FFFu) > INF ? ONE : 0u) | (hi == want || (hi & 0x7FFFu) > INF ? ONE << 16 : 0u);
     }
 
     __device__ __forceinline__ float maxOverQuads(float x)
@@ -103,7 +151,7 @@ namespace
     }
 
     template <typename T, uint32_t D, uint32_t WQ, uint32_t QB>
-    __global__ void __launch_bounds__(WAVES * 64) treeKernel(TreeParams p)
+    __global__ void __launch_bounds__(WAVES * 64, WQ == 1u ? 1 : 2) treeKernel(TreeParams p)
     {
         constexpr uint32_t WK    = WAVES / WQ;
         constexpr uint32_t NP    = D == 256u ? 16u : 32u; // positions of a tile
@@ -117,6 +165,8 @@ namespace
         constexpr uint32_t MERGE = WK > 1u ? WK * QB * 16u * (D + 2u) * 4u : 0u;
         // weights are held relative to 2^-SHIFT of the largest: in f16 those under 2^-14 of it, of which a long row has many, stay normal numbers
         constexpr float SHIFT = std::is_same_v<T, __bf16> ? 0.0f : 10.0f;
+        // ... and the maximum is taken as it was until it has grown by more than this: the sums are scaled anew in few tiles, and the largest weight is 2^(SHIFT + SLACK)
+        constexpr float SLACK = 4.0f;
         static_assert(LDS <= 160u * 1024u, "LDS");
         __shared__ __attribute__((aligned(1024))) char lds[LDS > MERGE ? LDS : MERGE];
 
@@ -125,7 +175,7 @@ namespace
         const uint32_t head = bh % p.kvHeads, b = bh / p.kvHeads;
         if(b >= p.batch)
             return;
-        const Sequence seq  = sequenceOf(p, b);
+        const Sequence seq  = sequenceOf(p, __builtin_amdgcn_readfirstlane(p.qStart[b]), __builtin_amdgcn_readfirstlane(p.qStart[b + 1u]), __builtin_amdgcn_readfirstlane(p.kvLen[b]));
         const uint32_t rows = seq.tokens * p.group, row0 = tile0 * WQ * QB * 16u;
         if(row0 >= rows)
             return;
@@ -156,38 +206,67 @@ namespace
             for(uint32_t i = 0; i < D / 32u; ++i)
             {
                 const uint32_t d = i * 32u + quad * 8u;
-                qf[a][i]         = rowValid[a] && d < p.dim ? *reinterpret_cast<const u32x4*>(at + d) : u32x4{0u, 0u, 0u, 0u};
+                qf[a][i]         = rowValid[a] && d < p.dim ? *reinterpret_cast<const u32x4*>(at + d) ^ p.signs : u32x4{0u, 0u, 0u, 0u};
             }
         }
 
-        // ---- direct loads.  A tile is NP / 16 blocks of 16 positions, each within one page.
+        // ---- direct loads.  A tile is PB blocks of 16 positions, each within one page.  Lane i holds where the blocks 64 g + i of the chunk
+        // lie, in blocks of the cache, for GROUPS of 64 at a time: a load of the table within the loop would have the compiler wait for every
+        // direct load before it (the positions of a chunk and more are read at the start).
         const uint32_t ldsBase = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
         const uint32_t myTiles = wk * BUFS * 2u * TILE;
-        constexpr uint32_t OUTSIDE = 0x7FFFFF00u, RECORDS = 0x7FFF0000u; // (a lane's offset past the buffer's end loads zeros)
+        const uint32_t pageBlocks = p.pageSize / 16u, lastBlocks = end > begin ? (end - begin + 15u) / 16u : 0u;
+        constexpr uint32_t GROUPS = 4;
+        uint32_t           group = 0u, here, ahead[GROUPS];
+#pragma unroll
+        for(uint32_t g = 0; g < GROUPS; ++g)
+            ahead[g] = placeOf(p, b, begin / 16u, g * 64u + lane, lastBlocks, pageBlocks);
+#pragma unroll
+        for(uint32_t g = 0; g < GROUPS; ++g)
+            asm volatile("" : "+v"(ahead[g])); // (they are there from here on)
+        here = ahead[0];
+        // a lane's offsets: RPL rows a load, 16-byte pieces exchanged within the row; past the width of a head: outside the buffer, which loads zeros
         const uint32_t loadRow = lane / SLOTS, loadSlot = lane % SLOTS;
-        // pieces of 16 rows that one load covers lie in one 16-position block (RPL <= 16)
-        auto issue = [&](uint32_t pos0, uint32_t buf) {
+        uint32_t       offK[LOADS], offV[LOADS];
+#pragma unroll
+        for(uint32_t j = 0; j < LOADS; ++j)
+        {
+            const uint32_t inTile = (wq * LOADS + j) * RPL + loadRow;
+            const uint32_t pieceK = loadSlot ^ swizzleK<D>(inTile), pieceV = loadSlot ^ swizzleV<D>(inTile);
+            offK[j] = pieceK * 8u < p.dim ? inTile % 16u * (uint32_t)(p.kSlot * 2) + pieceK * 16u : OUTSIDE;
+            offV[j] = pieceV * 8u < p.dim ? inTile % 16u * (uint32_t)(p.vSlot * 2) + pieceV * 16u : OUTSIDE;
+        }
+        const uint64_t baseK = reinterpret_cast<uint64_t>(p.k) + 2u * (uint64_t)(head * p.kHead), baseV = reinterpret_cast<uint64_t>(p.v) + 2u * (uint64_t)(head * p.vHead);
+        auto issue = [&](uint32_t tile, uint32_t buf) __attribute__((always_inline)) {
+            if(const uint32_t of = tile * PB / 64u; of != group)
+            {
+                group = of;
+                if(of % GROUPS == 0u)
+                {
+#pragma unroll
+                    for(uint32_t g = 0; g < GROUPS; ++g)
+                        ahead[g] = placeOf(p, b, begin / 16u, (of + g) * 64u + lane, lastBlocks, pageBlocks);
+#pragma unroll
+                    for(uint32_t g = 0; g < GROUPS; ++g)
+                        asm volatile("" : "+v"(ahead[g]));
+                    here = ahead[0];
+                }
+                else
+                    here = of % GROUPS == 1u ? ahead[1] : of % GROUPS == 2u ? ahead[2] : ahead[3];
+            }
 #pragma unroll
             for(uint32_t j = 0; j < LOADS; ++j)
             {
-                const uint32_t piece = WQ == 1u ? j : wq * LOADS + j; // which RPL rows of the tile
-                const uint32_t block = pos0 + piece * RPL / 16u * 16u; // its 16 positions
-                const uint32_t inBlock = piece * RPL % 16u + loadRow, inTile = piece * RPL + loadRow;
-                uint32_t       page = 0u;
-                if(block < end)
-                    page = static_cast<uint32_t>(p.table[(uint64_t)b * p.tableStride + block / p.pageSize]);
-                const bool     there = block < end && page < p.pages;
-                const uint64_t slot  = (uint64_t)(there ? page : 0u) * p.pageSize + block % p.pageSize;
-                const bool     inside = there && block + inBlock < end;
-                const uint32_t pieceK = loadSlot ^ swizzleK<D>(inTile), pieceV = loadSlot ^ swizzleV<D>(inTile);
-                const uint32_t offK   = inside && pieceK * 8u < p.dim ? inBlock * (uint32_t)(p.kSlot * 2) + pieceK * 16u : OUTSIDE;
-                const uint32_t offV   = inside && pieceV * 8u < p.dim ? inBlock * (uint32_t)(p.vSlot * 2) + pieceV * 16u : OUTSIDE;
-                r355::dma_i32x4 bufK  = r355::rawBuffer(reinterpret_cast<uint64_t>(p.k) + 2u * (slot * p.kSlot + (int64_t)head * p.kHead));
-                r355::dma_i32x4 bufV  = r355::rawBuffer(reinterpret_cast<uint64_t>(p.v) + 2u * (slot * p.vSlot + (int64_t)head * p.vHead));
-                bufK[2] = bufV[2] = RECORDS;
+                const uint32_t piece = wq * LOADS + j; // which RPL rows of the tile
+                const uint32_t block = tile * PB + piece * RPL / 16u; // of the chunk
+                const uint32_t at   = __builtin_amdgcn_readlane(here, block % 64u);
+                const uint32_t rows = at == ABSENT ? 0u : end - begin - block * 16u < 16u ? end - begin - block * 16u : 16u;
+                // (a buffer that ends with the last row that there is: the others load zeros)
+                r355::dma_i32x4 bufK = r355::rawBuffer(baseK + (uint64_t)at * (uint32_t)(p.kSlot * 32)), bufV = r355::rawBuffer(baseV + (uint64_t)at * (uint32_t)(p.vSlot * 32));
+                bufK[2] = __builtin_amdgcn_readfirstlane(rows * (uint32_t)(p.kSlot * 2)), bufV[2] = __builtin_amdgcn_readfirstlane(rows * (uint32_t)(p.vSlot * 2));
                 const uint32_t to = __builtin_amdgcn_readfirstlane(ldsBase + myTiles + buf * 2u * TILE + piece * 1024u);
-                r355::loadToLds(bufK, offK, 0u, to);
-                r355::loadToLds(bufV, offV, 0u, to + TILE);
+                r355::loadToLds(bufK, offK[j], 0u, to);
+                r355::loadToLds(bufV, offV[j], 0u, to + TILE);
             }
         };
 
@@ -202,52 +281,44 @@ namespace
                 o[a][d] = f32x4{0, 0, 0, 0};
         }
 
-        auto compute = [&](uint32_t pos0, uint32_t buf) {
-            const char* tileK = lds + myTiles + buf * 2u * TILE;
-            const char* tileV = tileK + TILE;
-            f32x4       s[QB][PB];
+        // MASKED: some row does not see all of the tile
+        auto compute = [&](auto maskedTile, uint32_t pos0, uint32_t buf) __attribute__((always_inline)) {
+            constexpr bool MASKED = decltype(maskedTile)::value;
+            // LDS addresses of the lane's row: the pieces of a row differ in an exclusive or with a constant (rows start on multiples of their
+            // size), the blocks of 16 rows in a constant offset
+            const uint32_t tileK = ldsBase + myTiles + buf * 2u * TILE, tileV = tileK + TILE;
+            const uint32_t rowV = quad * 4u + (col >> 2);
+            const uint32_t fromK = tileK + col * ROWB + (quad ^ swizzleK<D>(col)) * 16u, fromV = tileV + rowV * ROWB + (((col >> 1) & 1u) ^ swizzleV<D>(rowV)) * 16u + (col & 1u) * 8u;
+            f32x4          s[QB][PB];
 #pragma unroll
             for(uint32_t n = 0; n < PB; ++n)
-            {
 #pragma unroll
                 for(uint32_t a = 0; a < QB; ++a)
                     s[a][n] = f32x4{0, 0, 0, 0};
-                const uint32_t row = n * 16u + col;
 #pragma unroll
-                for(uint32_t i = 0; i < D / 32u; ++i)
+            for(uint32_t i = 0; i < D / 32u; ++i)
+#pragma unroll
+                for(uint32_t n = 0; n < PB; ++n)
                 {
-                    const u32x4 kf = *reinterpret_cast<const u32x4*>(tileK + row * ROWB + ((i * 4u + quad) ^ swizzleK<D>(row)) * 16u);
+                    const u32x4 kf = *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)((fromK ^ (i * 64u)) + n * 16u * ROWB);
 #pragma unroll
                     for(uint32_t a = 0; a < QB; ++a)
                         s[a][n] = r355::mfma32<T>(kf, qf[a][i], s[a][n]);
                 }
-            }
-            const bool masked = (int64_t)pos0 + NP > prefix || pos0 + NP > end; // some row does not see all of the tile
-            if(masked)
+            if constexpr(MASKED)
             {
 #pragma unroll
                 for(uint32_t a = 0; a < QB; ++a)
+                {
+                    // bit i: the row sees position pos0 + i
+                    const uint32_t seen = rowValid[a] ? seenOf(p, seq.first + token[a], token[a], (int64_t)pos0 - prefix) : 0u;
+                    const uint32_t mine = (end - pos0 < 32u ? seen & ((1u << (end - pos0)) - 1u) : seen) >> (quad * 4u);
 #pragma unroll
                     for(uint32_t n = 0; n < PB; ++n)
 #pragma unroll
                         for(uint32_t j = 0; j < 4; ++j)
-                        {
-                            const uint32_t pos  = pos0 + n * 16u + quad * 4u + j;
-                            const int64_t  past = (int64_t)pos - prefix; // which drafted token, from 0 on
-                            bool           seen = pos < end && rowValid[a];
-                            if(seen && past >= 0)
-                                seen = p.mask ? (p.mask[(uint64_t)(seq.first + token[a]) * p.maskWords + (uint32_t)past / 64u] >> ((uint32_t)past % 64u)) & 1u
-                                              : past <= (int64_t)token[a];
-                            s[a][n][j] = seen ? s[a][n][j] * p.scale2 : -INFINITY;
-                        }
-            }
-            else
-            {
-#pragma unroll
-                for(uint32_t a = 0; a < QB; ++a)
-#pragma unroll
-                    for(uint32_t n = 0; n < PB; ++n)
-                        s[a][n] *= p.scale2;
+                            s[a][n][j] = (mine >> (n * 16u + j)) & 1u ? s[a][n][j] : -INFINITY;
+                }
             }
             uint32_t pf[QB][PB][2];
 #pragma unroll
@@ -257,8 +328,9 @@ namespace
 #pragma unroll
                 for(uint32_t n = 0; n < PB; ++n)
                     most = fmaxf(fmaxf(fmaxf(s[a][n][0], s[a][n][1]), fmaxf(s[a][n][2], s[a][n][3])), most);
+                most = most == -INFINITY ? most : most * p.scale2;
                 most = maxOverQuads(most) - SHIFT;
-                if(__any(most > top[a]))
+                if(__any(most > top[a] + SLACK))
                 {
                     const float next = fmaxf(most, top[a]);
                     const float keep = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[a] - next);
@@ -275,52 +347,24 @@ namespace
 #pragma unroll
                     for(uint32_t j = 0; j < 4; ++j)
                     {
-                        s[a][n][j] = __builtin_amdgcn_exp2f(s[a][n][j] - base);
+                        s[a][n][j] = __builtin_amdgcn_exp2f(fmaf(s[a][n][j], p.scale2, -base));
                         sum[a] += s[a][n][j];
                     }
                     pf[a][n][0] = r355::pack2<T>(s[a][n][0], s[a][n][1]), pf[a][n][1] = r355::pack2<T>(s[a][n][2], s[a][n][3]);
                 }
             }
-            // A position that a row does not see has weight 0, and 0 times an infinity or a NaN is a NaN: where the tile holds one, the sums
-            // are made without the matrix instructions, a position at a time and only for the rows that see it.
+            // A position that a row does not see has weight 0, and 0 times an infinity or a NaN is a NaN: where the tile holds one, those are
+            // taken out of the product, and the rows that give them weight get them by two more (where (+inf or NaN) and where (-inf or NaN)).
             bool unfit = false;
-            if(masked)
+            if constexpr(MASKED)
             {
-                constexpr uint32_t EXPONENT = std::is_same_v<T, __bf16> ? 0x7F807F80u : 0x7C007C00u, ULP = std::is_same_v<T, __bf16> ? 0x00800080u : 0x04000400u;
-                uint32_t           found = 0u;
+                uint32_t found = 0u;
                 for(uint32_t at = lane * 16u; at < TILE; at += 1024u)
                 {
-                    const u32x4 v = *reinterpret_cast<const u32x4*>(tileV + at);
-                    found |= ((v[0] & EXPONENT) + ULP) | ((v[1] & EXPONENT) + ULP) | ((v[2] & EXPONENT) + ULP) | ((v[3] & EXPONENT) + ULP);
+                    const u32x4 v = *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)(tileV + at);
+                    found |= unfitHalves<T>(v[0]) | unfitHalves<T>(v[1]) | unfitHalves<T>(v[2]) | unfitHalves<T>(v[3]);
                 }
-                unfit = __any((found & 0x80008000u) != 0u);
-            }
-            if(unfit)
-            {
-#pragma unroll
-                for(uint32_t n = 0; n < PB; ++n)
-#pragma unroll
-                    for(uint32_t j = 0; j < 4; ++j)
-#pragma unroll 1
-                        for(uint32_t from = 0; from < 4; ++from)
-                        {
-                            const uint32_t row = n * 16u + from * 4u + j;
-                            float          weight[QB];
-#pragma unroll
-                            for(uint32_t a = 0; a < QB; ++a)
-                                weight[a] = __shfl(s[a][n][j], from * 16u + col);
-#pragma unroll
-                            for(uint32_t d = 0; d < D / 16u; ++d)
-                            {
-                                const vec<T, 4> v = *reinterpret_cast<const vec<T, 4>*>(tileV + row * ROWB + ((d * 2u + (quad >> 1)) ^ swizzleV<D>(row)) * 16u + (quad & 1u) * 8u);
-#pragma unroll
-                                for(uint32_t a = 0; a < QB; ++a)
-#pragma unroll
-                                    for(uint32_t e = 0; e < 4; ++e)
-                                        o[a][d][e] += weight[a] != 0.0f ? weight[a] * static_cast<float>(v[e]) : 0.0f;
-                            }
-                        }
-                return;
+                unfit = __any(found != 0u);
             }
             // V^T: lane t of 16 names four consecutive d of position t / 4 and receives four positions of d = t
             using lp = __attribute__((address_space(3))) vec<short, 4>*;
@@ -330,51 +374,66 @@ namespace
                 u32x2 vf[PB];
 #pragma unroll
                 for(uint32_t n = 0; n < PB; ++n)
-                {
-                    const uint32_t row  = n * 16u + quad * 4u + (col >> 2);
-                    const char*    from = tileV + row * ROWB + ((d * 2u + ((col & 3u) >> 1)) ^ swizzleV<D>(row)) * 16u + (col & 1u) * 8u;
-                    vf[n]               = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)from));
-                }
+                    vf[n] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(uintptr_t)((fromV ^ (d * 32u)) + n * 16u * ROWB)));
+                auto times = [&](const u32x2(&v)[PB], uint32_t a, f32x4 c) __attribute__((always_inline)) {
+                    if constexpr(PB == 2u)
+                        return r355::mfma32<T>(u32x4{v[0][0], v[0][1], v[1][0], v[1][1]}, u32x4{pf[a][0][0], pf[a][0][1], pf[a][1][0], pf[a][1][1]}, c);
+                    else
+                        return r355::mfma16<T>(v[0], u32x2{pf[a][0][0], pf[a][0][1]}, c);
+                };
+                if constexpr(MASKED)
+                    if(unfit)
+                    {
+                        u32x2 up[PB], down[PB];
+#pragma unroll
+                        for(uint32_t n = 0; n < PB; ++n)
+#pragma unroll
+                            for(uint32_t w = 0; w < 2; ++w)
+                            {
+                                up[n][w] = unfitOnes<T>(vf[n][w], false), down[n][w] = unfitOnes<T>(vf[n][w], true);
+                                vf[n][w] &= ~(unfitHalves<T>(vf[n][w]) * 0xFFFFu);
+                            }
+#pragma unroll
+                        for(uint32_t a = 0; a < QB; ++a)
+                        {
+                            const f32x4 above = times(up, a, f32x4{0, 0, 0, 0}), below = times(down, a, f32x4{0, 0, 0, 0});
+#pragma unroll
+                            for(uint32_t e = 0; e < 4; ++e)
+                            {
+                                o[a][d][e] += above[e] != 0.0f ? INFINITY : 0.0f;
+                                o[a][d][e] -= below[e] != 0.0f ? INFINITY : 0.0f;
+                            }
+                        }
+                    }
 #pragma unroll
                 for(uint32_t a = 0; a < QB; ++a)
-                {
-                    if constexpr(PB == 2u)
-                        o[a][d] = r355::mfma32<T>(u32x4{vf[0][0], vf[0][1], vf[1][0], vf[1][1]}, u32x4{pf[a][0][0], pf[a][0][1], pf[a][1][0], pf[a][1][1]}, o[a][d]);
-                    else
-                        o[a][d] = r355::mfma16<T>(vf[0], u32x2{pf[a][0][0], pf[a][0][1]}, o[a][d]);
-                }
+                    o[a][d] = times(vf, a, o[a][d]);
             }
         };
 
         const uint32_t tiles = begin < end ? (end - begin + NP - 1u) / NP : 0u;
-        if constexpr(WQ == 1u)
-        {
-            // tiles wk, wk + 4, ... of the chunk; those past the end load zeros and are not computed
-            if(wk < tiles)
-                issue(begin + wk * NP, 0u);
-            uint32_t buf = 0u;
-            for(uint32_t t = wk; t < tiles; t += WK, buf ^= 1u)
+        // the tiles that every row sees all of come first
+        const int64_t  open = prefix < (int64_t)end ? prefix : (int64_t)end;
+        const uint32_t clear = open > (int64_t)begin ? static_cast<uint32_t>(open - begin) / NP : 0u;
+        uint32_t       buf = 0u, t = WQ == 1u ? wk : 0u;
+        // tile t (of tiles wk, wk + 4, ... where every wave has its own)
+        auto step = [&](auto maskedTile) __attribute__((always_inline)) {
+            if constexpr(WQ == 1u)
             {
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the reads of the buffer that is filled next have returned
                 if(t + WK < tiles)
                 {
-                    issue(begin + (t + WK) * NP, buf ^ 1u);
+                    issue(t + WK, buf ^ 1u);
                     r355::waitVmcnt<2u * LOADS>();
                 }
                 else
                     r355::waitVmcnt<0>();
                 asm volatile("" ::: "memory");
-                compute(begin + t * NP, buf);
+                compute(maskedTile, begin + t * NP, buf);
+                buf ^= 1u;
+                t += WK;
             }
-        }
-        else
-        {
-            if(tiles > 0u)
-                issue(begin, 0u);
-            if(tiles > 1u)
-                issue(begin + NP, 1u);
-            uint32_t buf = 0u;
-            for(uint32_t t = 0; t < tiles; ++t)
+            else
             {
                 if(t + 1u < tiles)
                     r355::waitVmcnt<2u * LOADS>();
@@ -383,11 +442,20 @@ namespace
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 r355::ldsBarrier(); // everyone's part of tile t is there, and everyone is done with the buffer of tile t - 1
                 if(t + 2u < tiles)
-                    issue(begin + (t + 2u) * NP, buf == 0u ? 2u : buf - 1u);
-                compute(begin + t * NP, buf);
+                    issue(t + 2u, buf == 0u ? 2u : buf - 1u);
+                compute(maskedTile, begin + t * NP, buf);
                 buf = buf == 2u ? 0u : buf + 1u;
+                t += 1u;
             }
-        }
+        };
+        if(t < tiles)
+            issue(t, 0u);
+        if(WQ > 1u && tiles > 1u)
+            issue(1u, 1u);
+        while(t < clear)
+            step(std::false_type{});
+        while(t < tiles)
+            step(std::true_type{});
 #pragma unroll
         for(uint32_t a = 0; a < QB; ++a)
             sum[a] = sumOverQuads(sum[a]);
@@ -475,36 +543,49 @@ namespace
         }
     }
 
-    // adds up the splits of a row, in order: one wave per row
-    template <typename T>
+    // Adds up the splits of a row, in order.  L = D / 4 lanes a row, each four elements; the lanes take the splits' maxima and sums side by side.
+    template <typename T, uint32_t D>
     __global__ void __launch_bounds__(256) treeMergeKernel(TreeParams p)
     {
-        const uint32_t lane = threadIdx.x & 63u;
-        const uint64_t item = (uint64_t)blockIdx.x * 4u + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); // (sequence, drafted token, head)
-        const uint32_t head = static_cast<uint32_t>(item % p.heads);
-        const uint64_t bt = item / p.heads;
-        const uint32_t b = static_cast<uint32_t>(bt / p.maxTokens), t = static_cast<uint32_t>(bt % p.maxTokens);
+        constexpr uint32_t L = D / 4u;
+        const uint32_t     lane = threadIdx.x % L;
+        const uint64_t     item = (uint64_t)blockIdx.x * (256u / L) + threadIdx.x / L; // (sequence, drafted token, head)
+        const uint32_t     head = static_cast<uint32_t>(item % p.heads);
+        const uint64_t     bt = item / p.heads;
+        const uint32_t     b = static_cast<uint32_t>(bt / p.maxTokens), t = static_cast<uint32_t>(bt % p.maxTokens);
         if(b >= p.batch)
             return;
-        const Sequence seq = sequenceOf(p, b);
+        const Sequence seq = sequenceOf(p, p.qStart[b], p.qStart[b + 1u], p.kvLen[b]);
         const uint32_t chunk = chunkOf(seq.length, p.splits);
         if(t >= seq.tokens || seq.length <= chunk)
             return;
         const uint32_t splits = (seq.length + chunk - 1u) / chunk;
         const uint64_t row = (uint64_t)(seq.first + t) * p.heads + head, allRows = (uint64_t)p.totalTokens * p.heads;
         const float*   ends = p.partial + (uint64_t)p.splits * allRows * p.dim + row * 2u;
+        const float*   from = p.partial + row * p.dim + lane * 4u;
         float          most = -INFINITY;
-        for(uint32_t s = 0; s < splits; ++s)
+        for(uint32_t s = lane; s < splits; s += L)
             most = fmaxf(most, ends[s * allRows * 2u]);
+#pragma unroll
+        for(uint32_t x = 1u; x < L; x *= 2u)
+            most = fmaxf(most, __shfl_xor(most, x));
         float total = 0.0f;
         f32x4 all{0, 0, 0, 0};
-        for(uint32_t s = 0; s < splits; ++s)
+        for(uint32_t s0 = 0; s0 < splits; s0 += L)
         {
-            const float theirs = ends[s * allRows * 2u];
-            const float factor = theirs == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(theirs - most);
-            total += factor * ends[s * allRows * 2u + 1u];
-            if(lane * 4u < p.dim)
-                all += factor * *reinterpret_cast<const f32x4*>(p.partial + (s * allRows + row) * p.dim + lane * 4u);
+            float theirs = -INFINITY, sum = 0.0f;
+            if(s0 + lane < splits)
+                theirs = ends[(s0 + lane) * allRows * 2u], sum = ends[(s0 + lane) * allRows * 2u + 1u];
+            const float    factor = theirs == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(theirs - most);
+            const uint32_t here   = splits - s0 < L ? splits - s0 : L;
+#pragma unroll 8
+            for(uint32_t s = 0; s < here; ++s)
+            {
+                const float f = __shfl(factor, s, L);
+                total += f * __shfl(sum, s, L);
+                if(lane * 4u < p.dim)
+                    all += f * *reinterpret_cast<const f32x4*>(from + (s0 + s) * allRows * p.dim);
+            }
         }
         const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
         if(lane * 4u < p.dim)
@@ -527,7 +608,9 @@ namespace
         plan.rowTiles     = static_cast<uint32_t>((rows + plan.rowsPerGroup - 1u) / plan.rowsPerGroup);
         const uint64_t groups = (uint64_t)a.batch * a.kv_heads * plan.rowTiles;
         const uint64_t cus    = r355::computeUnits();
-        uint64_t       want   = (2u * cus + groups - 1u) / groups;
+        // one row tile for all rows: four workgroups a CU, as sequences differ in length (32 x 1 token of 820..8192 positions, 32 / 8 heads of 128:
+        // two 136 us, four 128, eight 136); tiles of 128 rows: two (2 x 64 tokens over 65600: two 207, four 237: more partial results)
+        uint64_t       want   = ((plan.rowsPerGroup <= 64u && a.head_dim <= 128u ? 4u : 2u) * cus + groups - 1u) / groups;
         const uint64_t least  = ((uint64_t)a.max_kv + LEAST_CHUNK - 1u) / LEAST_CHUNK;
         want                  = want < least ? want : least;
         want                  = want < mostSplits ? want : mostSplits;
@@ -561,6 +644,11 @@ namespace
                 launchTree<T, D, 1, 4>(p, plan, s);
             else
                 launchTree<T, D, 4, 2>(p, plan, s);
+            if(plan.splits > 1u)
+            {
+                const uint64_t items = (uint64_t)p.batch * p.maxTokens * p.heads;
+                hipLaunchKernelGGL((treeMergeKernel<T, D>), dim3(static_cast<uint32_t>((items + 1024u / D - 1u) / (1024u / D))), dim3(256), 0, s, p);
+            }
         };
         using std::integral_constant;
         if(p.dim <= 64u)
@@ -569,11 +657,6 @@ namespace
             byRows(integral_constant<uint32_t, 128>{});
         else
             byRows(integral_constant<uint32_t, 256>{});
-        if(plan.splits > 1u)
-        {
-            const uint64_t items = (uint64_t)p.batch * p.maxTokens * p.heads;
-            hipLaunchKernelGGL(treeMergeKernel<T>, dim3(static_cast<uint32_t>((items + 3u) / 4u)), dim3(256), 0, s, p);
-        }
     }
 
     // everything that the sizes alone decide
@@ -634,8 +717,10 @@ extern "C" int r355_tree_attention(const r355_tree_attention_args* args, void* s
         return r355::fail(R355_ERR_MISALIGNED, "tree_attention: lse needs 4-byte alignment");
     if(a.mask && !r355::aligned(a.mask, 8))
         return r355::fail(R355_ERR_MISALIGNED, "tree_attention: the mask needs 8-byte alignment");
-    if(a.k_slot_stride < 0 || a.v_slot_stride < 0 || a.k_slot_stride > (1 << 25) || a.v_slot_stride > (1 << 25))
-        return r355::fail(R355_ERR_BAD_SIZE, "tree_attention: slot strides must be 0 to 2^25 elements");
+    if(a.k_slot_stride < (int64_t)a.head_dim || a.v_slot_stride < (int64_t)a.head_dim || a.k_slot_stride > (1 << 25) || a.v_slot_stride > (1 << 25))
+        return r355::fail(R355_ERR_BAD_SIZE, "tree_attention: slot strides must be head_dim to 2^25 elements");
+    if((uint64_t)a.pages * (a.page_size / 16u) >= 0xFFFFFFFFull)
+        return r355::fail(R355_ERR_BAD_SIZE, "tree_attention: a cache of 2^36 slots and more");
     if(a.workspace && !r355::aligned(a.workspace, 16))
         return r355::fail(R355_ERR_MISALIGNED, "tree_attention: the workspace needs 16-byte alignment");
     const uint64_t perSplit = (uint64_t)a.total_tokens * a.heads * (a.head_dim + 2u) * 4u;
@@ -651,7 +736,8 @@ extern "C" int r355_tree_attention(const r355_tree_attention_args* args, void* s
     p.totalTokens = a.total_tokens, p.maxTokens = a.max_tokens, p.maxKv = a.max_kv;
     p.pageSize = a.page_size, p.pages = a.pages, p.tableStride = a.table_stride, p.maskWords = a.mask_words;
     p.splits = plan.splits, p.columns = (a.batch * a.kv_heads * plan.splits + 7u) / 8u * 8u; // (row tiles of one split on one XCD)
-    p.scale2 = static_cast<float>(a.scale * 1.4426950408889634);
+    p.scale2 = std::fmax(static_cast<float>(std::fabs(a.scale) * 1.4426950408889634), 1.17549435e-38f);
+    p.signs  = a.scale < 0.0 ? 0x80008000u : 0u;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     r355::beginCall();
     if(a.type == R355_F16)

@@ -335,6 +335,8 @@ def test_tree_refusals():
     _refused(-3, max_kv=257)
     _refused(-3, max_kv=(1 << 30) + 1)
     _refused(-3, k_strides=(1 << 26, 64))
+    _refused(-3, v_strides=(56, 64))
+    _refused(-3, pages=1 << 31, page_size=48)
     _refused(-3, batch=1 << 24)
     _refused(-4, q=0x1008)
     _refused(-4, k=0x2008)
