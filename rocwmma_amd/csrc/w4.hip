@@ -38,73 +38,130 @@ namespace
         uint32_t       tokens, n, k, group, groups;
         uint32_t       ldx, ldc, ldy;
         uint32_t       blocksN, blocksK; // of 16 rows, of 128 k
-        uint32_t       tilesN, tilesT, perXcd; // workgroups along n and tokens; tiles of n for each XCD
+        uint32_t       perGroup, groupMagic; // blocks of 128 k per group of 128 and more, and 2^32 over it, rounded up (exact: both numbers of blocks are at most 2^15)
+        uint32_t       tilesN, tilesT, perXcd; // workgroups along n and tokens, and of each XCD
         uint32_t       outF32, wideN; // wideN: 4-element accesses of c and y
         float          alpha, beta;
     };
 
-    // two weights of a dword (nibbles p and p + 4) as 16 + q each
+    constexpr uint32_t OUTSIDE = 0x7FFFFFF0u; // a lane's offset past the end of any buffer: it loads zeros
+
+    // Eight weights of a dword as 16 + q each, two (nibbles p and p + 4) a register.  The two constants are kept from the compiler, which otherwise makes
+    // an and and an or with literals of what is one instruction with registers.
     template <typename T>
-    __device__ __forceinline__ u32x4 expand(uint32_t d)
+    struct Expand
+    {
+        uint32_t mask, sixteen;
+        __device__ __forceinline__ Expand()
+        {
+            mask = std::is_same_v<T, __bf16> ? 0x00780078u : 0x03C003C0u, sixteen = std::is_same_v<T, __bf16> ? 0x41804180u : 0x4C004C00u;
+            asm volatile("" : "+s"(mask), "+v"(sixteen));
+        }
+        __device__ __forceinline__ u32x4 operator()(uint32_t d) const
+        {
+            if constexpr(std::is_same_v<T, __bf16>)
+                return u32x4{((d << 3) & mask) | sixteen, ((d >> 1) & mask) | sixteen, ((d >> 5) & mask) | sixteen, ((d >> 9) & mask) | sixteen};
+            else
+                return u32x4{((d << 6) & mask) | sixteen, ((d << 2) & mask) | sixteen, ((d >> 2) & mask) | sixteen, ((d >> 6) & mask) | sixteen};
+        }
+    };
+
+    template <typename T>
+    __device__ __forceinline__ u32x4 onesOf()
+    {
+        constexpr uint32_t ONE = std::is_same_v<T, __bf16> ? 0x3F803F80u : 0x3C003C00u;
+        return u32x4{ONE, ONE, ONE, ONE};
+    }
+
+    // a 16-bit scale in the low half of a dword
+    template <typename T>
+    __device__ __forceinline__ float scaleOf(uint32_t v)
     {
         if constexpr(std::is_same_v<T, __bf16>)
-            return u32x4{((d << 3) & 0x00780078u) | 0x41804180u, ((d >> 1) & 0x00780078u) | 0x41804180u, ((d >> 5) & 0x00780078u) | 0x41804180u,
-                         ((d >> 9) & 0x00780078u) | 0x41804180u};
+            return __uint_as_float(v << 16);
         else
-            return u32x4{((d << 6) & 0x03C003C0u) | 0x4C004C00u, ((d << 2) & 0x03C003C0u) | 0x4C004C00u, ((d >> 2) & 0x03C003C0u) | 0x4C004C00u,
-                         ((d >> 6) & 0x03C003C0u) | 0x4C004C00u};
+            return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(v)));
     }
 
-    template <typename T>
-    constexpr uint32_t ONES = std::is_same_v<T, __bf16> ? 0x3F803F80u : 0x3C003C00u;
+    // scales of four rows, and 16 + z of their zero points
+    struct Values
+    {
+        f32x4 scale, zero;
+    };
 
-    template <typename T>
-    __device__ __forceinline__ f32x4 floats(u32x2 v)
+    // the first group of block kb of 128 k
+    template <uint32_t STEPS>
+    __device__ __forceinline__ uint32_t groupOf(const W4Params& p, uint32_t kb)
     {
-        const vec<T, 4> t = __builtin_bit_cast(vec<T, 4>, v);
-        return f32x4{static_cast<float>(t[0]), static_cast<float>(t[1]), static_cast<float>(t[2]), static_cast<float>(t[3])};
-    }
-    // 16 + z of four zero points
-    __device__ __forceinline__ f32x4 offsets(uint32_t v)
-    {
-        return f32x4{16.0f + static_cast<float>(v & 255u), 16.0f + static_cast<float>((v >> 8) & 255u), 16.0f + static_cast<float>((v >> 16) & 255u), 16.0f + static_cast<float>(v >> 24)};
+        return STEPS < 4u ? kb * (4u / STEPS) : p.perGroup == 1u ? kb : __umulhi(kb, p.groupMagic);
     }
 
-    struct __attribute__((packed, aligned(2))) Four16
+    // calls f with the integral constants 0 .. N - 1
+    template <uint32_t N, typename F>
+    __device__ __forceinline__ void each(F&& f)
     {
-        u32x2 v;
-    };
-    struct __attribute__((packed, aligned(1))) Four8
-    {
-        uint32_t v;
-    };
+        if constexpr(N > 0u)
+        {
+            each<N - 1u>(f);
+            f(std::integral_constant<uint32_t, N - 1u>{});
+        }
+    }
 
-    // The scales (zero points) of four rows of a group.  At the end of a row of them the last four are read and moved down.
-    struct RowsOf4
+    // One group (STEPS matrix instructions of 32 k): acc += s (sum x (16 + q) - (16 + z) sum x).  Every row of the product with ones is sum x.
+    // EARLY: with z = 8 everywhere the product of all rows starts from -24 sum x instead of zero; x(c, i) is held meanwhile.
+    template <typename T, uint32_t RB, uint32_t CB, uint32_t STEPS, bool ZEROS, bool EARLY, typename X, typename W, typename V>
+    __device__ __forceinline__ void accumulate(f32x4 (&acc)[RB][CB], const Expand<T>& expand, X&& x, W&& weights, V&& values)
     {
-        uint32_t at, past; // the first row read, and by how much the rows wanted lie behind it
-        __device__ __forceinline__ RowsOf4(uint32_t row, uint32_t n)
+        static_assert(!(ZEROS && EARLY), "one start for all rows");
+        const u32x4 ones = onesOf<T>();
+        f32x4       sumX[CB], sum[RB][CB];
+        u32x4       held[CB][EARLY ? STEPS : 1u];
+#pragma unroll
+        for(uint32_t c = 0; c < CB; ++c)
+            sumX[c] = f32x4{0, 0, 0, 0};
+        if constexpr(EARLY)
+#pragma unroll
+            for(uint32_t c = 0; c < CB; ++c)
+            {
+#pragma unroll
+                for(uint32_t i = 0; i < STEPS; ++i)
+                {
+                    held[c][i] = x(c, i);
+                    sumX[c]    = r355::mfma32<T>(ones, held[c][i], sumX[c]);
+                }
+                const float t = -24.0f * sumX[c][0];
+                sumX[c]       = f32x4{t, t, t, t};
+            }
+#pragma unroll
+        for(uint32_t i = 0; i < STEPS; ++i)
         {
-            at   = row + 4u <= n ? row : n - 4u;
-            past = row - at < 3u ? row - at : 3u;
+            if constexpr(!EARLY)
+#pragma unroll
+                for(uint32_t c = 0; c < CB; ++c)
+                {
+                    held[c][0] = x(c, i);
+                    sumX[c]    = r355::mfma32<T>(ones, held[c][0], sumX[c]);
+                }
+#pragma unroll
+            for(uint32_t r = 0; r < RB; ++r)
+            {
+                const u32x4 a = expand(weights(r, i));
+#pragma unroll
+                for(uint32_t c = 0; c < CB; ++c)
+                    sum[r][c] = r355::mfma32<T>(a, held[c][EARLY ? i : 0u], i != 0u ? sum[r][c] : EARLY ? sumX[c] : f32x4{0, 0, 0, 0});
+            }
         }
-        __device__ __forceinline__ u32x2 scales(const W4Params& p, uint32_t g) const
+#pragma unroll
+        for(uint32_t r = 0; r < RB; ++r)
         {
-            return reinterpret_cast<const Four16*>(p.scales + 2u * ((uint64_t)g * p.n + at))->v;
+            const Values v = values(r);
+#pragma unroll
+            for(uint32_t c = 0; c < CB; ++c)
+#pragma unroll
+                for(uint32_t j = 0; j < 4; ++j)
+                    acc[r][c][j] = fmaf(v.scale[j], EARLY ? sum[r][c][j] : fmaf(ZEROS ? -v.zero[j] : -24.0f, sumX[c][0], sum[r][c][j]), acc[r][c][j]);
         }
-        __device__ __forceinline__ uint32_t zeros(const W4Params& p, uint32_t g) const
-        {
-            return reinterpret_cast<const Four8*>(p.zeros + (uint64_t)g * p.n + at)->v;
-        }
-        __device__ __forceinline__ u32x2 moved(u32x2 v) const
-        {
-            return __builtin_bit_cast(u32x2, __builtin_bit_cast(uint64_t, v) >> (16u * past));
-        }
-        __device__ __forceinline__ uint32_t moved(uint32_t v) const
-        {
-            return v >> (8u * past);
-        }
-    };
+    }
 
     template <typename O>
     __device__ __forceinline__ void storeRows(const W4Params& p, uint32_t token, uint32_t row, f32x4 sum)
@@ -117,6 +174,7 @@ namespace
             if(p.beta != 0.0f)
             {
                 const vec<O, 4> was = *reinterpret_cast<const vec<O, 4>*>(c);
+#pragma unroll
                 for(uint32_t e = 0; e < 4; ++e)
                     out[e] += p.beta * static_cast<float>(was[e]);
             }
@@ -139,20 +197,29 @@ namespace
             storeRows<T>(p, token, row, sum);
     }
 
-    // Tile of n and tile of tokens of a workgroup: workgroups id, id + 8, ... run on one XCD and take a contiguous stretch of n (the scales of
-    // neighbouring rows share cache lines), all tiles of tokens of one tile of n after another.
+    // Tile of n and tile of tokens of a workgroup: workgroups id, id + 8, ... run on one XCD and take a contiguous stretch of the tiles, those of one tile of
+    // n after another (the scales of neighbouring rows share cache lines, the weights a tile of n).
     __device__ __forceinline__ bool tileOf(const W4Params& p, uint32_t& tileN, uint32_t& tileT)
     {
-        const uint32_t id = blockIdx.x / 8u;
-        tileN = blockIdx.x % 8u * p.perXcd + id / p.tilesT, tileT = id % p.tilesT;
-        return id / p.tilesT < p.perXcd && tileN < p.tilesN;
+        const uint32_t id = blockIdx.x % 8u * p.perXcd + blockIdx.x / 8u;
+        tileN = id / p.tilesT, tileT = id % p.tilesT;
+        return tileN < p.tilesN;
     }
 
-    // ---- few tokens.  A workgroup's waves share 16 RB rows x 16 CB tokens and take the 128-k blocks in turn; their sums meet in LDS in the order
-    // of the waves, so the result does not depend on scheduling.  STEPS: matrix instructions (32 k) per scale.  FAST: rows of x on 16-byte
-    // boundaries; everything that a block of k needs is requested, without branches, while the one before it is multiplied.
-    template <typename T, uint32_t RB, uint32_t CB, uint32_t STEPS, bool ZEROS, bool FAST>
-    __global__ void __launch_bounds__(512) w4Kernel(W4Params p)
+    // ---- A few tokens, or rows of x off 16-byte boundaries (FAST false).  A workgroup's waves share 16 RB rows x 16 CB tokens and take the 128-k blocks in
+    // turn, x and the weights straight from global memory; their sums meet in LDS in the order of the waves, so the result does not depend on
+    // scheduling.  STEPS: matrix instructions (32 k) per scale.  DEPTH blocks in flight, each in registers of its own.
+    struct __attribute__((packed, aligned(2))) Four16
+    {
+        u32x2 v;
+    };
+    struct __attribute__((packed, aligned(1))) Four8
+    {
+        uint32_t v;
+    };
+
+    template <typename T, uint32_t RB, uint32_t CB, uint32_t DEPTH, uint32_t STEPS, bool ZEROS, bool FAST>
+    __global__ void __launch_bounds__(512, FAST ? 2 : 1) w4Kernel(W4Params p)
     {
         extern __shared__ __attribute__((aligned(16))) float sums[]; // [waves][RB * CB][64][4]
         constexpr uint32_t PARTS = 4u / STEPS;
@@ -161,136 +228,135 @@ namespace
             return;
         const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
         const uint32_t col = lane & 15u, quad = lane >> 4;
-        const uint32_t block0 = tileN * RB, token0 = tileT * 16u * CB;
-        const u32x4    ones{ONES<T>, ONES<T>, ONES<T>, ONES<T>};
-        const f32x4    none{0, 0, 0, 0};
-        f32x4          acc[RB][CB];
+        const uint32_t block0 = tileN * RB, token0 = tileT * 16u * CB, left = p.tokens - token0;
+        const Expand<T> expand;
+        f32x4           acc[RB][CB];
 #pragma unroll
         for(uint32_t r = 0; r < RB; ++r)
 #pragma unroll
             for(uint32_t c = 0; c < CB; ++c)
-                acc[r][c] = none;
+                acc[r][c] = f32x4{0, 0, 0, 0};
 
+        // Where a block of 128 k has several groups, neighbouring lanes read one each and exchange them: one load instead of four.
         struct Stage
         {
             u32x4    w[RB], x[CB][4];
-            u32x2    scale[RB][PARTS];
-            uint32_t zero[RB][PARTS];
+            u32x2    scale[RB];
+            uint32_t zero[RB];
         };
-        const uint32_t left = p.tokens - token0;
+        const uint32_t mine = lane % PARTS;
         // (a buffer over the rows of x from token0 on, which ends with the last element; lanes without a token lie past it)
-        constexpr uint32_t OUTSIDE = 0x7FFFFFF0u;
         const auto bufX = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p.x) + (uint64_t)token0 * p.ldx * 2u, 0,
                                                             FAST ? ((left < 16u * CB ? left : 16u * CB) - 1u) * p.ldx * 2u + p.k * 2u : 0u, 0x00020000);
+        uint32_t offX[CB];
+#pragma unroll
+        for(uint32_t c = 0; c < CB; ++c)
+            offX[c] = c * 16u + col < left ? (c * 16u + col) * p.ldx * 2u + quad * 16u : OUTSIDE;
+        // FAST: at the end of a row of scales (n is 4 at least) the last four are read and moved down
+        auto rowOf = [&](uint32_t r) __attribute__((always_inline)) { return (block0 + r) * 16u + quad * 4u; };
+        auto readOf = [&](uint32_t r) __attribute__((always_inline)) { return rowOf(r) + 4u <= p.n ? rowOf(r) : p.n - 4u; };
         auto load = [&](uint32_t kb) __attribute__((always_inline)) {
-            Stage s;
+            Stage          s;
+            const uint32_t of = groupOf<STEPS>(p, kb) + mine;
+            const uint64_t g  = of < p.groups ? of : p.groups - 1u; // (past k: x is zero there)
 #pragma unroll
             for(uint32_t r = 0; r < RB; ++r)
             {
                 const uint32_t b = block0 + r < p.blocksN ? block0 + r : p.blocksN - 1u;
                 s.w[r]           = *reinterpret_cast<const u32x4*>(p.w + ((uint64_t)b * p.blocksK + kb) * 1024u + lane * 16u);
+                if constexpr(FAST)
+                {
+                    s.scale[r] = reinterpret_cast<const Four16*>(p.scales + 2u * (g * p.n + readOf(r)))->v;
+                    s.zero[r]  = ZEROS ? reinterpret_cast<const Four8*>(p.zeros + g * p.n + readOf(r))->v : 0u;
+                }
+                else
+                {
+                    s.scale[r] = u32x2{0u, 0u}, s.zero[r] = 0u;
+#pragma unroll
+                    for(uint32_t e = 0; e < 4; ++e)
+                        if(rowOf(r) + e < p.n)
+                        {
+                            s.scale[r][e / 2u] |= (uint32_t)reinterpret_cast<const uint16_t*>(p.scales)[g * p.n + rowOf(r) + e] << (e % 2u * 16u);
+                            if(ZEROS)
+                                s.zero[r] |= (uint32_t)p.zeros[g * p.n + rowOf(r) + e] << (e * 8u);
+                        }
+                }
             }
 #pragma unroll
             for(uint32_t c = 0; c < CB; ++c)
 #pragma unroll
                 for(uint32_t i = 0; i < 4u; ++i)
                 {
-                    const uint32_t k = kb * 128u + i * 32u + quad * 8u;
                     if constexpr(FAST)
-                        s.x[c][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(bufX, c * 16u + col < left && k < p.k ? (c * 16u + col) * p.ldx * 2u + k * 2u : OUTSIDE, 0, 0));
+                        s.x[c][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(bufX, offX[c] + i * 64u, kb * 256u, 0));
                     else
                     {
-                        vec<T, 8> v;
+                        const uint32_t k = kb * 128u + i * 32u + quad * 8u;
+                        vec<T, 8>      v;
 #pragma unroll
                         for(uint32_t e = 0; e < 8; ++e)
                             v[e] = c * 16u + col < left && k + e < p.k ? reinterpret_cast<const T*>(p.x)[(uint64_t)(token0 + c * 16u + col) * p.ldx + k + e] : T(0.0f);
                         s.x[c][i] = __builtin_bit_cast(u32x4, v);
                     }
                 }
-#pragma unroll
-            for(uint32_t part = 0; part < PARTS; ++part)
-            {
-                const uint32_t of = (kb * 128u + part * STEPS * 32u) / p.group, g = of < p.groups ? of : p.groups - 1u;
-#pragma unroll
-                for(uint32_t r = 0; r < RB; ++r)
-                {
-                    const uint32_t row = (block0 + r) * 16u + quad * 4u;
-                    if constexpr(FAST)
-                    {
-                        const RowsOf4 rows(row, p.n);
-                        s.scale[r][part] = rows.scales(p, g);
-                        s.zero[r][part]  = ZEROS ? rows.zeros(p, g) : 0u;
-                    }
-                    else
-                    {
-                        s.scale[r][part] = u32x2{0u, 0u}, s.zero[r][part] = 0u;
-#pragma unroll
-                        for(uint32_t e = 0; e < 4; ++e)
-                            if(row + e < p.n)
-                            {
-                                s.scale[r][part][e / 2u] |= (uint32_t)reinterpret_cast<const uint16_t*>(p.scales)[(uint64_t)g * p.n + row + e] << (e % 2u * 16u);
-                                if(ZEROS)
-                                    s.zero[r][part] |= (uint32_t)p.zeros[(uint64_t)g * p.n + row + e] << (e * 8u);
-                            }
-                    }
-                }
-            }
             return s;
         };
+        // (in the last block of k a lane's pieces past k are those of the next token or of what lies between the rows)
+        auto trim = [&](Stage& s, uint32_t kb) __attribute__((always_inline)) {
+#pragma unroll
+            for(uint32_t i = 0; i < 4u; ++i)
+                if(kb * 128u + i * 32u + quad * 8u >= p.k)
+#pragma unroll
+                    for(uint32_t c = 0; c < CB; ++c)
+                        s.x[c][i] = u32x4{0u, 0u, 0u, 0u};
+        };
         auto multiply = [&](const Stage& s) __attribute__((always_inline)) {
+            u32x2    scales[RB]; // of the lane's group
+            uint32_t zeros[RB];
 #pragma unroll
-            for(uint32_t part = 0; part < PARTS; ++part)
+            for(uint32_t r = 0; r < RB; ++r)
             {
-                f32x4 sum[RB][CB], sumX[CB];
-#pragma unroll
-                for(uint32_t i = 0; i < STEPS; ++i)
-                {
-#pragma unroll
-                    for(uint32_t c = 0; c < CB; ++c)
-                        sumX[c] = r355::mfma32<T>(ones, s.x[c][part * STEPS + i], i == 0u ? none : sumX[c]);
-#pragma unroll
-                    for(uint32_t r = 0; r < RB; ++r)
-                    {
-                        const u32x4 a = expand<T>(s.w[r][part * STEPS + i]);
-#pragma unroll
-                        for(uint32_t c = 0; c < CB; ++c)
-                            sum[r][c] = r355::mfma32<T>(a, s.x[c][part * STEPS + i], i == 0u ? none : sum[r][c]);
-                    }
-                }
-#pragma unroll
-                for(uint32_t r = 0; r < RB; ++r)
-                {
-                    const RowsOf4 rows((block0 + r) * 16u + quad * 4u, p.n);
-                    const f32x4   scale = floats<T>(FAST ? rows.moved(s.scale[r][part]) : s.scale[r][part]);
-                    f32x4         zero{24.0f, 24.0f, 24.0f, 24.0f};
-                    if constexpr(ZEROS)
-                        zero = offsets(FAST ? rows.moved(s.zero[r][part]) : s.zero[r][part]);
-#pragma unroll
-                    for(uint32_t c = 0; c < CB; ++c)
+                const uint32_t past = !FAST ? 0u : rowOf(r) - readOf(r) < 3u ? rowOf(r) - readOf(r) : 3u;
+                scales[r] = __builtin_bit_cast(u32x2, __builtin_bit_cast(uint64_t, s.scale[r]) >> (16u * past)), zeros[r] = s.zero[r] >> (8u * past);
+            }
+            each<PARTS>([&](auto partAt) __attribute__((always_inline)) {
+                constexpr uint32_t part = decltype(partAt)::value;
+                auto               of   = [](uint32_t v) __attribute__((always_inline)) {
+                    return PARTS > 1u ? static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), part * 0x55, 0xF, 0xF, true)) : v;
+                };
+                accumulate<T, RB, CB, STEPS, ZEROS, !ZEROS>(
+                    acc, expand, [&](uint32_t c, uint32_t i) __attribute__((always_inline)) { return s.x[c][part * STEPS + i]; },
+                    [&](uint32_t r, uint32_t i) __attribute__((always_inline)) { return s.w[r][part * STEPS + i]; },
+                    [&](uint32_t r) __attribute__((always_inline)) {
+                        const uint32_t lo = of(scales[r][0]), hi = of(scales[r][1]), z = ZEROS ? of(zeros[r]) : 0u;
+                        Values         v;
+                        v.scale = f32x4{scaleOf<T>(lo & 0xFFFFu), scaleOf<T>(lo >> 16), scaleOf<T>(hi & 0xFFFFu), scaleOf<T>(hi >> 16)};
 #pragma unroll
                         for(uint32_t j = 0; j < 4; ++j)
-                            acc[r][c][j] = fmaf(scale[j], fmaf(-zero[j], sumX[c][j], sum[r][c][j]), acc[r][c][j]);
-                }
-            }
+                            v.zero[j] = 16.0f + static_cast<float>((z >> (8u * j)) & 255u);
+                        return v;
+                    });
+            });
         };
-        if(wave < p.blocksK)
-        {
-            Stage now = load(wave);
-            for(uint32_t kb = wave;;)
-            {
-                const uint32_t next = kb + waves;
-                if(next >= p.blocksK)
+        Stage stage[DEPTH]; // (a copy from one stage to the next would wait for its loads)
+        each<DEPTH>([&](auto at) __attribute__((always_inline)) {
+            constexpr uint32_t d = decltype(at)::value;
+            if(wave + d * waves < p.blocksK)
+                stage[d] = load(wave + d * waves);
+        });
+        for(uint32_t first = wave; first < p.blocksK; first += DEPTH * waves)
+            each<DEPTH>([&](auto at) __attribute__((always_inline)) {
+                constexpr uint32_t d  = decltype(at)::value;
+                const uint32_t     kb = first + d * waves;
+                if(kb < p.blocksK)
                 {
-                    multiply(now);
-                    break;
+                    if(FAST && kb + 1u == p.blocksK && p.k % 128u != 0u)
+                        trim(stage[d], kb);
+                    multiply(stage[d]);
+                    if(kb + DEPTH * waves < p.blocksK)
+                        stage[d] = load(kb + DEPTH * waves);
                 }
-                const Stage then = load(next);
-                __builtin_amdgcn_sched_barrier(0);
-                multiply(now);
-                __builtin_amdgcn_sched_barrier(0);
-                now = then, kb = next;
-            }
-        }
+            });
 
 #pragma unroll
         for(uint32_t r = 0; r < RB; ++r)
@@ -300,139 +366,195 @@ namespace
         __syncthreads();
         for(uint32_t u = wave; u < RB * CB; u += waves)
         {
-            f32x4 sum = none;
+            f32x4 sum{0, 0, 0, 0};
             for(uint32_t v = 0; v < waves; ++v)
                 sum += *reinterpret_cast<const f32x4*>(sums + ((v * RB * CB + u) * 64u + lane) * 4u);
             store<T>(p, token0 + u % CB * 16u + col, (block0 + u / CB) * 16u + quad * 4u, sum);
         }
     }
 
-    // ---- many tokens: 128 rows x 128 tokens a workgroup, 64 x 64 a wave.  x goes to LDS by direct loads a block of 128 k ahead (16-byte pieces of a
-    // row in slots that depend on the row: a wave reads 16 rows at one place), the weights of a wave's own rows straight to its registers.
-    // Bound by the vector ALU: of 64 k (group 64) a wave's 40 matrix instructions take 640 cycles, two operands for each of its 4096 weights 290
-    // and scaling its 4096 sums 510.
-    template <typename T, uint32_t STEPS, bool ZEROS>
-    __global__ void __launch_bounds__(256, 2) w4TileKernel(W4Params p)
+    // ---- More tokens: 16 RB WN rows x 16 CB WT tokens a workgroup, 16 RB x 16 CB a wave; WK sets of such waves take the blocks of 128 k in turn.
+    // Everything comes by direct loads into a ring of LDS buffers, as many steps ahead as fit: x in rows of 256 bytes (16-byte pieces in slots that depend on the
+    // row: a wave reads 16 rows at one place), the weights as they are packed, a wave's scales and zero points one to a dword.  (Loads into registers among the
+    // direct ones would have the compiler wait for all of them.)
+    __device__ __forceinline__ void loadShortToLds(r355::dma_i32x4 rsrc, uint32_t laneOffset, uint32_t ldsAddr)
     {
-        constexpr uint32_t PARTS = 4u / STEPS, TILE = 128u * 256u, LOADS = 8, OUTSIDE = 0x7FFFFFF0u;
-        __shared__ __attribute__((aligned(1024))) char lds[2u * TILE];
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_ushort %0, %1, 0 offen lds" : : "v"(laneOffset), "s"(rsrc), "s"(ldsAddr) : "memory");
+    }
+    __device__ __forceinline__ void loadByteToLds(r355::dma_i32x4 rsrc, uint32_t laneOffset, uint32_t ldsAddr)
+    {
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_ubyte %0, %1, 0 offen lds" : : "v"(laneOffset), "s"(rsrc), "s"(ldsAddr) : "memory");
+    }
+
+    template <uint32_t RB, uint32_t CB, uint32_t WN, uint32_t WT, uint32_t WK, uint32_t STEPS, bool ZEROS>
+    struct Ring
+    {
+        static constexpr uint32_t WAVES = WN * WT * WK, TOKENS = 16u * CB * WT, PARTS = 4u / STEPS;
+        static constexpr uint32_t X = WK * TOKENS * 256u, W = WK * WN * RB * 1024u; // bytes of a step
+        static constexpr uint32_t SCALES = (RB * PARTS + 3u) / 4u; // loads of 64 scales
+        static constexpr uint32_t STAGE = X + W + WAVES * SCALES * 256u * (ZEROS ? 2u : 1u);
+        static constexpr uint32_t LOADS_X = WK * TOKENS / 4u / WAVES, LOADS_W = W / 1024u / WAVES; // of a wave
+        static constexpr uint32_t LOADS = LOADS_X + LOADS_W + SCALES * (ZEROS ? 2u : 1u);
+        static constexpr uint32_t MERGE = WK > 1u ? WAVES * RB * CB * 1024u : 0u;
+        static constexpr uint32_t FIT = 160u * 1024u / STAGE, BUFS = FIT > 4u ? 4u : FIT;
+        static constexpr uint32_t LDS = BUFS * STAGE > MERGE ? BUFS * STAGE : MERGE;
+        static_assert(LOADS_X * WAVES * 4u == WK * TOKENS && LOADS_W * WAVES * 1024u == W, "whole loads for every wave");
+        static_assert(BUFS >= 2u && LOADS * (BUFS - 2u) < 64u && LDS <= 160u * 1024u, "LDS and counters");
+    };
+
+    template <typename T, uint32_t RB, uint32_t CB, uint32_t WN, uint32_t WT, uint32_t WK, uint32_t STEPS, bool ZEROS>
+    __global__ void __launch_bounds__(64 * WN * WT * WK, 1) w4RingKernel(W4Params p)
+    {
+        using R                  = Ring<RB, CB, WN, WT, WK, STEPS, ZEROS>;
+        constexpr uint32_t WAVES = R::WAVES, TOKENS = R::TOKENS, PARTS = R::PARTS, BUFS = R::BUFS;
+        __shared__ __attribute__((aligned(1024))) char lds[R::LDS];
         uint32_t tileN, tileT;
         if(!tileOf(p, tileN, tileT))
             return;
         const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        const uint32_t col = lane & 15u, quad = lane >> 4, waveN = wave & 1u, waveT = wave >> 1;
-        const uint32_t block0 = tileN * 8u + waveN * 4u, token0 = tileT * 128u, left = p.tokens - token0 < 128u ? p.tokens - token0 : 128u;
+        const uint32_t col = lane & 15u, quad = lane >> 4, waveN = wave % WN, waveT = wave / WN % WT, waveK = wave / (WN * WT);
+        const uint32_t group0 = tileN * WN * RB, block0 = group0 + waveN * RB, token0 = tileT * TOKENS, left = p.tokens - token0 < TOKENS ? p.tokens - token0 : TOKENS;
         const uint32_t ldsBase = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
+        constexpr uint32_t RECORDS = 0x7FFF0000u;
 
-        // rows 4 j + lane / 16 of the wave's 32 tokens; past the tokens and past k: outside the buffer, which loads zeros
+        // x: a load brings four rows of one block of k; past the tokens and past k: outside the buffer
         r355::dma_i32x4 bufX = r355::rawBuffer(reinterpret_cast<uint64_t>(p.x) + (uint64_t)token0 * p.ldx * 2u);
         bufX[2]              = __builtin_amdgcn_readfirstlane((left - 1u) * p.ldx * 2u + p.k * 2u);
-        uint32_t offX[LOADS], pieceK[LOADS];
+        uint32_t offX[R::LOADS_X];
 #pragma unroll
-        for(uint32_t j = 0; j < LOADS; ++j)
+        for(uint32_t j = 0; j < R::LOADS_X; ++j)
         {
-            const uint32_t row = wave * 32u + j * 4u + (lane >> 4), piece = col ^ (row & 15u);
-            offX[j] = row < left ? row * p.ldx * 2u + piece * 16u : OUTSIDE, pieceK[j] = piece * 8u;
+            const uint32_t row = (wave * R::LOADS_X + j) * 4u % TOKENS + quad;
+            offX[j] = row < left ? row * p.ldx * 2u + (col ^ (row & 15u)) * 16u : OUTSIDE;
         }
-        auto issue = [&](uint32_t kb, uint32_t buf) __attribute__((always_inline)) {
-            const uint32_t to = __builtin_amdgcn_readfirstlane(ldsBase + buf * TILE + wave * 8192u);
+        // scales: element (row block r, group of the block, row), 64 to a load
+        uint32_t offS[R::SCALES], partS[R::SCALES];
 #pragma unroll
-            for(uint32_t j = 0; j < LOADS; ++j)
-                r355::loadToLds(bufX, kb * 128u + pieceK[j] < p.k ? offX[j] : OUTSIDE, kb * 256u, to + j * 1024u);
-        };
-
-        struct Stage
+        for(uint32_t j = 0; j < R::SCALES; ++j)
         {
-            u32x4    w[4];
-            u32x2    scale[4][PARTS];
-            uint32_t zero[4][PARTS];
-        };
-        auto load = [&](uint32_t kb) __attribute__((always_inline)) {
-            Stage s;
+            const uint32_t e = j * 64u + lane, r = e / (16u * PARTS), row = (block0 + r) * 16u + e % 16u;
+            partS[j] = e / 16u % PARTS;
+            offS[j]  = r < RB && row < p.n ? partS[j] * p.n + row : OUTSIDE / 2u;
+        }
+        auto issue = [&](uint32_t step, uint32_t buf) __attribute__((always_inline)) {
+            const uint32_t to = ldsBase + buf * R::STAGE;
 #pragma unroll
-            for(uint32_t r = 0; r < 4u; ++r)
+            for(uint32_t j = 0; j < R::LOADS_X; ++j)
             {
-                const uint32_t b = block0 + r < p.blocksN ? block0 + r : p.blocksN - 1u;
-                s.w[r]           = *reinterpret_cast<const u32x4*>(p.w + ((uint64_t)b * p.blocksK + kb) * 1024u + lane * 16u);
-                const RowsOf4 rows((block0 + r) * 16u + quad * 4u, p.n);
-#pragma unroll
-                for(uint32_t part = 0; part < PARTS; ++part)
-                {
-                    const uint32_t of = (kb * 128u + part * STEPS * 32u) / p.group, g = of < p.groups ? of : p.groups - 1u;
-                    s.scale[r][part] = rows.scales(p, g);
-                    s.zero[r][part]  = ZEROS ? rows.zeros(p, g) : 0u;
-                }
+                const uint32_t at = wave * R::LOADS_X + j, kb = step * WK + at * 4u / TOKENS;
+                const uint32_t k  = kb * 128u + (col ^ ((at * 4u % TOKENS + quad) & 15u)) * 8u;
+                r355::loadToLds(bufX, k < p.k ? offX[j] : OUTSIDE, __builtin_amdgcn_readfirstlane(kb * 256u), __builtin_amdgcn_readfirstlane(to + at * 1024u));
             }
-            return s;
+#pragma unroll
+            for(uint32_t j = 0; j < R::LOADS_W; ++j)
+            {
+                const uint32_t at = wave * R::LOADS_W + j, kb = step * WK + at / (WN * RB), block = group0 + at % (WN * RB);
+                r355::dma_i32x4 bufW = r355::rawBuffer(reinterpret_cast<uint64_t>(p.w) + ((uint64_t)block * p.blocksK + kb) * 1024u);
+                bufW[2]              = __builtin_amdgcn_readfirstlane(block < p.blocksN && kb < p.blocksK ? 1024u : 0u);
+                r355::loadToLds(bufW, lane * 16u, 0u, __builtin_amdgcn_readfirstlane(to + R::X + at * 1024u));
+            }
+            const uint32_t  g    = groupOf<STEPS>(p, step * WK + waveK);
+            r355::dma_i32x4 bufS = r355::rawBuffer(reinterpret_cast<uint64_t>(p.scales) + (uint64_t)g * p.n * 2u);
+            bufS[2]              = RECORDS;
+#pragma unroll
+            for(uint32_t j = 0; j < R::SCALES; ++j)
+                loadShortToLds(bufS, (g + partS[j] < p.groups ? offS[j] : OUTSIDE / 2u) * 2u, __builtin_amdgcn_readfirstlane(to + R::X + R::W + (wave * R::SCALES + j) * 256u));
+            if constexpr(ZEROS)
+            {
+                r355::dma_i32x4 bufZ = r355::rawBuffer(reinterpret_cast<uint64_t>(p.zeros) + (uint64_t)g * p.n);
+                bufZ[2]              = RECORDS;
+#pragma unroll
+                for(uint32_t j = 0; j < R::SCALES; ++j)
+                    loadByteToLds(bufZ, g + partS[j] < p.groups && offS[j] != OUTSIDE / 2u ? offS[j] : OUTSIDE,
+                                  __builtin_amdgcn_readfirstlane(to + R::X + R::W + ((WAVES + wave) * R::SCALES + j) * 256u));
+            }
         };
-        const u32x4 ones{ONES<T>, ONES<T>, ONES<T>, ONES<T>};
-        const f32x4 none{0, 0, 0, 0};
-        f32x4       acc[4][4];
-#pragma unroll
-        for(uint32_t r = 0; r < 4; ++r)
-#pragma unroll
-            for(uint32_t c = 0; c < 4; ++c)
-                acc[r][c] = none;
 
-        issue(0u, 0u);
-        Stage now = load(0u);
-        for(uint32_t kb = 0; kb < p.blocksK; ++kb)
+        const Expand<T> expand;
+        f32x4           acc[RB][CB];
+#pragma unroll
+        for(uint32_t r = 0; r < RB; ++r)
+#pragma unroll
+            for(uint32_t c = 0; c < CB; ++c)
+                acc[r][c] = f32x4{0, 0, 0, 0};
+
+        using lds4 = const __attribute__((address_space(3))) u32x4*;
+        using lds1 = const __attribute__((address_space(3))) uint32_t*;
+        const uint32_t steps = (p.blocksK + WK - 1u) / WK;
+        each<BUFS - 1u>([&](auto at) __attribute__((always_inline)) {
+            if(decltype(at)::value < steps)
+                issue(decltype(at)::value, decltype(at)::value);
+        });
+        uint32_t buf = 0u;
+        for(uint32_t step = 0; step < steps; ++step)
         {
-            r355::waitVmcnt<0>();
+            const uint32_t after = steps - 1u - step; // steps whose loads may be outstanding
+            if(BUFS == 4u && after >= 2u)
+                r355::waitVmcnt<BUFS == 4u ? 2u * R::LOADS : 0u>();
+            else if(BUFS >= 3u && after >= 1u)
+                r355::waitVmcnt<BUFS >= 3u ? R::LOADS : 0u>();
+            else
+                r355::waitVmcnt<0>();
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            r355::ldsBarrier(); // everyone's part of block kb is there, and everyone is done with the other buffer
-            Stage then = now;
-            if(kb + 1u < p.blocksK)
-            {
-                issue(kb + 1u, (kb + 1u) & 1u);
-                then = load(kb + 1u);
-            }
-            const uint32_t from = ldsBase + (kb & 1u) * TILE + (waveT * 64u + col) * 256u + (quad ^ col) * 16u;
-#pragma unroll
-            for(uint32_t part = 0; part < PARTS; ++part)
-            {
-                f32x4 sum[4][4], sumX[4];
-#pragma unroll
-                for(uint32_t i = 0; i < STEPS; ++i)
-                {
-                    u32x4 x[4];
-#pragma unroll
-                    for(uint32_t c = 0; c < 4; ++c)
-                    {
-                        x[c]    = *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)((from ^ ((part * STEPS + i) * 64u)) + c * 4096u);
-                        sumX[c] = r355::mfma32<T>(ones, x[c], i == 0u ? none : sumX[c]);
-                    }
-#pragma unroll
-                    for(uint32_t r = 0; r < 4; ++r)
-                    {
-                        const u32x4 a = expand<T>(now.w[r][part * STEPS + i]);
-#pragma unroll
-                        for(uint32_t c = 0; c < 4; ++c)
-                            sum[r][c] = r355::mfma32<T>(a, x[c], i == 0u ? none : sum[r][c]);
-                    }
-                }
-#pragma unroll
-                for(uint32_t r = 0; r < 4; ++r)
-                {
-                    const RowsOf4 rows((block0 + r) * 16u + quad * 4u, p.n);
-                    const f32x4   scale = floats<T>(rows.moved(now.scale[r][part]));
-                    f32x4         zero{24.0f, 24.0f, 24.0f, 24.0f};
-                    if constexpr(ZEROS)
-                        zero = offsets(rows.moved(now.zero[r][part]));
-#pragma unroll
-                    for(uint32_t c = 0; c < 4; ++c)
+            r355::ldsBarrier(); // everyone's part of this step is there, and everyone is done with the step before
+            if(step + BUFS - 1u < steps)
+                issue(step + BUFS - 1u, buf == 0u ? BUFS - 1u : buf - 1u);
+            const uint32_t stage = ldsBase + buf * R::STAGE;
+            const uint32_t fromX = stage + waveK * TOKENS * 256u + (waveT * CB * 16u + col) * 256u + (quad ^ col) * 16u;
+            const uint32_t fromW = stage + R::X + ((waveK * WN + waveN) * RB * 64u + lane) * 16u;
+            const uint32_t fromS = stage + R::X + R::W + wave * R::SCALES * 256u + quad * 16u;
+            each<PARTS>([&](auto partAt) __attribute__((always_inline)) {
+                constexpr uint32_t part = decltype(partAt)::value;
+                accumulate<T, RB, CB, STEPS, ZEROS, !ZEROS && (STEPS * CB <= 8u)>(
+                    acc, expand,
+                    [&](uint32_t c, uint32_t i) __attribute__((always_inline)) { return *(lds4)(uintptr_t)((fromX ^ ((part * STEPS + i) * 64u)) + c * 4096u); },
+                    [&](uint32_t r, uint32_t i) __attribute__((always_inline)) { return *(lds1)(uintptr_t)(fromW + r * 1024u + (part * STEPS + i) * 4u); },
+                    [&](uint32_t r) __attribute__((always_inline)) {
+                        const u32x4 s = *(lds4)(uintptr_t)(fromS + (r * PARTS + part) * 64u);
+                        Values      v;
 #pragma unroll
                         for(uint32_t j = 0; j < 4; ++j)
-                            acc[r][c][j] = fmaf(scale[j], fmaf(-zero[j], sumX[c][j], sum[r][c][j]), acc[r][c][j]);
-                }
-            }
-            now = then;
+                            v.scale[j] = scaleOf<T>(s[j]), v.zero[j] = 24.0f;
+                        if constexpr(ZEROS)
+                        {
+                            const u32x4 z = *(lds4)(uintptr_t)(fromS + WAVES * R::SCALES * 256u + (r * PARTS + part) * 64u);
+#pragma unroll
+                            for(uint32_t j = 0; j < 4; ++j)
+                                v.zero[j] = __uint_as_float(0x41800000u | (z[j] << 19)); // 16 + z for z < 16
+                        }
+                        return v;
+                    });
+            });
+            buf = buf + 1u == BUFS ? 0u : buf + 1u;
         }
+        if constexpr(WK == 1u)
+        {
 #pragma unroll
-        for(uint32_t r = 0; r < 4; ++r)
+            for(uint32_t r = 0; r < RB; ++r)
 #pragma unroll
-            for(uint32_t c = 0; c < 4; ++c)
-                store<T>(p, token0 + waveT * 64u + c * 16u + col, (block0 + r) * 16u + quad * 4u, acc[r][c]);
+                for(uint32_t c = 0; c < CB; ++c)
+                    store<T>(p, token0 + (waveT * CB + c) * 16u + col, (block0 + r) * 16u + quad * 4u, acc[r][c]);
+        }
+        else
+        {
+            // the sets of waves meet in LDS, in order: set i adds up and stores the blocks i, i + WK, ... of its waves' place
+            __syncthreads();
+            float* const sums = reinterpret_cast<float*>(lds); // [WAVES][RB * CB][64][4]
+#pragma unroll
+            for(uint32_t r = 0; r < RB; ++r)
+#pragma unroll
+                for(uint32_t c = 0; c < CB; ++c)
+                    *reinterpret_cast<f32x4*>(sums + ((wave * RB * CB + r * CB + c) * 64u + lane) * 4u) = acc[r][c];
+            __syncthreads();
+            for(uint32_t u = waveK; u < RB * CB; u += WK)
+            {
+                f32x4 sum{0, 0, 0, 0};
+#pragma unroll
+                for(uint32_t v = 0; v < WK; ++v)
+                    sum += *reinterpret_cast<const f32x4*>(sums + (((wave % (WN * WT) + v * WN * WT) * RB * CB + u) * 64u + lane) * 4u);
+                store<T>(p, token0 + (waveT * CB + u % CB) * 16u + col, (block0 + u / CB) * 16u + quad * 4u, sum);
+            }
+        }
     }
 
     // one dword of the packed storage per thread: block of 16 rows, block of 128 k, lane, 32-k step
@@ -456,45 +578,90 @@ namespace
         }
     }
 
-    constexpr uint32_t MOST_ROWS = 1u << 24, MOST_TOKENS = 1u << 19;
+    constexpr uint32_t MOST_ROWS = 1u << 24, MOST_TOKENS = 1u << 19, MOST_K = 1u << 22;
 
-    // workgroups: a multiple of eight, every XCD a stretch of the tiles of n
+    // workgroups: a multiple of eight, every XCD a stretch of the tiles
     dim3 gridOf(W4Params& p, uint32_t rows, uint32_t tokens)
     {
         p.tilesN = (p.n + rows - 1u) / rows, p.tilesT = (p.tokens + tokens - 1u) / tokens;
-        p.perXcd = (p.tilesN + 7u) / 8u;
-        return dim3(p.perXcd * 8u * p.tilesT);
+        p.perXcd = (p.tilesN * p.tilesT + 7u) / 8u;
+        return dim3(p.perXcd * 8u);
     }
 
-    template <typename T, uint32_t RB, uint32_t CB, uint32_t STEPS, bool FAST>
-    void launchFew(W4Params& p, uint32_t waves, hipStream_t s)
+    template <typename T, uint32_t RB, uint32_t CB, uint32_t DEPTH, uint32_t STEPS, bool FAST>
+    void launchFew(W4Params& p, hipStream_t s)
     {
-        const dim3 grid = gridOf(p, 16u * RB, 16u * CB);
+        const uint32_t waves = p.blocksK >= 8u ? 8u : p.blocksK >= 4u ? 4u : 1u;
+        const dim3     grid  = gridOf(p, 16u * RB, 16u * CB);
         if(p.zeros)
-            hipLaunchKernelGGL((w4Kernel<T, RB, CB, STEPS, true, FAST>), grid, dim3(waves * 64u), waves * RB * CB * 1024u, s, p);
+            hipLaunchKernelGGL((w4Kernel<T, RB, CB, DEPTH, STEPS, true, FAST>), grid, dim3(waves * 64u), waves * RB * CB * 1024u, s, p);
         else
-            hipLaunchKernelGGL((w4Kernel<T, RB, CB, STEPS, false, FAST>), grid, dim3(waves * 64u), waves * RB * CB * 1024u, s, p);
+            hipLaunchKernelGGL((w4Kernel<T, RB, CB, DEPTH, STEPS, false, FAST>), grid, dim3(waves * 64u), waves * RB * CB * 1024u, s, p);
+    }
+
+    template <typename T, uint32_t RB, uint32_t CB, uint32_t WN, uint32_t WT, uint32_t WK, uint32_t STEPS>
+    void launchRing(W4Params& p, hipStream_t s)
+    {
+        const dim3 grid = gridOf(p, 16u * RB * WN, 16u * CB * WT);
+        if(p.zeros)
+            hipLaunchKernelGGL((w4RingKernel<T, RB, CB, WN, WT, WK, STEPS, true>), grid, dim3(64u * WN * WT * WK), 0, s, p);
+        else
+            hipLaunchKernelGGL((w4RingKernel<T, RB, CB, WN, WT, WK, STEPS, false>), grid, dim3(64u * WN * WT * WK), 0, s, p);
+    }
+
+    // The kernels that are launched, with what a workgroup of each takes for a block of 128 k while it has its CU to itself (hundredths of
+    // a microsecond; groups of 128, of 64 and of 32; measured over 1024 .. 16384 rows and 2048 .. 16384 k).
+    struct Variant
+    {
+        uint32_t rows, tokens, time[3];
+    };
+    constexpr Variant VARIANTS[] = {
+        {16, 16, {14, 15, 18}}, {32, 16, {16, 18, 22}}, {48, 16, {18, 21, 28}}, {64, 16, {19, 24, 36}}, // few tokens, one to four blocks of 16 rows
+        {16, 32, {21, 23, 26}}, {32, 32, {23, 25, 31}}, {48, 32, {25, 29, 38}}, {64, 32, {27, 34, 90}}, // (the last with groups of 32: registers spill)
+        {64, 32, {29, 34, 44}}, {128, 32, {51, 60, 78}}, {64, 64, {53, 60, 73}}, {128, 64, {77, 84, 114}}, // the ring
+        {128, 128, {147, 160, 200}}, {256, 128, {242, 245, 300}}};
+
+    // The least time of all, counting a round of workgroups over the CUs as long as one.  (16384 x 8192, 24 tokens, groups of 128: one to four blocks
+    // of rows 51, 31, 34, 20 us; 10250 x 4168, groups of 32: 21, 22, 15, 35 us.)
+    uint32_t variantOf(const W4Params& p)
+    {
+        const uint32_t by = p.group == 32u ? 2u : p.group == 64u ? 1u : 0u, cus = r355::computeUnits();
+        uint32_t       best = 0u;
+        uint64_t       least = ~0ull;
+        for(uint32_t v = 0; v < sizeof(VARIANTS) / sizeof(VARIANTS[0]); ++v)
+        {
+            // up to four tokens x costs next to nothing, and two workgroups of up to three blocks share a CU well (16384 x 8192, one token: two blocks 13.6, four 14.8 us)
+            if(p.tokens <= 4u && v > 2u)
+                break;
+            const uint64_t groups = (uint64_t)((p.n + VARIANTS[v].rows - 1u) / VARIANTS[v].rows) * ((p.tokens + VARIANTS[v].tokens - 1u) / VARIANTS[v].tokens);
+            const uint64_t time   = ((groups + 7u) / 8u * 8u + cus - 1u) / cus * VARIANTS[v].time[by];
+            if(time < least)
+                least = time, best = v;
+        }
+        return best;
     }
 
     template <typename T, uint32_t STEPS>
     void launchSteps(W4Params& p, bool fast, hipStream_t s)
     {
-        const uint32_t waves = p.blocksK >= 8u ? 8u : p.blocksK >= 4u ? 4u : 1u;
         if(!fast)
-            launchFew<T, 1, 2, STEPS, false>(p, waves, s);
-        else if(p.tokens <= 16u)
-            launchFew<T, 1, 1, STEPS, true>(p, waves, s);
-        else if(p.tokens <= 32u)
-            launchFew<T, 1, 2, STEPS, true>(p, waves, s);
-        else if(p.tokens <= 64u)
-            launchFew<T, 1, 4, STEPS, true>(p, waves, s);
-        else
+            return launchFew<T, 1, 2, 1, STEPS, false>(p, s);
+        switch(variantOf(p))
         {
-            const dim3 grid = gridOf(p, 128u, 128u);
-            if(p.zeros)
-                hipLaunchKernelGGL((w4TileKernel<T, STEPS, true>), grid, dim3(256), 0, s, p);
-            else
-                hipLaunchKernelGGL((w4TileKernel<T, STEPS, false>), grid, dim3(256), 0, s, p);
+        case 0: return launchFew<T, 1, 1, 2, STEPS, true>(p, s);
+        case 1: return launchFew<T, 2, 1, 1, STEPS, true>(p, s);
+        case 2: return launchFew<T, 3, 1, 1, STEPS, true>(p, s);
+        case 3: return launchFew<T, 4, 1, 1, STEPS, true>(p, s);
+        case 4: return launchFew<T, 1, 2, 1, STEPS, true>(p, s);
+        case 5: return launchFew<T, 2, 2, 1, STEPS, true>(p, s);
+        case 6: return launchFew<T, 3, 2, 1, STEPS, true>(p, s);
+        case 7: return launchFew<T, 4, 2, 1, STEPS == 1u ? 2u : STEPS, true>(p, s); // (never chosen for groups of 32)
+        case 8: return launchRing<T, 2, 2, 2, 1, 4, STEPS>(p, s);
+        case 9: return launchRing<T, 2, 2, 4, 1, 2, STEPS>(p, s);
+        case 10: return launchRing<T, 1, 4, 4, 1, 2, STEPS>(p, s);
+        case 11: return launchRing<T, 2, 4, 4, 1, 2, STEPS>(p, s);
+        case 12: return launchRing<T, 2, 4, 4, 2, 1, STEPS>(p, s);
+        default: return launchRing<T, 4, 4, 4, 2, 1, STEPS>(p, s);
         }
     }
 
@@ -521,8 +688,8 @@ extern "C" int r355_w4_pack(const uint8_t* q, uint32_t n, uint32_t k, uint32_t l
         return r355::fail(R355_ERR_BAD_ARG, "w4_pack: null pointer");
     if(n == 0 || k == 0)
         return r355::fail(R355_ERR_BAD_ARG, "w4_pack: n and k must be non-zero");
-    if(n > MOST_ROWS || k > 0xFFFFFF00u)
-        return r355::fail(R355_ERR_BAD_SIZE, "w4_pack: at most %u rows and 0xFFFFFF00 columns, got %u and %u", MOST_ROWS, n, k);
+    if(n > MOST_ROWS || k > MOST_K)
+        return r355::fail(R355_ERR_BAD_SIZE, "w4_pack: at most %u rows and %u columns, got %u and %u", MOST_ROWS, MOST_K, n, k);
     if(ldq < (k + 1u) / 2u)
         return r355::fail(R355_ERR_BAD_ARG, "w4_pack: ldq=%u is less than the %u bytes of a row", ldq, (k + 1u) / 2u);
     if(!r355::aligned(packed, 16))
@@ -545,8 +712,8 @@ extern "C" int r355_w4_matmul(const r355_w4_args* args, void* stream)
         return r355::fail(R355_ERR_UNSUPPORTED, "w4_matmul: the result has the type of x or is f32");
     if(a.n == 0 || a.k == 0)
         return r355::fail(R355_ERR_BAD_ARG, "w4_matmul: n and k must be non-zero");
-    if(a.n > MOST_ROWS || a.tokens > MOST_TOKENS || a.k > 0xFFFFFF00u)
-        return r355::fail(R355_ERR_BAD_SIZE, "w4_matmul: at most %u rows, %u tokens and 0xFFFFFF00 columns, got %u, %u and %u", MOST_ROWS, MOST_TOKENS, a.n, a.tokens, a.k);
+    if(a.n > MOST_ROWS || a.tokens > MOST_TOKENS || a.k > MOST_K)
+        return r355::fail(R355_ERR_BAD_SIZE, "w4_matmul: at most %u rows, %u tokens and %u columns, got %u, %u and %u", MOST_ROWS, MOST_TOKENS, MOST_K, a.n, a.tokens, a.k);
     if(a.group != 32u && a.group != 64u && (a.group == 0u || a.group % 128u))
         return r355::fail(R355_ERR_BAD_SIZE, "w4_matmul: group=%u must be 32, 64 or a multiple of 128", a.group);
     if(((uint64_t)a.n + 15u) / 16u * (((uint64_t)a.tokens + 15u) / 16u) > r355::MAX_GROUPS / 4u)
@@ -567,6 +734,8 @@ extern "C" int r355_w4_matmul(const r355_w4_args* args, void* stream)
     p.c = static_cast<const char*>(a.c), p.y = static_cast<char*>(a.y);
     p.tokens = a.tokens, p.n = a.n, p.k = a.k, p.group = a.group, p.groups = (a.k + a.group - 1u) / a.group, p.ldx = a.ldx, p.ldc = a.ldc, p.ldy = a.ldy;
     p.blocksN = (a.n + 15u) / 16u, p.blocksK = (a.k + 127u) / 128u;
+    p.perGroup = a.group / 128u < p.blocksK ? a.group / 128u : p.blocksK; // (a group longer than k)
+    p.groupMagic = p.perGroup > 1u ? static_cast<uint32_t>(((1ull << 32) + p.perGroup - 1u) / p.perGroup) : 0u;
     p.outF32 = a.out_type == R355_F32;
     p.wideN  = a.ldy % 4u == 0u && r355::aligned(a.y, 4u * outBytes) && (a.beta == 0.0 || (a.ldc % 4u == 0u && r355::aligned(a.c, 4u * outBytes)));
     p.alpha = static_cast<float>(a.alpha), p.beta = static_cast<float>(a.beta);

@@ -82,6 +82,9 @@ def test_w4_shapes(n, k):
 @pytest.mark.gpu
 @pytest.mark.parametrize("k", [1, 7, 31, 129, 1001])
 def test_w4_k_off_the_vectors(k):
+    """(k = 1001 with groups of 384 and of more than k as well)"""
+    _case("f16", "f16", 3, 36, 8 * k, 384, zeros=True, seed=k)
+    _case("bf16", "f32", 70, 36, 8 * k, 1 << 20, seed=k)
     _case("bf16", "bf16", 5, 40, k, 32, seed=k)
     _case("f16", "f32", 20, 41, k, 128, zeros=True, seed=k)
 
@@ -147,6 +150,8 @@ def test_w4_refusals():
     _refused(-3, group=16)
     _refused(-3, n=(1 << 24) + 1)
     _refused(-3, tokens=(1 << 19) + 1)
+    _refused(-3, k=(1 << 22) + 128)
+    _refused(-3, n=1 << 24, tokens=1 << 10)
     _refused(-4, w=0x2008)
     _refused(-4, x=0x1001)
     _refused(-4, out_type=R.F32, y=0x4002)
