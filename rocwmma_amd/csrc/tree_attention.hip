@@ -30,8 +30,8 @@ namespace
     using r355::u32x4;
     using r355::vec;
 
-    constexpr uint32_t WAVES = 4;
     constexpr uint32_t LEAST_CHUNK = 256; // positions of a workgroup at least
+    constexpr uint32_t WHOLE = 0xFFFFFF80u; // a chunk that no sequence fills
     constexpr uint32_t ABSENT = 0xFFFFFFFFu; // no such block of the cache
     constexpr uint32_t OUTSIDE = 0x7FFFFFF0u; // a lane's offset past the end of any buffer
 
@@ -46,21 +46,57 @@ namespace
         const int32_t*  qStart;
         const int32_t*  kvLen;
         const uint64_t* mask;
-        float*          partial; // [splits][rows][dim], then [splits][rows][2]: maximum (in powers of two) and sum
+        float*          partial; // [shares][maxTokens * heads][dim], then [shares][maxTokens * heads][2]: maximum (in powers of two) and sum
         int64_t         qToken, qHead, kSlot, kHead, vSlot, vHead, oToken, oHead; // strides in elements
         uint32_t        batch, heads, kvHeads, group, dim, totalTokens, maxTokens, maxKv;
         uint32_t        pageSize, pages, tableStride, maskWords;
-        uint32_t        splits, columns; // columns: (sequence, key head, split) triples
+        uint32_t        shares, columns; // shares of all sequences' positions (as many as sequences: none is split); (share, key head) pairs, a multiple of eight
         float           scale2; // |scale| * log2(e), at least the smallest normal number (times minus infinity it is minus infinity)
         uint32_t        signs; // what turns the signs of two elements of q: the scale's
     };
 
-    // the positions of one sequence that a workgroup takes
-    __device__ __forceinline__ uint32_t chunkOf(uint32_t length, uint32_t splits)
+    // The positions of all sequences are split into at most `shares` shares of the same length (LEAST_CHUNK at least, a multiple of it), each of one
+    // sequence: a long sequence gets as many more of them as it is longer.  With L positions in all and n sequences a share of
+    // L / (shares - n) leaves room for the last, shorter share of every sequence.
+    struct Share
     {
-        const uint32_t even = (length + splits - 1u) / splits;
-        const uint32_t most = even > LEAST_CHUNK ? even : LEAST_CHUNK;
-        return (most + 127u) / 128u * 128u;
+        uint32_t sequence, split, chunk; // whose share, which of its, positions of a share
+    };
+    __device__ __forceinline__ uint32_t lengthOf(const TreeParams& p, int32_t length)
+    {
+        const uint32_t n = length < 0 ? 0u : static_cast<uint32_t>(length);
+        return n < p.maxKv ? n : p.maxKv;
+    }
+    // (by a whole wave)
+    __device__ __forceinline__ uint32_t chunkFrom(const TreeParams& p, uint32_t blocks)
+    {
+#pragma unroll
+        for(uint32_t x = 1u; x < 64u; x *= 2u)
+            blocks += __shfl_xor(blocks, x);
+        const uint32_t each = (blocks + p.shares - p.batch - 1u) / (p.shares - p.batch);
+        return __builtin_amdgcn_readfirstlane((each > 1u ? each : 1u) * LEAST_CHUNK);
+    }
+    // the same of one sequence
+    __device__ __forceinline__ uint32_t chunkAlone(const TreeParams& p, uint32_t length)
+    {
+        const uint32_t each = ((length + LEAST_CHUNK - 1u) / LEAST_CHUNK + p.shares - 1u) / p.shares;
+        return (each > 1u ? each : 1u) * LEAST_CHUNK;
+    }
+    __device__ __forceinline__ uint32_t chunkOf(const TreeParams& p, uint32_t lane)
+    {
+        if(p.shares <= p.batch)
+            return WHOLE;
+        if(p.batch == 1u)
+            return chunkAlone(p, __builtin_amdgcn_readfirstlane(lengthOf(p, p.kvLen[0])));
+        uint32_t blocks = 0u; // of LEAST_CHUNK positions
+        for(uint32_t first = 0; first < p.batch; first += 64u)
+            if(first + lane < p.batch)
+                blocks += (lengthOf(p, p.kvLen[first + lane]) + LEAST_CHUNK - 1u) / LEAST_CHUNK;
+        return chunkFrom(p, blocks);
+    }
+    __device__ __forceinline__ uint32_t splitsOf(uint32_t length, uint32_t chunk)
+    {
+        return length > chunk ? (length + chunk - 1u) / chunk : 1u; // (a sequence without positions has a share, which writes its zeros)
     }
 
     struct Sequence
@@ -71,15 +107,72 @@ namespace
     // what the arrays say of a sequence, held to what the host was told
     __device__ __forceinline__ Sequence sequenceOf(const TreeParams& p, int32_t from, int32_t to, int32_t len)
     {
-        Sequence      s;
+        Sequence s;
         s.first  = from < 0 ? 0u : static_cast<uint32_t>(from);
         s.first  = s.first < p.totalTokens ? s.first : p.totalTokens;
         s.tokens = to > static_cast<int32_t>(s.first) ? static_cast<uint32_t>(to) - s.first : 0u;
         s.tokens = s.tokens < p.maxTokens ? s.tokens : p.maxTokens;
         s.tokens = s.tokens < p.totalTokens - s.first ? s.tokens : p.totalTokens - s.first;
-        s.length = len < 0 ? 0u : static_cast<uint32_t>(len);
-        s.length = s.length < p.maxKv ? s.length : p.maxKv;
+        s.length = lengthOf(p, len);
         return s;
+    }
+
+    // The sequence and split of share `share`, and the sequence itself (share.sequence: batch where there is no such share).  The arrays are read by
+    // the lanes, all three before anything of them is used.
+    __device__ __forceinline__ Share shareOf(const TreeParams& p, uint32_t share, uint32_t lane, Sequence& seq)
+    {
+        const bool split = p.shares > p.batch;
+        if(p.batch == 1u)
+        {
+            seq = sequenceOf(p, __builtin_amdgcn_readfirstlane(p.qStart[0]), __builtin_amdgcn_readfirstlane(p.qStart[1]), __builtin_amdgcn_readfirstlane(p.kvLen[0]));
+            const uint32_t chunk = split ? chunkAlone(p, seq.length) : WHOLE;
+            return Share{share < splitsOf(seq.length, chunk) ? 0u : 1u, share, chunk};
+        }
+        Share      s{p.batch, 0u, WHOLE};
+        uint32_t   before = 0u;
+        for(uint32_t first = split ? 0u : share; first < p.batch; first += 64u)
+        {
+            const uint32_t i = first + lane < p.batch ? first + lane : p.batch - 1u;
+            const int32_t  from = p.qStart[i], to = p.qStart[i + 1u], len = p.kvLen[i];
+            uint32_t       at = 0u;
+            if(split)
+            {
+                const uint32_t length = lengthOf(p, len);
+                if(first == 0u)
+                    s.chunk = p.batch <= 64u ? chunkFrom(p, lane < p.batch ? (length + LEAST_CHUNK - 1u) / LEAST_CHUNK : 0u) : chunkOf(p, lane);
+                const uint32_t own  = first + lane < p.batch ? splitsOf(length, s.chunk) : 0u;
+                uint32_t       upTo = own;
+#pragma unroll
+                for(uint32_t x = 1u; x < 64u; x *= 2u)
+                {
+                    const uint32_t left = __shfl_up(upTo, x);
+                    upTo += lane >= x ? left : 0u;
+                }
+                const uint64_t holds = __ballot(own != 0u && share < before + upTo);
+                if(holds == 0u)
+                {
+                    before += __builtin_amdgcn_readlane(upTo, 63);
+                    continue;
+                }
+                at      = static_cast<uint32_t>(__builtin_ctzll(holds));
+                s.split = share - before - (__builtin_amdgcn_readlane(upTo, at) - __builtin_amdgcn_readlane(own, at));
+            }
+            s.sequence = first + at;
+            seq        = sequenceOf(p, __builtin_amdgcn_readlane(from, at), __builtin_amdgcn_readlane(to, at), __builtin_amdgcn_readlane(len, at));
+            break;
+        }
+        return s;
+    }
+    // the first share of sequence b
+    __device__ __forceinline__ uint32_t firstShareOf(const TreeParams& p, uint32_t b, uint32_t chunk, uint32_t lane)
+    {
+        uint32_t before = 0u;
+        for(uint32_t i = lane; i < b; i += 64u)
+            before += splitsOf(lengthOf(p, p.kvLen[i]), chunk);
+#pragma unroll
+        for(uint32_t x = 1u; x < 64u; x *= 2u)
+            before += __shfl_xor(before, x);
+        return __builtin_amdgcn_readfirstlane(before);
     }
 
     // where block `inChunk` (of 16 positions) of the chunk that begins at block `first` of sequence b lies, in blocks of the cache
@@ -130,13 +223,15 @@ namespace
         constexpr uint32_t EXPONENT = std::is_same_v<T, __bf16> ? 0x7F807F80u : 0x7C007C00u, ULP = std::is_same_v<T, __bf16> ? 0x00800080u : 0x04000400u;
         return (((v & EXPONENT) + ULP) >> 15) & 0x00010001u;
     }
-    // 1.0 in each half that holds a NaN or the infinity of the given sign, otherwise zero
-    template <typename T>
-    __device__ __forceinline__ uint32_t unfitOnes(uint32_t v, bool negative)
+    // calls f with the integral constants 0 .. N - 1
+    template <uint32_t N, typename F>
+    __device__ __forceinline__ void each(F&& f)
     {
-        constexpr uint32_t INF = std::is_same_v<T, __bf16> ? 0x7F80u : 0x7C00u, ONE = std::is_same_v<T, __bf16> ? 0x3F80u : 0x3C00u;
-        const uint32_t     lo = v & 0xFFFFu, hi = v >> 16, want = negative ? INF | 0x8000u : INF;
-        return (lo == want || (lo & 0x7FFFu) > INF ? ONE : 0u) | (hi == want || (hi & 0x7FFFu) > INF ? ONE << 16 : 0u);
+        if constexpr(N > 0u)
+        {
+            each<N - 1u>(f);
+            f(std::integral_constant<uint32_t, N - 1u>{});
+        }
     }
 
     __device__ __forceinline__ float maxOverQuads(float x)
@@ -151,16 +246,16 @@ namespace
     }
 
     template <typename T, uint32_t D, uint32_t WQ, uint32_t QB>
-    __global__ void __launch_bounds__(WAVES * 64, WQ == 1u ? 1 : 2) treeKernel(TreeParams p)
+    __global__ void __launch_bounds__(WQ == 8u ? 512 : 256, WQ == 4u ? 2 : 1) treeKernel(TreeParams p)
     {
-        constexpr uint32_t WK    = WAVES / WQ;
-        constexpr uint32_t NP    = D == 256u ? 16u : 32u; // positions of a tile
+        constexpr uint32_t WAVES = WQ == 8u ? 8u : 4u, WK = WAVES / WQ;
+        constexpr uint32_t NP    = D == 256u ? 16u : D == 128u || WQ > 1u ? 32u : 64u; // positions of a tile
         constexpr uint32_t PB    = NP / 16u;
         constexpr uint32_t ROWB  = D * 2u, SLOTS = ROWB / 16u; // bytes and 16-byte pieces of a row
         constexpr uint32_t RPL   = 64u / SLOTS; // rows of a direct load
         constexpr uint32_t TILE  = NP * ROWB;
-        constexpr uint32_t BUFS  = WQ == 1u ? 2u : 3u;
-        constexpr uint32_t LOADS = NP / RPL / WQ; // direct loads of a wave per tile, of K or of V
+        constexpr uint32_t BUFS  = WQ == 1u ? 2u : 4u;
+        constexpr uint32_t LOADS = 2u * NP / RPL / WQ; // direct loads of a wave per tile: those of K, then those of V, shared out
         constexpr uint32_t LDS   = WK * BUFS * 2u * TILE;
         constexpr uint32_t MERGE = WK > 1u ? WK * QB * 16u * (D + 2u) * 4u : 0u;
         // weights are held relative to 2^-SHIFT of the largest: in f16 those under 2^-14 of it, of which a long row has many, stay normal numbers
@@ -170,20 +265,20 @@ namespace
         static_assert(LDS <= 160u * 1024u, "LDS");
         __shared__ __attribute__((aligned(1024))) char lds[LDS > MERGE ? LDS : MERGE];
 
-        const uint32_t tile0 = blockIdx.x / p.columns, column = blockIdx.x % p.columns;
-        const uint32_t split = column % p.splits, bh = column / p.splits;
-        const uint32_t head = bh % p.kvHeads, b = bh / p.kvHeads;
+        const uint32_t tile0 = blockIdx.x / p.columns, column = blockIdx.x % p.columns, head = column % p.kvHeads, index = column / p.kvHeads;
+        if(index >= p.shares)
+            return;
+        Sequence       seq;
+        const Share    share = shareOf(p, index, threadIdx.x & 63u, seq);
+        const uint32_t b     = share.sequence;
         if(b >= p.batch)
             return;
-        const Sequence seq  = sequenceOf(p, __builtin_amdgcn_readfirstlane(p.qStart[b]), __builtin_amdgcn_readfirstlane(p.qStart[b + 1u]), __builtin_amdgcn_readfirstlane(p.kvLen[b]));
         const uint32_t rows = seq.tokens * p.group, row0 = tile0 * WQ * QB * 16u;
         if(row0 >= rows)
             return;
-        const uint32_t chunk = chunkOf(seq.length, p.splits), begin = split * chunk;
-        if(begin >= seq.length && split != 0u)
-            return;
-        const uint32_t end = seq.length - begin < chunk ? seq.length : begin + chunk;
-        const bool     whole = seq.length <= chunk; // no other workgroup has positions of this sequence
+        const bool     whole = seq.length <= share.chunk; // no other workgroup has positions of this sequence
+        const uint32_t begin = whole ? 0u : share.split * share.chunk;
+        const uint32_t end   = seq.length - begin < share.chunk ? seq.length : begin + share.chunk;
 
         const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const uint32_t col = lane & 15u, quad = lane >> 4;
@@ -216,7 +311,7 @@ namespace
         const uint32_t ldsBase = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
         const uint32_t myTiles = wk * BUFS * 2u * TILE;
         const uint32_t pageBlocks = p.pageSize / 16u, lastBlocks = end > begin ? (end - begin + 15u) / 16u : 0u;
-        constexpr uint32_t GROUPS = 4;
+        constexpr uint32_t GROUPS = WQ == 1u ? 4u : 2u;
         uint32_t           group = 0u, here, ahead[GROUPS];
 #pragma unroll
         for(uint32_t g = 0; g < GROUPS; ++g)
@@ -227,14 +322,13 @@ namespace
         here = ahead[0];
         // a lane's offsets: RPL rows a load, 16-byte pieces exchanged within the row; past the width of a head: outside the buffer, which loads zeros
         const uint32_t loadRow = lane / SLOTS, loadSlot = lane % SLOTS;
-        uint32_t       offK[LOADS], offV[LOADS];
+        uint32_t       off[LOADS];
 #pragma unroll
         for(uint32_t j = 0; j < LOADS; ++j)
         {
-            const uint32_t inTile = (wq * LOADS + j) * RPL + loadRow;
-            const uint32_t pieceK = loadSlot ^ swizzleK<D>(inTile), pieceV = loadSlot ^ swizzleV<D>(inTile);
-            offK[j] = pieceK * 8u < p.dim ? inTile % 16u * (uint32_t)(p.kSlot * 2) + pieceK * 16u : OUTSIDE;
-            offV[j] = pieceV * 8u < p.dim ? inTile % 16u * (uint32_t)(p.vSlot * 2) + pieceV * 16u : OUTSIDE;
+            const uint32_t item = wq * LOADS + j, inTile = item % (NP / RPL) * RPL + loadRow;
+            const uint32_t piece = loadSlot ^ (item < NP / RPL ? swizzleK<D>(inTile) : swizzleV<D>(inTile));
+            off[j] = piece * 8u < p.dim ? inTile % 16u * (uint32_t)((item < NP / RPL ? p.kSlot : p.vSlot) * 2) + piece * 16u : OUTSIDE;
         }
         const uint64_t baseK = reinterpret_cast<uint64_t>(p.k) + 2u * (uint64_t)(head * p.kHead), baseV = reinterpret_cast<uint64_t>(p.v) + 2u * (uint64_t)(head * p.vHead);
         auto issue = [&](uint32_t tile, uint32_t buf) __attribute__((always_inline)) {
@@ -252,21 +346,21 @@ namespace
                     here = ahead[0];
                 }
                 else
-                    here = of % GROUPS == 1u ? ahead[1] : of % GROUPS == 2u ? ahead[2] : ahead[3];
+                    here = of % GROUPS == 1u ? ahead[1] : of % GROUPS == 2u ? ahead[GROUPS - 2u] : ahead[GROUPS - 1u];
             }
 #pragma unroll
             for(uint32_t j = 0; j < LOADS; ++j)
             {
-                const uint32_t piece = wq * LOADS + j; // which RPL rows of the tile
+                const uint32_t item = wq * LOADS + j, piece = item % (NP / RPL); // K or V, and which RPL rows of the tile
+                const bool     isK  = item < NP / RPL;
                 const uint32_t block = tile * PB + piece * RPL / 16u; // of the chunk
-                const uint32_t at   = __builtin_amdgcn_readlane(here, block % 64u);
-                const uint32_t rows = at == ABSENT ? 0u : end - begin - block * 16u < 16u ? end - begin - block * 16u : 16u;
+                const uint32_t at    = __builtin_amdgcn_readlane(here, block % 64u);
+                const uint32_t rows  = at == ABSENT ? 0u : end - begin - block * 16u < 16u ? end - begin - block * 16u : 16u;
+                const uint32_t slot  = static_cast<uint32_t>(isK ? p.kSlot : p.vSlot);
                 // (a buffer that ends with the last row that there is: the others load zeros)
-                r355::dma_i32x4 bufK = r355::rawBuffer(baseK + (uint64_t)at * (uint32_t)(p.kSlot * 32)), bufV = r355::rawBuffer(baseV + (uint64_t)at * (uint32_t)(p.vSlot * 32));
-                bufK[2] = __builtin_amdgcn_readfirstlane(rows * (uint32_t)(p.kSlot * 2)), bufV[2] = __builtin_amdgcn_readfirstlane(rows * (uint32_t)(p.vSlot * 2));
-                const uint32_t to = __builtin_amdgcn_readfirstlane(ldsBase + myTiles + buf * 2u * TILE + piece * 1024u);
-                r355::loadToLds(bufK, offK[j], 0u, to);
-                r355::loadToLds(bufV, offV[j], 0u, to + TILE);
+                r355::dma_i32x4 rsrc = r355::rawBuffer((isK ? baseK : baseV) + (uint64_t)at * (slot * 32u));
+                rsrc[2]              = __builtin_amdgcn_readfirstlane(rows * slot * 2u);
+                r355::loadToLds(rsrc, off[j], 0u, __builtin_amdgcn_readfirstlane(ldsBase + myTiles + buf * 2u * TILE + (isK ? 0u : TILE) + piece * 1024u));
             }
         };
 
@@ -281,58 +375,65 @@ namespace
                 o[a][d] = f32x4{0, 0, 0, 0};
         }
 
-        // MASKED: some row does not see all of the tile
-        auto compute = [&](auto maskedTile, uint32_t pos0, uint32_t buf) __attribute__((always_inline)) {
-            constexpr bool MASKED = decltype(maskedTile)::value;
-            // LDS addresses of the lane's row: the pieces of a row differ in an exclusive or with a constant (rows start on multiples of their
-            // size), the blocks of 16 rows in a constant offset
-            const uint32_t tileK = ldsBase + myTiles + buf * 2u * TILE, tileV = tileK + TILE;
-            const uint32_t rowV = quad * 4u + (col >> 2);
-            const uint32_t fromK = tileK + col * ROWB + (quad ^ swizzleK<D>(col)) * 16u, fromV = tileV + rowV * ROWB + (((col >> 1) & 1u) ^ swizzleV<D>(rowV)) * 16u + (col & 1u) * 8u;
-            f32x4          s[QB][PB];
+        // S^T of a tile.  LDS addresses of the lane's row: the pieces of a row differ in an exclusive or with a constant (rows start on multiples of their
+        // size), the blocks of 16 rows in a constant offset.
+        uint32_t atK[D / 32u], atV[D / 16u]; // in the first buffer
+        {
+            const uint32_t rowV = quad * 4u + (col >> 2), tile = ldsBase + myTiles;
 #pragma unroll
-            for(uint32_t n = 0; n < PB; ++n)
+            for(uint32_t i = 0; i < D / 32u; ++i)
+                atK[i] = (tile + col * ROWB + (quad ^ swizzleK<D>(col)) * 16u) ^ (i * 64u);
 #pragma unroll
-                for(uint32_t a = 0; a < QB; ++a)
-                    s[a][n] = f32x4{0, 0, 0, 0};
+            for(uint32_t d = 0; d < D / 16u; ++d)
+                atV[d] = (tile + TILE + rowV * ROWB + (((col >> 1) & 1u) ^ swizzleV<D>(rowV)) * 16u + (col & 1u) * 8u) ^ (d * 32u);
+        }
+        auto scores = [&](auto buf, f32x4(&s)[QB][PB]) __attribute__((always_inline)) {
 #pragma unroll
             for(uint32_t i = 0; i < D / 32u; ++i)
 #pragma unroll
                 for(uint32_t n = 0; n < PB; ++n)
                 {
-                    const u32x4 kf = *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)((fromK ^ (i * 64u)) + n * 16u * ROWB);
+                    const u32x4 kf = *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)(atK[i] + (buf * 2u * TILE + n * 16u * ROWB));
 #pragma unroll
                     for(uint32_t a = 0; a < QB; ++a)
-                        s[a][n] = r355::mfma32<T>(kf, qf[a][i], s[a][n]);
+                        s[a][n] = r355::mfma32<T>(kf, qf[a][i], i != 0u ? s[a][n] : f32x4{0, 0, 0, 0});
                 }
-            if constexpr(MASKED)
+        };
+        // The weights of a tile and their product with V.  masked: some row does not see all of the tile.  between(): what can go on beside the exponentials.
+        // (With few rows one copy of the code for both: a call over few positions takes about as long as its instructions take to arrive, some 25 ns for 64 bytes.)
+        auto weigh = [&](auto ahead, auto masked, uint32_t pos0, auto buf, f32x4(&s)[QB][PB], auto&& between) __attribute__((always_inline)) {
+            if(masked)
             {
 #pragma unroll
                 for(uint32_t a = 0; a < QB; ++a)
                 {
-                    // bit i: the row sees position pos0 + i
-                    const uint32_t seen = rowValid[a] ? seenOf(p, seq.first + token[a], token[a], (int64_t)pos0 - prefix) : 0u;
-                    const uint32_t mine = (end - pos0 < 32u ? seen & ((1u << (end - pos0)) - 1u) : seen) >> (quad * 4u);
 #pragma unroll
-                    for(uint32_t n = 0; n < PB; ++n)
+                    for(uint32_t w = 0; w < PB; w += 2u)
+                    {
+                        // bit i: the row sees position from + i
+                        const uint32_t from = pos0 + w * 16u;
+                        const uint32_t seen = rowValid[a] && from < end ? seenOf(p, seq.first + token[a], token[a], (int64_t)from - prefix) : 0u;
+                        const uint32_t mine = (from < end && end - from < 32u ? seen & ((1u << (end - from)) - 1u) : seen) >> (quad * 4u);
 #pragma unroll
-                        for(uint32_t j = 0; j < 4; ++j)
-                            s[a][n][j] = (mine >> (n * 16u + j)) & 1u ? s[a][n][j] : -INFINITY;
+                        for(uint32_t n = w; n < w + 2u && n < PB; ++n)
+#pragma unroll
+                            for(uint32_t j = 0; j < 4; ++j)
+                                s[a][n][j] = (mine >> ((n - w) * 16u + j)) & 1u ? s[a][n][j] : -INFINITY;
+                    }
                 }
             }
-            uint32_t pf[QB][PB][2];
 #pragma unroll
             for(uint32_t a = 0; a < QB; ++a)
             {
+                // the lane's largest score; what the row's four lanes have is compared only where one has grown too large
                 float most = -INFINITY;
 #pragma unroll
                 for(uint32_t n = 0; n < PB; ++n)
                     most = fmaxf(fmaxf(fmaxf(s[a][n][0], s[a][n][1]), fmaxf(s[a][n][2], s[a][n][3])), most);
-                most = most == -INFINITY ? most : most * p.scale2;
-                most = maxOverQuads(most) - SHIFT;
+                most = most == -INFINITY ? most : most * p.scale2 - SHIFT;
                 if(__any(most > top[a] + SLACK))
                 {
-                    const float next = fmaxf(most, top[a]);
+                    const float next = fmaxf(maxOverQuads(most), top[a]);
                     const float keep = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[a] - next);
                     top[a]           = next;
                     sum[a] *= keep;
@@ -340,6 +441,31 @@ namespace
                     for(uint32_t d = 0; d < D / 16u; ++d)
                         o[a][d] *= keep;
                 }
+            }
+            // V^T: lane t of 16 names four consecutive d of position t / 4 and receives four positions of d = t.  (ahead: all of it is asked for
+            // before the exponentials; next to the product each read is waited for.)
+            using lp = __attribute__((address_space(3))) vec<short, 4>*;
+            auto v   = [&](uint32_t d, u32x2(&to)[PB]) __attribute__((always_inline)) {
+#pragma unroll
+                for(uint32_t n = 0; n < PB; ++n)
+                    to[n] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(uintptr_t)(atV[d] + (buf * 2u * TILE + n * 16u * ROWB))));
+            };
+            constexpr uint32_t EARLY = decltype(ahead)::value ? D / 16u : 0u;
+            u32x2              early[EARLY + 1u][PB];
+#pragma unroll
+            for(uint32_t d = 0; d < EARLY; ++d)
+                v(d, early[d]);
+            if constexpr(EARLY != 0u)
+                __builtin_amdgcn_sched_barrier(0);
+            uint32_t pf[QB][PB][2];
+            between();
+            // (shared tiles that are masked: nothing is moved up here, for want of registers)
+            constexpr bool TIGHT = WQ > 1u && !decltype(ahead)::value;
+            if constexpr(TIGHT)
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for(uint32_t a = 0; a < QB; ++a)
+            {
                 const float base = top[a] == -INFINITY ? 0.0f : top[a];
 #pragma unroll
                 for(uint32_t n = 0; n < PB; ++n)
@@ -353,58 +479,102 @@ namespace
                     pf[a][n][0] = r355::pack2<T>(s[a][n][0], s[a][n][1]), pf[a][n][1] = r355::pack2<T>(s[a][n][2], s[a][n][3]);
                 }
             }
-            // A position that a row does not see has weight 0, and 0 times an infinity or a NaN is a NaN: where the tile holds one, those are
-            // taken out of the product, and the rows that give them weight get them by two more (where (+inf or NaN) and where (-inf or NaN)).
-            bool unfit = false;
-            if constexpr(MASKED)
+            auto times = [&](const u32x2(&of)[PB], uint32_t a, f32x4 c) __attribute__((always_inline)) {
+                if constexpr(PB == 1u)
+                    return r355::mfma16<T>(of[0], u32x2{pf[a][0][0], pf[a][0][1]}, c);
+                else
+                {
+#pragma unroll
+                    for(uint32_t n = 0; n < PB; n += 2u)
+                        c = r355::mfma32<T>(u32x4{of[n][0], of[n][1], of[n + 1u][0], of[n + 1u][1]}, u32x4{pf[a][n][0], pf[a][n][1], pf[a][n + 1u][0], pf[a][n + 1u][1]}, c);
+                    return c;
+                }
+            };
+            // A position that a row does not see has weight 0, and 0 times an infinity or a NaN is a NaN.  Where the tile holds one, the rows that give it no
+            // weight take the product with zeros in the place of all of them.
+            if(masked)
             {
                 uint32_t found = 0u;
+#pragma unroll 1
                 for(uint32_t at = lane * 16u; at < TILE; at += 1024u)
                 {
-                    const u32x4 v = *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)(tileV + at);
-                    found |= unfitHalves<T>(v[0]) | unfitHalves<T>(v[1]) | unfitHalves<T>(v[2]) | unfitHalves<T>(v[3]);
+                    const u32x4 x = *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)(ldsBase + myTiles + buf * 2u * TILE + TILE + at);
+                    found |= unfitHalves<T>(x[0]) | unfitHalves<T>(x[1]) | unfitHalves<T>(x[2]) | unfitHalves<T>(x[3]);
                 }
-                unfit = __any(found != 0u);
+                if(__any(found != 0u))
+                {
+                    u32x2 bad[PB]; // of the lane's positions, over all d
+#pragma unroll
+                    for(uint32_t n = 0; n < PB; ++n)
+                        bad[n] = u32x2{0u, 0u};
+#pragma unroll
+                    for(uint32_t d = 0; d < D / 16u; ++d)
+                    {
+                        u32x2 x[PB];
+                        if constexpr(TIGHT)
+                            __builtin_amdgcn_sched_barrier(0);
+                        v(d, x);
+#pragma unroll
+                        for(uint32_t n = 0; n < PB; ++n)
+                            bad[n] |= u32x2{unfitHalves<T>(x[n][0]), unfitHalves<T>(x[n][1])};
+                    }
+                    bool hit[QB];
+#pragma unroll
+                    for(uint32_t a = 0; a < QB; ++a)
+                        hit[a] = false;
+#pragma unroll
+                    for(uint32_t n = 0; n < PB; ++n)
+#pragma unroll
+                        for(uint32_t w = 0; w < 2u; ++w)
+                        {
+                            uint32_t all = bad[n][w];
+#pragma unroll
+                            for(uint32_t x = 1u; x < 16u; x *= 2u)
+                                all |= __shfl_xor(all, x);
+#pragma unroll
+                            for(uint32_t a = 0; a < QB; ++a)
+                                hit[a] = hit[a] || (pf[a][n][w] & (all * 0x7FFFu)) != 0u; // (a weight in each half)
+                        }
+#pragma unroll
+                    for(uint32_t a = 0; a < QB; ++a)
+                        hit[a] = maxOverQuads(hit[a] ? 1.0f : 0.0f) != 0.0f;
+#pragma unroll
+                    for(uint32_t d = 0; d < D / 16u; ++d)
+                    {
+                        u32x2 as[PB], fit[PB];
+                        if constexpr(TIGHT)
+                            __builtin_amdgcn_sched_barrier(0);
+                        v(d, as);
+#pragma unroll
+                        for(uint32_t n = 0; n < PB; ++n)
+                            fit[n] = u32x2{as[n][0] & ~(unfitHalves<T>(as[n][0]) * 0xFFFFu), as[n][1] & ~(unfitHalves<T>(as[n][1]) * 0xFFFFu)};
+#pragma unroll
+                        for(uint32_t a = 0; a < QB; ++a)
+                        {
+                            const f32x4 seen = times(as, a, o[a][d]), unseen = times(fit, a, o[a][d]);
+#pragma unroll
+                            for(uint32_t e = 0; e < 4u; ++e)
+                                o[a][d][e] = hit[a] ? seen[e] : unseen[e];
+                        }
+                    }
+                    return;
+                }
             }
-            // V^T: lane t of 16 names four consecutive d of position t / 4 and receives four positions of d = t
-            using lp = __attribute__((address_space(3))) vec<short, 4>*;
 #pragma unroll
             for(uint32_t d = 0; d < D / 16u; ++d)
             {
                 u32x2 vf[PB];
+                if constexpr(EARLY != 0u)
 #pragma unroll
-                for(uint32_t n = 0; n < PB; ++n)
-                    vf[n] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(uintptr_t)((fromV ^ (d * 32u)) + n * 16u * ROWB)));
-                auto times = [&](const u32x2(&v)[PB], uint32_t a, f32x4 c) __attribute__((always_inline)) {
-                    if constexpr(PB == 2u)
-                        return r355::mfma32<T>(u32x4{v[0][0], v[0][1], v[1][0], v[1][1]}, u32x4{pf[a][0][0], pf[a][0][1], pf[a][1][0], pf[a][1][1]}, c);
-                    else
-                        return r355::mfma16<T>(v[0], u32x2{pf[a][0][0], pf[a][0][1]}, c);
-                };
-                if constexpr(MASKED)
-                    if(unfit)
-                    {
-                        u32x2 up[PB], down[PB];
-#pragma unroll
-                        for(uint32_t n = 0; n < PB; ++n)
-#pragma unroll
-                            for(uint32_t w = 0; w < 2; ++w)
-                            {
-                                up[n][w] = unfitOnes<T>(vf[n][w], false), down[n][w] = unfitOnes<T>(vf[n][w], true);
-                                vf[n][w] &= ~(unfitHalves<T>(vf[n][w]) * 0xFFFFu);
-                            }
-#pragma unroll
-                        for(uint32_t a = 0; a < QB; ++a)
-                        {
-                            const f32x4 above = times(up, a, f32x4{0, 0, 0, 0}), below = times(down, a, f32x4{0, 0, 0, 0});
-#pragma unroll
-                            for(uint32_t e = 0; e < 4; ++e)
-                            {
-                                o[a][d][e] += above[e] != 0.0f ? INFINITY : 0.0f;
-                                o[a][d][e] -= below[e] != 0.0f ? INFINITY : 0.0f;
-                            }
-                        }
-                    }
+                    for(uint32_t n = 0; n < PB; ++n)
+                        vf[n] = early[d < EARLY ? d : 0u][n];
+                else
+                {
+                    if constexpr(TIGHT)
+                        if(d % 4u == 0u)
+                            __builtin_amdgcn_sched_barrier(0);
+                    v(d, vf);
+                }
 #pragma unroll
                 for(uint32_t a = 0; a < QB; ++a)
                     o[a][d] = times(vf, a, o[a][d]);
@@ -417,45 +587,101 @@ namespace
         const uint32_t clear = open > (int64_t)begin ? static_cast<uint32_t>(open - begin) / NP : 0u;
         uint32_t       buf = 0u, t = WQ == 1u ? wk : 0u;
         // tile t (of tiles wk, wk + 4, ... where every wave has its own)
-        auto step = [&](auto maskedTile) __attribute__((always_inline)) {
+        f32x4 held[QB][PB];
+        // WQ > 1: the scores of tile t + 1 are made beside the exponentials of tile t (after the last tile: of what the buffer holds, and not used)
+        [[maybe_unused]] f32x4 other[QB][PB];
+        auto arrive = [&]() __attribute__((always_inline)) {
+            if(t + 2u < tiles)
+                r355::waitVmcnt<LOADS>();
+            else
+                r355::waitVmcnt<0>();
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            r355::ldsBarrier(); // everyone's part of tile t + 1 is there, and everyone is done with the buffer of tile t - 1
+        };
+        auto step = [&](auto ahead, auto masked) __attribute__((always_inline)) {
             if constexpr(WQ == 1u)
             {
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the reads of the buffer that is filled next have returned
                 if(t + WK < tiles)
                 {
                     issue(t + WK, buf ^ 1u);
-                    r355::waitVmcnt<2u * LOADS>();
+                    r355::waitVmcnt<LOADS>();
                 }
                 else
                     r355::waitVmcnt<0>();
                 asm volatile("" ::: "memory");
-                compute(maskedTile, begin + t * NP, buf);
+                scores(buf, held);
+                weigh(ahead, masked, begin + t * NP, buf, held, [] {});
                 buf ^= 1u;
                 t += WK;
             }
             else
             {
-                if(t + 1u < tiles)
-                    r355::waitVmcnt<2u * LOADS>();
-                else
-                    r355::waitVmcnt<0>();
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                r355::ldsBarrier(); // everyone's part of tile t is there, and everyone is done with the buffer of tile t - 1
-                if(t + 2u < tiles)
-                    issue(t + 2u, buf == 0u ? 2u : buf - 1u);
-                compute(maskedTile, begin + t * NP, buf);
-                buf = buf == 2u ? 0u : buf + 1u;
+                arrive();
+                if(t + 3u < tiles)
+                    issue(t + 3u, (buf + 3u) % BUFS);
+                if constexpr(decltype(ahead)::value)
+                {
+                    weigh(ahead, masked, begin + t * NP, buf, held, [&]() __attribute__((always_inline)) { scores((buf + 1u) % BUFS, other); });
+#pragma unroll
+                    for(uint32_t a = 0; a < QB; ++a)
+#pragma unroll
+                        for(uint32_t n = 0; n < PB; ++n)
+                            held[a][n] = other[a][n];
+                }
+                else // (the few masked tiles: one after the other, for want of registers)
+                {
+                    weigh(ahead, masked, begin + t * NP, buf, held, [] {});
+                    scores((buf + 1u) % BUFS, held);
+                }
+                buf = (buf + 1u) % BUFS;
                 t += 1u;
             }
         };
         if(t < tiles)
             issue(t, 0u);
-        if(WQ > 1u && tiles > 1u)
-            issue(1u, 1u);
-        while(t < clear)
-            step(std::false_type{});
-        while(t < tiles)
-            step(std::true_type{});
+        if constexpr(WQ > 1u)
+        {
+            if(tiles > 1u)
+                issue(1u, 1u);
+            if(tiles > 2u)
+                issue(2u, 2u);
+            if(tiles > 2u)
+                r355::waitVmcnt<2u * LOADS>();
+            else if(tiles > 1u)
+                r355::waitVmcnt<LOADS>();
+            else
+                r355::waitVmcnt<0>();
+            r355::ldsBarrier();
+            scores(0u, held);
+            // Long caches: four tiles at a time, so that LDS addresses and the places of the scores are the same each time around (2 x 64 tokens over 65600:
+            // 163 -> 154 us; where a workgroup has few tiles the code takes longer to arrive: 8 trees of up to 48 tokens over 4099 28 -> 33 us)
+            static_assert(BUFS == 4u, "one tile of a turn for each buffer");
+            while(WQ == 8u && t + 3u < clear)
+                each<WQ == 8u ? 4u : 0u>([&](auto at) __attribute__((always_inline)) {
+                    constexpr uint32_t i = decltype(at)::value;
+                    arrive();
+                    if(t + 3u < tiles)
+                        issue(t + 3u, (i + 3u) % 4u);
+                    const std::integral_constant<uint32_t, i> here;
+                    const std::integral_constant<uint32_t, (i + 1u) % 4u> next;
+                    if constexpr(i % 2u == 0u)
+                        weigh(std::true_type{}, std::false_type{}, begin + t * NP, here, held, [&]() __attribute__((always_inline)) { scores(next, other); });
+                    else
+                        weigh(std::true_type{}, std::false_type{}, begin + t * NP, here, other, [&]() __attribute__((always_inline)) { scores(next, held); });
+                    t += 1u;
+                });
+        }
+        if constexpr(WQ == 1u)
+            while(t < tiles)
+                step(std::false_type{}, t >= clear);
+        else
+        {
+            while(t < clear)
+                step(std::true_type{}, std::false_type{});
+            while(t < tiles)
+                step(std::false_type{}, std::true_type{});
+        }
 #pragma unroll
         for(uint32_t a = 0; a < QB; ++a)
             sum[a] = sumOverQuads(sum[a]);
@@ -514,7 +740,7 @@ namespace
         {
             if(!rowValid[a])
                 continue;
-            const uint64_t row = (uint64_t)(seq.first + token[a]) * p.heads + qHead[a], allRows = (uint64_t)p.totalTokens * p.heads;
+            const uint64_t row = (uint64_t)(seq.first + token[a]) * p.heads + qHead[a];
             if(whole)
             {
                 const float inverse = sum[a] == 0.0f ? 0.0f : 1.0f / sum[a];
@@ -529,104 +755,140 @@ namespace
             }
             else
             {
-                float* const to = p.partial + ((uint64_t)split * allRows + row) * p.dim;
+                const uint64_t all = (uint64_t)p.maxTokens * p.heads, at = index * all + token[a] * p.heads + qHead[a];
+                float* const   to  = p.partial + at * p.dim;
 #pragma unroll
                 for(uint32_t d = 0; d < D / 16u; ++d)
                     if(d % WK == wk && d * 16u + quad * 4u < p.dim)
                         *reinterpret_cast<f32x4*>(to + d * 16u + quad * 4u) = o[a][d];
                 if(wk == 0u && quad == 0u)
                 {
-                    float* const ends = p.partial + (uint64_t)p.splits * allRows * p.dim + ((uint64_t)split * allRows + row) * 2u;
+                    float* const ends = p.partial + p.shares * all * p.dim + at * 2u;
                     ends[0] = top[a], ends[1] = sum[a];
                 }
             }
         }
     }
 
-    // Adds up the splits of a row, in order.  L = D / 4 lanes a row, each four elements; the lanes take the splits' maxima and sums side by side.
-    template <typename T, uint32_t D>
+    // Adds up the shares of a row.  L = D / 4 lanes take four elements each, of four shares at once.  A workgroup has 256 / L sets of such lanes: one set a row, or
+    // (ALL: few rows) all of them for one row, each every (256 / L)-th share, and their sums meet in LDS, in order.  (64 rows of 16 shares: 8.0 us with a set a
+    // row, 4.0 with all; 4600 rows of 9 shares: 5 and 14 us.)  blockIdx.x: drafted tokens and heads, blockIdx.y: the sequence.
+    template <typename T, uint32_t D, bool ALL>
     __global__ void __launch_bounds__(256) treeMergeKernel(TreeParams p)
     {
-        constexpr uint32_t L = D / 4u;
-        const uint32_t     lane = threadIdx.x % L;
-        const uint64_t     item = (uint64_t)blockIdx.x * (256u / L) + threadIdx.x / L; // (sequence, drafted token, head)
-        const uint32_t     head = static_cast<uint32_t>(item % p.heads);
-        const uint64_t     bt = item / p.heads;
-        const uint32_t     b = static_cast<uint32_t>(bt / p.maxTokens), t = static_cast<uint32_t>(bt % p.maxTokens);
-        if(b >= p.batch)
+        constexpr uint32_t L = D / 4u, SETS = 256u / L, UNROLL = 4, STEP = ALL ? SETS : 1u;
+        __shared__ __attribute__((aligned(16))) f32x4 sums[SETS][L];
+        __shared__ float ends[SETS][2];
+        const uint32_t   lane = threadIdx.x % L, set = threadIdx.x / L, item = ALL ? blockIdx.x : blockIdx.x * SETS + set;
+        const uint32_t   b = blockIdx.y, t = item / p.heads, head = item % p.heads;
+        const Sequence   seq = sequenceOf(p, p.qStart[b], p.qStart[b + 1u], p.kvLen[b]);
+        const uint32_t   chunk = chunkOf(p, threadIdx.x & 63u);
+        if(seq.length <= chunk)
             return;
-        const Sequence seq = sequenceOf(p, p.qStart[b], p.qStart[b + 1u], p.kvLen[b]);
-        const uint32_t chunk = chunkOf(seq.length, p.splits);
-        if(t >= seq.tokens || seq.length <= chunk)
+        const uint32_t splits = splitsOf(seq.length, chunk), begin = ALL ? set : 0u;
+        const uint64_t all = (uint64_t)p.maxTokens * p.heads, at = firstShareOf(p, b, chunk, threadIdx.x & 63u) * all + item;
+        if(t >= seq.tokens)
             return;
-        const uint32_t splits = (seq.length + chunk - 1u) / chunk;
-        const uint64_t row = (uint64_t)(seq.first + t) * p.heads + head, allRows = (uint64_t)p.totalTokens * p.heads;
-        const float*   ends = p.partial + (uint64_t)p.splits * allRows * p.dim + row * 2u;
-        const float*   from = p.partial + row * p.dim + lane * 4u;
-        float          most = -INFINITY;
-        for(uint32_t s = lane; s < splits; s += L)
-            most = fmaxf(most, ends[s * allRows * 2u]);
-#pragma unroll
-        for(uint32_t x = 1u; x < L; x *= 2u)
-            most = fmaxf(most, __shfl_xor(most, x));
-        float total = 0.0f;
-        f32x4 all{0, 0, 0, 0};
-        for(uint32_t s0 = 0; s0 < splits; s0 += L)
+        const float*   endsOf = p.partial + p.shares * all * p.dim + at * 2u;
+        const float*   sumsOf = p.partial + at * p.dim + lane * 4u;
+        float          top = -INFINITY, total = 0.0f;
+        f32x4          sum{0, 0, 0, 0};
+        for(uint32_t first = begin; first < splits; first += STEP * UNROLL)
         {
-            float theirs = -INFINITY, sum = 0.0f;
-            if(s0 + lane < splits)
-                theirs = ends[(s0 + lane) * allRows * 2u], sum = ends[(s0 + lane) * allRows * 2u + 1u];
-            const float    factor = theirs == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(theirs - most);
-            const uint32_t here   = splits - s0 < L ? splits - s0 : L;
-#pragma unroll 8
-            for(uint32_t s = 0; s < here; ++s)
+            float theirs[UNROLL], weight[UNROLL], next = top;
+            f32x4 v[UNROLL];
+#pragma unroll
+            for(uint32_t u = 0; u < UNROLL; ++u)
             {
-                const float f = __shfl(factor, s, L);
-                total += f * __shfl(sum, s, L);
-                if(lane * 4u < p.dim)
-                    all += f * *reinterpret_cast<const f32x4*>(from + (s0 + s) * allRows * p.dim);
+                const uint32_t s = first + u * STEP, i = s < splits ? s : begin; // (those past the last: the first again, without weight)
+                theirs[u]        = endsOf[i * all * 2u], weight[u] = endsOf[i * all * 2u + 1u];
+                v[u]             = lane * 4u < p.dim ? *reinterpret_cast<const f32x4*>(sumsOf + i * all * p.dim) : f32x4{0, 0, 0, 0};
+            }
+#pragma unroll
+            for(uint32_t u = 0; u < UNROLL; ++u)
+            {
+                theirs[u] = first + u * STEP < splits ? theirs[u] : -INFINITY;
+                next      = fmaxf(next, theirs[u]);
+            }
+            const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - next);
+            total *= keep, sum *= keep, top = next;
+#pragma unroll
+            for(uint32_t u = 0; u < UNROLL; ++u)
+            {
+                const float factor = theirs[u] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(theirs[u] - next);
+                total += factor * weight[u];
+                sum += factor * v[u];
             }
         }
-        const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+        if constexpr(ALL)
+        {
+            sums[set][lane] = sum;
+            if(lane == 0u)
+                ends[set][0] = top, ends[set][1] = total;
+            __syncthreads();
+            if(set != 0u)
+                return;
+            for(uint32_t s = 1u; s < SETS; ++s)
+                top = fmaxf(top, ends[s][0]);
+            total = 0.0f, sum = f32x4{0, 0, 0, 0};
+            for(uint32_t s = 0; s < SETS; ++s)
+            {
+                const float factor = ends[s][0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ends[s][0] - top);
+                total += factor * ends[s][1];
+                sum += factor * sums[s][lane];
+            }
+        }
+        const float    inverse = total == 0.0f ? 0.0f : 1.0f / total;
+        const uint64_t row = seq.first + t;
         if(lane * 4u < p.dim)
-            *reinterpret_cast<u32x2*>(reinterpret_cast<T*>(p.out) + (int64_t)(seq.first + t) * p.oToken + (int64_t)head * p.oHead + lane * 4u)
-                = u32x2{r355::pack2<T>(all[0] * inverse, all[1] * inverse), r355::pack2<T>(all[2] * inverse, all[3] * inverse)};
+            *reinterpret_cast<u32x2*>(reinterpret_cast<T*>(p.out) + (int64_t)row * p.oToken + (int64_t)head * p.oHead + lane * 4u)
+                = u32x2{r355::pack2<T>(sum[0] * inverse, sum[1] * inverse), r355::pack2<T>(sum[2] * inverse, sum[3] * inverse)};
         if(p.lse && lane == 0u)
-            p.lse[row] = total == 0.0f ? -INFINITY : (most + __builtin_amdgcn_logf(total)) * 0.693147180559945309f;
+            p.lse[row * p.heads + head] = total == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * 0.693147180559945309f;
     }
 
     struct Plan
     {
-        uint32_t rowsPerGroup, rowTiles, splits;
+        uint32_t rowsPerGroup, rowTiles, shares;
     };
 
-    Plan planOf(const r355_tree_attention_args& a, uint32_t mostSplits)
+    uint64_t bytesOfShare(const r355_tree_attention_args& a)
     {
-        const uint64_t rows = (uint64_t)a.max_tokens * (a.heads / a.kv_heads);
-        Plan           plan;
-        plan.rowsPerGroup = rows <= 16u ? 16u : rows <= 32u ? 32u : a.head_dim <= 128u ? (rows <= 64u ? 64u : 128u) : 64u;
-        plan.rowTiles     = static_cast<uint32_t>((rows + plan.rowsPerGroup - 1u) / plan.rowsPerGroup);
-        const uint64_t groups = (uint64_t)a.batch * a.kv_heads * plan.rowTiles;
-        const uint64_t cus    = r355::computeUnits();
-        // one row tile for all rows: four workgroups a CU, as sequences differ in length (32 x 1 token of 820..8192 positions, 32 / 8 heads of 128:
-        // two 136 us, four 128, eight 136); tiles of 128 rows: two (2 x 64 tokens over 65600: two 207, four 237: more partial results)
-        uint64_t       want   = ((plan.rowsPerGroup <= 64u && a.head_dim <= 128u ? 4u : 2u) * cus + groups - 1u) / groups;
-        const uint64_t least  = ((uint64_t)a.max_kv + LEAST_CHUNK - 1u) / LEAST_CHUNK;
-        want                  = want < least ? want : least;
-        want                  = want < mostSplits ? want : mostSplits;
-        plan.splits           = static_cast<uint32_t>(want < 1u ? 1u : want > 256u ? 256u : want);
-        return plan;
+        return (uint64_t)a.max_tokens * a.heads * (a.head_dim + 2u) * 4u;
     }
 
-    uint64_t bytesOf(const r355_tree_attention_args& a, uint32_t splits)
+    Plan planOf(const r355_tree_attention_args& a, uint64_t workspaceBytes)
     {
-        return splits > 1u ? (uint64_t)splits * a.total_tokens * a.heads * (a.head_dim + 2u) * 4u : 0u;
+        const uint64_t rows = (uint64_t)a.max_tokens * (a.heads / a.kv_heads), cus = r355::computeUnits();
+        const uint64_t cache = (uint64_t)a.batch * a.max_kv * a.kv_heads * a.head_dim * 4u; // bytes, at most
+        Plan           plan;
+        // 16 and 32 rows: all four waves on positions; 64 and 128: on rows (50 rows of 16 heads, 4 x 16 tokens over 16000: 50 us, with the waves on positions 133).
+        plan.rowsPerGroup = rows <= 16u ? 16u : rows <= 32u && a.head_dim <= 128u ? 32u : a.head_dim <= 128u ? (rows <= 64u ? 64u : 128u) : 64u;
+        // A cache that the memory-side cache does not hold is read by one workgroup of eight waves instead of two of four, which drift apart further than
+        // an XCD's L2 reaches (2 x 64 tokens over 65600, 32 / 8 heads of 128: 890 instead of 450 MB past the L2, 180 and 163 us)
+        if(rows > 128u && cache >= 192ull << 20)
+            plan.rowsPerGroup = a.head_dim <= 128u ? 256u : 128u;
+        plan.rowTiles         = static_cast<uint32_t>((rows + plan.rowsPerGroup - 1u) / plan.rowsPerGroup);
+        const uint64_t groups = (uint64_t)a.kv_heads * plan.rowTiles; // workgroups of a share
+        // Workgroups a CU that are aimed at.  Eight waves: one (1 x 64 tokens over 65600, 32 / 8 heads of 128: 100 us, two 127).  One tile of rows: two, and four for
+        // single tokens with heads of 128, whose workgroups are the shortest (32 x 1 token over 820 .. 8192 positions: one 134 us, two 145, four 124, eight 141).
+        // Several tiles, of which shorter sequences have fewer: four (8 trees of up to 48 tokens over 4099, 24 / 4 heads of 64: two 34 us, three 33, four 25),
+        // three of heads of 256 (4 x 64 tokens over 8000: two 69 us, three 60, four 74).
+        const bool     eight  = plan.rowsPerGroup == 256u || (a.head_dim > 128u && plan.rowsPerGroup == 128u);
+        const uint64_t target = eight ? 1u : rows <= 16u && a.head_dim > 64u && a.head_dim <= 128u ? 4u : plan.rowTiles == 1u ? 2u : a.head_dim > 128u ? 3u : 4u;
+        uint64_t       shares = (target * cus + groups - 1u) / groups;
+        const uint64_t most   = (uint64_t)a.batch * (((uint64_t)a.max_kv + LEAST_CHUNK - 1u) / LEAST_CHUNK);
+        shares                = shares < most ? shares : most;
+        const uint64_t fit    = workspaceBytes / bytesOfShare(a);
+        shares                = shares < fit ? shares : fit;
+        plan.shares           = static_cast<uint32_t>(shares > a.batch ? shares : a.batch);
+        return plan;
     }
 
     template <typename T, uint32_t D, uint32_t WQ, uint32_t QB>
     void launchTree(const TreeParams& p, const Plan& plan, hipStream_t s)
     {
-        hipLaunchKernelGGL((treeKernel<T, D, WQ, QB>), dim3(p.columns * plan.rowTiles), dim3(WAVES * 64u), 0, s, p);
+        hipLaunchKernelGGL((treeKernel<T, D, WQ, QB>), dim3(p.columns * plan.rowTiles), dim3(WQ == 8u ? 512u : 256u), 0, s, p);
     }
 
     template <typename T>
@@ -636,18 +898,28 @@ namespace
             constexpr uint32_t D = decltype(width)::value;
             if(plan.rowsPerGroup == 16u)
                 launchTree<T, D, 1, 1>(p, plan, s);
+            else if constexpr(D == 256u)
+            {
+                if(plan.rowsPerGroup == 64u)
+                    launchTree<T, D, 4, 1>(p, plan, s);
+                else
+                    launchTree<T, D, 8, 1>(p, plan, s);
+            }
             else if(plan.rowsPerGroup == 32u)
                 launchTree<T, D, 1, 2>(p, plan, s);
-            else if constexpr(D == 256u)
-                launchTree<T, D, 4, 1>(p, plan, s);
             else if(plan.rowsPerGroup == 64u)
-                launchTree<T, D, 1, 4>(p, plan, s);
-            else
+                launchTree<T, D, 4, 1>(p, plan, s);
+            else if(plan.rowsPerGroup == 128u)
                 launchTree<T, D, 4, 2>(p, plan, s);
-            if(plan.splits > 1u)
+            else
+                launchTree<T, D, 8, 2>(p, plan, s);
+            if(plan.shares > p.batch)
             {
-                const uint64_t items = (uint64_t)p.batch * p.maxTokens * p.heads;
-                hipLaunchKernelGGL((treeMergeKernel<T, D>), dim3(static_cast<uint32_t>((items + 1024u / D - 1u) / (1024u / D))), dim3(256), 0, s, p);
+                const uint32_t rows = p.maxTokens * p.heads;
+                if((uint64_t)p.batch * rows <= 2048u)
+                    hipLaunchKernelGGL((treeMergeKernel<T, D, true>), dim3(rows, p.batch), dim3(256), 0, s, p);
+                else
+                    hipLaunchKernelGGL((treeMergeKernel<T, D, false>), dim3((rows + 1024u / D - 1u) / (1024u / D), p.batch), dim3(256), 0, s, p);
             }
         };
         using std::integral_constant;
@@ -680,8 +952,8 @@ namespace
             return r355::fail(R355_ERR_BAD_SIZE, "tree_attention: rows of %u pages hold fewer than max_kv=%u positions", a.table_stride, a.max_kv);
         if((uint64_t)a.max_tokens * (a.heads / a.kv_heads) > 0x40000000u)
             return r355::fail(R355_ERR_BAD_SIZE, "tree_attention: max_tokens=%u times %u heads per key head is over 2^30", a.max_tokens, a.heads / a.kv_heads);
-        const uint64_t groups = ((uint64_t)a.batch * a.kv_heads + 8u) * (((uint64_t)a.max_tokens * (a.heads / a.kv_heads) + 15u) / 16u);
-        if(groups > r355::MAX_GROUPS || (uint64_t)a.batch * a.max_tokens * a.heads / 4u >= r355::MAX_GROUPS)
+        const uint64_t groups = ((uint64_t)a.batch * a.kv_heads + 8192u) * (((uint64_t)a.max_tokens * (a.heads / a.kv_heads) + 15u) / 16u);
+        if(groups > r355::MAX_GROUPS / 2u || a.batch > 65535u || (uint64_t)a.max_tokens * a.heads >= r355::MAX_GROUPS)
             return r355::fail(R355_ERR_BAD_SIZE, "tree_attention: too many sequences, heads and drafted tokens for one launch");
         return R355_OK;
     }
@@ -691,7 +963,8 @@ extern "C" size_t r355_tree_attention_workspace_bytes(const r355_tree_attention_
 {
     if(!args || checkSizes(*args) != R355_OK || args->batch == 0 || args->total_tokens == 0 || args->max_tokens == 0)
         return 0;
-    return bytesOf(*args, planOf(*args, 256u).splits);
+    const Plan plan = planOf(*args, ~0ull);
+    return plan.shares > args->batch ? plan.shares * bytesOfShare(*args) : 0u;
 }
 
 extern "C" int r355_tree_attention(const r355_tree_attention_args* args, void* stream)
@@ -723,9 +996,7 @@ extern "C" int r355_tree_attention(const r355_tree_attention_args* args, void* s
         return r355::fail(R355_ERR_BAD_SIZE, "tree_attention: a cache of 2^36 slots and more");
     if(a.workspace && !r355::aligned(a.workspace, 16))
         return r355::fail(R355_ERR_MISALIGNED, "tree_attention: the workspace needs 16-byte alignment");
-    const uint64_t perSplit = (uint64_t)a.total_tokens * a.heads * (a.head_dim + 2u) * 4u;
-    const uint64_t fit      = a.workspace ? a.workspace_bytes / perSplit : 0u;
-    const Plan     plan     = planOf(a, static_cast<uint32_t>(fit < 256u ? fit : 256u));
+    const Plan plan = planOf(a, a.workspace ? a.workspace_bytes : 0u);
 
     TreeParams p;
     p.q = static_cast<const char*>(a.q), p.k = static_cast<const char*>(a.k), p.v = static_cast<const char*>(a.v), p.out = static_cast<char*>(a.out), p.lse = a.lse;
@@ -735,7 +1006,7 @@ extern "C" int r355_tree_attention(const r355_tree_attention_args* args, void* s
     p.batch = a.batch, p.heads = a.heads, p.kvHeads = a.kv_heads, p.group = a.heads / a.kv_heads, p.dim = a.head_dim;
     p.totalTokens = a.total_tokens, p.maxTokens = a.max_tokens, p.maxKv = a.max_kv;
     p.pageSize = a.page_size, p.pages = a.pages, p.tableStride = a.table_stride, p.maskWords = a.mask_words;
-    p.splits = plan.splits, p.columns = (a.batch * a.kv_heads * plan.splits + 7u) / 8u * 8u; // (row tiles of one split on one XCD)
+    p.shares = plan.shares, p.columns = (plan.shares * a.kv_heads + 7u) / 8u * 8u; // (the row tiles of a share on one XCD)
     p.scale2 = std::fmax(static_cast<float>(std::fabs(a.scale) * 1.4426950408889634), 1.17549435e-38f);
     p.signs  = a.scale < 0.0 ? 0x80008000u : 0u;
     const hipStream_t s = static_cast<hipStream_t>(stream);
