@@ -80,20 +80,22 @@ class W4Args(ctypes.Structure):
     ]
 
 
-class RopePart(ctypes.Structure):
-    _fields_ = [
-        ("x", ctypes.c_void_p), ("y", ctypes.c_void_p), ("heads", ctypes.c_uint32),
-        ("rotate", ctypes.c_int32), ("to_slots", ctypes.c_int32),
-        ("x_token_stride", ctypes.c_int64), ("x_head_stride", ctypes.c_int64),
-        ("y_token_stride", ctypes.c_int64), ("y_head_stride", ctypes.c_int64),
-    ]
+_ROPE_PART = (
+    ("x", ctypes.c_void_p), ("y", ctypes.c_void_p), ("heads", ctypes.c_uint32),
+    ("rotate", ctypes.c_int32), ("to_slots", ctypes.c_int32), ("pad", ctypes.c_int32),
+    ("x_token_stride", ctypes.c_int64), ("x_head_stride", ctypes.c_int64),
+    ("y_token_stride", ctypes.c_int64), ("y_head_stride", ctypes.c_int64),
+)
+_NO_ROPE_PART = (None, None, 0, 0, 0, 0, 0, 0, 0, 0)
 
 
 class RopeArgs(ctypes.Structure):
+    """r355_rope_args with its three r355_rope_part flat in it, x0 .. y_head_stride2: made by one call, where an array of structures takes more."""
     _fields_ = [
         ("type", ctypes.c_int32), ("layout", ctypes.c_int32),
         ("tokens", ctypes.c_uint32), ("head_dim", ctypes.c_uint32), ("rotary_dim", ctypes.c_uint32), ("parts", ctypes.c_uint32),
-        ("part", RopePart * 3),
+        *((name + "0", kind) for name, kind in _ROPE_PART), *((name + "1", kind) for name, kind in _ROPE_PART),
+        *((name + "2", kind) for name, kind in _ROPE_PART),
         ("positions", ctypes.c_void_p), ("turns", ctypes.c_void_p), ("slots", ctypes.c_void_p),
         ("slot_count", ctypes.c_uint32), ("inverse", ctypes.c_int32), ("scale", ctypes.c_double),
     ]
@@ -405,16 +407,17 @@ def rope_turns(rotary_dim, base=10000.0, factor=1.0, original_length=0, slow=1.0
 
 def rope_part(x, y, heads, x_strides, y_strides, rotate=True, to_slots=False):
     """One of up to three tensors of a rope() call; strides: (token, head) in elements."""
-    return RopePart(_ptr(x), _ptr(y), heads, rotate, to_slots, x_strides[0], x_strides[1], y_strides[0], y_strides[1])
+    return (_ptr(x), _ptr(y), heads, rotate, to_slots, 0, x_strides[0], x_strides[1], y_strides[0], y_strides[1])
 
 
 def rope(dtype, layout, tokens, head_dim, rotary_dim, parts, positions, turns, scale=1.0, inverse=False, slots=None, slot_count=0, stream=None):
     """Rotates (inverse: back) the first rotary_dim elements of every head of the parts by their token's position, in one launch; parts with
     to_slots go to rows slots[token] of a cache."""
-    if not 1 <= len(parts) <= 3:
-        raise ValueError("rope: 1 to 3 parts, got %d" % len(parts))
-    a = RopeArgs(dtype, layout, tokens, head_dim, rotary_dim, len(parts), tuple(parts), _ptr(positions), _ptr(turns), _ptr(slots), slot_count,
-                 inverse, scale)
+    n = len(parts)
+    if not 1 <= n <= 3:
+        raise ValueError("rope: 1 to 3 parts, got %d" % n)
+    p0, p1, p2 = (*parts, _NO_ROPE_PART, _NO_ROPE_PART)[:3]
+    a = RopeArgs(dtype, layout, tokens, head_dim, rotary_dim, n, *p0, *p1, *p2, _ptr(positions), _ptr(turns), _ptr(slots), slot_count, inverse, scale)
     _check(lib().r355_rope(ctypes.byref(a), _stream_handle(stream)))
 
 
