@@ -154,6 +154,8 @@ namespace
 #pragma unroll
         for(uint32_t r = 0; r < RB; ++r)
         {
+            if constexpr(ZEROS && RB * CB >= 16u)
+                __builtin_amdgcn_sched_barrier(0); // (the values of several blocks of rows at once would not fit beside the sums)
             const Values v = values(r);
 #pragma unroll
             for(uint32_t c = 0; c < CB; ++c)
@@ -209,6 +211,9 @@ namespace
     // ---- A few tokens, or rows of x off 16-byte boundaries (FAST false).  A workgroup's waves share 16 RB rows x 16 CB tokens and take the 128-k blocks in
     // turn, x and the weights straight from global memory; their sums meet in LDS in the order of the waves, so the result does not depend on
     // scheduling.  STEPS: matrix instructions (32 k) per scale.  DEPTH blocks in flight, each in registers of its own.
+    // Bound by the bytes of the weights from one wide row of workgroups on (16384 x 8192, groups of 128 with zero points, one token: 15.2 us, 4.63 TB/s of
+    // weights, scales and zero points), below that by one load's latency and the launch (1024 x 2048: 6.0 us); with small groups by the vector instructions that make operands
+    // and apply scales (10250 x 4168, groups of 32, 24 tokens: 15.0 us in one round of 214 workgroups).  No LDS: no other wave reads the same weights.
     struct __attribute__((packed, aligned(2))) Four16
     {
         u32x2 v;
@@ -377,6 +382,8 @@ namespace
     // Everything comes by direct loads into a ring of LDS buffers, as many steps ahead as fit: x in rows of 256 bytes (16-byte pieces in slots that depend on the
     // row: a wave reads 16 rows at one place), the weights as they are packed, a wave's scales and zero points one to a dword.  (Loads into registers among the
     // direct ones would have the compiler wait for all of them.)
+    // Bound by the vector instructions that make operands, once per tile of tokens, and by LDS reads beside the matrix instructions: 8192 x 4096, groups of 64,
+    // 1000 tokens, residual added: 88 us, 761 TFLOP/s (a library product of the same size, weights made 16 bits beforehand and not counted: some 1200).
     __device__ __forceinline__ void loadShortToLds(r355::dma_i32x4 rsrc, uint32_t laneOffset, uint32_t ldsAddr)
     {
         asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_ushort %0, %1, 0 offen lds" : : "v"(laneOffset), "s"(rsrc), "s"(ldsAddr) : "memory");
@@ -617,8 +624,9 @@ namespace
     };
     constexpr Variant VARIANTS[] = {
         {16, 16, {14, 15, 18}}, {32, 16, {16, 18, 22}}, {48, 16, {18, 21, 28}}, {64, 16, {19, 24, 36}}, // few tokens, one to four blocks of 16 rows
-        {16, 32, {21, 23, 26}}, {32, 32, {23, 25, 31}}, {48, 32, {25, 29, 38}}, {64, 32, {27, 34, 90}}, // (the last with groups of 32: registers spill)
-        {64, 32, {29, 34, 44}}, {128, 32, {51, 60, 78}}, {64, 64, {53, 60, 73}}, {128, 64, {77, 84, 114}}, // the ring
+        {16, 32, {21, 23, 26}}, {32, 32, {23, 25, 31}}, {48, 32, {25, 29, 38}},
+        {64, 32, {27, 34, 44}}, // (groups of 32: the ring, the others' registers spill: 90; with longer groups the ring takes 29 and 34)
+        {128, 32, {51, 60, 78}}, {64, 64, {53, 60, 73}}, {128, 64, {77, 84, 114}}, // the ring
         {128, 128, {147, 160, 200}}, {256, 128, {242, 245, 300}}};
 
     // The least time of all, counting a round of workgroups over the CUs as long as one.  (16384 x 8192, 24 tokens, groups of 128: one to four blocks
@@ -655,12 +663,15 @@ namespace
         case 4: return launchFew<T, 1, 2, 1, STEPS, true>(p, s);
         case 5: return launchFew<T, 2, 2, 1, STEPS, true>(p, s);
         case 6: return launchFew<T, 3, 2, 1, STEPS, true>(p, s);
-        case 7: return launchFew<T, 4, 2, 1, STEPS == 1u ? 2u : STEPS, true>(p, s); // (never chosen for groups of 32)
-        case 8: return launchRing<T, 2, 2, 2, 1, 4, STEPS>(p, s);
-        case 9: return launchRing<T, 2, 2, 4, 1, 2, STEPS>(p, s);
-        case 10: return launchRing<T, 1, 4, 4, 1, 2, STEPS>(p, s);
-        case 11: return launchRing<T, 2, 4, 4, 1, 2, STEPS>(p, s);
-        case 12: return launchRing<T, 2, 4, 4, 2, 1, STEPS>(p, s);
+        case 7:
+            if constexpr(STEPS == 1u)
+                return launchRing<T, 2, 2, 2, 1, 4, STEPS>(p, s);
+            else
+                return launchFew<T, 4, 2, 1, STEPS, true>(p, s);
+        case 8: return launchRing<T, 2, 2, 4, 1, 2, STEPS>(p, s);
+        case 9: return launchRing<T, 1, 4, 4, 1, 2, STEPS>(p, s);
+        case 10: return launchRing<T, 2, 4, 4, 1, 2, STEPS>(p, s);
+        case 11: return launchRing<T, 2, 4, 4, 2, 1, STEPS>(p, s);
         default: return launchRing<T, 4, 4, 4, 2, 1, STEPS>(p, s);
         }
     }
