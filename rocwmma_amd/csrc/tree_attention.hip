@@ -5,15 +5,19 @@
 // over the positions j that row i sees: all of the prefix and, of the drafted tokens (whose keys and values are the last rows of the
 // cache), those whose bit is set in the row's mask; without a mask those up to the row itself.
 //
-// The rows of a key head are its query heads times the drafted tokens of a sequence: 16 QB of them per wave.  A wave multiplies
+// The rows of a key head are its query heads times the drafted tokens of a sequence, 16 QB of them to a wave.  A wave multiplies
 // S^T = K Q^T (16 positions x 16 rows a matrix instruction), so that a lane holds four consecutive positions of one row: the running
 // maximum and sum of the softmax stay within a lane's registers but for two exchanges, and P^T is, as it lies, the B operand
 // of O^T = V^T P^T.  K and V go to LDS by direct loads, a 16-byte piece of a row in a slot that depends on the row, so that neither the reads
 // of K (16 rows at one place) nor the transposing reads of V meet in a bank.
 //
-// WQ waves of the four take different rows (and share the tiles), 4 / WQ different positions.  With all four on positions every wave fills
-// and reads tiles of its own and the loop has no barrier.
-// The positions of a sequence are split over workgroups where there are few; partial results (f32) meet in a second kernel, in order.
+// WQ waves of a workgroup take different rows (and share the tiles), the others different positions.  WQ = 1: four waves on positions, each of which fills and
+// reads tiles of its own, without a barrier.  WQ = 4 and 8: as many waves, all on rows, with the scores of the next tile made beside the exponentials of this one.
+// The positions of all sequences are split into shares of one length; partial results (f32) meet in a second kernel, in order.
+//
+// What bounds it, 32 / 8 heads of 128: with single tokens the bytes of the cache (32 tokens over 820 .. 8192 positions: 124 us, 4.9 TB/s), with a
+// short cache two launches and the first reads' latency (one token over 700: 11.7 us); with 64 tokens over 65600 positions the matrix and vector
+// instructions under the power limit (two sequences: 155 us, 665 TFLOP/s; their bytes alone are 94 us).
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -862,7 +866,7 @@ namespace
         const uint64_t rows = (uint64_t)a.max_tokens * (a.heads / a.kv_heads), cus = r355::computeUnits();
         const uint64_t cache = (uint64_t)a.batch * a.max_kv * a.kv_heads * a.head_dim * 4u; // bytes, at most
         Plan           plan;
-        // 16 and 32 rows: all four waves on positions; 64 and 128: on rows (50 rows of 16 heads, 4 x 16 tokens over 16000: 50 us, with the waves on positions 133).
+        // 16 and 32 rows: all four waves on positions; 64 and 128: on rows (64 rows, 4 x 16 tokens over 16000, 32 / 8 heads of 128: 50 us, with the waves on positions 133).
         plan.rowsPerGroup = rows <= 16u ? 16u : rows <= 32u && a.head_dim <= 128u ? 32u : a.head_dim <= 128u ? (rows <= 64u ? 64u : 128u) : 64u;
         // A cache that the memory-side cache does not hold is read by one workgroup of eight waves instead of two of four, which drift apart further than
         // an XCD's L2 reaches (2 x 64 tokens over 65600, 32 / 8 heads of 128: 890 instead of 450 MB past the L2, 180 and 163 us)
@@ -986,6 +990,8 @@ extern "C" int r355_tree_attention(const r355_tree_attention_args* args, void* s
         return r355::fail(R355_ERR_MISALIGNED, "tree_attention: strides of out must be multiples of 4 elements");
     if(!r355::aligned(a.q, 16) || !r355::aligned(a.k, 16) || !r355::aligned(a.v, 16) || !r355::aligned(a.out, 8))
         return r355::fail(R355_ERR_MISALIGNED, "tree_attention: q, k and v need 16-byte alignment, out 8-byte alignment");
+    if(!std::isfinite(static_cast<float>(a.scale)))
+        return r355::fail(R355_ERR_BAD_ARG, "tree_attention: the scale must be finite");
     if(a.lse && !r355::aligned(a.lse, 4))
         return r355::fail(R355_ERR_MISALIGNED, "tree_attention: lse needs 4-byte alignment");
     if(a.mask && !r355::aligned(a.mask, 8))

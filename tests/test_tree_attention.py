@@ -356,3 +356,8 @@ def test_tree_workspace_is_for_long_sequences():
     need = R.tree_attention_workspace_bytes(_args(max_kv=16384, table_stride=1024))
     assert need > 0 and need % (4 * 8 * (64 + 2) * 4) == 0
     assert R.tree_attention_workspace_bytes(_args(heads=7)) == 0
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), 1e300])
+def test_tree_refuses_a_scale_that_is_not_finite(scale):
+    _refused(-1, scale=scale)
