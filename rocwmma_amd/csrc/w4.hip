@@ -83,11 +83,15 @@ namespace
             return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(v)));
     }
 
-    // scales of four rows, and 16 + z of their zero points
+    // scale of the lane's row, and 16 + z of its zero point
     struct Values
     {
-        f32x4 scale, zero;
+        float scale, zero;
     };
+    __device__ __forceinline__ float zeroOf(uint32_t z)
+    {
+        return __uint_as_float(0x41800000u | (z << 19)); // (z < 16)
+    }
 
     // the first group of block kb of 128 k
     template <uint32_t STEPS>
@@ -107,7 +111,8 @@ namespace
         }
     }
 
-    // One group (STEPS matrix instructions of 32 k): acc += s (sum x (16 + q) - (16 + z) sum x).  Every row of the product with ones is sum x.
+    // One group (STEPS matrix instructions of 32 k): acc += s (sum x (16 + q) - (16 + z) sum x).  x is the first operand: a lane holds four tokens of one
+    // row, so that it needs one scale and one zero point.  Every column of the product with ones is sum x.
     // EARLY: with z = 8 everywhere the product of all rows starts from -24 sum x instead of zero; x(c, i) is held meanwhile.
     template <typename T, uint32_t RB, uint32_t CB, uint32_t STEPS, bool ZEROS, bool EARLY, typename X, typename W, typename V>
     __device__ __forceinline__ void accumulate(f32x4 (&acc)[RB][CB], const Expand<T>& expand, X&& x, W&& weights, V&& values)
@@ -127,10 +132,9 @@ namespace
                 for(uint32_t i = 0; i < STEPS; ++i)
                 {
                     held[c][i] = x(c, i);
-                    sumX[c]    = r355::mfma32<T>(ones, held[c][i], sumX[c]);
+                    sumX[c]    = r355::mfma32<T>(held[c][i], ones, sumX[c]);
                 }
-                const float t = -24.0f * sumX[c][0];
-                sumX[c]       = f32x4{t, t, t, t};
+                sumX[c] *= -24.0f;
             }
 #pragma unroll
         for(uint32_t i = 0; i < STEPS; ++i)
@@ -140,15 +144,15 @@ namespace
                 for(uint32_t c = 0; c < CB; ++c)
                 {
                     held[c][0] = x(c, i);
-                    sumX[c]    = r355::mfma32<T>(ones, held[c][0], sumX[c]);
+                    sumX[c]    = r355::mfma32<T>(held[c][0], ones, sumX[c]);
                 }
 #pragma unroll
             for(uint32_t r = 0; r < RB; ++r)
             {
-                const u32x4 a = expand(weights(r, i));
+                const u32x4 b = expand(weights(r, i));
 #pragma unroll
                 for(uint32_t c = 0; c < CB; ++c)
-                    sum[r][c] = r355::mfma32<T>(a, held[c][EARLY ? i : 0u], i != 0u ? sum[r][c] : EARLY ? sumX[c] : f32x4{0, 0, 0, 0});
+                    sum[r][c] = r355::mfma32<T>(held[c][EARLY ? i : 0u], b, i != 0u ? sum[r][c] : EARLY ? sumX[c] : f32x4{0, 0, 0, 0});
             }
         }
 #pragma unroll
@@ -161,7 +165,7 @@ namespace
             for(uint32_t c = 0; c < CB; ++c)
 #pragma unroll
                 for(uint32_t j = 0; j < 4; ++j)
-                    acc[r][c][j] = fmaf(v.scale[j], EARLY ? sum[r][c][j] : fmaf(ZEROS ? -v.zero[j] : -24.0f, sumX[c][0], sum[r][c][j]), acc[r][c][j]);
+                    acc[r][c][j] = fmaf(v.scale, EARLY ? sum[r][c][j] : fmaf(ZEROS ? -v.zero : -24.0f, sumX[c][j], sum[r][c][j]), acc[r][c][j]);
         }
     }
 
@@ -199,6 +203,21 @@ namespace
             storeRows<T>(p, token, row, sum);
     }
 
+    // The sums of `sets` sets of waves, [token][STRIDE] with ROWS rows each, added up in order and stored, four rows of a token to a thread.
+    template <typename T, uint32_t ROWS, uint32_t TOKENS, uint32_t STRIDE>
+    __device__ __forceinline__ void storeTile(const W4Params& p, const float* sums, uint32_t sets, uint32_t token0, uint32_t row0)
+    {
+        const uint32_t left = p.tokens - token0 < TOKENS ? p.tokens - token0 : TOKENS;
+        for(uint32_t i = threadIdx.x; i < left * (ROWS / 4u); i += blockDim.x)
+        {
+            const uint32_t token = i / (ROWS / 4u), row = i % (ROWS / 4u) * 4u;
+            f32x4          sum   = *reinterpret_cast<const f32x4*>(sums + token * STRIDE + row);
+            for(uint32_t v = 1u; v < sets; ++v)
+                sum += *reinterpret_cast<const f32x4*>(sums + (v * TOKENS + token) * STRIDE + row);
+            store<T>(p, token0 + token, row0 + row, sum);
+        }
+    }
+
     // Tile of n and tile of tokens of a workgroup: workgroups id, id + 8, ... run on one XCD and take a contiguous stretch of the tiles, those of one tile of
     // n after another (the scales of neighbouring rows share cache lines, the weights a tile of n).
     __device__ __forceinline__ bool tileOf(const W4Params& p, uint32_t& tileN, uint32_t& tileT)
@@ -214,19 +233,10 @@ namespace
     // Bound by the bytes of the weights from one wide row of workgroups on (16384 x 8192, groups of 128 with zero points, one token: 15.2 us, 4.63 TB/s of
     // weights, scales and zero points), below that by one load's latency and the launch (1024 x 2048: 6.0 us); with small groups by the vector instructions that make operands
     // and apply scales (10250 x 4168, groups of 32, 24 tokens: 15.0 us in one round of 214 workgroups).  No LDS: no other wave reads the same weights.
-    struct __attribute__((packed, aligned(2))) Four16
-    {
-        u32x2 v;
-    };
-    struct __attribute__((packed, aligned(1))) Four8
-    {
-        uint32_t v;
-    };
-
     template <typename T, uint32_t RB, uint32_t CB, uint32_t DEPTH, uint32_t STEPS, bool ZEROS, bool FAST>
     __global__ void __launch_bounds__(512, FAST ? 2 : 1) w4Kernel(W4Params p)
     {
-        extern __shared__ __attribute__((aligned(16))) float sums[]; // [waves][RB * CB][64][4]
+        extern __shared__ __attribute__((aligned(16))) float sums[]; // [waves][16 CB tokens][16 RB rows]
         constexpr uint32_t PARTS = 4u / STEPS;
         uint32_t           tileN, tileT;
         if(!tileOf(p, tileN, tileT))
@@ -242,14 +252,13 @@ namespace
             for(uint32_t c = 0; c < CB; ++c)
                 acc[r][c] = f32x4{0, 0, 0, 0};
 
-        // Where a block of 128 k has several groups, neighbouring lanes read one each and exchange them: one load instead of four.
+        // Where a block of 128 k has several groups, the lanes of one row read one each and exchange them: one load instead of four.
         struct Stage
         {
             u32x4    w[RB], x[CB][4];
-            u32x2    scale[RB];
-            uint32_t zero[RB];
+            uint32_t scale[RB], zero[RB];
         };
-        const uint32_t mine = lane % PARTS;
+        const uint32_t mine = quad % PARTS;
         // (a buffer over the rows of x from token0 on, which ends with the last element; lanes without a token lie past it)
         const auto bufX = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p.x) + (uint64_t)token0 * p.ldx * 2u, 0,
                                                             FAST ? ((left < 16u * CB ? left : 16u * CB) - 1u) * p.ldx * 2u + p.k * 2u : 0u, 0x00020000);
@@ -257,9 +266,6 @@ namespace
 #pragma unroll
         for(uint32_t c = 0; c < CB; ++c)
             offX[c] = c * 16u + col < left ? (c * 16u + col) * p.ldx * 2u + quad * 16u : OUTSIDE;
-        // FAST: at the end of a row of scales (n is 4 at least) the last four are read and moved down
-        auto rowOf = [&](uint32_t r) __attribute__((always_inline)) { return (block0 + r) * 16u + quad * 4u; };
-        auto readOf = [&](uint32_t r) __attribute__((always_inline)) { return rowOf(r) + 4u <= p.n ? rowOf(r) : p.n - 4u; };
         auto load = [&](uint32_t kb) __attribute__((always_inline)) {
             Stage          s;
             const uint32_t of = groupOf<STEPS>(p, kb) + mine;
@@ -269,23 +275,10 @@ namespace
             {
                 const uint32_t b = block0 + r < p.blocksN ? block0 + r : p.blocksN - 1u;
                 s.w[r]           = *reinterpret_cast<const u32x4*>(p.w + ((uint64_t)b * p.blocksK + kb) * 1024u + lane * 16u);
-                if constexpr(FAST)
-                {
-                    s.scale[r] = reinterpret_cast<const Four16*>(p.scales + 2u * (g * p.n + readOf(r)))->v;
-                    s.zero[r]  = ZEROS ? reinterpret_cast<const Four8*>(p.zeros + g * p.n + readOf(r))->v : 0u;
-                }
-                else
-                {
-                    s.scale[r] = u32x2{0u, 0u}, s.zero[r] = 0u;
-#pragma unroll
-                    for(uint32_t e = 0; e < 4; ++e)
-                        if(rowOf(r) + e < p.n)
-                        {
-                            s.scale[r][e / 2u] |= (uint32_t)reinterpret_cast<const uint16_t*>(p.scales)[g * p.n + rowOf(r) + e] << (e % 2u * 16u);
-                            if(ZEROS)
-                                s.zero[r] |= (uint32_t)p.zeros[g * p.n + rowOf(r) + e] << (e * 8u);
-                        }
-                }
+                const uint32_t row = (block0 + r) * 16u + col;
+                const uint64_t at  = g * p.n + (row < p.n ? row : p.n - 1u);
+                s.scale[r]         = reinterpret_cast<const uint16_t*>(p.scales)[at];
+                s.zero[r]          = ZEROS ? p.zeros[at] : 0u;
             }
 #pragma unroll
             for(uint32_t c = 0; c < CB; ++c)
@@ -316,31 +309,31 @@ namespace
                         s.x[c][i] = u32x4{0u, 0u, 0u, 0u};
         };
         auto multiply = [&](const Stage& s) __attribute__((always_inline)) {
-            u32x2    scales[RB]; // of the lane's group
-            uint32_t zeros[RB];
+            uint32_t of[RB][PARTS]; // of each group: the scale and, in the upper half, the zero point
 #pragma unroll
             for(uint32_t r = 0; r < RB; ++r)
             {
-                const uint32_t past = !FAST ? 0u : rowOf(r) - readOf(r) < 3u ? rowOf(r) - readOf(r) : 3u;
-                scales[r] = __builtin_bit_cast(u32x2, __builtin_bit_cast(uint64_t, s.scale[r]) >> (16u * past)), zeros[r] = s.zero[r] >> (8u * past);
+                const uint32_t v = ZEROS ? s.scale[r] | (s.zero[r] << 16) : s.scale[r];
+                if constexpr(PARTS == 1u)
+                    of[r][0] = v;
+                else if constexpr(PARTS == 2u)
+                {
+                    const auto pair = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+                    of[r][0] = pair[0], of[r][1] = pair[1];
+                }
+                else
+                {
+                    const auto half = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+                    const auto low = __builtin_amdgcn_permlane16_swap(half[0], half[0], false, false), high = __builtin_amdgcn_permlane16_swap(half[1], half[1], false, false);
+                    of[r][0] = low[0], of[r][1] = low[1], of[r][2] = high[0], of[r][3] = high[1];
+                }
             }
             each<PARTS>([&](auto partAt) __attribute__((always_inline)) {
                 constexpr uint32_t part = decltype(partAt)::value;
-                auto               of   = [](uint32_t v) __attribute__((always_inline)) {
-                    return PARTS > 1u ? static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), part * 0x55, 0xF, 0xF, true)) : v;
-                };
                 accumulate<T, RB, CB, STEPS, ZEROS, !ZEROS>(
                     acc, expand, [&](uint32_t c, uint32_t i) __attribute__((always_inline)) { return s.x[c][part * STEPS + i]; },
                     [&](uint32_t r, uint32_t i) __attribute__((always_inline)) { return s.w[r][part * STEPS + i]; },
-                    [&](uint32_t r) __attribute__((always_inline)) {
-                        const uint32_t lo = of(scales[r][0]), hi = of(scales[r][1]), z = ZEROS ? of(zeros[r]) : 0u;
-                        Values         v;
-                        v.scale = f32x4{scaleOf<T>(lo & 0xFFFFu), scaleOf<T>(lo >> 16), scaleOf<T>(hi & 0xFFFFu), scaleOf<T>(hi >> 16)};
-#pragma unroll
-                        for(uint32_t j = 0; j < 4; ++j)
-                            v.zero[j] = 16.0f + static_cast<float>((z >> (8u * j)) & 255u);
-                        return v;
-                    });
+                    [&](uint32_t r) __attribute__((always_inline)) { return Values{scaleOf<T>(of[r][part]), zeroOf(of[r][part] >> 16)}; });
             });
         };
         Stage stage[DEPTH]; // (a copy from one stage to the next would wait for its loads)
@@ -364,18 +357,15 @@ namespace
             });
 
 #pragma unroll
-        for(uint32_t r = 0; r < RB; ++r)
+        for(uint32_t c = 0; c < CB; ++c)
 #pragma unroll
-            for(uint32_t c = 0; c < CB; ++c)
-                *reinterpret_cast<f32x4*>(sums + ((wave * RB * CB + r * CB + c) * 64u + lane) * 4u) = acc[r][c];
+            for(uint32_t j = 0; j < 4; ++j)
+                if(c * 16u + quad * 4u + j < left)
+#pragma unroll
+                    for(uint32_t r = 0; r < RB; ++r)
+                        sums[((wave * CB + c) * 16u + quad * 4u + j) * (16u * RB) + r * 16u + col] = acc[r][c][j];
         __syncthreads();
-        for(uint32_t u = wave; u < RB * CB; u += waves)
-        {
-            f32x4 sum{0, 0, 0, 0};
-            for(uint32_t v = 0; v < waves; ++v)
-                sum += *reinterpret_cast<const f32x4*>(sums + ((v * RB * CB + u) * 64u + lane) * 4u);
-            store<T>(p, token0 + u % CB * 16u + col, (block0 + u / CB) * 16u + quad * 4u, sum);
-        }
+        storeTile<T, 16u * RB, 16u * CB, 16u * RB>(p, sums, waves, token0, block0 * 16u);
     }
 
     // ---- More tokens: 16 RB WN rows x 16 CB WT tokens a workgroup, 16 RB x 16 CB a wave; WK sets of such waves take the blocks of 128 k in turn.
@@ -402,7 +392,7 @@ namespace
         static constexpr uint32_t STAGE = X + W + WAVES * SCALES * 256u * (ZEROS ? 2u : 1u);
         static constexpr uint32_t LOADS_X = WK * TOKENS / 4u / WAVES, LOADS_W = W / 1024u / WAVES; // of a wave
         static constexpr uint32_t LOADS = LOADS_X + LOADS_W + SCALES * (ZEROS ? 2u : 1u);
-        static constexpr uint32_t MERGE = WK > 1u ? WAVES * RB * CB * 1024u : 0u;
+        static constexpr uint32_t STRIDE = 16u * RB * WN + 4u, MERGE = WK * TOKENS * STRIDE * 4u; // of the sums, at the end
         static constexpr uint32_t FIT = 160u * 1024u / STAGE, BUFS = FIT > 4u ? 4u : FIT;
         static constexpr uint32_t LDS = BUFS * STAGE > MERGE ? BUFS * STAGE : MERGE;
         static_assert(LOADS_X * WAVES * 4u == WK * TOKENS && LOADS_W * WAVES * 1024u == W, "whole loads for every wave");
@@ -509,7 +499,7 @@ namespace
             const uint32_t stage = ldsBase + buf * R::STAGE;
             const uint32_t fromX = stage + waveK * TOKENS * 256u + (waveT * CB * 16u + col) * 256u + (quad ^ col) * 16u;
             const uint32_t fromW = stage + R::X + ((waveK * WN + waveN) * RB * 64u + lane) * 16u;
-            const uint32_t fromS = stage + R::X + R::W + wave * R::SCALES * 256u + quad * 16u;
+            const uint32_t fromS = stage + R::X + R::W + wave * R::SCALES * 256u + col * 4u;
             each<PARTS>([&](auto partAt) __attribute__((always_inline)) {
                 constexpr uint32_t part = decltype(partAt)::value;
                 accumulate<T, RB, CB, STEPS, ZEROS, !ZEROS && (STEPS * CB <= 8u)>(
@@ -517,51 +507,23 @@ namespace
                     [&](uint32_t c, uint32_t i) __attribute__((always_inline)) { return *(lds4)(uintptr_t)((fromX ^ ((part * STEPS + i) * 64u)) + c * 4096u); },
                     [&](uint32_t r, uint32_t i) __attribute__((always_inline)) { return *(lds1)(uintptr_t)(fromW + r * 1024u + (part * STEPS + i) * 4u); },
                     [&](uint32_t r) __attribute__((always_inline)) {
-                        const u32x4 s = *(lds4)(uintptr_t)(fromS + (r * PARTS + part) * 64u);
-                        Values      v;
-#pragma unroll
-                        for(uint32_t j = 0; j < 4; ++j)
-                            v.scale[j] = scaleOf<T>(s[j]), v.zero[j] = 24.0f;
-                        if constexpr(ZEROS)
-                        {
-                            const u32x4 z = *(lds4)(uintptr_t)(fromS + WAVES * R::SCALES * 256u + (r * PARTS + part) * 64u);
-#pragma unroll
-                            for(uint32_t j = 0; j < 4; ++j)
-                                v.zero[j] = __uint_as_float(0x41800000u | (z[j] << 19)); // 16 + z for z < 16
-                        }
-                        return v;
+                        const uint32_t at = fromS + (r * PARTS + part) * 64u;
+                        return Values{scaleOf<T>(*(lds1)(uintptr_t)at), ZEROS ? zeroOf(*(lds1)(uintptr_t)(at + WAVES * R::SCALES * 256u)) : 24.0f};
                     });
             });
             buf = buf + 1u == BUFS ? 0u : buf + 1u;
         }
-        if constexpr(WK == 1u)
-        {
+        __syncthreads();
+        float* const sums = reinterpret_cast<float*>(lds);
 #pragma unroll
-            for(uint32_t r = 0; r < RB; ++r)
+        for(uint32_t c = 0; c < CB; ++c)
 #pragma unroll
-                for(uint32_t c = 0; c < CB; ++c)
-                    store<T>(p, token0 + (waveT * CB + c) * 16u + col, (block0 + r) * 16u + quad * 4u, acc[r][c]);
-        }
-        else
-        {
-            // the sets of waves meet in LDS, in order: set i adds up and stores the blocks i, i + WK, ... of its waves' place
-            __syncthreads();
-            float* const sums = reinterpret_cast<float*>(lds); // [WAVES][RB * CB][64][4]
+            for(uint32_t j = 0; j < 4; ++j)
 #pragma unroll
-            for(uint32_t r = 0; r < RB; ++r)
-#pragma unroll
-                for(uint32_t c = 0; c < CB; ++c)
-                    *reinterpret_cast<f32x4*>(sums + ((wave * RB * CB + r * CB + c) * 64u + lane) * 4u) = acc[r][c];
-            __syncthreads();
-            for(uint32_t u = waveK; u < RB * CB; u += WK)
-            {
-                f32x4 sum{0, 0, 0, 0};
-#pragma unroll
-                for(uint32_t v = 0; v < WK; ++v)
-                    sum += *reinterpret_cast<const f32x4*>(sums + (((wave % (WN * WT) + v * WN * WT) * RB * CB + u) * 64u + lane) * 4u);
-                store<T>(p, token0 + (waveT * CB + u % CB) * 16u + col, (block0 + u / CB) * 16u + quad * 4u, sum);
-            }
-        }
+                for(uint32_t r = 0; r < RB; ++r)
+                    sums[(waveK * TOKENS + (waveT * CB + c) * 16u + quad * 4u + j) * R::STRIDE + (waveN * RB + r) * 16u + col] = acc[r][c][j];
+        __syncthreads();
+        storeTile<T, 16u * RB * WN, TOKENS, R::STRIDE>(p, sums, WK, token0, group0 * 16u);
     }
 
     // one dword of the packed storage per thread: block of 16 rows, block of 128 k, lane, 32-k step
@@ -751,7 +713,7 @@ extern "C" int r355_w4_matmul(const r355_w4_args* args, void* stream)
     p.wideN  = a.ldy % 4u == 0u && r355::aligned(a.y, 4u * outBytes) && (a.beta == 0.0 || (a.ldc % 4u == 0u && r355::aligned(a.c, 4u * outBytes)));
     p.alpha = static_cast<float>(a.alpha), p.beta = static_cast<float>(a.beta);
     // (the rows of x that a workgroup takes, 128 at most, lie within 2^31 bytes)
-    const bool        fast = a.k % 8u == 0u && a.ldx % 8u == 0u && r355::aligned(a.x, 16) && a.n >= 4u && a.ldx <= (1u << 22);
+    const bool        fast = a.k % 8u == 0u && a.ldx % 8u == 0u && r355::aligned(a.x, 16) && a.ldx <= (1u << 22);
     const hipStream_t s    = static_cast<hipStream_t>(stream);
     r355::beginCall();
     if(a.in_type == R355_F16)
