@@ -66,11 +66,12 @@ namespace
         }
     };
 
-    template <typename T>
-    __device__ __forceinline__ u32x4 onesOf()
+    // all 1, or all -24
+    template <typename T, bool EARLY>
+    __device__ __forceinline__ u32x4 timesOf()
     {
-        constexpr uint32_t ONE = std::is_same_v<T, __bf16> ? 0x3F803F80u : 0x3C003C00u;
-        return u32x4{ONE, ONE, ONE, ONE};
+        constexpr uint32_t V = std::is_same_v<T, __bf16> ? (EARLY ? 0xC1C0C1C0u : 0x3F803F80u) : (EARLY ? 0xCE00CE00u : 0x3C003C00u);
+        return u32x4{V, V, V, V};
     }
 
     // a 16-bit scale in the low half of a dword
@@ -113,12 +114,12 @@ namespace
 
     // One group (STEPS matrix instructions of 32 k): acc += s (sum x (16 + q) - (16 + z) sum x).  x is the first operand: a lane holds four tokens of one
     // row, so that it needs one scale and one zero point.  Every column of the product with ones is sum x.
-    // EARLY: with z = 8 everywhere the product of all rows starts from -24 sum x instead of zero; x(c, i) is held meanwhile.
+    // EARLY: with z = 8 everywhere the product of all rows starts from -24 sum x, a product with that, instead of zero; x(c, i) is held meanwhile.
     template <typename T, uint32_t RB, uint32_t CB, uint32_t STEPS, bool ZEROS, bool EARLY, typename X, typename W, typename V>
     __device__ __forceinline__ void accumulate(f32x4 (&acc)[RB][CB], const Expand<T>& expand, X&& x, W&& weights, V&& values)
     {
         static_assert(!(ZEROS && EARLY), "one start for all rows");
-        const u32x4 ones = onesOf<T>();
+        const u32x4 times = timesOf<T, EARLY>();
         f32x4       sumX[CB], sum[RB][CB];
         u32x4       held[CB][EARLY ? STEPS : 1u];
 #pragma unroll
@@ -127,15 +128,12 @@ namespace
         if constexpr(EARLY)
 #pragma unroll
             for(uint32_t c = 0; c < CB; ++c)
-            {
 #pragma unroll
                 for(uint32_t i = 0; i < STEPS; ++i)
                 {
                     held[c][i] = x(c, i);
-                    sumX[c]    = r355::mfma32<T>(held[c][i], ones, sumX[c]);
+                    sumX[c]    = r355::mfma32<T>(held[c][i], times, sumX[c]);
                 }
-                sumX[c] *= -24.0f;
-            }
 #pragma unroll
         for(uint32_t i = 0; i < STEPS; ++i)
         {
@@ -144,7 +142,7 @@ namespace
                 for(uint32_t c = 0; c < CB; ++c)
                 {
                     held[c][0] = x(c, i);
-                    sumX[c]    = r355::mfma32<T>(held[c][0], ones, sumX[c]);
+                    sumX[c]    = r355::mfma32<T>(held[c][0], times, sumX[c]);
                 }
 #pragma unroll
             for(uint32_t r = 0; r < RB; ++r)
@@ -230,9 +228,9 @@ namespace
     // ---- A few tokens, or rows of x off 16-byte boundaries (FAST false).  A workgroup's waves share 16 RB rows x 16 CB tokens and take the 128-k blocks in
     // turn, x and the weights straight from global memory; their sums meet in LDS in the order of the waves, so the result does not depend on
     // scheduling.  STEPS: matrix instructions (32 k) per scale.  DEPTH blocks in flight, each in registers of its own.
-    // Bound by the bytes of the weights from one wide row of workgroups on (16384 x 8192, groups of 128 with zero points, one token: 15.2 us, 4.63 TB/s of
-    // weights, scales and zero points), below that by one load's latency and the launch (1024 x 2048: 6.0 us); with small groups by the vector instructions that make operands
-    // and apply scales (10250 x 4168, groups of 32, 24 tokens: 15.0 us in one round of 214 workgroups).  No LDS: no other wave reads the same weights.
+    // Bound by the bytes of the weights from one wide row of workgroups on (16384 x 8192, groups of 128 with zero points, one token: 14.2 us, 4.95 TB/s of
+    // weights, scales and zero points), below that by one load's latency and the launch (1024 x 2048: 5.6 us); with more tokens by x out of the L2 and, with small groups,
+    // the vector instructions that make operands and apply scales (10250 x 4168, groups of 32, 24 tokens: 13.1 us in one round of 214 workgroups).  No LDS: no other wave reads the same weights.
     template <typename T, uint32_t RB, uint32_t CB, uint32_t DEPTH, uint32_t STEPS, bool ZEROS, bool FAST>
     __global__ void __launch_bounds__(512, FAST ? 2 : 1) w4Kernel(W4Params p)
     {
@@ -373,7 +371,7 @@ namespace
     // row: a wave reads 16 rows at one place), the weights as they are packed, a wave's scales and zero points one to a dword.  (Loads into registers among the
     // direct ones would have the compiler wait for all of them.)
     // Bound by the vector instructions that make operands, once per tile of tokens, and by LDS reads beside the matrix instructions: 8192 x 4096, groups of 64,
-    // 1000 tokens, residual added: 88 us, 761 TFLOP/s (a library product of the same size, weights made 16 bits beforehand and not counted: some 1200).
+    // 1000 tokens, residual added: 87 us, 771 TFLOP/s (a library product of the same size, weights made 16 bits beforehand and not counted: some 1200).
     __device__ __forceinline__ void loadShortToLds(r355::dma_i32x4 rsrc, uint32_t laneOffset, uint32_t ldsAddr)
     {
         asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_ushort %0, %1, 0 offen lds" : : "v"(laneOffset), "s"(rsrc), "s"(ldsAddr) : "memory");
@@ -494,8 +492,14 @@ namespace
                 r355::waitVmcnt<0>();
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             r355::ldsBarrier(); // everyone's part of this step is there, and everyone is done with the step before
-            if(step + BUFS - 1u < steps)
-                issue(step + BUFS - 1u, buf == 0u ? BUFS - 1u : buf - 1u);
+            // The next loads, into the buffer of the step before: with groups of 128 behind the products (4096 x 4096, 512 tokens 77.4 -> 74.6 us), with smaller ones
+            // before them, for want of registers.
+            auto next = [&]() __attribute__((always_inline)) {
+                if(step + BUFS - 1u < steps)
+                    issue(step + BUFS - 1u, buf == 0u ? BUFS - 1u : buf - 1u);
+            };
+            if constexpr(PARTS > 1u)
+                next();
             const uint32_t stage = ldsBase + buf * R::STAGE;
             const uint32_t fromX = stage + waveK * TOKENS * 256u + (waveT * CB * 16u + col) * 256u + (quad ^ col) * 16u;
             const uint32_t fromW = stage + R::X + ((waveK * WN + waveN) * RB * 64u + lane) * 16u;
@@ -511,6 +515,8 @@ namespace
                         return Values{scaleOf<T>(*(lds1)(uintptr_t)at), ZEROS ? zeroOf(*(lds1)(uintptr_t)(at + WAVES * R::SCALES * 256u)) : 24.0f};
                     });
             });
+            if constexpr(PARTS == 1u)
+                next();
             buf = buf + 1u == BUFS ? 0u : buf + 1u;
         }
         __syncthreads();
@@ -585,14 +591,14 @@ namespace
         uint32_t rows, tokens, time[3];
     };
     constexpr Variant VARIANTS[] = {
-        {16, 16, {14, 15, 18}}, {32, 16, {16, 18, 22}}, {48, 16, {18, 21, 28}}, {64, 16, {19, 24, 36}}, // few tokens, one to four blocks of 16 rows
-        {16, 32, {21, 23, 26}}, {32, 32, {23, 25, 31}}, {48, 32, {25, 29, 38}},
-        {64, 32, {27, 34, 44}}, // (groups of 32: the ring, the others' registers spill: 90; with longer groups the ring takes 29 and 34)
-        {128, 32, {51, 60, 78}}, {64, 64, {53, 60, 73}}, {128, 64, {77, 84, 114}}, // the ring
-        {128, 128, {147, 160, 200}}, {256, 128, {242, 245, 300}}};
+        {16, 16, {13, 13, 13}}, {32, 16, {15, 14, 15}}, {48, 16, {16, 17, 19}}, {64, 16, {18, 19, 23}}, // few tokens, one to four blocks of 16 rows
+        {16, 32, {24, 25, 24}}, {32, 32, {26, 25, 26}}, {48, 32, {27, 27, 28}},
+        {64, 32, {27, 29, 34}}, // (groups of 32: the ring, the others' registers spill)
+        {128, 32, {49, 56, 63}}, {64, 64, {52, 57, 65}}, {128, 64, {78, 84, 106}}, // the ring
+        {128, 128, {147, 161, 199}}, {256, 128, {251, 262, 319}}};
 
-    // The least time of all, counting a round of workgroups over the CUs as long as one.  (16384 x 8192, 24 tokens, groups of 128: one to four blocks
-    // of rows 51, 31, 34, 20 us; 10250 x 4168, groups of 32: 21, 22, 15, 35 us.)
+    // The least time of all, counting a round of workgroups over the CUs as long as one.  (24 tokens: 16384 x 8192, groups of 128: one to four blocks of rows
+    // 55, 31, 34, 20 us; 10250 x 4168, groups of 32: 21, 20, 13, 16 us.)
     uint32_t variantOf(const W4Params& p)
     {
         const uint32_t by = p.group == 32u ? 2u : p.group == 64u ? 1u : 0u, cus = r355::computeUnits();
@@ -600,7 +606,7 @@ namespace
         uint64_t       least = ~0ull;
         for(uint32_t v = 0; v < sizeof(VARIANTS) / sizeof(VARIANTS[0]); ++v)
         {
-            // up to four tokens x costs next to nothing, and two workgroups of up to three blocks share a CU well (16384 x 8192, one token: two blocks 13.6, four 14.8 us)
+            // up to four tokens x costs next to nothing, and two workgroups of up to three blocks share a CU well (16384 x 8192, one token: two blocks 14.3, four 15.2 us)
             if(p.tokens <= 4u && v > 2u)
                 break;
             const uint64_t groups = (uint64_t)((p.n + VARIANTS[v].rows - 1u) / VARIANTS[v].rows) * ((p.tokens + VARIANTS[v].tokens - 1u) / VARIANTS[v].tokens);
