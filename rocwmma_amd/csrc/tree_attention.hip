@@ -874,12 +874,15 @@ namespace
             plan.rowsPerGroup = a.head_dim <= 128u ? 256u : 128u;
         plan.rowTiles         = static_cast<uint32_t>((rows + plan.rowsPerGroup - 1u) / plan.rowsPerGroup);
         const uint64_t groups = (uint64_t)a.kv_heads * plan.rowTiles; // workgroups of a share
-        // Workgroups a CU that are aimed at.  Eight waves: one (1 x 64 tokens over 65600, 32 / 8 heads of 128: 100 us, two 127).  One tile of rows: two, and four for
+        // Workgroups a CU that are aimed at.  Eight waves: one (1 x 64 tokens over 65600, 32 / 8 heads of 128: 100 us, two 127).  Waves on positions, of which a CU holds
+        // one workgroup: one, where that makes eight shares of a sequence and more, so that the last share of each, which is shorter, weighs little (one token, 32 / 8 heads of 128:
+        // 1 x 16000 18.8 us, two 23.7, four 23.7; 4 x 16000 56, 61, 64; 8 tokens, 1 x 65536: 59, 66, 81).  Else, with one tile of rows: two, and four for
         // single tokens with heads of 128, whose workgroups are the shortest (32 x 1 token over 820 .. 8192 positions: one 134 us, two 145, four 124, eight 141).
         // Several tiles, of which shorter sequences have fewer: four (8 trees of up to 48 tokens over 4099, 24 / 4 heads of 64: two 34 us, three 33, four 25),
         // three of heads of 256 (4 x 64 tokens over 8000: two 69 us, three 60, four 74).
         const bool     eight  = plan.rowsPerGroup == 256u || (a.head_dim > 128u && plan.rowsPerGroup == 128u);
-        const uint64_t target = eight ? 1u : rows <= 16u && a.head_dim > 64u && a.head_dim <= 128u ? 4u : plan.rowTiles == 1u ? 2u : a.head_dim > 128u ? 3u : 4u;
+        const bool     one    = eight || (plan.rowsPerGroup <= 32u && (a.batch == 1u || a.batch * 8u <= cus / groups));
+        const uint64_t target = one ? 1u : rows <= 16u && a.head_dim > 64u && a.head_dim <= 128u ? 4u : plan.rowTiles == 1u ? 2u : a.head_dim > 128u ? 3u : 4u;
         uint64_t       shares = (target * cus + groups - 1u) / groups;
         const uint64_t most   = (uint64_t)a.batch * (((uint64_t)a.max_kv + LEAST_CHUNK - 1u) / LEAST_CHUNK);
         shares                = shares < most ? shares : most;
