@@ -10,6 +10,7 @@ Argument order follows the reference kernel signature (test/gemm/gemm_kernel_bas
 """
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "librocwmma_amd.so")
@@ -80,25 +81,10 @@ class W4Args(ctypes.Structure):
     ]
 
 
-_ROPE_PART = (
-    ("x", ctypes.c_void_p), ("y", ctypes.c_void_p), ("heads", ctypes.c_uint32),
-    ("rotate", ctypes.c_int32), ("to_slots", ctypes.c_int32), ("pad", ctypes.c_int32),
-    ("x_token_stride", ctypes.c_int64), ("x_head_stride", ctypes.c_int64),
-    ("y_token_stride", ctypes.c_int64), ("y_head_stride", ctypes.c_int64),
-)
-_NO_ROPE_PART = (None, None, 0, 0, 0, 0, 0, 0, 0, 0)
-
-
-class RopeArgs(ctypes.Structure):
-    """r355_rope_args with its three r355_rope_part flat in it, x0 .. y_head_stride2: made by one call, where an array of structures takes more."""
-    _fields_ = [
-        ("type", ctypes.c_int32), ("layout", ctypes.c_int32),
-        ("tokens", ctypes.c_uint32), ("head_dim", ctypes.c_uint32), ("rotary_dim", ctypes.c_uint32), ("parts", ctypes.c_uint32),
-        *((name + "0", kind) for name, kind in _ROPE_PART), *((name + "1", kind) for name, kind in _ROPE_PART),
-        *((name + "2", kind) for name, kind in _ROPE_PART),
-        ("positions", ctypes.c_void_p), ("turns", ctypes.c_void_p), ("slots", ctypes.c_void_p),
-        ("slot_count", ctypes.c_uint32), ("inverse", ctypes.c_int32), ("scale", ctypes.c_double),
-    ]
+# r355_rope_args as bytes: a structure of 42 fields takes 2 us longer to make, a quarter of a call for a few tokens.  Sizes and strides; per part: x, y, heads, rotate,
+# to_slots, padding, strides of x and of y; then positions, turns, slots, slot_count, inverse, scale.
+_ROPE_ARGS = struct.Struct("=iiIIII" + 3 * "QQIiiiqqqq" + "QQQIid")
+_NO_ROPE_PART = (0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
 
 
 class TreeAttentionArgs(ctypes.Structure):
@@ -162,7 +148,7 @@ def lib():
         L.r355_w4_matmul.argtypes = [ctypes.POINTER(W4Args), vp]
         L.r355_w4_packed_bytes.argtypes = [u32, u32]
         L.r355_w4_pack.argtypes = [vp, u32, u32, u32, vp, vp]
-        L.r355_rope.argtypes = [ctypes.POINTER(RopeArgs), vp]
+        L.r355_rope.argtypes = [ctypes.c_char_p, vp]
         L.r355_rope_turns.argtypes = [u32, ctypes.c_double, ctypes.c_double, u32, ctypes.c_double, ctypes.c_double, vp]
         L.r355_tree_attention.argtypes = [ctypes.POINTER(TreeAttentionArgs), vp]
         L.r355_tree_attention_workspace_bytes.argtypes = [ctypes.POINTER(TreeAttentionArgs)]
@@ -407,7 +393,7 @@ def rope_turns(rotary_dim, base=10000.0, factor=1.0, original_length=0, slow=1.0
 
 def rope_part(x, y, heads, x_strides, y_strides, rotate=True, to_slots=False):
     """One of up to three tensors of a rope() call; strides: (token, head) in elements."""
-    return (_ptr(x), _ptr(y), heads, rotate, to_slots, 0, x_strides[0], x_strides[1], y_strides[0], y_strides[1])
+    return (_ptr(x) or 0, _ptr(y) or 0, heads, rotate, to_slots, 0, x_strides[0], x_strides[1], y_strides[0], y_strides[1])
 
 
 def rope(dtype, layout, tokens, head_dim, rotary_dim, parts, positions, turns, scale=1.0, inverse=False, slots=None, slot_count=0, stream=None):
@@ -417,8 +403,9 @@ def rope(dtype, layout, tokens, head_dim, rotary_dim, parts, positions, turns, s
     if not 1 <= n <= 3:
         raise ValueError("rope: 1 to 3 parts, got %d" % n)
     p0, p1, p2 = (*parts, _NO_ROPE_PART, _NO_ROPE_PART)[:3]
-    a = RopeArgs(dtype, layout, tokens, head_dim, rotary_dim, n, *p0, *p1, *p2, _ptr(positions), _ptr(turns), _ptr(slots), slot_count, inverse, scale)
-    _check(lib().r355_rope(ctypes.byref(a), _stream_handle(stream)))
+    a = _ROPE_ARGS.pack(dtype, layout, tokens, head_dim, rotary_dim, n, *p0, *p1, *p2, _ptr(positions) or 0, _ptr(turns) or 0, _ptr(slots) or 0, slot_count,
+                        inverse, scale)
+    _check(lib().r355_rope(a, _stream_handle(stream)))
 
 
 def tree_attention_args(dtype, batch, total_tokens, heads, kv_heads, head_dim, q, k, v, out, table, page_size, pages, q_start, kv_len, max_tokens,
