@@ -3,12 +3,12 @@
 //   y[t][r] = alpha * sum_k x[t][k] (q[r][k] - z[k / g][r]) s[k / g][r] + beta c[t][r]
 //
 // No counterpart in the reference.  The weights q are stored in blocks of 16 rows x 128 k (r355_w4_pack), 1 KiB each in the order in
-// which a wave's lanes load them, 16 bytes a lane: the four dwords of a lane are its A operands of four v_mfma_f32_16x16x32, x is the B
-// operand, and up to 16 tokens cost what one costs.
+// which a wave's lanes load them, 16 bytes a lane: the four dwords of a lane are its second operands of four v_mfma_f32_16x16x32, x is the
+// first, and up to 16 tokens cost what one costs.
 //
 // A nibble becomes an operand without a conversion: with the nibble in the four leading bits of the mantissa of 16.0 the 16-bit number
 // is 16 + q, so a shift and an and-or make two operands.  The matrix instruction sums x (16 + q) over a group exactly as it would sum x q,
-// one more instruction with ones for A leaves sum x in the same lanes, and
+// one more instruction with ones for weights leaves sum x in the same lanes, and
 //   sum x (q - z) = sum x (16 + q) - (16 + z) sum x
 // in f32: the sums are about five times as large as the difference (16 + 7.5 against the spread of q), so their rounding costs about
 // two bits of 24.  The scale of the group is applied to the f32 sum, never to a 16-bit weight.
