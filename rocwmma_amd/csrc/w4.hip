@@ -585,7 +585,7 @@ namespace
     }
 
     // The kernels that are launched, with what a workgroup of each takes for a block of 128 k while it has its CU to itself (hundredths of
-    // a microsecond; groups of 128, of 64 and of 32; measured over 1024 .. 16384 rows and 2048 .. 16384 k).
+    // a microsecond; groups of 128, of 64 and of 32; bf16, with and without zero points, 240 workgroups, from k = 4096 to 8192).
     struct Variant
     {
         uint32_t rows, tokens, time[3];
