@@ -438,7 +438,9 @@ namespace
             {
                 const uint32_t at = wave * R::LOADS_X + j, kb = step * WK + at * 4u / TOKENS;
                 const uint32_t k  = kb * 128u + (col ^ ((at * 4u % TOKENS + quad) & 15u)) * 8u;
-                r355::loadToLds(bufX, k < p.k ? offX[j] : OUTSIDE, __builtin_amdgcn_readfirstlane(kb * 256u), __builtin_amdgcn_readfirstlane(to + at * 1024u));
+                // (A lane's offset is held against the length of the buffer less the uniform one: that must not be more than the length, which with one token is 2 k
+                // bytes, or the difference wraps around and OUTSIDE is inside.)
+                r355::loadToLds(bufX, k < p.k ? offX[j] : OUTSIDE, __builtin_amdgcn_readfirstlane(kb < p.blocksK ? kb * 256u : 0u), __builtin_amdgcn_readfirstlane(to + at * 1024u));
             }
 #pragma unroll
             for(uint32_t j = 0; j < R::LOADS_W; ++j)
