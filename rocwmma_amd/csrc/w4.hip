@@ -713,7 +713,7 @@ extern "C" int r355_w4_matmul(const r355_w4_args* args, void* stream)
     W4Params p;
     p.x = static_cast<const char*>(a.x), p.w = static_cast<const char*>(a.w), p.scales = static_cast<const char*>(a.scales), p.zeros = a.zeros;
     p.c = static_cast<const char*>(a.c), p.y = static_cast<char*>(a.y);
-    p.tokens = a.tokens, p.n = a.n, p.k = a.k, p.group = a.group, p.groups = (a.k + a.group - 1u) / a.group, p.ldx = a.ldx, p.ldc = a.ldc, p.ldy = a.ldy;
+    p.tokens = a.tokens, p.n = a.n, p.k = a.k, p.group = a.group, p.groups = static_cast<uint32_t>(((uint64_t)a.k + a.group - 1u) / a.group), p.ldx = a.ldx, p.ldc = a.ldc, p.ldy = a.ldy;
     p.blocksN = (a.n + 15u) / 16u, p.blocksK = (a.k + 127u) / 128u;
     p.perGroup = a.group / 128u < p.blocksK ? a.group / 128u : p.blocksK; // (a group longer than k)
     p.groupMagic = p.perGroup > 1u ? static_cast<uint32_t>(((1ull << 32) + p.perGroup - 1u) / p.perGroup) : 0u;
