@@ -41,7 +41,8 @@ class AttentionLayer:
         return rows, packed, scales
 
     def reserve(self, total_tokens, max_tokens, max_kv, batch, table_stride):
-        """The buffers of steps of up to that size, kept for all of them."""
+        """The buffers of steps of up to that size, kept for all of them: tokens in all, drafted tokens of a sequence, cached positions of one (those of the
+        step among them), sequences and entries of a row of the table."""
         import torch
 
         import rocwmma_amd as R
@@ -50,16 +51,32 @@ class AttentionLayer:
         self.qkv = empty(total_tokens, self.qkv_heads, self.head_dim)
         self.q, self.attended = empty(total_tokens, self.heads, self.head_dim), empty(total_tokens, self.heads, self.head_dim)
         self.y = empty(total_tokens, self.hidden)
-        self.max_tokens, self.max_kv = max_tokens, max_kv
+        self.total_tokens, self.batch, self.max_tokens, self.max_kv = total_tokens, batch, max_tokens, max_kv
         sizes = R.tree_attention_args(self.dtype, batch, total_tokens, self.heads, self.kv_heads, self.head_dim, None, None, None, None, None,
                                       self.page_size, self.pages, None, None, max_tokens, max_kv, table_stride=table_stride)
         self.workspace = empty(max(R.tree_attention_workspace_bytes(sizes), 16), dtype=torch.uint8)
 
+    def _holds(self, x, positions, slots, table, q_start, kv_len, mask):
+        """ValueError unless the step is one that the buffers of reserve() and the kernels' strides were made for"""
+        tokens, batch = x.shape[0], table.shape[0]
+        if tokens > self.total_tokens or batch > self.batch:
+            raise ValueError("step: %d tokens of %d sequences, reserved are %d of %d" % (tokens, batch, self.total_tokens, self.batch))
+        if tuple(x.shape) != (tokens, self.hidden) or x.dtype != self.torch_type or not x.is_contiguous():
+            raise ValueError("step: x must be contiguous rows of %d %s, got %s of %s" % (self.hidden, self.torch_type, tuple(x.shape), x.dtype))
+        if positions.numel() != tokens or slots.numel() != tokens:
+            raise ValueError("step: %d tokens, but %d positions and %d slots" % (tokens, positions.numel(), slots.numel()))
+        if q_start.numel() <= batch or kv_len.numel() < batch:
+            raise ValueError("step: %d sequences, but q_start has %d elements and kv_len %d" % (batch, q_start.numel(), kv_len.numel()))
+        if mask is not None and (mask.dim() != 2 or mask.shape[0] < tokens):
+            raise ValueError("step: the mask needs a row of words for each of the %d tokens, got %s" % (tokens, tuple(mask.shape)))
+
     def step(self, x, positions, slots, table, q_start, kv_len, mask=None, stream=None):
         """x [tokens][hidden] -> x + attention(x) W_o^T.  positions, slots: of every token, its place in the sequence and in the cache; table, q_start,
-        kv_len (which counts the tokens of this step), mask: as of tree_attention()."""
+        kv_len (which counts the tokens of this step), mask: as of tree_attention().  What q_start and kv_len hold stays in device memory and is not looked at here:
+        a sequence has at most reserve()'s max_tokens of the step's tokens and max_kv positions (of one with more, the rows of the result mean nothing)."""
         import rocwmma_amd as R
 
+        self._holds(x, positions, slots, table, q_start, kv_len, mask)
         tokens, batch, d, f = x.shape[0], table.shape[0], self.head_dim, self.qkv_heads * self.head_dim
         R.w4_matmul(self.dtype, self.dtype, tokens, f, self.hidden, self.group, x, self.wqkv[1], self.wqkv[2], self.qkv, stream=stream)
         keys, values = self.qkv[:, self.heads:], self.qkv[:, self.heads + self.kv_heads:]
