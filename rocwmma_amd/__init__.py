@@ -392,8 +392,8 @@ def rope_turns(rotary_dim, base=10000.0, factor=1.0, original_length=0, slow=1.0
 
 
 def rope_part(x, y, heads, x_strides, y_strides, rotate=True, to_slots=False):
-    """One of up to three tensors of a rope() call; strides: (token, head) in elements."""
-    return (_ptr(x) or 0, _ptr(y) or 0, heads, rotate, to_slots, 0, x_strides[0], x_strides[1], y_strides[0], y_strides[1])
+    """One of up to three tensors of a rope() call; strides: (token, head) in elements.  The part holds x and y themselves as well, so that they live until the call."""
+    return (_ptr(x) or 0, _ptr(y) or 0, heads, rotate, to_slots, 0, x_strides[0], x_strides[1], y_strides[0], y_strides[1], x, y)
 
 
 def rope(dtype, layout, tokens, head_dim, rotary_dim, parts, positions, turns, scale=1.0, inverse=False, slots=None, slot_count=0, stream=None):
@@ -403,7 +403,7 @@ def rope(dtype, layout, tokens, head_dim, rotary_dim, parts, positions, turns, s
     if not 1 <= n <= 3:
         raise ValueError("rope: 1 to 3 parts, got %d" % n)
     p0, p1, p2 = (*parts, _NO_ROPE_PART, _NO_ROPE_PART)[:3]
-    a = _ROPE_ARGS.pack(dtype, layout, tokens, head_dim, rotary_dim, n, *p0, *p1, *p2, _ptr(positions) or 0, _ptr(turns) or 0, _ptr(slots) or 0, slot_count,
+    a = _ROPE_ARGS.pack(dtype, layout, tokens, head_dim, rotary_dim, n, *p0[:10], *p1[:10], *p2[:10], _ptr(positions) or 0, _ptr(turns) or 0, _ptr(slots) or 0, slot_count,
                         inverse, scale)
     _check(lib().r355_rope(a, _stream_handle(stream)))
 
