@@ -206,6 +206,39 @@ def _ptr(t):
         return t if isinstance(t, int) else t.ctypes.data
 
 
+_WHOLE_BYTES = {}  # bytes of the whole numbers of a type: dtype -> 1, 2, 4 or 8 (0: not whole numbers)
+
+
+def _whole_bytes(dtype):
+    if dtype not in _WHOLE_BYTES:
+        whole = dtype.kind in "iu" if hasattr(dtype, "kind") else not (dtype.is_floating_point or dtype.is_complex or str(dtype) == "torch.bool")
+        _WHOLE_BYTES[dtype] = dtype.itemsize if whole else 0
+    return _WHOLE_BYTES[dtype]
+
+
+def _index(name, t, size, count):
+    """Address of `count` whole numbers of `size` bytes that a kernel reads one after the other (a raw address is taken as it is).  A tensor of other ones (torch makes 64-bit
+    ones unless told otherwise), with gaps, too short or out of the GPU's reach raises: read as what it is not it would give other positions and slots, without an error."""
+    if t is None:
+        return None
+    try:
+        if _WHOLE_BYTES[t.dtype] == size and t.is_cuda and t.is_contiguous() and t.numel() >= count:
+            return t.data_ptr()
+    except (AttributeError, KeyError):
+        pass
+    if not hasattr(t, "dtype"):
+        return t
+    if _whole_bytes(t.dtype) != size:
+        raise ValueError("%s must hold whole numbers of %d bits, got %s" % (name, 8 * size, t.dtype))
+    if not hasattr(t, "is_cuda") or not (t.is_cuda or t.is_pinned()):
+        raise ValueError("%s must lie in device memory or in pinned host memory" % name)
+    if not t.is_contiguous():
+        raise ValueError("%s must be contiguous, got strides %s" % (name, t.stride()))
+    if t.numel() < count:
+        raise ValueError("%s has %d elements, %d are needed" % (name, t.numel(), count))
+    return t.data_ptr()
+
+
 def _stream_handle(stream):
     if stream is None:
         return None
@@ -376,7 +409,7 @@ def w4_pack(q, n, k, packed, ldq=None, stream=None):
 def w4_matmul(in_type, out_type, tokens, n, k, group, x, w, scales, y, zeros=None, c=None, alpha=1.0, beta=0.0, ldx=None, ldc=None,
               ldy=None, stream=None):
     """y = alpha * x W^T + beta * c for packed 4-bit W (n x k) with scales (and zero points; default 8) per `group` of k."""
-    a = W4Args(in_type, out_type, tokens, n, k, group, _ptr(x), _ptr(w), _ptr(scales), _ptr(zeros), _ptr(c), _ptr(y),
+    a = W4Args(in_type, out_type, tokens, n, k, group, _ptr(x), _ptr(w), _ptr(scales), _index("w4_matmul: zeros", zeros, 1, -(-k // group) * n if group else 0), _ptr(c), _ptr(y),
                k if ldx is None else ldx, n if ldc is None else ldc, n if ldy is None else ldy, alpha, beta)
     _check(lib().r355_w4_matmul(ctypes.byref(a), _stream_handle(stream)))
 
@@ -403,9 +436,39 @@ def rope(dtype, layout, tokens, head_dim, rotary_dim, parts, positions, turns, s
     if not 1 <= n <= 3:
         raise ValueError("rope: 1 to 3 parts, got %d" % n)
     p0, p1, p2 = (*parts, _NO_ROPE_PART, _NO_ROPE_PART)[:3]
-    a = _ROPE_ARGS.pack(dtype, layout, tokens, head_dim, rotary_dim, n, *p0[:10], *p1[:10], *p2[:10], _ptr(positions) or 0, _ptr(turns) or 0, _ptr(slots) or 0, slot_count,
-                        inverse, scale)
+    a = _ROPE_ARGS.pack(dtype, layout, tokens, head_dim, rotary_dim, n, *p0[:10], *p1[:10], *p2[:10], _index("rope: positions", positions, 4, tokens) or 0,
+                        _index("rope: turns", turns, 8, rotary_dim // 2) or 0, _index("rope: slots", slots, 4, tokens) or 0, slot_count, inverse, scale)
     _check(lib().r355_rope(a, _stream_handle(stream)))
+
+
+def _row_stride(table, max_kv, page_size):
+    """Elements between the rows of a table of pages, which may be a slice of a wider one; of one whose rows are too short for max_kv positions their
+    length (which is refused as that)."""
+    pages = table.shape[1]
+    if not hasattr(table, "stride") or table.is_contiguous() or table.shape[0] <= 1 or pages * page_size < max_kv:
+        return pages
+    return table.stride(0)
+
+
+def _table(table, batch, stride, page_size, max_kv):
+    """_index() of a table of pages: of all of it, or of the first row of a slice of a wider one"""
+    if batch == 0 or stride * page_size < max_kv:  # (rows that are too short are refused as that)
+        return
+    pages = -(-max_kv // page_size) if page_size else 0
+    try:
+        if _WHOLE_BYTES[table.dtype] == 4 and table.is_cuda and table.is_contiguous() and table.numel() >= (batch - 1) * stride + pages:
+            return
+    except (AttributeError, KeyError):
+        pass
+    if not hasattr(table, "dtype"):
+        return
+    rows = table.shape[0] if table.ndim == 2 else batch
+    if rows < batch:
+        raise ValueError("tree_attention: the table has %d rows, %d are needed" % (rows, batch))
+    if table.ndim == 2 and hasattr(table, "stride") and not table.is_contiguous():
+        _index("tree_attention: a row of the table", table[0], 4, pages)
+    else:
+        _index("tree_attention: the table", table, 4, (batch - 1) * stride + pages)
 
 
 def tree_attention_args(dtype, batch, total_tokens, heads, kv_heads, head_dim, q, k, v, out, table, page_size, pages, q_start, kv_len, max_tokens,
@@ -417,7 +480,7 @@ def tree_attention_args(dtype, batch, total_tokens, heads, kv_heads, head_dim, q
         workspace_bytes = workspace.numel() * workspace.element_size() if hasattr(workspace, "numel") else 0
     return TreeAttentionArgs(
         dtype, batch, total_tokens, heads, kv_heads, head_dim, max_tokens, max_kv, _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse),
-        qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os_[0], os_[1], _ptr(table), table.shape[1] if table_stride is None else table_stride,
+        qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os_[0], os_[1], _ptr(table), _row_stride(table, max_kv, page_size) if table_stride is None else table_stride,
         page_size, pages, _ptr(q_start), _ptr(kv_len), _ptr(mask), mask_words, head_dim ** -0.5 if scale is None else scale,
         _ptr(workspace), workspace_bytes)
 
@@ -428,6 +491,10 @@ def tree_attention(dtype, batch, total_tokens, heads, kv_heads, head_dim, q, k, 
     1 / sqrt(head_dim); strides: q_strides, k_strides, v_strides, out_strides as (token or slot, head) in elements, table_stride."""
     a = tree_attention_args(dtype, batch, total_tokens, heads, kv_heads, head_dim, q, k, v, out, table, page_size, pages, q_start, kv_len,
                             max_tokens, max_kv, mask, mask_words, lse, scale, workspace, **strides)
+    _index("tree_attention: q_start", q_start, 4, batch + 1)
+    _index("tree_attention: kv_len", kv_len, 4, batch)
+    _index("tree_attention: the mask", mask, 8, total_tokens * mask_words)
+    _table(table, batch, a.table_stride, page_size, max_kv)
     _check(lib().r355_tree_attention(ctypes.byref(a), _stream_handle(stream)))
 
 
