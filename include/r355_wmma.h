@@ -350,7 +350,9 @@ int r355_rope_turns(uint32_t rotary_dim, double base, double factor, uint32_t or
  * table[b * table_stride + p / page_size] * page_size + p % page_size.  A page outside [0, pages) reads as zeros.
  * Query head h uses key head h / (heads / kv_heads).  head_dim: a multiple of 8 up to 256; page_size: a multiple of 16; type: R355_F16 or R355_BF16
  * for q, k, v and out.  Scores, softmax and sums are f32; the weights are rounded to `type` for the product with v.
- * Strides of q, k and v: multiples of 8 elements, those of slots head_dim to 2^25; of out: of 4.  scale: finite.  Up to 65535 sequences.
+ * Strides of q, k and v: multiples of 8 elements, those of slots head_dim to 2^25; of out: of 4.  scale: finite.
+ * Up to 65535 sequences, 2^30 positions and 2^30 rows (max_tokens times the query heads of a key head) of a sequence; batch * kv_heads, rounded up to a
+ * multiple of 8, times the tiles of 64 rows (32 / 8 heads: of 16 tokens) up to 2^23 - 4.
  * max_tokens and max_kv: bounds of what q_start and kv_len hold (device memory, not read by the host): what lies beyond is left out.
  * workspace (16-byte aligned, contents irrelevant): with it the positions of a sequence are split over workgroups where there are few,
  * up to what r355_tree_attention_workspace_bytes asks for; with less, fewer.  Calls that overlap need one each.  The result depends on

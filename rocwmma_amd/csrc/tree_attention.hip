@@ -892,6 +892,17 @@ namespace
         return plan;
     }
 
+    // shares times key heads, a multiple of the XCDs (the row tiles of a share on one of them)
+    uint64_t columnsOf(const r355_tree_attention_args& a, const Plan& plan)
+    {
+        return ((uint64_t)plan.shares * a.kv_heads + 7u) / 8u * 8u;
+    }
+    // of a workgroup: eight waves on 256 rows, with heads over 128 on 128; else four
+    uint32_t threadsOf(const r355_tree_attention_args& a, const Plan& plan)
+    {
+        return plan.rowsPerGroup == 256u || (a.head_dim > 128u && plan.rowsPerGroup == 128u) ? 512u : 256u;
+    }
+
     template <typename T, uint32_t D, uint32_t WQ, uint32_t QB>
     void launchTree(const TreeParams& p, const Plan& plan, hipStream_t s)
     {
@@ -920,7 +931,7 @@ namespace
                 launchTree<T, D, 4, 2>(p, plan, s);
             else
                 launchTree<T, D, 8, 2>(p, plan, s);
-            if(plan.shares > p.batch)
+            if(plan.shares > p.batch) // (planOf: batch * kv_heads * row tiles of up to 256 rows are fewer than four times the CUs then)
             {
                 const uint32_t rows = p.maxTokens * p.heads;
                 if((uint64_t)p.batch * rows <= 2048u)
@@ -959,9 +970,16 @@ namespace
             return r355::fail(R355_ERR_BAD_SIZE, "tree_attention: rows of %u pages hold fewer than max_kv=%u positions", a.table_stride, a.max_kv);
         if((uint64_t)a.max_tokens * (a.heads / a.kv_heads) > 0x40000000u)
             return r355::fail(R355_ERR_BAD_SIZE, "tree_attention: max_tokens=%u times %u heads per key head is over 2^30", a.max_tokens, a.heads / a.kv_heads);
-        const uint64_t groups = ((uint64_t)a.batch * a.kv_heads + 8192u) * (((uint64_t)a.max_tokens * (a.heads / a.kv_heads) + 15u) / 16u);
-        if(groups > r355::MAX_GROUPS / 2u || a.batch > 65535u || (uint64_t)a.max_tokens * a.heads >= r355::MAX_GROUPS)
-            return r355::fail(R355_ERR_BAD_SIZE, "tree_attention: too many sequences, heads and drafted tokens for one launch");
+        if(a.batch > 65535u)
+            return r355::fail(R355_ERR_BAD_SIZE, "tree_attention: batch=%u is over 65535", a.batch);
+        if(a.batch == 0 || a.total_tokens == 0 || a.max_tokens == 0)
+            return R355_OK;
+        // (the most workgroups that there can be: those with all of the workspace asked for)
+        const Plan     plan   = planOf(a, ~0ull);
+        const uint64_t groups = columnsOf(a, plan) * plan.rowTiles;
+        if(groups * (threadsOf(a, plan) / 256u) > r355::MAX_GROUPS)
+            return r355::fail(R355_ERR_BAD_SIZE, "tree_attention: %llu workgroups of %u threads for the sequences, heads and drafted tokens are too many for one launch",
+                              (unsigned long long)groups, threadsOf(a, plan));
         return R355_OK;
     }
 } // namespace
@@ -1015,7 +1033,7 @@ extern "C" int r355_tree_attention(const r355_tree_attention_args* args, void* s
     p.batch = a.batch, p.heads = a.heads, p.kvHeads = a.kv_heads, p.group = a.heads / a.kv_heads, p.dim = a.head_dim;
     p.totalTokens = a.total_tokens, p.maxTokens = a.max_tokens, p.maxKv = a.max_kv;
     p.pageSize = a.page_size, p.pages = a.pages, p.tableStride = a.table_stride, p.maskWords = a.mask_words;
-    p.shares = plan.shares, p.columns = (plan.shares * a.kv_heads + 7u) / 8u * 8u; // (the row tiles of a share on one XCD)
+    p.shares = plan.shares, p.columns = static_cast<uint32_t>(columnsOf(a, plan));
     p.scale2 = std::fmax(static_cast<float>(std::fabs(a.scale) * 1.4426950408889634), 1.17549435e-38f);
     p.signs  = a.scale < 0.0 ? 0x80008000u : 0u;
     const hipStream_t s = static_cast<hipStream_t>(stream);
