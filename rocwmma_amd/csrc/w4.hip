@@ -556,34 +556,53 @@ namespace
     }
 
     constexpr uint32_t MOST_ROWS = 1u << 24, MOST_TOKENS = 1u << 19, MOST_K = 1u << 22;
+    constexpr uint64_t MOST_RESULTS = 1ull << 34;
 
-    // workgroups: a multiple of eight, every XCD a stretch of the tiles
-    dim3 gridOf(W4Params& p, uint32_t rows, uint32_t tokens)
+    // most workgroups of a launch, a multiple of the XCDs (they have up to 512 threads, and the threads of a launch are counted in 32 bits)
+    constexpr uint32_t MOST_GROUPS = r355::MAX_GROUPS / 16u * 8u;
+
+    // Calls launch(parameters, workgroups) for tiles of rows x tokens, every XCD a stretch of them; several times, each with some of the tokens, where a
+    // launch does not hold them all.
+    template <typename F>
+    void inLaunches(const W4Params& whole, uint32_t rows, uint32_t tokens, F&& launch)
     {
-        p.tilesN = (p.n + rows - 1u) / rows, p.tilesT = (p.tokens + tokens - 1u) / tokens;
-        p.perXcd = (p.tilesN * p.tilesT + 7u) / 8u;
-        return dim3(p.perXcd * 8u);
+        const uint64_t outBytes = whole.outF32 ? 4u : 2u;
+        W4Params       p        = whole;
+        p.tilesN                = (p.n + rows - 1u) / rows;
+        const uint32_t most     = MOST_GROUPS / p.tilesN * tokens; // (tilesN: 2^20 at most)
+        for(uint32_t first = 0; first < whole.tokens; first += p.tokens)
+        {
+            p.tokens = whole.tokens - first < most ? whole.tokens - first : most;
+            p.x      = whole.x + (uint64_t)first * p.ldx * 2u;
+            p.y      = whole.y + (uint64_t)first * p.ldy * outBytes;
+            p.c      = whole.c ? whole.c + (uint64_t)first * p.ldc * outBytes : nullptr;
+            p.tilesT = (p.tokens + tokens - 1u) / tokens;
+            p.perXcd = (p.tilesN * p.tilesT + 7u) / 8u;
+            launch(p, dim3(p.perXcd * 8u));
+        }
     }
 
     template <typename T, uint32_t RB, uint32_t CB, uint32_t DEPTH, uint32_t STEPS, bool FAST>
-    void launchFew(W4Params& p, hipStream_t s)
+    void launchFew(const W4Params& whole, hipStream_t s)
     {
-        const uint32_t waves = p.blocksK >= 8u ? 8u : p.blocksK >= 4u ? 4u : 1u;
-        const dim3     grid  = gridOf(p, 16u * RB, 16u * CB);
-        if(p.zeros)
-            hipLaunchKernelGGL((w4Kernel<T, RB, CB, DEPTH, STEPS, true, FAST>), grid, dim3(waves * 64u), waves * RB * CB * 1024u, s, p);
-        else
-            hipLaunchKernelGGL((w4Kernel<T, RB, CB, DEPTH, STEPS, false, FAST>), grid, dim3(waves * 64u), waves * RB * CB * 1024u, s, p);
+        const uint32_t waves = whole.blocksK >= 8u ? 8u : whole.blocksK >= 4u ? 4u : 1u;
+        inLaunches(whole, 16u * RB, 16u * CB, [&](const W4Params& p, dim3 grid) {
+            if(p.zeros)
+                hipLaunchKernelGGL((w4Kernel<T, RB, CB, DEPTH, STEPS, true, FAST>), grid, dim3(waves * 64u), waves * RB * CB * 1024u, s, p);
+            else
+                hipLaunchKernelGGL((w4Kernel<T, RB, CB, DEPTH, STEPS, false, FAST>), grid, dim3(waves * 64u), waves * RB * CB * 1024u, s, p);
+        });
     }
 
     template <typename T, uint32_t RB, uint32_t CB, uint32_t WN, uint32_t WT, uint32_t WK, uint32_t STEPS>
-    void launchRing(W4Params& p, hipStream_t s)
+    void launchRing(const W4Params& whole, hipStream_t s)
     {
-        const dim3 grid = gridOf(p, 16u * RB * WN, 16u * CB * WT);
-        if(p.zeros)
-            hipLaunchKernelGGL((w4RingKernel<T, RB, CB, WN, WT, WK, STEPS, true>), grid, dim3(64u * WN * WT * WK), 0, s, p);
-        else
-            hipLaunchKernelGGL((w4RingKernel<T, RB, CB, WN, WT, WK, STEPS, false>), grid, dim3(64u * WN * WT * WK), 0, s, p);
+        inLaunches(whole, 16u * RB * WN, 16u * CB * WT, [&](const W4Params& p, dim3 grid) {
+            if(p.zeros)
+                hipLaunchKernelGGL((w4RingKernel<T, RB, CB, WN, WT, WK, STEPS, true>), grid, dim3(64u * WN * WT * WK), 0, s, p);
+            else
+                hipLaunchKernelGGL((w4RingKernel<T, RB, CB, WN, WT, WK, STEPS, false>), grid, dim3(64u * WN * WT * WK), 0, s, p);
+        });
     }
 
     // The kernels that are launched, with what a workgroup of each takes for a block of 128 k while it has its CU to itself (hundredths of
@@ -620,7 +639,7 @@ namespace
     }
 
     template <typename T, uint32_t STEPS>
-    void launchSteps(W4Params& p, bool fast, hipStream_t s)
+    void launchSteps(const W4Params& p, bool fast, hipStream_t s)
     {
         if(!fast)
             return launchFew<T, 1, 2, 1, STEPS, false>(p, s);
@@ -647,7 +666,7 @@ namespace
     }
 
     template <typename T>
-    void launchType(W4Params& p, bool fast, hipStream_t s)
+    void launchType(const W4Params& p, bool fast, hipStream_t s)
     {
         if(p.group == 32u)
             launchSteps<T, 1>(p, fast, s);
@@ -697,8 +716,8 @@ extern "C" int r355_w4_matmul(const r355_w4_args* args, void* stream)
         return r355::fail(R355_ERR_BAD_SIZE, "w4_matmul: at most %u rows, %u tokens and %u columns, got %u, %u and %u", MOST_ROWS, MOST_TOKENS, MOST_K, a.n, a.tokens, a.k);
     if(a.group != 32u && a.group != 64u && (a.group == 0u || a.group % 128u))
         return r355::fail(R355_ERR_BAD_SIZE, "w4_matmul: group=%u must be 32, 64 or a multiple of 128", a.group);
-    if(((uint64_t)a.n + 15u) / 16u * (((uint64_t)a.tokens + 15u) / 16u) > r355::MAX_GROUPS / 4u)
-        return r355::fail(R355_ERR_BAD_SIZE, "w4_matmul: too many blocks of 16 rows x 16 tokens for one launch");
+    if((uint64_t)a.n * a.tokens >= MOST_RESULTS)
+        return r355::fail(R355_ERR_BAD_SIZE, "w4_matmul: n=%u times tokens=%u are 2^34 results and more", a.n, a.tokens);
     if(a.tokens == 0)
         return R355_OK;
     if(!a.x || !a.w || !a.scales || !a.y || (a.beta != 0.0 && !a.c))
