@@ -343,9 +343,8 @@ int r355_rope_turns(uint32_t rotary_dim, double base, double factor, uint32_t or
  * Sequence b has the rows q_start[b] .. q_start[b + 1] of q (its drafted tokens, their keys and values being the last rows of its cache) and
  * kv_len[b] cached positions, the drafted among them.  A row sees every position before the drafted ones and, of those, the tokens whose bit is
  * set in its row of `mask` (bit j % 64 of word j / 64: token j of the same sequence; as a rule its ancestors and itself); with mask = NULL those
- * up to itself: one token, or a chunk of a prompt.  What a row does not see does not count, whatever the cache holds there (but where a row does see an infinity
- * or a NaN in v, elements of it may become NaN by those of positions nearby that it does not see).  A row that sees nothing gives zeros, and
- * lse = -infinity.
+ * up to itself: one token, or a chunk of a prompt.  What a row does not see does not count, whatever the cache holds there.  An infinity or a NaN in v makes
+ * that element of the rows that give its position a weight an infinity or a NaN, and no other.  A row that sees nothing gives zeros, and lse = -infinity.
  * k, v: [pages * page_size slots][kv_heads][head_dim] by strides; position p of sequence b lies in slot
  * table[b * table_stride + p / page_size] * page_size + p % page_size.  A page outside [0, pages) reads as zeros.
  * Query head h uses key head h / (heads / kv_heads).  head_dim: a multiple of 8 up to 256; page_size: a multiple of 16; type: R355_F16 or R355_BF16

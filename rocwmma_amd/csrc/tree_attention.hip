@@ -227,6 +227,15 @@ namespace
         constexpr uint32_t EXPONENT = std::is_same_v<T, __bf16> ? 0x7F807F80u : 0x7C007C00u, ULP = std::is_same_v<T, __bf16> ? 0x00800080u : 0x04000400u;
         return (((v & EXPONENT) + ULP) >> 15) & 0x00010001u;
     }
+    // ... 1 in each half whose mantissa is not zero
+    template <typename T>
+    __device__ __forceinline__ uint32_t mantissaHalves(uint32_t v)
+    {
+        constexpr uint32_t MANTISSA = std::is_same_v<T, __bf16> ? 0x007F007Fu : 0x03FF03FFu, BITS = std::is_same_v<T, __bf16> ? 7u : 10u;
+        return (((v & MANTISSA) + MANTISSA) >> BITS) & 0x00010001u;
+    }
+    template <typename T>
+    constexpr uint32_t ONE = std::is_same_v<T, __bf16> ? 0x3F80u : 0x3C00u;
     // calls f with the integral constants 0 .. N - 1
     template <uint32_t N, typename F>
     __device__ __forceinline__ void each(F&& f)
@@ -494,8 +503,8 @@ namespace
                     return c;
                 }
             };
-            // A position that a row does not see has weight 0, and 0 times an infinity or a NaN is a NaN.  Where the tile holds one, the rows that give it no
-            // weight take the product with zeros in the place of all of them.
+            // A position that a row does not see has weight 0, and 0 times an infinity or a NaN is a NaN.  Where the tile holds one, the product is made with zeros in
+            // their place; two more, with ones in the place of each sign's (a NaN: of both) and zeros elsewhere, are more than 0 where a row gives one a weight.
             if(masked)
             {
                 uint32_t found = 0u;
@@ -507,58 +516,36 @@ namespace
                 }
                 if(__any(found != 0u))
                 {
-                    u32x2 bad[PB]; // of the lane's positions, over all d
-#pragma unroll
-                    for(uint32_t n = 0; n < PB; ++n)
-                        bad[n] = u32x2{0u, 0u};
 #pragma unroll
                     for(uint32_t d = 0; d < D / 16u; ++d)
                     {
-                        u32x2 x[PB];
-                        if constexpr(TIGHT)
-                            __builtin_amdgcn_sched_barrier(0);
-                        v(d, x);
 #pragma unroll
-                        for(uint32_t n = 0; n < PB; ++n)
-                            bad[n] |= u32x2{unfitHalves<T>(x[n][0]), unfitHalves<T>(x[n][1])};
-                    }
-                    bool hit[QB];
-#pragma unroll
-                    for(uint32_t a = 0; a < QB; ++a)
-                        hit[a] = false;
-#pragma unroll
-                    for(uint32_t n = 0; n < PB; ++n)
-#pragma unroll
-                        for(uint32_t w = 0; w < 2u; ++w)
+                        for(uint32_t of = 0; of < 3u; ++of) // the numbers, the positive ones, the negative ones
                         {
-                            uint32_t all = bad[n][w];
+                            u32x2 x[PB];
+                            asm volatile("" ::: "memory"); // (read again each time: kept, they would not fit)
+                            if constexpr(TIGHT)
+                                __builtin_amdgcn_sched_barrier(0);
+                            v(d, x);
 #pragma unroll
-                            for(uint32_t x = 1u; x < 16u; x *= 2u)
-                                all |= __shfl_xor(all, x);
+                            for(uint32_t n = 0; n < PB; ++n)
+#pragma unroll
+                                for(uint32_t w = 0; w < 2u; ++w)
+                                {
+                                    const uint32_t was = x[n][w], unfit = unfitHalves<T>(was);
+                                    x[n][w] = of == 0u ? was & ~(unfit * 0xFFFFu) : (unfit & ((of == 1u ? ~was : was) >> 15 | mantissaHalves<T>(was))) * ONE<T>;
+                                }
 #pragma unroll
                             for(uint32_t a = 0; a < QB; ++a)
-                                hit[a] = hit[a] || (pf[a][n][w] & (all * 0x7FFFu)) != 0u; // (a weight in each half)
-                        }
+                                if(of == 0u)
+                                    o[a][d] = times(x, a, o[a][d]);
+                                else
+                                {
+                                    const f32x4 seen = times(x, a, f32x4{0, 0, 0, 0});
 #pragma unroll
-                    for(uint32_t a = 0; a < QB; ++a)
-                        hit[a] = maxOverQuads(hit[a] ? 1.0f : 0.0f) != 0.0f;
-#pragma unroll
-                    for(uint32_t d = 0; d < D / 16u; ++d)
-                    {
-                        u32x2 as[PB], fit[PB];
-                        if constexpr(TIGHT)
-                            __builtin_amdgcn_sched_barrier(0);
-                        v(d, as);
-#pragma unroll
-                        for(uint32_t n = 0; n < PB; ++n)
-                            fit[n] = u32x2{as[n][0] & ~(unfitHalves<T>(as[n][0]) * 0xFFFFu), as[n][1] & ~(unfitHalves<T>(as[n][1]) * 0xFFFFu)};
-#pragma unroll
-                        for(uint32_t a = 0; a < QB; ++a)
-                        {
-                            const f32x4 seen = times(as, a, o[a][d]), unseen = times(fit, a, o[a][d]);
-#pragma unroll
-                            for(uint32_t e = 0; e < 4u; ++e)
-                                o[a][d][e] = hit[a] ? seen[e] : unseen[e];
+                                    for(uint32_t e = 0; e < 4u; ++e)
+                                        o[a][d][e] += seen[e] > 0.0f ? of == 1u ? INFINITY : -INFINITY : 0.0f;
+                                }
                         }
                     }
                     return;
