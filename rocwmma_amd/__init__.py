@@ -84,7 +84,7 @@ class W4Args(ctypes.Structure):
 # r355_rope_args as bytes: a structure of 42 fields takes 2 us longer to make, a quarter of a call for a few tokens.  Sizes and strides; per part: x, y, heads, rotate,
 # to_slots, padding, strides of x and of y; then positions, turns, slots, slot_count, inverse, scale.
 _ROPE_ARGS = struct.Struct("=iiIIII" + 3 * "QQIiiiqqqq" + "QQQIid")
-_NO_ROPE_PART = (0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+_NO_ROPE_PART = (0, 0, 0, 0, 0, 0, 0, 0, 0, 0), None, None
 
 
 class TreeAttentionArgs(ctypes.Structure):
@@ -101,6 +101,10 @@ class TreeAttentionArgs(ctypes.Structure):
         ("q_start", ctypes.c_void_p), ("kv_len", ctypes.c_void_p), ("mask", ctypes.c_void_p), ("mask_words", ctypes.c_uint32),
         ("scale", ctypes.c_double), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64),
     ]
+
+
+# ... the same for a call of the attention: packed and copied it takes half the time.  (Each address of an array is followed by its numbers, those by padding.)
+_TREE_ARGS = struct.Struct("=iIIIIIIIQQQQQqqqqqqqqQIIIiQQQIidQQ")
 
 
 class DeviceInfo(ctypes.Structure):
@@ -409,7 +413,9 @@ def w4_pack(q, n, k, packed, ldq=None, stream=None):
 def w4_matmul(in_type, out_type, tokens, n, k, group, x, w, scales, y, zeros=None, c=None, alpha=1.0, beta=0.0, ldx=None, ldc=None,
               ldy=None, stream=None):
     """y = alpha * x W^T + beta * c for packed 4-bit W (n x k) with scales (and zero points; default 8) per `group` of k."""
-    a = W4Args(in_type, out_type, tokens, n, k, group, _ptr(x), _ptr(w), _ptr(scales), _index("w4_matmul: zeros", zeros, 1, -(-k // group) * n if group else 0), _ptr(c), _ptr(y),
+    if zeros is not None:
+        zeros = _index("w4_matmul: zeros", zeros, 1, -(-k // group) * n if group else 0)
+    a = W4Args(in_type, out_type, tokens, n, k, group, _ptr(x), _ptr(w), _ptr(scales), zeros, _ptr(c), _ptr(y),
                k if ldx is None else ldx, n if ldc is None else ldc, n if ldy is None else ldy, alpha, beta)
     _check(lib().r355_w4_matmul(ctypes.byref(a), _stream_handle(stream)))
 
@@ -426,7 +432,11 @@ def rope_turns(rotary_dim, base=10000.0, factor=1.0, original_length=0, slow=1.0
 
 def rope_part(x, y, heads, x_strides, y_strides, rotate=True, to_slots=False):
     """One of up to three tensors of a rope() call; strides: (token, head) in elements.  The part holds x and y themselves as well, so that they live until the call."""
-    return (_ptr(x) or 0, _ptr(y) or 0, heads, rotate, to_slots, 0, x_strides[0], x_strides[1], y_strides[0], y_strides[1], x, y)
+    try:
+        at, to = x.data_ptr(), y.data_ptr()
+    except AttributeError:
+        at, to = _ptr(x) or 0, _ptr(y) or 0
+    return (at, to, heads, rotate, to_slots, 0, x_strides[0], x_strides[1], y_strides[0], y_strides[1]), x, y
 
 
 def rope(dtype, layout, tokens, head_dim, rotary_dim, parts, positions, turns, scale=1.0, inverse=False, slots=None, slot_count=0, stream=None):
@@ -435,10 +445,12 @@ def rope(dtype, layout, tokens, head_dim, rotary_dim, parts, positions, turns, s
     n = len(parts)
     if not 1 <= n <= 3:
         raise ValueError("rope: 1 to 3 parts, got %d" % n)
-    p0, p1, p2 = (*parts, _NO_ROPE_PART, _NO_ROPE_PART)[:3]
-    a = _ROPE_ARGS.pack(dtype, layout, tokens, head_dim, rotary_dim, n, *p0[:10], *p1[:10], *p2[:10], _index("rope: positions", positions, 4, tokens) or 0,
+    (p0, _, _), (p1, _, _), (p2, _, _) = parts if n == 3 else (*parts, _NO_ROPE_PART, _NO_ROPE_PART)[:3]
+    a = _ROPE_ARGS.pack(dtype, layout, tokens, head_dim, rotary_dim, n, *p0, *p1, *p2, _index("rope: positions", positions, 4, tokens) or 0,
                         _index("rope: turns", turns, 8, rotary_dim // 2) or 0, _index("rope: slots", slots, 4, tokens) or 0, slot_count, inverse, scale)
-    _check(lib().r355_rope(a, _stream_handle(stream)))
+    rc = lib().r355_rope(a, None if stream is None else _stream_handle(stream))
+    if rc != 0:
+        _check(rc)
 
 
 def _row_stride(table, max_kv, page_size):
@@ -453,49 +465,58 @@ def _row_stride(table, max_kv, page_size):
 def _table(table, batch, stride, page_size, max_kv):
     """_index() of a table of pages: of all of it, or of the first row of a slice of a wider one"""
     if batch == 0 or stride * page_size < max_kv:  # (rows that are too short are refused as that)
-        return
+        return _ptr(table)
     pages = -(-max_kv // page_size) if page_size else 0
     try:
         if _WHOLE_BYTES[table.dtype] == 4 and table.is_cuda and table.is_contiguous() and table.numel() >= (batch - 1) * stride + pages:
-            return
+            return table.data_ptr()
     except (AttributeError, KeyError):
         pass
     if not hasattr(table, "dtype"):
-        return
+        return table
     rows = table.shape[0] if table.ndim == 2 else batch
     if rows < batch:
         raise ValueError("tree_attention: the table has %d rows, %d are needed" % (rows, batch))
     if table.ndim == 2 and hasattr(table, "stride") and not table.is_contiguous():
-        _index("tree_attention: a row of the table", table[0], 4, pages)
-    else:
-        _index("tree_attention: the table", table, 4, (batch - 1) * stride + pages)
+        return _index("tree_attention: a row of the table", table[0], 4, pages)
+    return _index("tree_attention: the table", table, 4, (batch - 1) * stride + pages)
 
 
 def tree_attention_args(dtype, batch, total_tokens, heads, kv_heads, head_dim, q, k, v, out, table, page_size, pages, q_start, kv_len, max_tokens,
                         max_kv, mask=None, mask_words=0, lse=None, scale=None, workspace=None, workspace_bytes=None, q_strides=None,
                         k_strides=None, v_strides=None, out_strides=None, table_stride=None):
+    return _tree_args(dtype, batch, total_tokens, heads, kv_heads, head_dim, q, k, v, out, _ptr(table), page_size, pages, _ptr(q_start), _ptr(kv_len), max_tokens, max_kv,
+                      _ptr(mask), mask_words, lse, scale, workspace, workspace_bytes, q_strides, k_strides, v_strides, out_strides,
+                      _row_stride(table, max_kv, page_size) if table_stride is None else table_stride)
+
+
+def _tree_args(dtype, batch, total_tokens, heads, kv_heads, head_dim, q, k, v, out, table, page_size, pages, q_start, kv_len, max_tokens, max_kv, mask, mask_words, lse, scale,
+               workspace, workspace_bytes, q_strides, k_strides, v_strides, out_strides, table_stride):
+    """(table, q_start, kv_len and mask: addresses)"""
     row, slot = (heads * head_dim, head_dim), (kv_heads * head_dim, head_dim)
     qs, ks, vs, os_ = q_strides or row, k_strides or slot, v_strides or slot, out_strides or row
     if workspace_bytes is None:
         workspace_bytes = workspace.numel() * workspace.element_size() if hasattr(workspace, "numel") else 0
-    return TreeAttentionArgs(
-        dtype, batch, total_tokens, heads, kv_heads, head_dim, max_tokens, max_kv, _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse),
-        qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os_[0], os_[1], _ptr(table), _row_stride(table, max_kv, page_size) if table_stride is None else table_stride,
-        page_size, pages, _ptr(q_start), _ptr(kv_len), _ptr(mask), mask_words, head_dim ** -0.5 if scale is None else scale,
-        _ptr(workspace), workspace_bytes)
+    return TreeAttentionArgs.from_buffer_copy(_TREE_ARGS.pack(
+        dtype, batch, total_tokens, heads, kv_heads, head_dim, max_tokens, max_kv, _ptr(q) or 0, _ptr(k) or 0, _ptr(v) or 0, _ptr(out) or 0, _ptr(lse) or 0,
+        qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os_[0], os_[1], table or 0, table_stride, page_size, pages, 0, q_start or 0, kv_len or 0, mask or 0, mask_words, 0,
+        head_dim ** -0.5 if scale is None else scale, _ptr(workspace) or 0, workspace_bytes))
 
 
 def tree_attention(dtype, batch, total_tokens, heads, kv_heads, head_dim, q, k, v, out, table, page_size, pages, q_start, kv_len, max_tokens,
-                   max_kv, mask=None, mask_words=0, lse=None, scale=None, workspace=None, stream=None, **strides):
+                   max_kv, mask=None, mask_words=0, lse=None, scale=None, workspace=None, stream=None, workspace_bytes=None, q_strides=None, k_strides=None, v_strides=None,
+                   out_strides=None, table_stride=None):
     """Attention of the drafted tokens of `batch` sequences over a paged cache (include/r355_wmma.h).  scale: default
     1 / sqrt(head_dim); strides: q_strides, k_strides, v_strides, out_strides as (token or slot, head) in elements, table_stride."""
-    a = tree_attention_args(dtype, batch, total_tokens, heads, kv_heads, head_dim, q, k, v, out, table, page_size, pages, q_start, kv_len,
-                            max_tokens, max_kv, mask, mask_words, lse, scale, workspace, **strides)
-    _index("tree_attention: q_start", q_start, 4, batch + 1)
-    _index("tree_attention: kv_len", kv_len, 4, batch)
-    _index("tree_attention: the mask", mask, 8, total_tokens * mask_words)
-    _table(table, batch, a.table_stride, page_size, max_kv)
-    _check(lib().r355_tree_attention(ctypes.byref(a), _stream_handle(stream)))
+    if table_stride is None:
+        table_stride = _row_stride(table, max_kv, page_size)
+    a = _tree_args(dtype, batch, total_tokens, heads, kv_heads, head_dim, q, k, v, out, _table(table, batch, table_stride, page_size, max_kv), page_size, pages,
+                   _index("tree_attention: q_start", q_start, 4, batch + 1), _index("tree_attention: kv_len", kv_len, 4, batch), max_tokens, max_kv,
+                   _index("tree_attention: the mask", mask, 8, total_tokens * mask_words), mask_words, lse, scale, workspace, workspace_bytes, q_strides, k_strides,
+                   v_strides, out_strides, table_stride)
+    rc = lib().r355_tree_attention(ctypes.byref(a), None if stream is None else _stream_handle(stream))
+    if rc != 0:
+        _check(rc)
 
 
 def tree_attention_workspace_bytes(a):
