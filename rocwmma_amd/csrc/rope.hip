@@ -251,6 +251,8 @@ extern "C" int r355_rope(const r355_rope_args* args, void* stream)
         return R355_OK;
     if(!a.positions)
         return r355::fail(R355_ERR_BAD_ARG, "rope: null positions");
+    if(!r355::aligned(a.positions, 4) || !r355::aligned(a.slots, 4))
+        return r355::fail(R355_ERR_MISALIGNED, "rope: positions and slots need 4-byte alignment");
     p.positions = a.positions, p.turns = a.turns, p.slots = a.slots;
     p.tokens = a.tokens, p.headDim = a.head_dim, p.half = a.rotary_dim / 2u, p.slotCount = a.slot_count;
     p.inverse = a.inverse != 0, p.scale = static_cast<float>(a.scale);

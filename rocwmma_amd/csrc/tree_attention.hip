@@ -1000,6 +1000,8 @@ extern "C" int r355_tree_attention(const r355_tree_attention_args* args, void* s
         return r355::fail(R355_ERR_MISALIGNED, "tree_attention: q, k and v need 16-byte alignment, out 8-byte alignment");
     if(!std::isfinite(static_cast<float>(a.scale)))
         return r355::fail(R355_ERR_BAD_ARG, "tree_attention: the scale must be finite");
+    if(!r355::aligned(a.table, 4) || !r355::aligned(a.q_start, 4) || !r355::aligned(a.kv_len, 4))
+        return r355::fail(R355_ERR_MISALIGNED, "tree_attention: table, q_start and kv_len need 4-byte alignment");
     if(a.lse && !r355::aligned(a.lse, 4))
         return r355::fail(R355_ERR_MISALIGNED, "tree_attention: lse needs 4-byte alignment");
     if(a.mask && !r355::aligned(a.mask, 8))
