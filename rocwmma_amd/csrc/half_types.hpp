@@ -1,8 +1,9 @@
-// 16-bit element types of the decoding kernels (w4.hip, rope.hip, tree_attention.hip): vectors, conversions, matrix instructions.
+// 16-bit element types of the decoding kernels (w4.hip, rope.hip, tree_attention.hip): vectors, conversions, matrix instructions; loops over constants.
 #ifndef R355_HALF_TYPES_HPP
 #define R355_HALF_TYPES_HPP
 
 #include <cstdint>
+#include <type_traits>
 
 #include <hip/hip_runtime.h>
 
@@ -41,6 +42,17 @@ namespace r355
     __device__ __forceinline__ uint32_t pack2(float lo, float hi)
     {
         return __builtin_bit_cast(uint32_t, vec<T, 2>{static_cast<T>(lo), static_cast<T>(hi)});
+    }
+
+    // calls f with the integral constants 0 .. N - 1
+    template <uint32_t N, typename F>
+    __device__ __forceinline__ void each(F&& f)
+    {
+        if constexpr(N > 0u)
+        {
+            each<N - 1u>(f);
+            f(std::integral_constant<uint32_t, N - 1u>{});
+        }
     }
 } // namespace r355
 

@@ -29,6 +29,7 @@
 
 namespace
 {
+    using r355::each;
     using r355::f32x4;
     using r355::u32x2;
     using r355::u32x4;
@@ -236,16 +237,6 @@ namespace
     }
     template <typename T>
     constexpr uint32_t ONE = std::is_same_v<T, __bf16> ? 0x3F80u : 0x3C00u;
-    // calls f with the integral constants 0 .. N - 1
-    template <uint32_t N, typename F>
-    __device__ __forceinline__ void each(F&& f)
-    {
-        if constexpr(N > 0u)
-        {
-            each<N - 1u>(f);
-            f(std::integral_constant<uint32_t, N - 1u>{});
-        }
-    }
 
     __device__ __forceinline__ float maxOverQuads(float x)
     {

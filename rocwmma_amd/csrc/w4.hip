@@ -22,6 +22,7 @@
 
 namespace
 {
+    using r355::each;
     using r355::f32x4;
     using r355::u32x2;
     using r355::u32x4;
@@ -99,17 +100,6 @@ namespace
     __device__ __forceinline__ uint32_t groupOf(const W4Params& p, uint32_t kb)
     {
         return STEPS < 4u ? kb * (4u / STEPS) : p.perGroup == 1u ? kb : __umulhi(kb, p.groupMagic);
-    }
-
-    // calls f with the integral constants 0 .. N - 1
-    template <uint32_t N, typename F>
-    __device__ __forceinline__ void each(F&& f)
-    {
-        if constexpr(N > 0u)
-        {
-            each<N - 1u>(f);
-            f(std::integral_constant<uint32_t, N - 1u>{});
-        }
     }
 
     // One group (STEPS matrix instructions of 32 k): acc += s (sum x (16 + q) - (16 + z) sum x).  x is the first operand: a lane holds four tokens of one
