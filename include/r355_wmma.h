@@ -274,7 +274,8 @@ int r355_decompress_24_16(const uint16_t* values, const uint8_t* meta, uint32_t 
  * scales: [ceil(k / group)][n] of in_type; zeros: the same shape in bytes of 0..15, or NULL for 8 everywhere.  group: 32, 64 or a multiple
  * of 128.  out_type: in_type or R355_F32 (c and y).  Sums and scaling are f32; y is rounded once.  c may be y; it is not read, and may
  * be NULL, where beta is 0.  Up to 2^24 rows, 2^22 k and 2^19 tokens (0: nothing is done), fewer than 2^34 results, and any size within these; x, c and
- * y of any leading dimension and alignment of an element, fastest with rows of x on 16-byte boundaries and n, ldc and ldy multiples of 4.
+ * y of any leading dimension and alignment of an element, fastest with rows of x on 16-byte boundaries and n, ldc and ldy multiples of 4.  (Rows of x off
+ * them, or k no multiple of 8, take about three times as long for one token and 25 times for 1000: many tokens are worth a copy.)
  * Inside, a sum over a group is the difference of two that are about five times as large: where x (16 + q) summed over a group passes the
  * range of f32, or x holds an infinity, the result is a NaN.
  */

@@ -17,7 +17,9 @@
 //
 // What bounds it, 32 / 8 heads of 128: with single tokens the bytes of the cache (32 tokens over 820 .. 8192 positions: 124 us, 4.9 TB/s), with a
 // short cache two launches and the first reads' latency (one token over 700: 11.7 us); with 64 tokens over 65600 positions the matrix and vector
-// instructions under the power limit (two sequences: 155 us, 665 TFLOP/s; their bytes alone are 94 us).
+// instructions under the power limit (two sequences: 152 us, 675 TFLOP/s; their bytes alone are 62 us at the rate of reads).  A chunk of a prompt takes the
+// time of all its positions: every tile of rows goes over those after its last token too, masked (2048 tokens after 6144: 429 us, 561 TFLOP/s of what is seen;
+// 8192 without a prefix: 2109 us, 261).
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -480,6 +482,9 @@ namespace
                         s[a][n][j] = __builtin_amdgcn_exp2f(fmaf(s[a][n][j], p.scale2, -base));
                         sum[a] += s[a][n][j];
                     }
+                    // (Rounded to 16 bits, as the second operand of the product with V has to be: at most what the rounding of the result is, and averaged over the
+                    // positions.  Relative error of results in all, against 64 bits, 32 tokens over 820 .. 8192 positions: bf16 0.0020, of which the result's own
+                    // rounding is 0.0017; f16 0.00025 and 0.00021.  The sum takes them unrounded, so lse has none of it.)
                     pf[a][n][0] = r355::pack2<T>(s[a][n][0], s[a][n][1]), pf[a][n][1] = r355::pack2<T>(s[a][n][2], s[a][n][3]);
                 }
             }
@@ -846,18 +851,24 @@ namespace
         Plan           plan;
         // 16 and 32 rows: all four waves on positions; 64 and 128: on rows (64 rows, 4 x 16 tokens over 16000, 32 / 8 heads of 128: 50 us, with the waves on positions 133).
         plan.rowsPerGroup = rows <= 16u ? 16u : rows <= 32u && a.head_dim <= 128u ? 32u : a.head_dim <= 128u ? (rows <= 64u ? 64u : 128u) : 64u;
-        // A cache that the memory-side cache does not hold is read by one workgroup of eight waves instead of two of four, which drift apart further than
-        // an XCD's L2 reaches (2 x 64 tokens over 65600, 32 / 8 heads of 128: 890 instead of 450 MB past the L2, 180 and 163 us)
+        // More than 128 rows over a cache that the memory-side cache does not hold: one workgroup of eight waves reads it instead of two of four, which drift apart further than
+        // an XCD's L2 reaches (2 x 64 tokens over 65600, 32 / 8 heads of 128: 890 instead of 450 MB past the L2, 180 and 163 us).  (Heads over 128 have tiles of 64 rows on
+        // four waves and would gain from 65 rows on: 4 x 17 .. 32 tokens over 32768, 16 / 4 heads of 256: 193 .. 205 and 129 .. 137 us; 8 x 17 over up to 16000, 32 / 8
+        // of 192: 196 and 170.)
         if(rows > 128u && cache >= 192ull << 20)
             plan.rowsPerGroup = a.head_dim <= 128u ? 256u : 128u;
         plan.rowTiles         = static_cast<uint32_t>((rows + plan.rowsPerGroup - 1u) / plan.rowsPerGroup);
         const uint64_t groups = (uint64_t)a.kv_heads * plan.rowTiles; // workgroups of a share
         // Workgroups a CU that are aimed at.  Eight waves: one (1 x 64 tokens over 65600, 32 / 8 heads of 128: 100 us, two 127).  Waves on positions, of which a CU holds
         // one workgroup: one, where that makes eight shares of a sequence and more, so that the last share of each, which is shorter, weighs little (one token, 32 / 8 heads of 128:
-        // 1 x 16000 18.8 us, two 23.7, four 23.7; 4 x 16000 56, 61, 64; 8 tokens, 1 x 65536: 59, 66, 81).  Else, with one tile of rows: two, and four for
-        // single tokens with heads of 128, whose workgroups are the shortest (32 x 1 token over 820 .. 8192 positions: one 134 us, two 145, four 124, eight 141).
-        // Several tiles, of which shorter sequences have fewer: four (8 trees of up to 48 tokens over 4099, 24 / 4 heads of 64: two 34 us, three 33, four 25),
-        // three of heads of 256 (4 x 64 tokens over 8000: two 69 us, three 60, four 74).
+        // 1 x 16000 18.8 us, two 23.7, four 23.7; 4 x 16000 56, 61, 64; 8 tokens, 1 x 65536: 59, 66, 81).  With more sequences the lengths decide, which are not known here.
+        // Of 8 to 100 sequences of up to 2048 and 8192 positions, all equal, evenly spread or a few eight times as long as the rest, as many as a CU takes
+        // over the best of one to eight, mean and most, single tokens: 32 / 8 heads of 128 one 1.09 and 1.81, two 1.10 and 1.53, four 1.11 and 1.51; 16 / 4 of 128
+        // 1.07 and 2.28, 1.11 and 1.44, 1.14 and 1.52; 32 / 8 of 64 1.05 and 1.63, 1.12 and 1.63, 1.15 and 1.62; 16 / 2 of 256 1.06 and 1.92, 1.09 and 1.36, 1.12 and 1.45.  So
+        // not one, which leaves the longest sequence to run by itself, though with lengths that are near each other it is the best (8 x 8192 evenly spread, 32 / 8 heads of 128:
+        // 34, 37, 42 us; 32 x 820 .. 8192: 134, 145, 122): two, and four for single tokens with heads of 128, which differ by 3 % in the mean.
+        // Several tiles, of which shorter sequences have fewer: four (8 trees of up to 48 tokens over 4099, 24 / 4 heads of 64: two 34 us, three 33, four 25; 4 x 64 tokens over
+        // 2500 .. 8000, 16 / 4 of 64: 29 each; of 128: two 38, three 49, four 48), three of heads of 256 (4 x 64 tokens over 8000: two 69 us, three 60, four 74).
         const bool     eight  = plan.rowsPerGroup == 256u || (a.head_dim > 128u && plan.rowsPerGroup == 128u);
         const bool     one    = eight || (plan.rowsPerGroup <= 32u && (a.batch == 1u || a.batch * 8u <= cus / groups));
         const uint64_t target = one ? 1u : rows <= 16u && a.head_dim > 64u && a.head_dim <= 128u ? 4u : plan.rowTiles == 1u ? 2u : a.head_dim > 128u ? 3u : 4u;

@@ -215,10 +215,11 @@ namespace
         return tileN < p.tilesN;
     }
 
-    // ---- A few tokens, or rows of x off 16-byte boundaries (FAST false).  A workgroup's waves share 16 RB rows x 16 CB tokens and take the 128-k blocks in
+    // ---- A few tokens, or rows of x off 16-byte boundaries (FAST false: element by element, one tile for any number of tokens; 8192 x 4096, groups of 64, with rows 4097 apart
+    // 1 token 14.5 us instead of 5.4, 24 tokens 48 instead of 8.1, 1000 tokens 2040 instead of 81).  A workgroup's waves share 16 RB rows x 16 CB tokens and take the 128-k blocks in
     // turn, x and the weights straight from global memory; their sums meet in LDS in the order of the waves, so the result does not depend on
     // scheduling.  STEPS: matrix instructions (32 k) per scale.  DEPTH blocks in flight, each in registers of its own.
-    // Bound by the bytes of the weights from one wide row of workgroups on (16384 x 8192, groups of 128 with zero points, one token: 14.2 us, 4.95 TB/s of
+    // Bound by the bytes of the weights from one wide row of workgroups on (16384 x 8192, groups of 128 with zero points, one token: 14.4 us, 4.9 TB/s of
     // weights, scales and zero points), below that by one load's latency and the launch (1024 x 2048: 5.6 us); with more tokens by x out of the L2 and, with small groups,
     // the vector instructions that make operands and apply scales (10250 x 4168, groups of 32, 24 tokens: 13.1 us in one round of 214 workgroups).  No LDS: no other wave reads the same weights.
     template <typename T, uint32_t RB, uint32_t CB, uint32_t DEPTH, uint32_t STEPS, bool ZEROS, bool FAST>
@@ -361,7 +362,8 @@ namespace
     // row: a wave reads 16 rows at one place), the weights as they are packed, a wave's scales and zero points one to a dword.  (Loads into registers among the
     // direct ones would have the compiler wait for all of them.)
     // Bound by the vector instructions that make operands, once per tile of tokens, and by LDS reads beside the matrix instructions: 8192 x 4096, groups of 64,
-    // 1000 tokens, residual added: 87 us, 771 TFLOP/s (a library product of the same size, weights made 16 bits beforehand and not counted: some 1200).
+    // 1000 tokens, residual added: 85 us, 785 TFLOP/s (a product of the same size with weights made 16 bits beforehand, not counted: 57 us, 1180, in the vendor's
+    // library and, 992 tokens, in this one's GEMM).
     __device__ __forceinline__ void loadShortToLds(r355::dma_i32x4 rsrc, uint32_t laneOffset, uint32_t ldsAddr)
     {
         asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_ushort %0, %1, 0 offen lds" : : "v"(laneOffset), "s"(rsrc), "s"(ldsAddr) : "memory");
