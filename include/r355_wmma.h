@@ -382,6 +382,83 @@ typedef struct
 int    r355_tree_attention(const r355_tree_attention_args* args, void* stream);
 size_t r355_tree_attention_workspace_bytes(const r355_tree_attention_args* args);
 
+/*
+ * ---- The feed-forward half of a layer: products with an epilogue and their gradients, for one matrix of weights or one per group of rows (an expert's tokens),
+ * the router that makes the groups, and the rows' way there and back.  No counterpart in the reference.
+ */
+typedef enum
+{
+    R355_ACT_NONE      = 0,
+    R355_ACT_RELU      = 1,
+    R355_ACT_GELU      = 2, /* z (1 + erf(z / sqrt 2)) / 2 */
+    R355_ACT_GELU_TANH = 3, /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
+    R355_ACT_SILU      = 4  /* z / (1 + exp(-z)) */
+} r355_activation;
+
+/*
+ * z = x W^T + bias;  y = act(z) * gate + c.  x: [rows][k], w: [groups][n][k], bias: [groups][n], gate, z: [rows][n] of in_type (R355_F16 or R355_BF16); c, y: [rows][n] of
+ * out_type (in_type or R355_F32).  bias, gate, c and z (written) may be NULL.  Sums and the epilogue are f32; z and y are rounded once each, y from what z was rounded from.
+ * groups = 1, offsets = NULL: one matrix of weights.  Otherwise rows offsets[e] .. offsets[e + 1] - 1 use weights and bias of group e; offsets is device memory, not read by the host;
+ * rows in no group are left as they were, and what offsets holds beyond the rows is cut off.  (A slice of the offsets with w from its first group on: some of the experts.)
+ * source (device memory, or NULL): row r is row source[r] of x, which has x_rows of them; a number that is none of them reads as zeros.
+ * c may be y.  Any sizes up to 2^30 rows, n and k of 2^22 - 8 and 1024 groups; any leading dimension and alignment of an element, fastest (several times) with rows of x and w on
+ * 16-byte boundaries and k a multiple of 8; then with n a multiple of 8 and the other rows on 16-byte boundaries.  With source, x_rows times ldx up to 2^31 bytes.
+ * workspace (16-byte aligned, contents irrelevant): with it the sum is split over workgroups where the result has few tiles; r355_linear_workspace_bytes says how much is made use of.
+ * Calls that overlap need one each.  The result depends on the sizes and the workspace offered, not on scheduling.
+ */
+typedef struct
+{
+    int32_t        in_type, out_type, activation;
+    uint32_t       rows, n, k, groups, x_rows;
+    const void*    x;
+    const void*    w;
+    const void*    bias;
+    const void*    gate;
+    const void*    c;
+    void*          y;
+    void*          z;
+    const int32_t* offsets; /* [groups + 1], or NULL */
+    const int32_t* source;  /* [rows], or NULL */
+    uint32_t       ldx, ldw, ldg, ldc, ldy, ldz; /* elements */
+    int64_t        w_stride;                     /* elements from one group's weights to the next's */
+    void*          workspace;
+    uint64_t       workspace_bytes;
+} r355_linear_args;
+int    r355_linear(const r355_linear_args* args, void* stream);
+size_t r355_linear_workspace_bytes(const r355_linear_args* args);
+
+/*
+ * The gradients of r355_linear for dy = dL / dy [rows][n]:
+ *   dz = dy * gate * act'(z);  dgate = dy * act(z);  dx = dz W;  dw = dz^T x;  dbias = sum of dz over a group's rows      (of c: dy itself)
+ * z: as the forward call wrote it; gate, z: NULL where there is none or no activation.  dgate, dx, dw, dbias: NULL where not wanted.  dz (in_type, written) is needed with an
+ * activation or a gate; without either dz is dy.  It is rounded to in_type for the two products; dbias (f32) is summed before that rounding.  dw: grad_type (in_type
+ * or R355_F32), [groups][n][k]; of a group without rows zeros.  accumulate: dw and dbias are added to what is there.  All else is of in_type.
+ * x and dx are by rows, as dy is (rows taken by source: their gradient is the sum over the rows that took them, r355_combine).  Groups, sizes and strides as above; fastest with
+ * rows on 16-byte boundaries and, for dx, n a multiple of 8.  workspace: as above, and for the shares of dbias.
+ */
+typedef struct
+{
+    int32_t        in_type, grad_type, activation, accumulate;
+    uint32_t       rows, n, k, groups;
+    const void*    dy;
+    const void*    x;
+    const void*    w;
+    const void*    z;
+    const void*    gate;
+    void*          dz;
+    void*          dgate;
+    void*          dx;
+    void*          dw;
+    float*         dbias; /* [groups][n] */
+    const int32_t* offsets;
+    uint32_t       lddy, ldx, ldw, ldz, ldg, lddz, lddg, lddx, lddw;
+    int64_t        w_stride, dw_stride;
+    void*          workspace;
+    uint64_t       workspace_bytes;
+} r355_linear_backward_args;
+int    r355_linear_backward(const r355_linear_backward_args* args, void* stream);
+size_t r355_linear_backward_workspace_bytes(const r355_linear_backward_args* args);
+
 /* Device facts used by the roofline report (test/hip_device.hpp:101-119 in the reference). */
 typedef struct
 {

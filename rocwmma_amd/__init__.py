@@ -28,12 +28,16 @@ DLRM_KERNEL_SPECIALISED, DLRM_KERNEL_BLOCK_PER_WAVE, DLRM_KERNEL_REGISTER_BLOCKE
 # r355_rope_layout
 ROPE_HALF, ROPE_INTERLEAVED = 0, 1
 
+# r355_activation
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = range(5)
+
 DTYPE_BYTES = {F16: 2, BF16: 2, E4M3: 1, I8: 1, F32: 4, I32: 4, F64: 8, E5M2: 1}
 
 EXPORTS = [
     "r355_gemm", "r355_gemm_noalloc", "r355_gemm_query", "r355_gemm_launch_plan", "r355_gemm_timed", "r355_dlrm_fwd", "r355_dlrm_fwd_timed",
     "r355_dlrm_bwd", "r355_dlrm_kernel", "r355_gemv", "r355_gemv_timed", "r355_dgemv", "r355_gemv_workspace_bytes", "r355_gemv_ws", "r355_dgemv_ws", "r355_compress_24", "r355_decompress_24", "r355_compress_24_16", "r355_decompress_24_16",
     "r355_w4_matmul", "r355_w4_packed_bytes", "r355_w4_pack", "r355_rope", "r355_rope_turns", "r355_tree_attention", "r355_tree_attention_workspace_bytes",
+    "r355_linear", "r355_linear_workspace_bytes", "r355_linear_backward", "r355_linear_backward_workspace_bytes",
     "r355_get_device_info", "r355_last_error", "r355_version",
 ]
 
@@ -107,6 +111,29 @@ class TreeAttentionArgs(ctypes.Structure):
 _TREE_ARGS = struct.Struct("=iIIIIIIIQQQQQqqqqqqqqQIIIiQQQIidQQ")
 
 
+class LinearArgs(ctypes.Structure):
+    _fields_ = [
+        ("in_type", ctypes.c_int32), ("out_type", ctypes.c_int32), ("activation", ctypes.c_int32),
+        ("rows", ctypes.c_uint32), ("n", ctypes.c_uint32), ("k", ctypes.c_uint32), ("groups", ctypes.c_uint32), ("x_rows", ctypes.c_uint32),
+        ("x", ctypes.c_void_p), ("w", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("gate", ctypes.c_void_p), ("c", ctypes.c_void_p),
+        ("y", ctypes.c_void_p), ("z", ctypes.c_void_p), ("offsets", ctypes.c_void_p), ("source", ctypes.c_void_p),
+        ("ldx", ctypes.c_uint32), ("ldw", ctypes.c_uint32), ("ldg", ctypes.c_uint32), ("ldc", ctypes.c_uint32), ("ldy", ctypes.c_uint32),
+        ("ldz", ctypes.c_uint32), ("w_stride", ctypes.c_int64), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64),
+    ]
+
+
+class LinearBackwardArgs(ctypes.Structure):
+    _fields_ = [
+        ("in_type", ctypes.c_int32), ("grad_type", ctypes.c_int32), ("activation", ctypes.c_int32), ("accumulate", ctypes.c_int32),
+        ("rows", ctypes.c_uint32), ("n", ctypes.c_uint32), ("k", ctypes.c_uint32), ("groups", ctypes.c_uint32),
+        ("dy", ctypes.c_void_p), ("x", ctypes.c_void_p), ("w", ctypes.c_void_p), ("z", ctypes.c_void_p), ("gate", ctypes.c_void_p),
+        ("dz", ctypes.c_void_p), ("dgate", ctypes.c_void_p), ("dx", ctypes.c_void_p), ("dw", ctypes.c_void_p), ("dbias", ctypes.c_void_p),
+        ("offsets", ctypes.c_void_p), ("lddy", ctypes.c_uint32), ("ldx", ctypes.c_uint32), ("ldw", ctypes.c_uint32), ("ldz", ctypes.c_uint32),
+        ("ldg", ctypes.c_uint32), ("lddz", ctypes.c_uint32), ("lddg", ctypes.c_uint32), ("lddx", ctypes.c_uint32), ("lddw", ctypes.c_uint32),
+        ("w_stride", ctypes.c_int64), ("dw_stride", ctypes.c_int64), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64),
+    ]
+
+
 class DeviceInfo(ctypes.Structure):
     _fields_ = [
         ("arch", ctypes.c_char * 64), ("compute_units", ctypes.c_int32), ("wave_size", ctypes.c_int32),
@@ -156,6 +183,10 @@ def lib():
         L.r355_rope_turns.argtypes = [u32, ctypes.c_double, ctypes.c_double, u32, ctypes.c_double, ctypes.c_double, vp]
         L.r355_tree_attention.argtypes = [ctypes.POINTER(TreeAttentionArgs), vp]
         L.r355_tree_attention_workspace_bytes.argtypes = [ctypes.POINTER(TreeAttentionArgs)]
+        L.r355_linear.argtypes = [ctypes.POINTER(LinearArgs), vp]
+        L.r355_linear_workspace_bytes.argtypes = [ctypes.POINTER(LinearArgs)]
+        L.r355_linear_backward.argtypes = [ctypes.POINTER(LinearBackwardArgs), vp]
+        L.r355_linear_backward_workspace_bytes.argtypes = [ctypes.POINTER(LinearBackwardArgs)]
         L.r355_get_device_info.argtypes = [ctypes.POINTER(DeviceInfo)]
         L.r355_last_error.argtypes = []
         L.r355_version.argtypes = []
@@ -164,7 +195,7 @@ def lib():
         for name in EXPORTS:
             if name not in ("r355_last_error", "r355_version"):
                 getattr(L, name).restype = ctypes.c_int
-        for name in ("r355_w4_packed_bytes", "r355_tree_attention_workspace_bytes"):
+        for name in ("r355_w4_packed_bytes", "r355_tree_attention_workspace_bytes", "r355_linear_workspace_bytes", "r355_linear_backward_workspace_bytes"):
             getattr(L, name).restype = ctypes.c_size_t
         _lib = L
     return _lib
@@ -522,6 +553,66 @@ def tree_attention(dtype, batch, total_tokens, heads, kv_heads, head_dim, q, k, 
 def tree_attention_workspace_bytes(a):
     """Bytes of workspace that r355_tree_attention makes use of for TreeAttentionArgs (0: none)."""
     return lib().r355_tree_attention_workspace_bytes(ctypes.byref(a))
+
+
+def _workspace(workspace, workspace_bytes):
+    """Address and bytes of a workspace"""
+    if workspace_bytes is None:
+        workspace_bytes = workspace.numel() * workspace.element_size() if hasattr(workspace, "numel") else 0
+    return _ptr(workspace), workspace_bytes
+
+
+def linear_args(in_type, out_type, rows, n, k, x, w, y, bias=None, activation=ACT_NONE, gate=None, c=None, z=None, groups=1, offsets=None, source=None, x_rows=None, ldx=None,
+                ldw=None, ldg=None, ldc=None, ldy=None, ldz=None, w_stride=None, workspace=None, workspace_bytes=None):
+    ldw = k if ldw is None else ldw
+    at, size = _workspace(workspace, workspace_bytes)
+    return LinearArgs(in_type, out_type, activation, rows, n, k, groups, rows if x_rows is None else x_rows, _ptr(x), _ptr(w), _ptr(bias), _ptr(gate), _ptr(c), _ptr(y), _ptr(z),
+                      _index("linear: offsets", offsets, 4, groups + 1), _index("linear: source", source, 4, rows), k if ldx is None else ldx, ldw, n if ldg is None else ldg,
+                      n if ldc is None else ldc, n if ldy is None else ldy, n if ldz is None else ldz, n * ldw if w_stride is None else w_stride, at, size)
+
+
+def linear(in_type, out_type, rows, n, k, x, w, y, bias=None, activation=ACT_NONE, gate=None, c=None, z=None, groups=1, offsets=None, source=None, x_rows=None, ldx=None,
+           ldw=None, ldg=None, ldc=None, ldy=None, ldz=None, w_stride=None, workspace=None, workspace_bytes=None, stream=None):
+    """y = activation(x W^T + bias) * gate + c for w [groups][n][k] (include/r355_wmma.h); rows offsets[e] .. offsets[e + 1] - 1 use group e, row r is row source[r] of x (of
+    x_rows; default: rows) where source is given.  z: where the activation's argument is kept for linear_backward()."""
+    a = linear_args(in_type, out_type, rows, n, k, x, w, y, bias, activation, gate, c, z, groups, offsets, source, x_rows, ldx, ldw, ldg, ldc, ldy, ldz, w_stride, workspace,
+                    workspace_bytes)
+    rc = lib().r355_linear(ctypes.byref(a), None if stream is None else _stream_handle(stream))
+    if rc != 0:
+        _check(rc)
+
+
+def linear_workspace_bytes(a):
+    """Bytes of workspace that r355_linear makes use of for LinearArgs (0: none)."""
+    return lib().r355_linear_workspace_bytes(ctypes.byref(a))
+
+
+def linear_backward_args(in_type, grad_type, rows, n, k, dy, x, w, dx=None, dw=None, dbias=None, z=None, activation=ACT_NONE, gate=None, dgate=None, dz=None, accumulate=False,
+                         groups=1, offsets=None, lddy=None, ldx=None, ldw=None, ldz=None, ldg=None, lddz=None, lddg=None, lddx=None, lddw=None, w_stride=None, dw_stride=None,
+                         workspace=None, workspace_bytes=None):
+    of_n, of_k = lambda ld: n if ld is None else ld, lambda ld: k if ld is None else ld  # noqa: E731
+    at, size = _workspace(workspace, workspace_bytes)
+    return LinearBackwardArgs(in_type, grad_type, activation, accumulate, rows, n, k, groups, _ptr(dy), _ptr(x), _ptr(w), _ptr(z), _ptr(gate), _ptr(dz), _ptr(dgate), _ptr(dx),
+                              _ptr(dw), _ptr(dbias), _index("linear_backward: offsets", offsets, 4, groups + 1), of_n(lddy), of_k(ldx), of_k(ldw), of_n(ldz), of_n(ldg),
+                              of_n(lddz), of_n(lddg), of_k(lddx), of_k(lddw), n * of_k(ldw) if w_stride is None else w_stride,
+                              n * of_k(lddw) if dw_stride is None else dw_stride, at, size)
+
+
+def linear_backward(in_type, grad_type, rows, n, k, dy, x, w, dx=None, dw=None, dbias=None, z=None, activation=ACT_NONE, gate=None, dgate=None, dz=None, accumulate=False,
+                    groups=1, offsets=None, lddy=None, ldx=None, ldw=None, ldz=None, ldg=None, lddz=None, lddg=None, lddx=None, lddw=None, w_stride=None, dw_stride=None,
+                    workspace=None, workspace_bytes=None, stream=None):
+    """The gradients of linear() for dy (include/r355_wmma.h): those of dx, dw (grad_type), dbias (f32) and dgate that are given.  z: what linear() kept; dz: room for the gradient
+    of that, needed with an activation or a gate; accumulate: dw and dbias are added to what is there."""
+    a = linear_backward_args(in_type, grad_type, rows, n, k, dy, x, w, dx, dw, dbias, z, activation, gate, dgate, dz, accumulate, groups, offsets, lddy, ldx, ldw, ldz, ldg, lddz,
+                             lddg, lddx, lddw, w_stride, dw_stride, workspace, workspace_bytes)
+    rc = lib().r355_linear_backward(ctypes.byref(a), None if stream is None else _stream_handle(stream))
+    if rc != 0:
+        _check(rc)
+
+
+def linear_backward_workspace_bytes(a):
+    """Bytes of workspace that r355_linear_backward makes use of for LinearBackwardArgs (0: none)."""
+    return lib().r355_linear_backward_workspace_bytes(ctypes.byref(a))
 
 
 def device_info():

@@ -1,0 +1,536 @@
+// Products of a layer with bias, activation, gate and residual, and their gradients, for one matrix of weights or one per group of rows: the entry points, the kernel
+// for few rows and what the gradient does element by element.  The macro tiles are in linear_tiles.hip.
+//
+//   forward    z = x W^T + b;  y = act(z) gate + c
+//   backward   dz = dy gate act'(z);  dgate = dy act(z);  dx = dz W;  dW = dz^T x;  db = sum of dz over the rows
+//
+// No counterpart in the reference.
+#include <hip/hip_runtime.h>
+
+#include <type_traits>
+
+#include "linear.hpp"
+
+namespace
+{
+    using r355::each;
+    using r355::f32x4;
+    using r355::GroupTile;
+    using r355::GroupTiles;
+    using r355::LinearParams;
+    using r355::OUTSIDE;
+    using r355::Rows;
+    using r355::u32x4;
+    using r355::vec;
+
+    constexpr uint32_t WAVES = 8u;
+
+    // ---- Few rows of each group.  A workgroup's eight waves share 16 RB weight rows x 16 CB rows of x and take pieces of 64 of the sum in turn, both
+    // straight from global memory; their sums meet in LDS in the order of the waves.  The weights are the first operand: a lane then holds four of them of one row of x.
+    template <typename T, uint32_t RB, uint32_t CB, uint32_t DEPTH>
+    __global__ void __launch_bounds__(64 * WAVES, 2) linearFew(LinearParams p)
+    {
+        constexpr uint32_t ROWS = 16u * CB, COLS = 16u * RB, PITCH = COLS + 4u;
+        __shared__ __attribute__((aligned(16))) float sums[WAVES * ROWS * PITCH];
+        GroupTiles<ROWS> tiles{p};
+        const uint32_t   tilesM = tiles.total(), count = tilesM * p.tilesN, perXcd = (count + 7u) / 8u;
+        // (a group's tiles of rows one after another on one XCD: they read the same weights)
+        const uint32_t id = blockIdx.x % 8u * perXcd + blockIdx.x / 8u;
+        if(blockIdx.x / 8u >= perXcd || id >= count)
+            return;
+        const uint32_t  tn = id / tilesM;
+        const GroupTile t  = tiles.at(id % tilesM);
+        const uint32_t  group = __builtin_amdgcn_readfirstlane(t.group), first = __builtin_amdgcn_readfirstlane(t.first), rows = __builtin_amdgcn_readfirstlane(t.count);
+        const uint32_t  lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15u, quad = lane >> 4;
+        const uint32_t  col0 = tn * COLS, cols = p.n - col0 < COLS ? p.n - col0 : COLS;
+
+        // (buffers that end with the last element; rows that are not there lie outside)
+        const auto bufW = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p.b) + (uint64_t)group * p.strideB + (uint64_t)col0 * p.ldb * 2u, 0,
+                                                            static_cast<int>(((cols - 1u) * p.ldb + p.k) * 2u), 0x00020000);
+        const auto bufX = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p.a) + (p.source ? 0u : (uint64_t)first * p.lda * 2u), 0,
+                                                            static_cast<int>(((p.source ? p.sourceRows : rows) - 1u) * p.lda * 2u + p.k * 2u), 0x00020000);
+        uint32_t offW[RB], offX[CB];
+#pragma unroll
+        for(uint32_t r = 0; r < RB; ++r)
+            offW[r] = r * 16u + r16 < cols ? (r * 16u + r16) * p.ldb * 2u + quad * 16u : OUTSIDE;
+#pragma unroll
+        for(uint32_t c = 0; c < CB; ++c)
+        {
+            const uint32_t row  = c * 16u + r16;
+            uint32_t       from = row;
+            bool           in   = row < rows;
+            if(in && p.source)
+            {
+                from = static_cast<uint32_t>(p.source[(uint64_t)first + row]);
+                in   = from < p.sourceRows;
+            }
+            offX[c] = in ? from * p.lda * 2u + quad * 16u : OUTSIDE;
+        }
+        f32x4 acc[RB][CB];
+#pragma unroll
+        for(uint32_t r = 0; r < RB; ++r)
+#pragma unroll
+            for(uint32_t c = 0; c < CB; ++c)
+                acc[r][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        struct Stage
+        {
+            u32x4 w[RB][2], x[CB][2];
+        };
+        const uint32_t pieces = (p.k + 63u) / 64u;
+        auto load = [&](uint32_t piece) __attribute__((always_inline)) {
+            Stage s;
+#pragma unroll
+            for(uint32_t i = 0; i < 2u; ++i)
+            {
+                const bool in = piece * 64u + i * 32u + quad * 8u < p.k; // (what lies past the sum's end is another row's)
+#pragma unroll
+                for(uint32_t r = 0; r < RB; ++r)
+                    s.w[r][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(bufW, in ? offW[r] + i * 64u : OUTSIDE, piece * 128u, 0));
+#pragma unroll
+                for(uint32_t c = 0; c < CB; ++c)
+                    s.x[c][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(bufX, in ? offX[c] + i * 64u : OUTSIDE, piece * 128u, 0));
+            }
+            return s;
+        };
+        Stage stage[DEPTH];
+        each<DEPTH>([&](auto at) __attribute__((always_inline)) {
+            constexpr uint32_t d = decltype(at)::value;
+            if(wave + d * WAVES < pieces)
+                stage[d] = load(wave + d * WAVES);
+        });
+        for(uint32_t from = wave; from < pieces; from += DEPTH * WAVES)
+            each<DEPTH>([&](auto at) __attribute__((always_inline)) {
+                constexpr uint32_t d     = decltype(at)::value;
+                const uint32_t     piece = from + d * WAVES;
+                if(piece < pieces)
+                {
+#pragma unroll
+                    for(uint32_t i = 0; i < 2u; ++i)
+#pragma unroll
+                        for(uint32_t r = 0; r < RB; ++r)
+#pragma unroll
+                            for(uint32_t c = 0; c < CB; ++c)
+                                acc[r][c] = r355::mfma32<T>(stage[d].w[r][i], stage[d].x[c][i], acc[r][c]);
+                    if(piece + DEPTH * WAVES < pieces)
+                        stage[d] = load(piece + DEPTH * WAVES);
+                }
+            });
+#pragma unroll
+        for(uint32_t c = 0; c < CB; ++c)
+#pragma unroll
+            for(uint32_t r = 0; r < RB; ++r)
+                *reinterpret_cast<f32x4*>(&sums[(wave * ROWS + c * 16u + r16) * PITCH + r * 16u + quad * 4u]) = acc[r][c];
+        __syncthreads();
+        for(uint32_t i = threadIdx.x; i < rows * COLS; i += 64u * WAVES)
+        {
+            const uint32_t row = i / COLS, col = i % COLS;
+            if(col >= cols)
+                continue;
+            float sum = 0.0f;
+#pragma unroll
+            for(uint32_t v = 0; v < WAVES; ++v)
+                sum += sums[(v * ROWS + row) * PITCH + col];
+            const uint64_t at = (uint64_t)first + row;
+            if(p.bias)
+                sum += static_cast<float>(reinterpret_cast<const T*>(p.bias)[(uint64_t)group * p.n + col0 + col]);
+            if(p.z)
+                reinterpret_cast<T*>(p.z)[at * p.ldz + col0 + col] = static_cast<T>(sum);
+            sum = r355::activate(p.activation, sum);
+            if(p.gate)
+                sum *= static_cast<float>(reinterpret_cast<const T*>(p.gate)[at * p.ldg + col0 + col]);
+            if(p.outF32)
+                reinterpret_cast<float*>(p.y)[at * p.ldy + col0 + col] = p.c ? sum + reinterpret_cast<const float*>(p.c)[at * p.ldc + col0 + col] : sum;
+            else
+                reinterpret_cast<T*>(p.y)[at * p.ldy + col0 + col] = static_cast<T>(p.c ? sum + static_cast<float>(reinterpret_cast<const T*>(p.c)[at * p.ldc + col0 + col]) : sum);
+        }
+    }
+
+    // ---- The gradient's part element by element: dz, dgate and the bias's gradient, one pass over dy, z and gate.
+    struct GradParams
+    {
+        const char*    dy;
+        const char*    z;
+        const char*    gate;
+        char*          dz;    // NULL: dz is dy
+        char*          dgate; // or NULL
+        float*         sums;  // [groups][parts][n]; parts = 1: the gradient itself; NULL: none
+        const int32_t* offsets;
+        uint32_t       rows, n, groups, parts;
+        uint32_t       lddy, ldz, ldg, lddz, lddg;
+        int32_t        activation, accumulate;
+    };
+
+    // A workgroup takes EW columns a lane and one of `parts` shares of a group's rows, its four waves every fourth of them.
+    template <typename T, uint32_t EW>
+    __global__ void __launch_bounds__(256) linearGrad(GradParams p)
+    {
+        __shared__ float meet[4][64 * EW];
+        LinearParams     rowsArg{};
+        rowsArg.offsets = p.offsets, rowsArg.rows = p.rows;
+        const uint32_t group = blockIdx.z, lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+        const Rows     all   = r355::rowsOf(rowsArg, group);
+        const uint32_t from = all.first + static_cast<uint32_t>((uint64_t)all.count * blockIdx.y / p.parts);
+        const uint32_t to   = all.first + static_cast<uint32_t>((uint64_t)all.count * (blockIdx.y + 1u) / p.parts);
+        const uint32_t col  = (blockIdx.x * 64u + lane) * EW;
+        using V             = vec<T, EW>;
+        float total[EW];
+#pragma unroll
+        for(uint32_t e = 0; e < EW; ++e)
+            total[e] = 0.0f;
+        auto read = [&](const char* base, uint64_t row, uint32_t ld, float (&v)[EW]) {
+            const T* at = reinterpret_cast<const T*>(base) + row * ld + col;
+            if constexpr(EW == 1u)
+                v[0] = static_cast<float>(*at);
+            else
+            {
+                const V w = *reinterpret_cast<const V*>(at);
+#pragma unroll
+                for(uint32_t e = 0; e < EW; ++e)
+                    v[e] = static_cast<float>(w[e]);
+            }
+        };
+        auto write = [&](char* base, uint64_t row, uint32_t ld, const float (&v)[EW]) {
+            T* at = reinterpret_cast<T*>(base) + row * ld + col;
+            if constexpr(EW == 1u)
+                *at = static_cast<T>(v[0]);
+            else
+            {
+                V w;
+#pragma unroll
+                for(uint32_t e = 0; e < EW; ++e)
+                    w[e] = static_cast<T>(v[e]);
+                *reinterpret_cast<V*>(at) = w;
+            }
+        };
+        if(col < p.n)
+#pragma unroll 2
+            for(uint32_t row = from + wave; row < to; row += 4u)
+            {
+                float d[EW];
+                read(p.dy, row, p.lddy, d);
+                if(p.dz)
+                {
+                    float z[EW], value[EW], slope[EW];
+                    if(p.z)
+                    {
+                        read(p.z, row, p.ldz, z);
+#pragma unroll
+                        for(uint32_t e = 0; e < EW; ++e)
+                            r355::activateBoth(p.activation, z[e], value[e], slope[e]);
+                    }
+                    else
+#pragma unroll
+                        for(uint32_t e = 0; e < EW; ++e)
+                            value[e] = 0.0f, slope[e] = 1.0f;
+                    if(p.dgate)
+                    {
+                        float g[EW];
+#pragma unroll
+                        for(uint32_t e = 0; e < EW; ++e)
+                            g[e] = d[e] * value[e];
+                        write(p.dgate, row, p.lddg, g);
+                    }
+                    if(p.gate)
+                    {
+                        float g[EW];
+                        read(p.gate, row, p.ldg, g);
+#pragma unroll
+                        for(uint32_t e = 0; e < EW; ++e)
+                            d[e] *= g[e];
+                    }
+#pragma unroll
+                    for(uint32_t e = 0; e < EW; ++e)
+                        d[e] = p.activation == R355_ACT_RELU && slope[e] == 0.0f ? 0.0f : d[e] * slope[e];
+                    write(p.dz, row, p.lddz, d);
+                }
+#pragma unroll
+                for(uint32_t e = 0; e < EW; ++e)
+                    total[e] += d[e];
+            }
+        if(!p.sums)
+            return;
+#pragma unroll
+        for(uint32_t e = 0; e < EW; ++e)
+            meet[wave][lane * EW + e] = total[e];
+        __syncthreads();
+        for(uint32_t i = threadIdx.x; i < 64u * EW; i += 256u)
+        {
+            const uint32_t c = blockIdx.x * 64u * EW + i;
+            if(c < p.n)
+            {
+                const float sum = ((meet[0][i] + meet[1][i]) + meet[2][i]) + meet[3][i];
+                float*      to_ = p.sums + ((uint64_t)group * p.parts + blockIdx.y) * p.n + c;
+                *to_            = p.parts == 1u && p.accumulate ? *to_ + sum : sum;
+            }
+        }
+    }
+
+    __global__ void __launch_bounds__(256) linearGradSums(const float* sums, float* dbias, uint32_t parts, uint32_t n, int32_t accumulate)
+    {
+        const uint32_t col = blockIdx.x * 256u + threadIdx.x;
+        if(col >= n)
+            return;
+        const float* from = sums + (uint64_t)blockIdx.y * parts * n + col;
+        float        sum  = 0.0f;
+        for(uint32_t s = 0; s < parts; ++s)
+            sum += from[(uint64_t)s * n];
+        float* to = dbias + (uint64_t)blockIdx.y * n + col;
+        *to       = accumulate ? *to + sum : sum;
+    }
+
+    constexpr uint32_t MOST_ROWS = 1u << 30, MOST_LENGTH = (1u << 22) - 8u, MOST_GROUPS = 1024u;
+
+    uint64_t tilesOf(uint64_t n, uint32_t edge)
+    {
+        return (n + edge - 1u) / edge;
+    }
+    // tiles of `edge` rows that any division of the rows into groups fits in
+    uint64_t mostTiles(const LinearParams& p, uint32_t edge)
+    {
+        if(!p.offsets)
+            return tilesOf(p.rows, edge);
+        const uint64_t most = p.rows / edge + p.groups;
+        return most < p.rows ? most : p.rows;
+    }
+
+    // Macro tile of a ragged product by the rows that a group has on average.
+    uint32_t tileEdge(const LinearParams& p, uint64_t rows, uint64_t cols, uint32_t groups)
+    {
+        const uint64_t perGroup = rows / groups;
+        for(uint32_t edge = 256u; edge > 64u; edge /= 2u)
+            if(perGroup >= edge * 3u / 4u && tilesOf(perGroup, edge) * groups * tilesOf(cols, edge) >= r355::computeUnits() * 3u / 4u)
+                return edge;
+        (void)p;
+        return 64u;
+    }
+
+    template <typename T>
+    void launchFew(LinearParams p, hipStream_t s)
+    {
+        p.tilesN             = static_cast<uint32_t>(tilesOf(p.n, 16u));
+        const uint64_t groups = (mostTiles(p, 16u) * p.tilesN + 7u) / 8u * 8u;
+        hipLaunchKernelGGL((linearFew<T, 1, 1, 4>), dim3(static_cast<uint32_t>(groups)), dim3(64 * WAVES), 0, s, p);
+    }
+
+    int tooMany(const char* what)
+    {
+        return r355::fail(R355_ERR_BAD_SIZE, "%s: more than 2^24 tiles of the result", what);
+    }
+
+    // one product on macro tiles; rowsY, colsY: of a group's result, on average
+    int launchTiles(int32_t type, LinearParams p, bool aK, bool bK, bool any, hipStream_t s, const char* what)
+    {
+        const uint32_t edge = any ? 64u : tileEdge(p, aK ? p.rows : (uint64_t)p.m * p.groups, p.n, p.groups);
+        p.tilesN = static_cast<uint32_t>(tilesOf(p.n, edge)), p.tilesM = static_cast<uint32_t>(tilesOf(p.m, edge));
+        const uint64_t tiles = (aK ? mostTiles(p, edge) : (uint64_t)p.tilesM * p.groups) * p.tilesN;
+        if(tiles > r355::MAX_GROUPS)
+            return tooMany(what);
+        const uint32_t workgroups = static_cast<uint32_t>((tiles + 7u) / 8u * 8u);
+        if(type == R355_F16)
+            r355::linearTilesF16(p, aK, bK, edge, any, workgroups, s);
+        else
+            r355::linearTilesBF16(p, aK, bK, edge, any, workgroups, s);
+        return R355_OK;
+    }
+
+    bool evenRows(const void* at, uint32_t ld, uint32_t bytes) // rows on 16-byte boundaries
+    {
+        return !at || (r355::aligned(at, 16) && (uint64_t)ld * bytes % 16u == 0u);
+    }
+
+    int checkCommon(const char* what, int32_t type, int32_t activation, uint32_t rows, uint32_t n, uint32_t k, uint32_t groups, const int32_t* offsets)
+    {
+        if(type != R355_F16 && type != R355_BF16)
+            return r355::fail(R355_ERR_UNSUPPORTED, "%s: operands are f16 or bf16", what);
+        if(activation < R355_ACT_NONE || activation > R355_ACT_SILU)
+            return r355::fail(R355_ERR_BAD_ARG, "%s: unknown activation %d", what, activation);
+        if(n == 0 || k == 0 || groups == 0)
+            return r355::fail(R355_ERR_BAD_ARG, "%s: n, k and groups must be non-zero", what);
+        if(rows > MOST_ROWS || n > MOST_LENGTH || k > MOST_LENGTH || groups > MOST_GROUPS)
+            return r355::fail(R355_ERR_BAD_SIZE, "%s: at most %u rows, n and k of %u and %u groups, got %u, %u, %u and %u", what, MOST_ROWS, MOST_LENGTH, MOST_GROUPS, rows, n, k, groups);
+        if(groups > 1u && !offsets)
+            return r355::fail(R355_ERR_BAD_ARG, "%s: %u groups of rows need offsets", what, groups);
+        if(!r355::aligned(offsets, 4))
+            return r355::fail(R355_ERR_MISALIGNED, "%s: offsets need the alignment of their elements", what);
+        return R355_OK;
+    }
+    int checkMatrix(const char* what, const char* name, const void* at, uint32_t ld, uint32_t width, uint32_t bytes)
+    {
+        if(!at)
+            return R355_OK;
+        if(ld < width || ld > MOST_LENGTH)
+            return r355::fail(R355_ERR_BAD_ARG, "%s: the leading dimension %u of %s must be %u (its row) to %u", what, ld, name, width, MOST_LENGTH);
+        if(!r355::aligned(at, bytes))
+            return r355::fail(R355_ERR_MISALIGNED, "%s: %s needs the alignment of its elements", what, name);
+        return R355_OK;
+    }
+    int checkStride(const char* what, const char* name, int64_t stride, uint32_t groups, uint64_t least)
+    {
+        if(groups > 1u && (stride < 0 || static_cast<uint64_t>(stride) < least || stride > (int64_t{1} << 46)))
+            return r355::fail(R355_ERR_BAD_ARG, "%s: %s=%lld is less than the %llu elements of a group", what, name, static_cast<long long>(stride), static_cast<unsigned long long>(least));
+        return R355_OK;
+    }
+
+    // Shares of a group's rows in the gradient's pass: four workgroups a CU, 16 rows each at least
+    uint64_t gradParts(const r355_linear_backward_args& a, uint32_t strips)
+    {
+        const uint64_t parts = tilesOf(4u * r355::computeUnits(), strips * a.groups), most = tilesOf(a.rows, 16u * a.groups);
+        return most == 0u ? 1u : parts < most ? parts : most;
+    }
+} // namespace
+
+#define R355_TRY(call)          \
+    do                          \
+    {                           \
+        const int rc_ = (call); \
+        if(rc_ != R355_OK)      \
+            return rc_;         \
+    } while(0)
+
+extern "C" int r355_linear(const r355_linear_args* args, void* stream)
+{
+    constexpr const char* what = "linear";
+    if(!args)
+        return r355::fail(R355_ERR_BAD_ARG, "linear: null arguments");
+    const r355_linear_args& a = *args;
+    R355_TRY(checkCommon(what, a.in_type, a.activation, a.rows, a.n, a.k, a.groups, a.offsets));
+    if(a.out_type != a.in_type && a.out_type != R355_F32)
+        return r355::fail(R355_ERR_UNSUPPORTED, "linear: the result has the type of x or is f32");
+    if(a.rows == 0)
+        return R355_OK;
+    if(!a.x || !a.w || !a.y)
+        return r355::fail(R355_ERR_BAD_ARG, "linear: null pointer");
+    const uint32_t outBytes = r355::dtypeBytes(a.out_type);
+    R355_TRY(checkMatrix(what, "x", a.x, a.ldx, a.k, 2));
+    R355_TRY(checkMatrix(what, "w", a.w, a.ldw, a.k, 2));
+    R355_TRY(checkMatrix(what, "bias", a.bias, a.n, a.n, 2));
+    R355_TRY(checkMatrix(what, "gate", a.gate, a.ldg, a.n, 2));
+    R355_TRY(checkMatrix(what, "z", a.z, a.ldz, a.n, 2));
+    R355_TRY(checkMatrix(what, "c", a.c, a.ldc, a.n, outBytes));
+    R355_TRY(checkMatrix(what, "y", a.y, a.ldy, a.n, outBytes));
+    R355_TRY(checkStride(what, "w_stride", a.w_stride, a.groups, (uint64_t)(a.n - 1u) * a.ldw + a.k));
+    if(a.source)
+    {
+        if(!r355::aligned(a.source, 4))
+            return r355::fail(R355_ERR_MISALIGNED, "linear: source needs the alignment of its elements");
+        if(a.x_rows == 0 || (uint64_t)a.x_rows * a.ldx * 2u > 0x7FFFFFF0u)
+            return r355::fail(R355_ERR_BAD_SIZE, "linear: rows taken by their numbers must be of 1 to 2^31 bytes of x, got %u rows %u elements apart", a.x_rows, a.ldx);
+    }
+    LinearParams p{};
+    p.a = static_cast<const char*>(a.x), p.b = static_cast<const char*>(a.w), p.bias = static_cast<const char*>(a.bias), p.gate = static_cast<const char*>(a.gate);
+    p.c = static_cast<const char*>(a.c), p.y = static_cast<char*>(a.y), p.z = static_cast<char*>(a.z);
+    p.offsets = a.offsets, p.source = a.source, p.rows = a.rows, p.n = a.n, p.k = a.k, p.groups = a.groups, p.sourceRows = a.x_rows;
+    p.lda = a.ldx, p.ldb = a.ldw, p.ldy = a.ldy, p.ldz = a.ldz, p.ldg = a.ldg, p.ldc = a.ldc;
+    p.strideB = static_cast<uint64_t>(a.groups > 1u ? a.w_stride : 0) * 2u, p.splits = 1u, p.activation = a.activation, p.outF32 = a.out_type == R355_F32;
+    p.wide = a.n % 8u == 0u && evenRows(a.y, a.ldy, outBytes) && evenRows(a.c, a.ldc, outBytes) && evenRows(a.z, a.ldz, 2) && evenRows(a.gate, a.ldg, 2) && r355::aligned(a.bias, 16);
+    const bool        even = a.k % 8u == 0u && evenRows(a.x, a.ldx, 2) && evenRows(a.w, a.ldw, 2) && (a.groups == 1u || a.w_stride % 8 == 0);
+    const hipStream_t s    = static_cast<hipStream_t>(stream);
+    r355::beginCall();
+    if(even && a.rows / a.groups <= 16u)
+    {
+        if(mostTiles(p, 16u) * tilesOf(p.n, 16u) > r355::MAX_GROUPS / 2u)
+            return tooMany(what);
+        a.in_type == R355_F16 ? launchFew<_Float16>(p, s) : launchFew<__bf16>(p, s);
+    }
+    else
+        R355_TRY(launchTiles(a.in_type, p, true, true, !even, s, what));
+    return r355::checkLaunch(what);
+}
+
+extern "C" size_t r355_linear_workspace_bytes(const r355_linear_args* args)
+{
+    (void)args;
+    return 0;
+}
+
+extern "C" size_t r355_linear_backward_workspace_bytes(const r355_linear_backward_args* args)
+{
+    if(!args || args->n == 0 || args->groups == 0 || !args->dbias)
+        return 0;
+    const uint64_t parts = gradParts(*args, static_cast<uint32_t>(tilesOf(args->n, 512u)));
+    return parts > 1u ? static_cast<size_t>(parts * args->groups * args->n * 4u) : 0u;
+}
+
+extern "C" int r355_linear_backward(const r355_linear_backward_args* args, void* stream)
+{
+    constexpr const char* what = "linear_backward";
+    if(!args)
+        return r355::fail(R355_ERR_BAD_ARG, "linear_backward: null arguments");
+    const r355_linear_backward_args& a = *args;
+    R355_TRY(checkCommon(what, a.in_type, a.activation, a.rows, a.n, a.k, a.groups, a.offsets));
+    if(a.grad_type != a.in_type && a.grad_type != R355_F32)
+        return r355::fail(R355_ERR_UNSUPPORTED, "linear_backward: dw has the type of x or is f32");
+    const bool slope = a.activation != R355_ACT_NONE, element = slope || a.gate;
+    if(a.rows != 0 && (!a.dy || (a.dx && !a.w) || (a.dw && !a.x)))
+        return r355::fail(R355_ERR_BAD_ARG, "linear_backward: null pointer");
+    if(a.rows != 0 && slope && !a.z)
+        return r355::fail(R355_ERR_BAD_ARG, "linear_backward: an activation's gradient needs z");
+    if(a.dgate && (!a.gate || !a.z))
+        return r355::fail(R355_ERR_BAD_ARG, "linear_backward: dgate needs gate and z");
+    if(element && !a.dz)
+        return r355::fail(R355_ERR_BAD_ARG, "linear_backward: with an activation or a gate dz is needed");
+    const uint32_t gradBytes = r355::dtypeBytes(a.grad_type);
+    R355_TRY(checkMatrix(what, "dy", a.dy, a.lddy, a.n, 2));
+    R355_TRY(checkMatrix(what, "x", a.x, a.ldx, a.k, 2));
+    R355_TRY(checkMatrix(what, "w", a.w, a.ldw, a.k, 2));
+    R355_TRY(checkMatrix(what, "z", a.z, a.ldz, a.n, 2));
+    R355_TRY(checkMatrix(what, "gate", a.gate, a.ldg, a.n, 2));
+    R355_TRY(checkMatrix(what, "dz", element ? a.dz : nullptr, a.lddz, a.n, 2));
+    R355_TRY(checkMatrix(what, "dgate", a.dgate, a.lddg, a.n, 2));
+    R355_TRY(checkMatrix(what, "dx", a.dx, a.lddx, a.k, 2));
+    R355_TRY(checkMatrix(what, "dw", a.dw, a.lddw, a.k, gradBytes));
+    R355_TRY(checkMatrix(what, "dbias", a.dbias, a.n, a.n, 4));
+    if(a.dx)
+        R355_TRY(checkStride(what, "w_stride", a.w_stride, a.groups, (uint64_t)(a.n - 1u) * a.ldw + a.k));
+    if(a.dw)
+        R355_TRY(checkStride(what, "dw_stride", a.dw_stride, a.groups, (uint64_t)(a.n - 1u) * a.lddw + a.k));
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    r355::beginCall();
+
+    if(element || a.dbias)
+    {
+        GradParams g{};
+        g.dy = static_cast<const char*>(a.dy), g.z = static_cast<const char*>(a.z), g.gate = static_cast<const char*>(a.gate);
+        g.dz = element ? static_cast<char*>(a.dz) : nullptr, g.dgate = static_cast<char*>(a.dgate), g.offsets = a.offsets;
+        g.rows = a.rows, g.n = a.n, g.groups = a.groups, g.lddy = a.lddy, g.ldz = a.ldz, g.ldg = a.ldg, g.lddz = a.lddz, g.lddg = a.lddg;
+        g.activation = a.activation, g.accumulate = a.accumulate;
+        const bool     wide   = a.n % 8u == 0u && evenRows(a.dy, a.lddy, 2) && evenRows(a.z, a.ldz, 2) && evenRows(a.gate, a.ldg, 2) && evenRows(g.dz, a.lddz, 2) && evenRows(a.dgate, a.lddg, 2);
+        const uint32_t strips = static_cast<uint32_t>(tilesOf(a.n, wide ? 512u : 64u));
+        const uint64_t wanted = gradParts(a, strips);
+        const uint64_t fit    = !a.dbias ? wanted : a.workspace && r355::aligned(a.workspace, 16) ? a.workspace_bytes / ((uint64_t)a.groups * a.n * 4u) : 1u;
+        const uint64_t parts  = wanted < fit ? wanted : fit ? fit : 1u;
+        g.parts = static_cast<uint32_t>(parts);
+        g.sums  = !a.dbias ? nullptr : parts > 1u ? static_cast<float*>(a.workspace) : a.dbias;
+        const dim3 grid(strips, g.parts, a.groups), block(256);
+        const bool f16 = a.in_type == R355_F16;
+        const auto kernel = wide ? (f16 ? linearGrad<_Float16, 8> : linearGrad<__bf16, 8>) : (f16 ? linearGrad<_Float16, 1> : linearGrad<__bf16, 1>);
+        hipLaunchKernelGGL(kernel, grid, block, 0, s, g);
+        if(a.dbias && parts > 1u)
+            hipLaunchKernelGGL(linearGradSums, dim3(static_cast<uint32_t>(tilesOf(a.n, 256u)), a.groups), block, 0, s, static_cast<const float*>(a.workspace), a.dbias, g.parts, a.n,
+                               a.accumulate);
+    }
+    const char*    dz   = static_cast<const char*>(element ? a.dz : a.dy);
+    const uint32_t lddz = element ? a.lddz : a.lddy;
+    LinearParams   p{};
+    p.offsets = a.offsets, p.rows = a.rows, p.groups = a.groups, p.splits = 1u;
+    if(a.dx && a.rows)
+    {
+        LinearParams d = p;
+        d.a = dz, d.lda = lddz, d.b = static_cast<const char*>(a.w), d.ldb = a.ldw, d.strideB = static_cast<uint64_t>(a.groups > 1u ? a.w_stride : 0) * 2u;
+        d.y = static_cast<char*>(a.dx), d.ldy = a.lddx, d.n = a.k, d.k = a.n;
+        d.wide          = a.k % 8u == 0u && evenRows(a.dx, a.lddx, 2);
+        const bool even = a.n % 8u == 0u && evenRows(dz, lddz, 2) && evenRows(a.w, a.ldw, 2) && (a.groups == 1u || a.w_stride % 8 == 0);
+        R355_TRY(launchTiles(a.in_type, d, true, false, !even, s, what));
+    }
+    if(a.dw)
+    {
+        LinearParams d = p;
+        d.a = dz, d.lda = lddz, d.b = static_cast<const char*>(a.x), d.ldb = a.ldx;
+        d.y = static_cast<char*>(a.dw), d.ldy = a.lddw, d.strideY = static_cast<uint64_t>(a.groups > 1u ? a.dw_stride : 0) * gradBytes, d.m = a.n, d.n = a.k;
+        d.c = a.accumulate ? static_cast<const char*>(a.dw) : nullptr, d.ldc = a.lddw, d.strideC = d.strideY, d.outF32 = a.grad_type == R355_F32;
+        d.wide          = a.k % 8u == 0u && evenRows(a.dw, a.lddw, gradBytes) && (a.groups == 1u || a.dw_stride * gradBytes % 16 == 0);
+        const bool even = evenRows(dz, lddz, 2) && evenRows(a.x, a.ldx, 2);
+        R355_TRY(launchTiles(a.in_type, d, false, false, !even, s, what));
+    }
+    return r355::checkLaunch(what);
+}

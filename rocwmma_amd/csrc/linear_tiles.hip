@@ -1,0 +1,587 @@
+// Products of a layer on macro tiles for gfx950: forward with bias, activation, gate and residual in the epilogue, and both gradients, for one
+// matrix of weights or for one per group of rows.  No counterpart in the reference.
+//
+// A macro tile of 32 WB x 32 WB results is four waves of 16 WB x 16 WB each, on v_mfma_f32_16x16x32 with the accumulators in place; a stage is 64 of the sum.  Operands go
+// to LDS by direct loads in the images of operand_tile.hpp and come back whole or, where they are not contiguous along the sum, through transposing reads.  LDS
+// holds two images of A and three of B, so that loads run two stages ahead (B of the small tiles three).  The buffers go round at run time: the loop is one stage long, and
+// what that costs, an addition for each address of a read, hides behind matrix instructions (six stages unrolled, as the GEMM has them, would be 36 KB of code for each epilogue).
+//
+// Rows are ragged: a workgroup finds its group from the offsets in device memory (GroupTiles).  A tile that has fewer rows reads its last one again, what that gives is not
+// stored; a sum that ends inside a stage is completed with zeros by loads past the end of their buffer.
+//
+// Compiled once per type.
+#include <hip/hip_runtime.h>
+
+#include <type_traits>
+
+#include "lds_dma.hpp"
+#include "linear.hpp"
+#include "operand_tile.hpp"
+
+namespace
+{
+    using r355::f32x4;
+    using r355::GroupTile;
+    using r355::GroupTiles;
+    using r355::ldsBarrier;
+    using r355::LinearParams;
+    using r355::loadToLds;
+    using r355::OUTSIDE;
+    using r355::u32x2;
+    using r355::u32x4;
+    using r355::vec;
+    using r355::waitVmcnt;
+    using r355::tile::CHUNK;
+    using r355::tile::i32x4;
+    using r355::tile::laneOffsets8;
+    using r355::tile::readBlock8;
+    using r355::tile::readOffsets8;
+    using r355::tile::STAGE_KB;
+    using r355::tile::swzK8;
+    using r355::tile::THREADS;
+
+#ifdef R355_LINEAR_BF16
+    using T = __bf16;
+#else
+    using T = _Float16;
+#endif
+    constexpr uint32_t TK = STAGE_KB / 2u; // of the sum per stage
+
+    // (inline assembly: of the builtin the compiler makes instructions whose result is not tied to their addend, and moves the accumulators about)
+    __device__ __forceinline__ void multiply(f32x4& acc, i32x4 x, i32x4 y)
+    {
+        if constexpr(__is_same(T, __bf16))
+            asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(x), "v"(y));
+        else
+            asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(acc) : "v"(x), "v"(y));
+    }
+
+    // What a workgroup multiplies: Y rows first .. first + rowsLeft, columns col0 .. col0 + colsLeft, of group `group`; the sum's share [kFirst, kFirst + k).
+    struct Work
+    {
+        uint32_t group, first, rowsLeft, col0, colsLeft, k, kFirst;
+        uint64_t sumRow; // weights' gradient: first row of the group
+    };
+
+    template <bool AK, uint32_t TILE>
+    __device__ __forceinline__ bool workOf(const LinearParams& p, Work& w)
+    {
+        uint32_t tm, tn, k;
+        if constexpr(AK)
+        {
+            GroupTiles<TILE> tiles{p};
+            const uint32_t   tilesM = tiles.total();
+            if(!r355::tileCoordRange(blockIdx.x, tilesM, p.tilesN, 0u, tilesM * p.tilesN, false, tm, tn))
+                return false;
+            const GroupTile t = tiles.at(tm);
+            w.group = t.group, w.first = t.first, w.rowsLeft = t.count, w.sumRow = 0u, k = p.k;
+        }
+        else
+        {
+            if(!r355::tileCoordRange(blockIdx.x, p.groups * p.tilesM, p.tilesN, 0u, p.groups * p.tilesM * p.tilesN, false, tm, tn))
+                return false;
+            w.group           = tm / p.tilesM;
+            w.first           = tm % p.tilesM * TILE;
+            w.rowsLeft        = p.m - w.first < TILE ? p.m - w.first : TILE;
+            const auto  rows  = r355::rowsOf(p, w.group);
+            w.sumRow = rows.first, k = rows.count;
+        }
+        w.col0     = tn * TILE;
+        w.colsLeft = p.n - w.col0 < TILE ? p.n - w.col0 : TILE;
+        // (whole stages for every share but the last ones)
+        const uint32_t stages = k / TK + (k % TK != 0u ? 1u : 0u), share = p.splits > 1u ? (stages + p.splits - 1u) / p.splits : stages;
+        w.kFirst = (p.splits > 1u ? blockIdx.y * share : 0u) * TK;
+        w.kFirst = w.kFirst < k ? w.kFirst : k;
+        w.k      = k - w.kFirst < share * TK ? k - w.kFirst : share * TK;
+        // (uniform, which the compiler does not see through the lanes' part in finding it)
+        w.group = __builtin_amdgcn_readfirstlane(w.group), w.first = __builtin_amdgcn_readfirstlane(w.first), w.rowsLeft = __builtin_amdgcn_readfirstlane(w.rowsLeft);
+        w.col0 = __builtin_amdgcn_readfirstlane(w.col0), w.colsLeft = __builtin_amdgcn_readfirstlane(w.colsLeft);
+        w.k = __builtin_amdgcn_readfirstlane(w.k), w.kFirst = __builtin_amdgcn_readfirstlane(w.kFirst);
+        return true;
+    }
+
+    // EW neighbouring elements of type E, as floats, from and to a buffer
+    template <typename E, uint32_t EW>
+    __device__ __forceinline__ void loadRow(__amdgpu_buffer_rsrc_t from, uint32_t offset, float (&v)[EW])
+    {
+        if constexpr(EW == 1u && sizeof(E) == 2u)
+            v[0] = static_cast<float>(__builtin_bit_cast(E, static_cast<uint16_t>(__builtin_amdgcn_raw_buffer_load_b16(from, offset, 0, 0))));
+        else if constexpr(EW == 1u)
+            v[0] = __builtin_bit_cast(E, __builtin_amdgcn_raw_buffer_load_b32(from, offset, 0, 0));
+        else
+#pragma unroll
+            for(uint32_t part = 0; part < EW * sizeof(E) / 16u; ++part)
+            {
+                const auto w = __builtin_bit_cast(vec<E, 16 / sizeof(E)>, __builtin_amdgcn_raw_buffer_load_b128(from, offset + part * 16u, 0, 0));
+#pragma unroll
+                for(uint32_t e = 0; e < 16u / sizeof(E); ++e)
+                    v[part * (16u / sizeof(E)) + e] = static_cast<float>(w[e]);
+            }
+    }
+    template <typename E, uint32_t EW>
+    __device__ __forceinline__ void storeRow(__amdgpu_buffer_rsrc_t to, uint32_t offset, const float (&v)[EW])
+    {
+        constexpr int NT = 2; // nontemporal: written once
+        if constexpr(EW == 1u && sizeof(E) == 2u)
+            __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, static_cast<E>(v[0])), to, offset, 0, 0);
+        else if constexpr(EW == 1u)
+            __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, static_cast<E>(v[0])), to, offset, 0, 0);
+        else
+#pragma unroll
+            for(uint32_t part = 0; part < EW * sizeof(E) / 16u; ++part)
+            {
+                vec<E, 16 / sizeof(E)> w;
+#pragma unroll
+                for(uint32_t e = 0; e < 16u / sizeof(E); ++e)
+                    w[e] = static_cast<E>(v[part * (16u / sizeof(E)) + e]);
+                // (the offset in the lane's register: gemm_tiled.hip says why)
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, w), to, offset + part * 16u, 0, NT);
+            }
+    }
+
+    // The buffer of `rows` rows of `cols` elements from (row, col) on, `bytes` an element: it ends with the last one
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t rowsBuffer(const char* base, uint64_t row, uint32_t col, uint32_t ld, uint32_t rows, uint32_t cols, uint32_t bytes)
+    {
+        const uint64_t addr    = r355::uniformAddress(base + (row * ld + col) * bytes);
+        const uint32_t records = rows && cols ? ((rows - 1u) * ld + cols) * bytes : 0u;
+        return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<char*>(addr), 0, static_cast<int>(__builtin_amdgcn_readfirstlane(records)), 0x00020000);
+    }
+
+    // Results of one wave's tile of 16 WB x 16 WB, rows row0 .. and columns col0 .. of Y, `rows` x `cols` of them there: staged in f32 through the wave's own LDS, so that an
+    // access covers whole rows of the wave's tile and the epilogue is taken of sums that nothing has rounded.
+    //   z = sum + bias;  y = act(z) gate + c     (FULL; otherwise y = sum + c)
+    // each rounded once.  Rows and columns that are not there lie outside the buffers: no branch around an access.
+    template <uint32_t WB, uint32_t EW, bool FULL, typename Out>
+    __device__ __forceinline__ void storeWave(f32x4 (&acc)[WB][WB], const LinearParams& p, const Work& w, uint32_t rowIn, uint32_t colIn, uint32_t lane, char* scratch)
+    {
+        constexpr uint32_t WT = 16u * WB, ROW = WT * 4u, PASS = WT < 64u ? WT : 64u; // LDS bytes of a row, rows at a time
+        constexpr uint32_t SWZ = WB * 4u < 16u ? WB * 4u - 1u : 15u;
+        constexpr uint32_t LANES = WT / EW < 64u ? WT / EW : 64u, ACROSS = WT / EW / LANES, RPI = 64u / LANES; // lanes and accesses of a row, rows an access
+        constexpr uint32_t ITERS = PASS / RPI, BATCH = ITERS < 4u ? ITERS : 4u, OS = sizeof(Out);
+        if(rowIn >= w.rowsLeft || colIn >= w.colsLeft)
+            return; // (uniform)
+        const uint32_t rows = w.rowsLeft - rowIn < WT ? w.rowsLeft - rowIn : WT, cols = w.colsLeft - colIn < WT ? w.colsLeft - colIn : WT;
+        const uint64_t row0 = (uint64_t)w.first + rowIn;
+        const uint32_t col0 = w.col0 + colIn, r16 = lane & 15u, quad = lane >> 4, rowLane = lane / LANES, at = lane % LANES;
+        // a share of a split sum goes to the workspace: [split][group, row of Y][column]
+        char* const y = p.y + (uint64_t)w.group * p.strideY + (p.splits > 1u ? (uint64_t)blockIdx.y * (p.groups * (uint64_t)p.m) * p.n * 4u : 0u);
+        const char* c = p.c ? p.c + (uint64_t)w.group * p.strideC : nullptr;
+
+        float bias[ACROSS][EW];
+        if constexpr(FULL)
+        {
+            const auto from = rowsBuffer(p.bias, w.group, col0, p.n, p.bias ? 1u : 0u, cols, 2u);
+#pragma unroll
+            for(uint32_t h = 0; h < ACROSS; ++h)
+                loadRow<T, EW>(from, (at + h * LANES) * EW < cols ? (at + h * LANES) * EW * 2u : OUTSIDE, bias[h]);
+        }
+#pragma unroll
+        for(uint32_t pass = 0; pass < WT / PASS; ++pass)
+        {
+            const uint32_t left = pass * PASS < rows ? rows - pass * PASS : 0u, here = left < PASS ? left : PASS;
+            const uint64_t row  = row0 + pass * PASS;
+#pragma unroll
+            for(uint32_t i = 0; i < PASS / 16u; ++i)
+#pragma unroll
+                for(uint32_t j = 0; j < WB; ++j)
+                {
+                    const uint32_t r = 16u * i + r16;
+                    *reinterpret_cast<f32x4*>(scratch + r * ROW + (((4u * j + quad) ^ (r & SWZ)) * CHUNK)) = acc[pass * (PASS / 16u) + i][j];
+                }
+            __builtin_amdgcn_wave_barrier(); // the same wave reads back what it wrote (LDS is in order per wave)
+            const auto toY = rowsBuffer(y, row, col0, p.ldy, here, cols, OS);
+            const auto fromC = rowsBuffer(c, row, col0, p.ldc, c ? here : 0u, cols, OS);
+            const auto toZ = rowsBuffer(p.z, row, col0, p.ldz, FULL && p.z ? here : 0u, cols, 2u), fromG = rowsBuffer(p.gate, row, col0, p.ldg, FULL && p.gate ? here : 0u, cols, 2u);
+#pragma unroll
+            for(uint32_t h = 0; h < ACROSS; ++h)
+            {
+                const uint32_t col = (at + h * LANES) * EW;
+                const bool     in  = col < cols;
+#pragma unroll 1
+                for(uint32_t b = 0; b < ITERS; b += BATCH)
+                {
+                    if(b * RPI >= here)
+                        break; // (uniform)
+                    float gate[BATCH][EW], add[BATCH][EW], sum[BATCH][EW];
+                    if(FULL && p.gate)
+#pragma unroll
+                        for(uint32_t u = 0; u < BATCH; ++u)
+                            loadRow<T, EW>(fromG, in ? (((b + u) * RPI + rowLane) * p.ldg + col) * 2u : OUTSIDE, gate[u]);
+                    if(c)
+#pragma unroll
+                        for(uint32_t u = 0; u < BATCH; ++u)
+                            loadRow<Out, EW>(fromC, in ? (((b + u) * RPI + rowLane) * p.ldc + col) * OS : OUTSIDE, add[u]);
+#pragma unroll
+                    for(uint32_t u = 0; u < BATCH; ++u)
+                    {
+                        const uint32_t r = (b + u) * RPI + rowLane;
+                        if constexpr(EW == 1u)
+                            sum[u][0] = *reinterpret_cast<const float*>(scratch + r * ROW + (((col >> 2) ^ (r & SWZ)) * CHUNK) + (col & 3u) * 4u);
+                        else
+#pragma unroll
+                            for(uint32_t part = 0; part < EW / 4u; ++part)
+                            {
+                                const f32x4 v = *reinterpret_cast<const f32x4*>(scratch + r * ROW + (((col / 4u + part) ^ (r & SWZ)) * CHUNK));
+#pragma unroll
+                                for(uint32_t e = 0; e < 4u; ++e)
+                                    sum[u][part * 4u + e] = v[e];
+                            }
+                    }
+                    if constexpr(FULL)
+                    {
+#pragma unroll
+                        for(uint32_t u = 0; u < BATCH; ++u)
+#pragma unroll
+                            for(uint32_t e = 0; e < EW; ++e)
+                                sum[u][e] += bias[h][e];
+                        if(p.z)
+#pragma unroll
+                            for(uint32_t u = 0; u < BATCH; ++u)
+                                storeRow<T, EW>(toZ, in ? (((b + u) * RPI + rowLane) * p.ldz + col) * 2u : OUTSIDE, sum[u]);
+                        if(p.activation != R355_ACT_NONE)
+#pragma unroll
+                            for(uint32_t u = 0; u < BATCH; ++u)
+#pragma unroll
+                                for(uint32_t e = 0; e < EW; ++e)
+                                    sum[u][e] = r355::activate(p.activation, sum[u][e]);
+                        if(p.gate)
+#pragma unroll
+                            for(uint32_t u = 0; u < BATCH; ++u)
+#pragma unroll
+                                for(uint32_t e = 0; e < EW; ++e)
+                                    sum[u][e] *= gate[u][e];
+                    }
+                    if(c)
+#pragma unroll
+                        for(uint32_t u = 0; u < BATCH; ++u)
+#pragma unroll
+                            for(uint32_t e = 0; e < EW; ++e)
+                                sum[u][e] += add[u][e];
+#pragma unroll
+                    for(uint32_t u = 0; u < BATCH; ++u)
+                        storeRow<Out, EW>(toY, in ? (((b + u) * RPI + rowLane) * p.ldy + col) * OS : OUTSIDE, sum[u]);
+                }
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
+    template <uint32_t WB, bool FULL>
+    __device__ __forceinline__ void storeTile(f32x4 (&acc)[WB][WB], const LinearParams& p, const Work& w, uint32_t rowIn, uint32_t colIn, uint32_t lane, char* scratch)
+    {
+        if(p.wide && p.outF32)
+            storeWave<WB, 8, FULL, float>(acc, p, w, rowIn, colIn, lane, scratch);
+        else if(p.wide)
+            storeWave<WB, 8, FULL, T>(acc, p, w, rowIn, colIn, lane, scratch);
+        else if(p.outF32)
+            storeWave<WB, 1, FULL, float>(acc, p, w, rowIn, colIn, lane, scratch);
+        else
+            storeWave<WB, 1, FULL, T>(acc, p, w, rowIn, colIn, lane, scratch);
+    }
+
+    // A stage of an operand that has `valid` bytes of the sum left per row: past its end the loads write zeros (K-contiguous: by tailOffset, otherwise the buffer ends there)
+    template <bool KCONTIG>
+    __device__ __forceinline__ i32x4 stageBuffer(uint64_t addr, uint32_t valid, uint32_t ld)
+    {
+        return i32x4{static_cast<int>(static_cast<uint32_t>(addr)), static_cast<int>(static_cast<uint32_t>(addr >> 32) & 0xFFFFu), static_cast<int>(KCONTIG ? 0x7FFFFFFFu : valid * ld),
+                     0x00020000};
+    }
+
+    template <bool AK, bool BK, uint32_t WB>
+    __device__ __forceinline__ void linearTile(const LinearParams& p)
+    {
+        static_assert(WB == 8 || WB == 4 || WB == 2, "wave tiles of 128, 64 or 32");
+        constexpr uint32_t TILE = 32u * WB, WT = 16u * WB, OPER = TILE * STAGE_KB; // macro and wave tile; bytes of an operand's stage
+        constexpr uint32_t NS = WB * WB, XS = 2u * WB, QS = WB / 2u, LOAD_Q = QS > 2u ? 2u : QS - 1u;
+        // the large tile's loads are dealt out over the whole stage, B two stages ahead; the small tiles', whose stages are a quarter as long and less, come in the
+        // second half, B three stages ahead (gemm_tiled.hip has both measured)
+        constexpr bool     SPREAD = WB == 8u;
+        constexpr uint32_t B_AHEAD = SPREAD ? 2u : 3u;
+        __shared__ __attribute__((aligned(1024))) char lds[5u * OPER]; // A at 0 and OPER, B at 2, 3 and 4 OPER
+
+        Work w;
+        if(!workOf<AK, TILE>(p, w))
+            return;
+        const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1u;
+        const uint32_t ldsBase = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
+        const uint32_t dma     = ldsBase + wave * 64u * CHUNK;
+
+        uint32_t offA[WB], offB[WB], stepA, stepB, kByteA, kByteB;
+        uint64_t stageA, stageB;
+        laneOffsets8<AK, WB, 2>(tid, p.lda, w.rowsLeft, offA, stepA, stageA, kByteA);
+        laneOffsets8<BK, WB, 2>(tid, p.ldb, w.colsLeft, offB, stepB, stageB, kByteB);
+        uint64_t fromA, fromB;
+        if constexpr(AK)
+        {
+            if(p.source) // rows by their numbers; one that is none of A's reads as zeros
+            {
+                const uint32_t r = tid >> 3, slot = tid & 7u;
+#pragma unroll
+                for(uint32_t j = 0; j < WB; ++j)
+                {
+                    const uint32_t row = r + 32u * j < w.rowsLeft ? r + 32u * j : w.rowsLeft - 1u, from = static_cast<uint32_t>(p.source[(uint64_t)w.first + row]);
+                    offA[j]            = from < p.sourceRows ? from * p.lda * 2u + ((slot ^ swzK8(r)) * CHUNK) : OUTSIDE;
+                }
+            }
+            fromA = r355::uniformAddress(p.a + ((p.source ? 0u : (uint64_t)w.first * p.lda) + w.kFirst) * 2u);
+            fromB = r355::uniformAddress(p.b + (uint64_t)w.group * p.strideB + (BK ? (uint64_t)w.col0 * p.ldb + w.kFirst : (uint64_t)w.kFirst * p.ldb + w.col0) * 2u);
+        }
+        else
+        {
+            fromA = r355::uniformAddress(p.a + ((w.sumRow + w.kFirst) * p.lda + w.first) * 2u);
+            fromB = r355::uniformAddress(p.b + ((w.sumRow + w.kFirst) * p.ldb + w.col0) * 2u);
+        }
+        // (an empty sum has one stage of zeros)
+        const uint32_t stages = w.k > TK ? (w.k - 1u) / TK + 1u : 1u, lastBytes = (w.k - (stages - 1u) * TK) * 2u;
+        auto validOf = [&](uint32_t s) { return s + 1u < stages ? STAGE_KB : s + 1u == stages ? lastBytes : 0u; };
+        auto tailA = [&](uint32_t j, uint32_t valid) { return AK && kByteA >= valid ? OUTSIDE : offA[j]; };
+        auto tailB = [&](uint32_t j, uint32_t valid) { return BK && kByteB >= valid ? OUTSIDE : offB[j]; };
+        auto addrA = [&](uint32_t s) { return fromA + (uint64_t)(s < stages ? s : stages - 1u) * stageA; }; // (of a stage that is not there no lane reads anything)
+        auto addrB = [&](uint32_t s) { return fromB + (uint64_t)(s < stages ? s : stages - 1u) * stageB; };
+        auto issueA = [&](uint32_t s, uint32_t at) {
+            const uint32_t valid = validOf(s);
+#pragma unroll
+            for(uint32_t j = 0; j < WB; ++j)
+                loadToLds(stageBuffer<AK>(addrA(s), valid, p.lda), tailA(j, valid), j * stepA, dma + at + j * THREADS * CHUNK);
+        };
+        auto issueB = [&](uint32_t s, uint32_t at) {
+            const uint32_t valid = validOf(s);
+#pragma unroll
+            for(uint32_t j = 0; j < WB; ++j)
+                loadToLds(stageBuffer<BK>(addrB(s), valid, p.ldb), tailB(j, valid), j * stepB, dma + at + j * THREADS * CHUNK);
+        };
+
+        uint32_t rdA[8], rdB[8];
+        readOffsets8<AK, WB, 2>(wm, lane, rdA);
+        readOffsets8<BK, WB, 2>(wn, lane, rdB);
+        f32x4 acc[WB][WB];
+#pragma unroll
+        for(uint32_t i = 0; i < WB; ++i)
+#pragma unroll
+            for(uint32_t j = 0; j < WB; ++j)
+                acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        i32x4 fa[2][WB], fb[2][WB];
+        // matrix instruction n of half a stage, in shells around block (0, 0), as the operand blocks A0 B0 A1 B1 ... come; the operands swapped: a lane holds four
+        // neighbouring columns of a row
+        auto multiplyAt = [&](uint32_t half, uint32_t n) {
+            uint32_t d = 0;
+            while((d + 1u) * (d + 1u) <= n)
+                ++d;
+            const uint32_t r = n - d * d, i = r <= d ? d : r - d - 1u, j = r <= d ? r : d;
+            multiply(acc[i][j], fb[half][j], fa[half][i]);
+        };
+        auto readAt = [&](uint32_t atA, uint32_t atB, uint32_t half, uint32_t x, uint32_t part) {
+            if(x & 1u)
+                readBlock8<BK, WB, 2>(lds + atB, rdB, x >> 1, half, part, fb[half][x >> 1], 0u);
+            else
+                readBlock8<AK, WB, 2>(lds + atA, rdA, x >> 1, half, part, fa[half][x >> 1], 0u);
+        };
+        auto after = [](uint32_t at) { return at == 4u * OPER ? 2u * OPER : at + OPER; }; // B's buffers go round
+
+        // prologue: stages 0 and 1 (and B of stage 2) requested in the order that the loop keeps
+        if constexpr(SPREAD)
+        {
+            issueB(0u, 2u * OPER), issueA(0u, 0u), issueB(1u, 3u * OPER), issueA(1u, OPER);
+            waitVmcnt<2u * WB>();
+        }
+        else
+        {
+            issueA(0u, 0u), issueB(0u, 2u * OPER), issueA(1u, OPER), issueB(1u, 3u * OPER), issueB(2u, 4u * OPER);
+            waitVmcnt<3u * WB>();
+        }
+        ldsBarrier();
+#pragma unroll
+        for(uint32_t x = 0; x < XS; ++x)
+        {
+            readAt(0u, 2u * OPER, 0, x, 0);
+            readAt(0u, 2u * OPER, 0, x, 1);
+        }
+        uint32_t aCur = 0u, bCur = 2u * OPER;
+        // One stage, its first half in registers: the second half arrives under the first's matrix instructions, then the first half of the next stage under the second's.
+        // FULL: all that this stage requests lies inside the sum.
+        auto stage = [&](auto full, uint32_t kt) {
+            constexpr bool FULL = decltype(full)::value;
+            const uint32_t aNxt = aCur ^ OPER, bNxt = after(bCur), bTo = SPREAD ? after(bNxt) : bCur;
+            const uint32_t vB   = FULL ? STAGE_KB : validOf(kt + B_AHEAD);
+            const i32x4    bufB = stageBuffer<BK>(addrB(kt + B_AHEAD), vB, p.ldb);
+#pragma unroll
+            for(uint32_t x = 0; x < XS; ++x)
+#pragma unroll
+                for(uint32_t q = 0; q < QS; ++q)
+                {
+                    multiplyAt(0, x * QS + q);
+                    if(q < 2u)
+                        readAt(aCur, bCur, 1, x, q);
+                    if constexpr(QS == 1u)
+                        readAt(aCur, bCur, 1, x, 1);
+                    if(SPREAD && q == LOAD_Q && (x & 1u))
+                        loadToLds(bufB, FULL ? offB[x >> 1] : tailB(x >> 1, vB), (x >> 1) * stepB, dma + bTo + (x >> 1) * THREADS * CHUNK);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            waitVmcnt<WB>(); // all but the youngest loads, B of stage kt + 2
+            ldsBarrier();
+            const uint32_t vA   = FULL ? STAGE_KB : validOf(kt + 2u);
+            const i32x4    bufA = stageBuffer<AK>(addrA(kt + 2u), vA, p.lda);
+#pragma unroll
+            for(uint32_t x = 0; x < XS; ++x)
+#pragma unroll
+                for(uint32_t q = 0; q < QS; ++q)
+                {
+                    multiplyAt(1, x * QS + q);
+                    if(q < 2u)
+                        readAt(aNxt, bNxt, 0, x, q);
+                    if constexpr(QS == 1u)
+                        readAt(aNxt, bNxt, 0, x, 1);
+                    if(q == LOAD_Q)
+                    {
+                        if(SPREAD ? (x & 1u) != 0u : x < WB)
+                        {
+                            const uint32_t j = SPREAD ? x >> 1 : x;
+                            loadToLds(bufA, FULL ? offA[j] : tailA(j, vA), j * stepA, dma + aCur + j * THREADS * CHUNK);
+                        }
+                        else if(!SPREAD)
+                            loadToLds(bufB, FULL ? offB[x - WB] : tailB(x - WB, vB), (x - WB) * stepB, dma + bTo + (x - WB) * THREADS * CHUNK);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            aCur = aNxt, bCur = bNxt;
+        };
+        const uint32_t whole = w.k / TK, main = whole > B_AHEAD ? whole - B_AHEAD : 0u;
+        uint32_t       kt    = 0u;
+        for(; kt < main; ++kt)
+            stage(std::true_type{}, kt);
+        for(; kt < stages; ++kt)
+            stage(std::false_type{}, kt);
+
+        // the last matrix instructions are still under way, which the compiler does not know, and loads past the last stage are writing zeros to buffers that the
+        // epilogue uses
+        asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+        waitVmcnt<0>();
+        ldsBarrier();
+        storeTile<WB, AK && BK>(acc, p, w, wm * WT, wn * WT, lane, lds + wave * (WB * 4096u));
+    }
+
+    // (a kernel per tile: the attribute cannot depend on a template parameter)
+    template <bool AK, bool BK>
+    __global__ void __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(1, 1))) linearTiles256(LinearParams p)
+    {
+        linearTile<AK, BK, 8>(p);
+    }
+    template <bool AK, bool BK>
+    __global__ void __launch_bounds__(THREADS, 2) linearTiles128(LinearParams p)
+    {
+        linearTile<AK, BK, 4>(p);
+    }
+    template <bool AK, bool BK>
+    __global__ void __launch_bounds__(THREADS, 4) linearTiles64(LinearParams p)
+    {
+        linearTile<AK, BK, 2>(p);
+    }
+
+    // The same on tiles of 64 x 64 for operands of any alignment, lengths and leading dimensions: loaded element by element through registers, 32 of the sum at a time.
+    template <bool AK, bool BK>
+    __global__ void __launch_bounds__(THREADS) linearAny(LinearParams p)
+    {
+        constexpr uint32_t TILE = 64u, STEP = 32u, PITCH = STEP + 8u; // (elements; rows 80 bytes apart: 16-byte reads of 16 rows meet in a bank at most twice)
+        __shared__ __attribute__((aligned(16))) T   image[2][TILE * PITCH];
+        __shared__ __attribute__((aligned(16))) char scratch[4u * 2u * 4096u];
+        Work w;
+        if(!workOf<AK, TILE>(p, w))
+            return;
+        const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1u;
+        // a thread's eight elements of a step: neighbours along the sum, or along the rows of Y (columns, for B)
+        const uint32_t rowA = AK ? tid >> 2 : (tid & 7u) * 8u, kA = AK ? (tid & 3u) * 8u : tid >> 3;
+        const uint32_t rowB = BK ? tid >> 2 : (tid & 7u) * 8u, kB = BK ? (tid & 3u) * 8u : tid >> 3;
+        const T* a = reinterpret_cast<const T*>(p.a);
+        const T* b = reinterpret_cast<const T*>(p.b) + w.group * (p.strideB / 2u);
+        bool     there = rowA < w.rowsLeft;
+        if constexpr(AK)
+        {
+            uint64_t row = (uint64_t)w.first + rowA;
+            if(there && p.source)
+            {
+                const uint32_t from = static_cast<uint32_t>(p.source[row]);
+                there = from < p.sourceRows, row = from;
+            }
+            a += row * p.lda + w.kFirst;
+            b += BK ? (uint64_t)(w.col0 + rowB) * p.ldb + w.kFirst : (uint64_t)w.kFirst * p.ldb + w.col0 + rowB;
+        }
+        else
+        {
+            a += (w.sumRow + w.kFirst) * p.lda + w.first + rowA;
+            b += (w.sumRow + w.kFirst) * p.ldb + w.col0 + rowB;
+        }
+        f32x4 acc[2][2];
+#pragma unroll
+        for(uint32_t i = 0; i < 2u; ++i)
+#pragma unroll
+            for(uint32_t j = 0; j < 2u; ++j)
+                acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for(uint32_t k0 = 0; k0 < w.k; k0 += STEP)
+        {
+            vec<T, 8> va, vb;
+#pragma unroll
+            for(uint32_t e = 0; e < 8u; ++e)
+            {
+                const bool inA = AK ? there && k0 + kA + e < w.k : rowA + e < w.rowsLeft && k0 + kA < w.k;
+                const bool inB = BK ? rowB < w.colsLeft && k0 + kB + e < w.k : rowB + e < w.colsLeft && k0 + kB < w.k;
+                va[e] = inA ? (AK ? a[k0 + kA + e] : a[(uint64_t)(k0 + kA) * p.lda + e]) : T(0.0f);
+                vb[e] = inB ? (BK ? b[k0 + kB + e] : b[(uint64_t)(k0 + kB) * p.ldb + e]) : T(0.0f);
+            }
+            __syncthreads();
+            if constexpr(AK)
+                *reinterpret_cast<vec<T, 8>*>(&image[0][rowA * PITCH + kA]) = va;
+            else
+#pragma unroll
+                for(uint32_t e = 0; e < 8u; ++e)
+                    image[0][(rowA + e) * PITCH + kA] = va[e];
+            if constexpr(BK)
+                *reinterpret_cast<vec<T, 8>*>(&image[1][rowB * PITCH + kB]) = vb;
+            else
+#pragma unroll
+                for(uint32_t e = 0; e < 8u; ++e)
+                    image[1][(rowB + e) * PITCH + kB] = vb[e];
+            __syncthreads();
+            u32x4 fa[2], fb[2];
+#pragma unroll
+            for(uint32_t i = 0; i < 2u; ++i)
+            {
+                fa[i] = *reinterpret_cast<const u32x4*>(&image[0][(wm * 32u + i * 16u + (lane & 15u)) * PITCH + (lane >> 4) * 8u]);
+                fb[i] = *reinterpret_cast<const u32x4*>(&image[1][(wn * 32u + i * 16u + (lane & 15u)) * PITCH + (lane >> 4) * 8u]);
+            }
+#pragma unroll
+            for(uint32_t i = 0; i < 2u; ++i)
+#pragma unroll
+                for(uint32_t j = 0; j < 2u; ++j)
+                    acc[i][j] = r355::mfma32<T>(fb[j], fa[i], acc[i][j]);
+        }
+        storeTile<2, AK && BK>(acc, p, w, wm * 32u, wn * 32u, lane, scratch + wave * 8192u);
+    }
+
+    template <bool AK, bool BK>
+    void launch(const LinearParams& p, uint32_t tile, bool any, uint32_t workgroups, hipStream_t s)
+    {
+        const dim3 grid(workgroups, p.splits), block(THREADS);
+        if(any)
+            hipLaunchKernelGGL((linearAny<AK, BK>), grid, block, 0, s, p);
+        else if(tile == 256u)
+            hipLaunchKernelGGL((linearTiles256<AK, BK>), grid, block, 0, s, p);
+        else if(tile == 128u)
+            hipLaunchKernelGGL((linearTiles128<AK, BK>), grid, block, 0, s, p);
+        else
+            hipLaunchKernelGGL((linearTiles64<AK, BK>), grid, block, 0, s, p);
+    }
+} // namespace
+
+#ifdef R355_LINEAR_BF16
+void r355::linearTilesBF16(const LinearParams& p, bool aK, bool bK, uint32_t tile, bool any, uint32_t workgroups, hipStream_t s)
+#else
+void r355::linearTilesF16(const LinearParams& p, bool aK, bool bK, uint32_t tile, bool any, uint32_t workgroups, hipStream_t s)
+#endif
+{
+    if(aK && bK)
+        launch<true, true>(p, tile, any, workgroups, s);
+    else if(aK)
+        launch<true, false>(p, tile, any, workgroups, s);
+    else
+        launch<false, false>(p, tile, any, workgroups, s);
+}
