@@ -459,6 +459,86 @@ typedef struct
 int    r355_linear_backward(const r355_linear_backward_args* args, void* stream);
 size_t r355_linear_backward_workspace_bytes(const r355_linear_backward_args* args);
 
+/*
+ * The router: for each token the `top` experts of the largest logit (plus bias [experts], where given: in f32, for the choice alone), the lowest expert of equal ones first, NaN behind
+ * every number.  weights [tokens][top]: softmax or sigmoid of the logits, over the chosen ones alone with chosen_only (their sum is then `scale`), times scale; an
+ * expert at -infinity has weight 0.  The rows of the experts' products are the tokens' choices in order of (expert, token, choice): chosen [tokens][top], place [tokens][top]
+ * (the row of a choice), source [tokens * top] (the token of a row), offsets [experts + 1] (an expert's first row).  logits: R355_F16, R355_BF16 or R355_F32, rows ldl elements apart.
+ * Up to 1024 experts, 32 choices and 2^30 rows.  workspace (16-byte aligned, contents irrelevant): r355_route_workspace_bytes are needed, 0 for a few tokens.  Calls that overlap need one each.
+ */
+typedef enum
+{
+    R355_ROUTE_SOFTMAX = 0,
+    R355_ROUTE_SIGMOID = 1
+} r355_route_score;
+typedef struct
+{
+    int32_t      type, score, chosen_only;
+    uint32_t     tokens, experts, top, ldl;
+    const void*  logits;
+    const float* bias; /* or NULL */
+    float*       weights;
+    int32_t*     chosen;
+    int32_t*     place;
+    int32_t*     source;
+    int32_t*     offsets;
+    double       scale;
+    void*        workspace;
+    uint64_t     workspace_bytes;
+} r355_route_args;
+int    r355_route(const r355_route_args* args, void* stream);
+size_t r355_route_workspace_bytes(uint32_t tokens, uint32_t experts, uint32_t top);
+
+/* dlogits [tokens][experts] for dweights [tokens][top] of the experts chosen, score, chosen_only and scale as in r355_route; every element is written.  A number
+ * in chosen that is no expert's is left out; one that is there twice counts twice. */
+typedef struct
+{
+    int32_t        type, score, chosen_only;
+    uint32_t       tokens, experts, top, ldl, ldd;
+    const void*    logits;
+    const int32_t* chosen;
+    const float*   dweights;
+    void*          dlogits;
+    double         scale;
+} r355_route_backward_args;
+int r355_route_backward(const r355_route_backward_args* args, void* stream);
+
+/*
+ * y[t] = sum_j weights[t][j] values[place[t][j]] + c[t]: the experts' rows put together, f32 sums, rounded once.  values: [rows][width] of type (R355_F16 or R355_BF16), as c and y;
+ * weights: f32, or NULL for ones; c: NULL, or y itself.  A place outside [0, rows) is left out.  Any width, leading dimension and alignment of an element, fastest in multiples of 16 bytes.
+ */
+typedef struct
+{
+    int32_t        type;
+    uint32_t       tokens, top, width, rows;
+    const void*    values;
+    const int32_t* place; /* [tokens][top] */
+    const float*   weights;
+    const void*    c;
+    void*          y;
+    uint32_t       ldv, ldc, ldy;
+} r355_combine_args;
+int r355_combine(const r355_combine_args* args, void* stream);
+
+/*
+ * out[place[t][j]] = weights[t][j] x[t] (weights NULL: x[t]): the tokens' rows to the experts, and the gradient of r355_combine with respect to its values; its weights'
+ * gradient is dweights[t][j] = x[t] . values[place[t][j]] (f32 sums; dweights NULL: not wanted, values then not read; out NULL: only that).  A place outside [0, rows) is left out (its
+ * dweights 0); rows that no place names are left as they were; no row is named twice.  out must not overlap x or values.  Sizes and types as above.
+ */
+typedef struct
+{
+    int32_t        type;
+    uint32_t       tokens, top, width, rows;
+    const void*    x;
+    const int32_t* place;
+    const float*   weights;
+    const void*    values;
+    void*          out;
+    float*         dweights;
+    uint32_t       ldx, ldv, ldo;
+} r355_dispatch_args;
+int r355_dispatch(const r355_dispatch_args* args, void* stream);
+
 /* Device facts used by the roofline report (test/hip_device.hpp:101-119 in the reference). */
 typedef struct
 {

@@ -30,6 +30,8 @@ ROPE_HALF, ROPE_INTERLEAVED = 0, 1
 
 # r355_activation
 ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = range(5)
+# r355_route_score
+ROUTE_SOFTMAX, ROUTE_SIGMOID = 0, 1
 
 DTYPE_BYTES = {F16: 2, BF16: 2, E4M3: 1, I8: 1, F32: 4, I32: 4, F64: 8, E5M2: 1}
 
@@ -38,6 +40,7 @@ EXPORTS = [
     "r355_dlrm_bwd", "r355_dlrm_kernel", "r355_gemv", "r355_gemv_timed", "r355_dgemv", "r355_gemv_workspace_bytes", "r355_gemv_ws", "r355_dgemv_ws", "r355_compress_24", "r355_decompress_24", "r355_compress_24_16", "r355_decompress_24_16",
     "r355_w4_matmul", "r355_w4_packed_bytes", "r355_w4_pack", "r355_rope", "r355_rope_turns", "r355_tree_attention", "r355_tree_attention_workspace_bytes",
     "r355_linear", "r355_linear_workspace_bytes", "r355_linear_backward", "r355_linear_backward_workspace_bytes",
+    "r355_route", "r355_route_workspace_bytes", "r355_route_backward", "r355_combine", "r355_dispatch",
     "r355_get_device_info", "r355_last_error", "r355_version",
 ]
 
@@ -134,6 +137,39 @@ class LinearBackwardArgs(ctypes.Structure):
     ]
 
 
+class RouteArgs(ctypes.Structure):
+    _fields_ = [
+        ("type", ctypes.c_int32), ("score", ctypes.c_int32), ("chosen_only", ctypes.c_int32),
+        ("tokens", ctypes.c_uint32), ("experts", ctypes.c_uint32), ("top", ctypes.c_uint32), ("ldl", ctypes.c_uint32),
+        ("logits", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("weights", ctypes.c_void_p), ("chosen", ctypes.c_void_p), ("place", ctypes.c_void_p),
+        ("source", ctypes.c_void_p), ("offsets", ctypes.c_void_p), ("scale", ctypes.c_double), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64),
+    ]
+
+
+class RouteBackwardArgs(ctypes.Structure):
+    _fields_ = [
+        ("type", ctypes.c_int32), ("score", ctypes.c_int32), ("chosen_only", ctypes.c_int32),
+        ("tokens", ctypes.c_uint32), ("experts", ctypes.c_uint32), ("top", ctypes.c_uint32), ("ldl", ctypes.c_uint32), ("ldd", ctypes.c_uint32),
+        ("logits", ctypes.c_void_p), ("chosen", ctypes.c_void_p), ("dweights", ctypes.c_void_p), ("dlogits", ctypes.c_void_p), ("scale", ctypes.c_double),
+    ]
+
+
+class CombineArgs(ctypes.Structure):
+    _fields_ = [
+        ("type", ctypes.c_int32), ("tokens", ctypes.c_uint32), ("top", ctypes.c_uint32), ("width", ctypes.c_uint32), ("rows", ctypes.c_uint32),
+        ("values", ctypes.c_void_p), ("place", ctypes.c_void_p), ("weights", ctypes.c_void_p), ("c", ctypes.c_void_p), ("y", ctypes.c_void_p),
+        ("ldv", ctypes.c_uint32), ("ldc", ctypes.c_uint32), ("ldy", ctypes.c_uint32),
+    ]
+
+
+class DispatchArgs(ctypes.Structure):
+    _fields_ = [
+        ("type", ctypes.c_int32), ("tokens", ctypes.c_uint32), ("top", ctypes.c_uint32), ("width", ctypes.c_uint32), ("rows", ctypes.c_uint32),
+        ("x", ctypes.c_void_p), ("place", ctypes.c_void_p), ("weights", ctypes.c_void_p), ("values", ctypes.c_void_p), ("out", ctypes.c_void_p),
+        ("dweights", ctypes.c_void_p), ("ldx", ctypes.c_uint32), ("ldv", ctypes.c_uint32), ("ldo", ctypes.c_uint32),
+    ]
+
+
 class DeviceInfo(ctypes.Structure):
     _fields_ = [
         ("arch", ctypes.c_char * 64), ("compute_units", ctypes.c_int32), ("wave_size", ctypes.c_int32),
@@ -187,6 +223,11 @@ def lib():
         L.r355_linear_workspace_bytes.argtypes = [ctypes.POINTER(LinearArgs)]
         L.r355_linear_backward.argtypes = [ctypes.POINTER(LinearBackwardArgs), vp]
         L.r355_linear_backward_workspace_bytes.argtypes = [ctypes.POINTER(LinearBackwardArgs)]
+        L.r355_route.argtypes = [ctypes.POINTER(RouteArgs), vp]
+        L.r355_route_workspace_bytes.argtypes = [u32, u32, u32]
+        L.r355_route_backward.argtypes = [ctypes.POINTER(RouteBackwardArgs), vp]
+        L.r355_combine.argtypes = [ctypes.POINTER(CombineArgs), vp]
+        L.r355_dispatch.argtypes = [ctypes.POINTER(DispatchArgs), vp]
         L.r355_get_device_info.argtypes = [ctypes.POINTER(DeviceInfo)]
         L.r355_last_error.argtypes = []
         L.r355_version.argtypes = []
@@ -195,7 +236,8 @@ def lib():
         for name in EXPORTS:
             if name not in ("r355_last_error", "r355_version"):
                 getattr(L, name).restype = ctypes.c_int
-        for name in ("r355_w4_packed_bytes", "r355_tree_attention_workspace_bytes", "r355_linear_workspace_bytes", "r355_linear_backward_workspace_bytes"):
+        for name in ("r355_w4_packed_bytes", "r355_tree_attention_workspace_bytes", "r355_linear_workspace_bytes", "r355_linear_backward_workspace_bytes",
+                     "r355_route_workspace_bytes"):
             getattr(L, name).restype = ctypes.c_size_t
         _lib = L
     return _lib
@@ -613,6 +655,65 @@ def linear_backward(in_type, grad_type, rows, n, k, dy, x, w, dx=None, dw=None, 
 def linear_backward_workspace_bytes(a):
     """Bytes of workspace that r355_linear_backward makes use of for LinearBackwardArgs (0: none)."""
     return lib().r355_linear_backward_workspace_bytes(ctypes.byref(a))
+
+
+def _floats(name, t, count):
+    """Address of `count` 32-bit floating numbers one after the other (a raw address is taken as it is)"""
+    if t is None or not hasattr(t, "dtype"):
+        return t
+    if str(t.dtype) not in ("torch.float32", "float32"):
+        raise ValueError("%s must hold 32-bit floating numbers, got %s" % (name, t.dtype))
+    if not getattr(t, "is_cuda", False):
+        raise ValueError("%s must lie in device memory" % name)
+    if not t.is_contiguous() or t.numel() < count:
+        raise ValueError("%s must be %d contiguous elements, got %s with strides %s" % (name, count, tuple(t.shape), t.stride()))
+    return t.data_ptr()
+
+
+def route_workspace_bytes(tokens, experts, top):
+    """Bytes of workspace that route() needs (0: none)."""
+    return lib().r355_route_workspace_bytes(tokens, experts, top)
+
+
+def route(dtype, tokens, experts, top, logits, weights, chosen, place, source, offsets, score=ROUTE_SOFTMAX, chosen_only=False, scale=1.0, bias=None, ldl=None, workspace=None,
+          workspace_bytes=None, stream=None):
+    """The `top` experts of each token by logits [tokens][experts] (plus bias, for the choice), their weights, and the rows in order of experts (include/r355_wmma.h): chosen, place
+    [tokens][top], source [tokens * top], offsets [experts + 1], what linear(), dispatch() and combine() take."""
+    slots = tokens * top
+    at, size = _workspace(workspace, workspace_bytes)
+    a = RouteArgs(dtype, score, chosen_only, tokens, experts, top, experts if ldl is None else ldl, _ptr(logits), _floats("route: bias", bias, experts),
+                  _floats("route: weights", weights, slots), _index("route: chosen", chosen, 4, slots), _index("route: place", place, 4, slots),
+                  _index("route: source", source, 4, slots), _index("route: offsets", offsets, 4, experts + 1), scale, at, size)
+    rc = lib().r355_route(ctypes.byref(a), None if stream is None else _stream_handle(stream))
+    if rc != 0:
+        _check(rc)
+
+
+def route_backward(dtype, tokens, experts, top, logits, chosen, dweights, dlogits, score=ROUTE_SOFTMAX, chosen_only=False, scale=1.0, ldl=None, ldd=None, stream=None):
+    """dlogits [tokens][experts] for the gradient of the weights that route() gave to the experts chosen."""
+    a = RouteBackwardArgs(dtype, score, chosen_only, tokens, experts, top, experts if ldl is None else ldl, experts if ldd is None else ldd, _ptr(logits),
+                          _index("route_backward: chosen", chosen, 4, tokens * top), _floats("route_backward: dweights", dweights, tokens * top), _ptr(dlogits), scale)
+    rc = lib().r355_route_backward(ctypes.byref(a), None if stream is None else _stream_handle(stream))
+    if rc != 0:
+        _check(rc)
+
+
+def combine(dtype, tokens, top, width, values, rows, place, y, weights=None, c=None, ldv=None, ldc=None, ldy=None, stream=None):
+    """y[t] = sum_j weights[t][j] values[place[t][j]] + c[t] over the `rows` rows of values; weights: default ones."""
+    a = CombineArgs(dtype, tokens, top, width, rows, _ptr(values), _index("combine: place", place, 4, tokens * top), _floats("combine: weights", weights, tokens * top), _ptr(c),
+                    _ptr(y), width if ldv is None else ldv, width if ldc is None else ldc, width if ldy is None else ldy)
+    rc = lib().r355_combine(ctypes.byref(a), None if stream is None else _stream_handle(stream))
+    if rc != 0:
+        _check(rc)
+
+
+def dispatch(dtype, tokens, top, width, x, out, rows, place, weights=None, values=None, dweights=None, ldx=None, ldv=None, ldo=None, stream=None):
+    """out[place[t][j]] = weights[t][j] x[t] (default: x[t]), of `rows` rows; with dweights also x[t] . values[place[t][j]], so that it is the gradient of combine() for x = dy."""
+    a = DispatchArgs(dtype, tokens, top, width, rows, _ptr(x), _index("dispatch: place", place, 4, tokens * top), _floats("dispatch: weights", weights, tokens * top), _ptr(values),
+                     _ptr(out), _floats("dispatch: dweights", dweights, tokens * top), width if ldx is None else ldx, width if ldv is None else ldv, width if ldo is None else ldo)
+    rc = lib().r355_dispatch(ctypes.byref(a), None if stream is None else _stream_handle(stream))
+    if rc != 0:
+        _check(rc)
 
 
 def device_info():

@@ -23,7 +23,7 @@ SOURCES = [("api.cpp", "api", []), ("gemm_simple.hip", "gemm_simple", []),
            ("gemm_tiled.hip", "gemm_tiled_p2", ["-DR355_TILED_PART=2"]), ("gemm_tiled.hip", "gemm_tiled_p3", ["-DR355_TILED_PART=3"]),
            ("gemm_f32.hip", "gemm_f32", []), ("dlrm.hip", "dlrm", []), ("dlrm_general.hip", "dlrm_general", []), ("sparse.hip", "sparse", []), ("gemv.hip", "gemv", []),
            ("w4.hip", "w4", []), ("rope.hip", "rope", []), ("tree_attention.hip", "tree_attention", []),
-           ("linear.hip", "linear", []), ("linear_tiles.hip", "linear_tiles_f16", []), ("linear_tiles.hip", "linear_tiles_bf16", ["-DR355_LINEAR_BF16"])]
+           ("linear.hip", "linear", []), ("experts.hip", "experts", []), ("linear_tiles.hip", "linear_tiles_f16", []), ("linear_tiles.hip", "linear_tiles_bf16", ["-DR355_LINEAR_BF16"])]
 
 # packed-fp32 instructions are disabled on purpose (device pass only; the host pass warns that it
 # does not know the feature, which is harmless)
