@@ -1,5 +1,5 @@
 // Products of a layer with bias, activation, gate and residual, and their gradients, for one matrix of weights or one per group of rows: the entry points, the kernel
-// for few rows and what the gradient does element by element.  The macro tiles are in linear_tiles.hip.
+// for few rows, what the gradient does element by element, and the sums of split products.  The macro tiles are in linear_tiles.hip.
 //
 //   forward    z = x W^T + b;  y = act(z) gate + c
 //   backward   dz = dy gate act'(z);  dgate = dy act(z);  dx = dz W;  dW = dz^T x;  db = sum of dz over the rows
@@ -135,13 +135,91 @@ namespace
                 sum += static_cast<float>(reinterpret_cast<const T*>(p.bias)[(uint64_t)group * p.n + col0 + col]);
             if(p.z)
                 reinterpret_cast<T*>(p.z)[at * p.ldz + col0 + col] = static_cast<T>(sum);
-            sum = r355::activate(p.activation, sum);
+            r355::withActivation(p.activation, [&](auto act) { sum = r355::activate<decltype(act)::value>(sum); });
             if(p.gate)
                 sum *= static_cast<float>(reinterpret_cast<const T*>(p.gate)[at * p.ldg + col0 + col]);
             if(p.outF32)
                 reinterpret_cast<float*>(p.y)[at * p.ldy + col0 + col] = p.c ? sum + reinterpret_cast<const float*>(p.c)[at * p.ldc + col0 + col] : sum;
             else
                 reinterpret_cast<T*>(p.y)[at * p.ldy + col0 + col] = static_cast<T>(p.c ? sum + static_cast<float>(reinterpret_cast<const T*>(p.c)[at * p.ldc + col0 + col]) : sum);
+        }
+    }
+
+    // ---- Sums of a split product: [splits][rows][pitch] of f32, added in order, then the epilogue of linear_tiles.hip.  Result rows are `p.m` to a group (weights' gradient), or
+    // all one group's.  Four columns a thread; what is not four columns wide, or past a row's end, goes element by element.
+    template <typename T, typename Out>
+    __global__ void __launch_bounds__(256) linearReduce(LinearParams p, const float* sums, uint64_t rows, uint32_t pitch)
+    {
+        const uint32_t col = (blockIdx.x * 256u + threadIdx.x) * 4u, left = col < p.n ? p.n - col : 0u;
+        if(left == 0u)
+            return;
+        // (rows anywhere: vectors of an element's alignment)
+        typedef T    TU __attribute__((ext_vector_type(4), aligned(2)));
+        typedef Out  OutU __attribute__((ext_vector_type(4), aligned(sizeof(Out))));
+        auto read = [&](const auto* from, float (&v)[4]) {
+            using E = std::remove_cv_t<std::remove_pointer_t<decltype(from)>>;
+            using U = std::conditional_t<std::is_same_v<E, T>, TU, OutU>;
+            if(left >= 4u)
+            {
+                const U w = *reinterpret_cast<const U*>(from);
+#pragma unroll
+                for(uint32_t e = 0; e < 4u; ++e)
+                    v[e] = static_cast<float>(w[e]);
+            }
+            else
+#pragma unroll
+                for(uint32_t e = 0; e < 4u; ++e)
+                    v[e] = e < left ? static_cast<float>(from[e]) : 0.0f;
+        };
+        auto write = [&](auto* to, const float (&v)[4]) {
+            using E = std::remove_pointer_t<decltype(to)>;
+            using U = std::conditional_t<std::is_same_v<E, T>, TU, OutU>;
+            if(left >= 4u)
+                *reinterpret_cast<U*>(to) = U{static_cast<E>(v[0]), static_cast<E>(v[1]), static_cast<E>(v[2]), static_cast<E>(v[3])};
+            else
+#pragma unroll
+                for(uint32_t e = 0; e < 4u; ++e)
+                    if(e < left)
+                        to[e] = static_cast<E>(v[e]);
+        };
+        float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if(p.bias)
+            read(reinterpret_cast<const T*>(p.bias) + col, bias);
+        const uint64_t share = rows * pitch;
+        for(uint64_t row = blockIdx.y; row < rows; row += gridDim.y)
+        {
+            const uint64_t group = p.m ? row / p.m : 0u, in = p.m ? row % p.m : row;
+            const float*   from = sums + row * pitch + col;
+            float          sum[4], more[4];
+            f32x4          all{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+            for(uint32_t s = 0; s < p.splits; ++s)
+                all += *reinterpret_cast<const f32x4*>(from + s * share);
+#pragma unroll
+            for(uint32_t e = 0; e < 4u; ++e)
+                sum[e] = all[e] + bias[e];
+            if(p.z)
+                write(reinterpret_cast<T*>(p.z) + row * p.ldz + col, sum);
+            r355::withActivation(p.activation, [&](auto act) __attribute__((always_inline)) {
+#pragma unroll
+                for(uint32_t e = 0; e < 4u; ++e)
+                    sum[e] = r355::activate<decltype(act)::value>(sum[e]);
+            });
+            if(p.gate)
+            {
+                read(reinterpret_cast<const T*>(p.gate) + row * p.ldg + col, more);
+#pragma unroll
+                for(uint32_t e = 0; e < 4u; ++e)
+                    sum[e] *= more[e];
+            }
+            if(p.c)
+            {
+                read(reinterpret_cast<const Out*>(p.c + group * p.strideC) + in * p.ldc + col, more);
+#pragma unroll
+                for(uint32_t e = 0; e < 4u; ++e)
+                    sum[e] += more[e];
+            }
+            write(reinterpret_cast<Out*>(p.y + group * p.strideY) + in * p.ldy + col, sum);
         }
     }
 
@@ -214,9 +292,11 @@ namespace
                     if(p.z)
                     {
                         read(p.z, row, p.ldz, z);
+                        r355::withActivation(p.activation, [&](auto act) __attribute__((always_inline)) {
 #pragma unroll
-                        for(uint32_t e = 0; e < EW; ++e)
-                            r355::activateBoth(p.activation, z[e], value[e], slope[e]);
+                            for(uint32_t e = 0; e < EW; ++e)
+                                r355::activateBoth<decltype(act)::value>(z[e], value[e], slope[e]);
+                        });
                     }
                     else
 #pragma unroll
@@ -265,17 +345,25 @@ namespace
         }
     }
 
+    // The shares of the bias's gradient: 64 columns a workgroup, a quarter of the shares a wave (of 128 shares of 4096 columns 38 us with one thread a column)
     __global__ void __launch_bounds__(256) linearGradSums(const float* sums, float* dbias, uint32_t parts, uint32_t n, int32_t accumulate)
     {
-        const uint32_t col = blockIdx.x * 256u + threadIdx.x;
-        if(col >= n)
-            return;
-        const float* from = sums + (uint64_t)blockIdx.y * parts * n + col;
-        float        sum  = 0.0f;
-        for(uint32_t s = 0; s < parts; ++s)
-            sum += from[(uint64_t)s * n];
-        float* to = dbias + (uint64_t)blockIdx.y * n + col;
-        *to       = accumulate ? *to + sum : sum;
+        __shared__ float meet[4][64];
+        const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, col = blockIdx.x * 64u + lane;
+        const float*   from = sums + (uint64_t)blockIdx.y * parts * n + col;
+        float          sum  = 0.0f;
+        if(col < n)
+#pragma unroll 8
+            for(uint32_t s = wave; s < parts; s += 4u)
+                sum += from[(uint64_t)s * n];
+        meet[wave][lane] = sum;
+        __syncthreads();
+        if(wave == 0u && col < n)
+        {
+            sum       = ((meet[0][lane] + meet[1][lane]) + meet[2][lane]) + meet[3][lane];
+            float* to = dbias + (uint64_t)blockIdx.y * n + col;
+            *to       = accumulate ? *to + sum : sum;
+        }
     }
 
     constexpr uint32_t MOST_ROWS = 1u << 30, MOST_LENGTH = (1u << 22) - 8u, MOST_GROUPS = 1024u;
@@ -293,15 +381,86 @@ namespace
         return most < p.rows ? most : p.rows;
     }
 
-    // Macro tile of a ragged product by the rows that a group has on average.
-    uint32_t tileEdge(const LinearParams& p, uint64_t rows, uint64_t cols, uint32_t groups)
+    // How a product on macro tiles is launched: `splits` workgroups along the sum; the first `tall` rows alone where the rest goes to other tiles.
+    struct Plan
     {
-        const uint64_t perGroup = rows / groups;
-        for(uint32_t edge = 256u; edge > 64u; edge /= 2u)
-            if(perGroup >= edge * 3u / 4u && tilesOf(perGroup, edge) * groups * tilesOf(cols, edge) >= r355::computeUnits() * 3u / 4u)
-                return edge;
-        (void)p;
-        return 64u;
+        r355::LinearTile tile, rest;
+        uint32_t         splits, tall;
+        double           us;
+    };
+
+    // What a launch takes, in us, of `tiles` with `stages` of 64 of the sum each (bf16, 256 CUs): rounds of as many tiles as the CUs hold at a time, the last one of fewer.  Per tile:
+    // how many a CU holds; a round's start and end; a stage with one, two, three, four of them on a CU (the large tile, which the power limit slows: on few CUs, on all).
+    struct TileTimes
+    {
+        uint32_t held;
+        double   ends, stage[4];
+    };
+    constexpr TileTimes TILE_TIMES[r355::LINEAR_TILES] = {{1u, 11.0, {1.05, 1.34}}, {1u, 6.0, {0.63, 0.80}}, {1u, 6.0, {0.63, 0.80}}, {2u, 4.5, {0.45, 0.88}}, {4u, 3.0, {0.37, 0.42, 0.56, 0.70}},
+                                                          {2u, 2.0, {1.40, 2.60}}};
+    double launchTime(uint32_t tile, double tiles, double stages)
+    {
+        const TileTimes& t    = TILE_TIMES[tile];
+        const double     cus  = r355::computeUnits(), round = cus * t.held;
+        const double     full = static_cast<double>(static_cast<uint64_t>(tiles / round)), rest = tiles - full * round;
+        double           us   = 2.0 + full * (t.ends + stages * t.stage[t.held == 1u ? 1u : t.held - 1u]);
+        if(rest > 0.0)
+        {
+            const uint32_t a = static_cast<uint32_t>((rest - 1e-9) / cus); // a + 1 tiles on a CU
+            us += t.ends + stages * (t.held == 1u ? t.stage[rest > 0.4 * cus ? 1u : 0u] : t.stage[a]);
+        }
+        return us;
+    }
+
+    // floats between the rows of the sums of a split product
+    uint32_t pitchOf(uint32_t n)
+    {
+        return (n + 3u) / 4u * 4u;
+    }
+
+    // The plan that takes the least by launchTime(), with as many splits as the workspace holds.
+    Plan planOf(const LinearParams& p, bool aK, bool any, uint64_t workspaceBytes)
+    {
+        using namespace r355;
+        // (of ragged groups on average: half a tile of each is empty; a weights' gradient has their rows for its sum)
+        const double   stages = aK ? static_cast<double>(tilesOf(p.k, 64u)) : p.offsets ? static_cast<double>(p.rows) / p.groups / 64.0 + 0.5 : static_cast<double>(tilesOf(p.rows, 64u));
+        const uint64_t rowsY  = aK ? p.rows : (uint64_t)p.m * p.groups;
+        auto tiles = [&](uint32_t tile, uint64_t rows) {
+            const double across = static_cast<double>(tilesOf(p.n, LINEAR_COLS[tile]));
+            if(!aK)
+                return static_cast<double>(tilesOf(p.m, LINEAR_ROWS[tile])) * p.groups * across;
+            if(!p.offsets)
+                return static_cast<double>(tilesOf(rows, LINEAR_ROWS[tile])) * across;
+            const double met = p.groups < rows ? p.groups : static_cast<double>(rows);
+            return (static_cast<double>(rows) / LINEAR_ROWS[tile] + 0.5 * met) * across;
+        };
+        Plan best{any ? TILE_ANY : TILE_64, TILE_64, 1u, 0u, 1e30};
+        for(uint32_t tile = any ? TILE_ANY : TILE_256; tile < (any ? LINEAR_TILES : TILE_ANY); ++tile)
+        {
+            const double all = tiles(tile, p.rows);
+            for(uint32_t splits = 1u; splits <= 64u; splits += splits < 4u ? 1u : splits / 2u)
+            {
+                // (a sum is split in whole stages, four of them at least; rows of no group are not to be written)
+                if(splits > 1u && ((aK && p.offsets) || stages < 4.0 * splits || rowsY * pitchOf(p.n) * 4u * splits > workspaceBytes || all > computeUnits()))
+                    break;
+                const double us = launchTime(tile, all * splits, stages / splits) + (splits > 1u ? 5.0 + static_cast<double>(rowsY) * p.n * 4.0 * (2u * splits + 1u) / 5e6 : 0.0);
+                if(us < best.us)
+                    best = Plan{static_cast<LinearTile>(tile), TILE_64, splits, 0u, us};
+            }
+            // whole rounds of large tiles, the rest on other ones
+            if(tile == TILE_256 && aK && !p.offsets)
+            {
+                const uint64_t across = tilesOf(p.n, 256u), rounds = static_cast<uint64_t>(all) / computeUnits(), tall = rounds * computeUnits() / across * 256u;
+                if(tall > 0u && tall < p.rows)
+                    for(uint32_t rest = TILE_256_128; rest <= TILE_64; ++rest)
+                    {
+                        const double us = launchTime(TILE_256, tiles(TILE_256, tall), stages) + launchTime(rest, tiles(rest, p.rows - tall), stages);
+                        if(us < best.us)
+                            best = Plan{TILE_256, static_cast<LinearTile>(rest), 1u, static_cast<uint32_t>(tall), us};
+                    }
+            }
+        }
+        return best;
     }
 
     template <typename T>
@@ -317,20 +476,62 @@ namespace
         return r355::fail(R355_ERR_BAD_SIZE, "%s: more than 2^24 tiles of the result", what);
     }
 
-    // one product on macro tiles; rowsY, colsY: of a group's result, on average
-    int launchTiles(int32_t type, LinearParams p, bool aK, bool bK, bool any, hipStream_t s, const char* what)
+    int launchTile(int32_t type, LinearParams p, bool aK, bool bK, r355::LinearTile tile, hipStream_t s, const char* what)
     {
-        const uint32_t edge = any ? 64u : tileEdge(p, aK ? p.rows : (uint64_t)p.m * p.groups, p.n, p.groups);
-        p.tilesN = static_cast<uint32_t>(tilesOf(p.n, edge)), p.tilesM = static_cast<uint32_t>(tilesOf(p.m, edge));
-        const uint64_t tiles = (aK ? mostTiles(p, edge) : (uint64_t)p.tilesM * p.groups) * p.tilesN;
+        const uint32_t rows = r355::LINEAR_ROWS[tile];
+        p.tilesN = static_cast<uint32_t>(tilesOf(p.n, r355::LINEAR_COLS[tile])), p.tilesM = static_cast<uint32_t>(tilesOf(p.m, rows));
+        const uint64_t tiles = (aK ? mostTiles(p, rows) : (uint64_t)p.tilesM * p.groups) * p.tilesN;
         if(tiles > r355::MAX_GROUPS)
             return tooMany(what);
         const uint32_t workgroups = static_cast<uint32_t>((tiles + 7u) / 8u * 8u);
         if(type == R355_F16)
-            r355::linearTilesF16(p, aK, bK, edge, any, workgroups, s);
+            r355::linearTilesF16(p, aK, bK, tile, workgroups, s);
         else
-            r355::linearTilesBF16(p, aK, bK, edge, any, workgroups, s);
+            r355::linearTilesBF16(p, aK, bK, tile, workgroups, s);
         return R355_OK;
+    }
+
+    uint64_t usable(const void* workspace, uint64_t bytes)
+    {
+        return workspace && r355::aligned(workspace, 16) ? bytes : 0u;
+    }
+
+    // one product on macro tiles
+    int launchTiles(int32_t type, const LinearParams& p, bool aK, bool bK, bool any, void* workspace, uint64_t workspaceBytes, hipStream_t s, const char* what)
+    {
+        const Plan plan = planOf(p, aK, any, usable(workspace, workspaceBytes));
+        if(plan.splits > 1u)
+        {
+            const uint64_t rowsY = aK ? p.rows : (uint64_t)p.m * p.groups;
+            const uint32_t pitch = pitchOf(p.n);
+            LinearParams   d     = p;
+            d.splits = plan.splits, d.y = static_cast<char*>(workspace), d.ldy = pitch, d.strideY = (uint64_t)p.m * pitch * 4u, d.strideSplit = rowsY * pitch * 4u, d.outF32 = 1u;
+            d.bias = d.gate = d.c = nullptr, d.z = nullptr, d.activation = R355_ACT_NONE;
+            if(const int rc = launchTile(type, d, aK, bK, plan.tile, s, what))
+                return rc;
+            LinearParams r = p;
+            r.splits       = plan.splits;
+            const dim3   grid(static_cast<uint32_t>(tilesOf(p.n, 1024u)), static_cast<uint32_t>(rowsY < 32768u ? rowsY : 32768u));
+            const float* sums   = static_cast<const float*>(workspace);
+            const auto   kernel = type == R355_F16 ? (p.outF32 ? linearReduce<_Float16, float> : linearReduce<_Float16, _Float16>)
+                                                   : (p.outF32 ? linearReduce<__bf16, float> : linearReduce<__bf16, __bf16>);
+            hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, r, sums, rowsY, pitch);
+            return R355_OK;
+        }
+        if(plan.tall == 0u)
+            return launchTile(type, p, aK, bK, plan.tile, s, what);
+        LinearParams first = p, rest = p;
+        first.rows = plan.tall, rest.rows = p.rows - plan.tall;
+        const uint64_t outBytes = p.outF32 ? 4u : 2u, by = plan.tall;
+        if(p.source)
+            rest.source += by;
+        else
+            rest.a += by * p.lda * 2u;
+        rest.y += by * p.ldy * outBytes;
+        rest.c = p.c ? p.c + by * p.ldc * outBytes : nullptr, rest.gate = p.gate ? p.gate + by * p.ldg * 2u : nullptr, rest.z = p.z ? p.z + by * p.ldz * 2u : nullptr;
+        if(const int rc = launchTile(type, first, aK, bK, plan.tile, s, what))
+            return rc;
+        return launchTile(type, rest, aK, bK, plan.rest, s, what);
     }
 
     bool evenRows(const void* at, uint32_t ld, uint32_t bytes) // rows on 16-byte boundaries
@@ -377,6 +578,56 @@ namespace
         const uint64_t parts = tilesOf(4u * r355::computeUnits(), strips * a.groups), most = tilesOf(a.rows, 16u * a.groups);
         return most == 0u ? 1u : parts < most ? parts : most;
     }
+
+    LinearParams forwardParams(const r355_linear_args& a)
+    {
+        LinearParams p{};
+        p.a = static_cast<const char*>(a.x), p.b = static_cast<const char*>(a.w), p.bias = static_cast<const char*>(a.bias), p.gate = static_cast<const char*>(a.gate);
+        p.c = static_cast<const char*>(a.c), p.y = static_cast<char*>(a.y), p.z = static_cast<char*>(a.z);
+        p.offsets = a.offsets, p.source = a.source, p.rows = a.rows, p.n = a.n, p.k = a.k, p.groups = a.groups, p.sourceRows = a.x_rows;
+        p.lda = a.ldx, p.ldb = a.ldw, p.ldy = a.ldy, p.ldz = a.ldz, p.ldg = a.ldg, p.ldc = a.ldc;
+        p.strideB = static_cast<uint64_t>(a.groups > 1u ? a.w_stride : 0) * 2u, p.splits = 1u, p.activation = a.activation, p.outF32 = a.out_type == R355_F32;
+        return p;
+    }
+    bool evenForward(const r355_linear_args& a)
+    {
+        return a.k % 8u == 0u && evenRows(a.x, a.ldx, 2) && evenRows(a.w, a.ldw, 2) && (a.groups == 1u || a.w_stride % 8 == 0);
+    }
+    bool fewRows(const r355_linear_args& a)
+    {
+        return a.rows / a.groups <= 16u;
+    }
+    LinearParams inputParams(const r355_linear_backward_args& a, const char* dz, uint32_t lddz)
+    {
+        LinearParams p{};
+        p.offsets = a.offsets, p.rows = a.rows, p.groups = a.groups, p.splits = 1u;
+        p.a = dz, p.lda = lddz, p.b = static_cast<const char*>(a.w), p.ldb = a.ldw, p.strideB = static_cast<uint64_t>(a.groups > 1u ? a.w_stride : 0) * 2u;
+        p.y = static_cast<char*>(a.dx), p.ldy = a.lddx, p.n = a.k, p.k = a.n;
+        return p;
+    }
+    LinearParams weightParams(const r355_linear_backward_args& a, const char* dz, uint32_t lddz)
+    {
+        LinearParams p{};
+        p.offsets = a.offsets, p.rows = a.rows, p.groups = a.groups, p.splits = 1u;
+        p.a = dz, p.lda = lddz, p.b = static_cast<const char*>(a.x), p.ldb = a.ldx, p.m = a.n, p.n = a.k;
+        p.y = static_cast<char*>(a.dw), p.ldy = a.lddw, p.strideY = static_cast<uint64_t>(a.groups > 1u ? a.dw_stride : 0) * r355::dtypeBytes(a.grad_type);
+        p.c = a.accumulate ? static_cast<const char*>(a.dw) : nullptr, p.ldc = a.lddw, p.strideC = p.strideY, p.outF32 = a.grad_type == R355_F32;
+        return p;
+    }
+    bool evenInput(const r355_linear_backward_args& a, const char* dz, uint32_t lddz)
+    {
+        return a.n % 8u == 0u && evenRows(dz, lddz, 2) && evenRows(a.w, a.ldw, 2) && (a.groups == 1u || a.w_stride % 8 == 0);
+    }
+    bool evenWeight(const r355_linear_backward_args& a, const char* dz, uint32_t lddz)
+    {
+        return evenRows(dz, lddz, 2) && evenRows(a.x, a.ldx, 2);
+    }
+    // what the sums of a split product take
+    size_t splitBytes(const LinearParams& p, bool aK, bool any)
+    {
+        const uint32_t splits = planOf(p, aK, any, ~0ull).splits;
+        return splits > 1u ? static_cast<size_t>((aK ? p.rows : (uint64_t)p.m * p.groups) * pitchOf(p.n) * 4u * splits) : 0u;
+    }
 } // namespace
 
 #define R355_TRY(call)          \
@@ -416,39 +667,51 @@ extern "C" int r355_linear(const r355_linear_args* args, void* stream)
         if(a.x_rows == 0 || (uint64_t)a.x_rows * a.ldx * 2u > 0x7FFFFFF0u)
             return r355::fail(R355_ERR_BAD_SIZE, "linear: rows taken by their numbers must be of 1 to 2^31 bytes of x, got %u rows %u elements apart", a.x_rows, a.ldx);
     }
-    LinearParams p{};
-    p.a = static_cast<const char*>(a.x), p.b = static_cast<const char*>(a.w), p.bias = static_cast<const char*>(a.bias), p.gate = static_cast<const char*>(a.gate);
-    p.c = static_cast<const char*>(a.c), p.y = static_cast<char*>(a.y), p.z = static_cast<char*>(a.z);
-    p.offsets = a.offsets, p.source = a.source, p.rows = a.rows, p.n = a.n, p.k = a.k, p.groups = a.groups, p.sourceRows = a.x_rows;
-    p.lda = a.ldx, p.ldb = a.ldw, p.ldy = a.ldy, p.ldz = a.ldz, p.ldg = a.ldg, p.ldc = a.ldc;
-    p.strideB = static_cast<uint64_t>(a.groups > 1u ? a.w_stride : 0) * 2u, p.splits = 1u, p.activation = a.activation, p.outF32 = a.out_type == R355_F32;
-    p.wide = a.n % 8u == 0u && evenRows(a.y, a.ldy, outBytes) && evenRows(a.c, a.ldc, outBytes) && evenRows(a.z, a.ldz, 2) && evenRows(a.gate, a.ldg, 2) && r355::aligned(a.bias, 16);
-    const bool        even = a.k % 8u == 0u && evenRows(a.x, a.ldx, 2) && evenRows(a.w, a.ldw, 2) && (a.groups == 1u || a.w_stride % 8 == 0);
-    const hipStream_t s    = static_cast<hipStream_t>(stream);
+    const LinearParams p    = forwardParams(a);
+    const bool         even = evenForward(a);
+    const hipStream_t  s    = static_cast<hipStream_t>(stream);
     r355::beginCall();
-    if(even && a.rows / a.groups <= 16u)
+    if(even && fewRows(a))
     {
         if(mostTiles(p, 16u) * tilesOf(p.n, 16u) > r355::MAX_GROUPS / 2u)
             return tooMany(what);
         a.in_type == R355_F16 ? launchFew<_Float16>(p, s) : launchFew<__bf16>(p, s);
     }
     else
-        R355_TRY(launchTiles(a.in_type, p, true, true, !even, s, what));
+        R355_TRY(launchTiles(a.in_type, p, true, true, !even, a.workspace, a.workspace_bytes, s, what));
     return r355::checkLaunch(what);
 }
 
 extern "C" size_t r355_linear_workspace_bytes(const r355_linear_args* args)
 {
-    (void)args;
-    return 0;
+    if(!args || args->rows == 0 || args->n == 0 || args->k == 0 || args->groups == 0 || (evenForward(*args) && fewRows(*args)))
+        return 0;
+    return splitBytes(forwardParams(*args), true, !evenForward(*args));
 }
 
 extern "C" size_t r355_linear_backward_workspace_bytes(const r355_linear_backward_args* args)
 {
-    if(!args || args->n == 0 || args->groups == 0 || !args->dbias)
+    if(!args || args->rows == 0 || args->n == 0 || args->k == 0 || args->groups == 0)
         return 0;
-    const uint64_t parts = gradParts(*args, static_cast<uint32_t>(tilesOf(args->n, 512u)));
-    return parts > 1u ? static_cast<size_t>(parts * args->groups * args->n * 4u) : 0u;
+    const r355_linear_backward_args& a = *args;
+    size_t                           most = 0u; // (one after the other)
+    if(a.dbias)
+        if(const uint64_t parts = gradParts(a, static_cast<uint32_t>(tilesOf(a.n, 512u))); parts > 1u)
+            most = static_cast<size_t>(parts * a.groups * a.n * 4u);
+    const bool     element = a.activation != R355_ACT_NONE || a.gate;
+    const char*    dz      = static_cast<const char*>(element ? a.dz : a.dy);
+    const uint32_t lddz    = element ? a.lddz : a.lddy;
+    if(a.dx)
+    {
+        const size_t bytes = splitBytes(inputParams(a, dz, lddz), true, !evenInput(a, dz, lddz));
+        most               = most > bytes ? most : bytes;
+    }
+    if(a.dw)
+    {
+        const size_t bytes = splitBytes(weightParams(a, dz, lddz), false, !evenWeight(a, dz, lddz));
+        most               = most > bytes ? most : bytes;
+    }
+    return most;
 }
 
 extern "C" int r355_linear_backward(const r355_linear_backward_args* args, void* stream)
@@ -497,7 +760,7 @@ extern "C" int r355_linear_backward(const r355_linear_backward_args* args, void*
         const bool     wide   = a.n % 8u == 0u && evenRows(a.dy, a.lddy, 2) && evenRows(a.z, a.ldz, 2) && evenRows(a.gate, a.ldg, 2) && evenRows(g.dz, a.lddz, 2) && evenRows(a.dgate, a.lddg, 2);
         const uint32_t strips = static_cast<uint32_t>(tilesOf(a.n, wide ? 512u : 64u));
         const uint64_t wanted = gradParts(a, strips);
-        const uint64_t fit    = !a.dbias ? wanted : a.workspace && r355::aligned(a.workspace, 16) ? a.workspace_bytes / ((uint64_t)a.groups * a.n * 4u) : 1u;
+        const uint64_t fit    = a.dbias ? usable(a.workspace, a.workspace_bytes) / ((uint64_t)a.groups * a.n * 4u) : wanted;
         const uint64_t parts  = wanted < fit ? wanted : fit ? fit : 1u;
         g.parts = static_cast<uint32_t>(parts);
         g.sums  = !a.dbias ? nullptr : parts > 1u ? static_cast<float*>(a.workspace) : a.dbias;
@@ -506,31 +769,18 @@ extern "C" int r355_linear_backward(const r355_linear_backward_args* args, void*
         const auto kernel = wide ? (f16 ? linearGrad<_Float16, 8> : linearGrad<__bf16, 8>) : (f16 ? linearGrad<_Float16, 1> : linearGrad<__bf16, 1>);
         hipLaunchKernelGGL(kernel, grid, block, 0, s, g);
         if(a.dbias && parts > 1u)
-            hipLaunchKernelGGL(linearGradSums, dim3(static_cast<uint32_t>(tilesOf(a.n, 256u)), a.groups), block, 0, s, static_cast<const float*>(a.workspace), a.dbias, g.parts, a.n,
+            hipLaunchKernelGGL(linearGradSums, dim3(static_cast<uint32_t>(tilesOf(a.n, 64u)), a.groups), block, 0, s, static_cast<const float*>(a.workspace), a.dbias, g.parts, a.n,
                                a.accumulate);
     }
     const char*    dz   = static_cast<const char*>(element ? a.dz : a.dy);
     const uint32_t lddz = element ? a.lddz : a.lddy;
-    LinearParams   p{};
-    p.offsets = a.offsets, p.rows = a.rows, p.groups = a.groups, p.splits = 1u;
     if(a.dx && a.rows)
     {
-        LinearParams d = p;
-        d.a = dz, d.lda = lddz, d.b = static_cast<const char*>(a.w), d.ldb = a.ldw, d.strideB = static_cast<uint64_t>(a.groups > 1u ? a.w_stride : 0) * 2u;
-        d.y = static_cast<char*>(a.dx), d.ldy = a.lddx, d.n = a.k, d.k = a.n;
-        d.wide          = a.k % 8u == 0u && evenRows(a.dx, a.lddx, 2);
-        const bool even = a.n % 8u == 0u && evenRows(dz, lddz, 2) && evenRows(a.w, a.ldw, 2) && (a.groups == 1u || a.w_stride % 8 == 0);
-        R355_TRY(launchTiles(a.in_type, d, true, false, !even, s, what));
+        R355_TRY(launchTiles(a.in_type, inputParams(a, dz, lddz), true, false, !evenInput(a, dz, lddz), a.workspace, a.workspace_bytes, s, what));
     }
     if(a.dw)
     {
-        LinearParams d = p;
-        d.a = dz, d.lda = lddz, d.b = static_cast<const char*>(a.x), d.ldb = a.ldx;
-        d.y = static_cast<char*>(a.dw), d.ldy = a.lddw, d.strideY = static_cast<uint64_t>(a.groups > 1u ? a.dw_stride : 0) * gradBytes, d.m = a.n, d.n = a.k;
-        d.c = a.accumulate ? static_cast<const char*>(a.dw) : nullptr, d.ldc = a.lddw, d.strideC = d.strideY, d.outF32 = a.grad_type == R355_F32;
-        d.wide          = a.k % 8u == 0u && evenRows(a.dw, a.lddw, gradBytes) && (a.groups == 1u || a.dw_stride * gradBytes % 16 == 0);
-        const bool even = evenRows(dz, lddz, 2) && evenRows(a.x, a.ldx, 2);
-        R355_TRY(launchTiles(a.in_type, d, false, false, !even, s, what));
+        R355_TRY(launchTiles(a.in_type, weightParams(a, dz, lddz), false, false, !evenWeight(a, dz, lddz), a.workspace, a.workspace_bytes, s, what));
     }
     return r355::checkLaunch(what);
 }

@@ -1,7 +1,7 @@
 // Products of a layer on macro tiles for gfx950: forward with bias, activation, gate and residual in the epilogue, and both gradients, for one
 // matrix of weights or for one per group of rows.  No counterpart in the reference.
 //
-// A macro tile of 32 WB x 32 WB results is four waves of 16 WB x 16 WB each, on v_mfma_f32_16x16x32 with the accumulators in place; a stage is 64 of the sum.  Operands go
+// A macro tile of 32 WM x 32 WN results is four waves of 16 WM x 16 WN each, on v_mfma_f32_16x16x32 with the accumulators in place; a stage is 64 of the sum.  Operands go
 // to LDS by direct loads in the images of operand_tile.hpp and come back whole or, where they are not contiguous along the sum, through transposing reads.  LDS
 // holds two images of A and three of B, so that loads run two stages ahead (B of the small tiles three).  The buffers go round at run time: the loop is one stage long, and
 // what that costs, an addition for each address of a read, hides behind matrix instructions (six stages unrolled, as the GEMM has them, would be 36 KB of code for each epilogue).
@@ -63,13 +63,13 @@ namespace
         uint64_t sumRow; // weights' gradient: first row of the group
     };
 
-    template <bool AK, uint32_t TILE>
+    template <bool AK, uint32_t ROWS, uint32_t COLS>
     __device__ __forceinline__ bool workOf(const LinearParams& p, Work& w)
     {
         uint32_t tm, tn, k;
         if constexpr(AK)
         {
-            GroupTiles<TILE> tiles{p};
+            GroupTiles<ROWS> tiles{p};
             const uint32_t   tilesM = tiles.total();
             if(!r355::tileCoordRange(blockIdx.x, tilesM, p.tilesN, 0u, tilesM * p.tilesN, false, tm, tn))
                 return false;
@@ -81,13 +81,13 @@ namespace
             if(!r355::tileCoordRange(blockIdx.x, p.groups * p.tilesM, p.tilesN, 0u, p.groups * p.tilesM * p.tilesN, false, tm, tn))
                 return false;
             w.group           = tm / p.tilesM;
-            w.first           = tm % p.tilesM * TILE;
-            w.rowsLeft        = p.m - w.first < TILE ? p.m - w.first : TILE;
+            w.first           = tm % p.tilesM * ROWS;
+            w.rowsLeft        = p.m - w.first < ROWS ? p.m - w.first : ROWS;
             const auto  rows  = r355::rowsOf(p, w.group);
             w.sumRow = rows.first, k = rows.count;
         }
-        w.col0     = tn * TILE;
-        w.colsLeft = p.n - w.col0 < TILE ? p.n - w.col0 : TILE;
+        w.col0     = tn * COLS;
+        w.colsLeft = p.n - w.col0 < COLS ? p.n - w.col0 : COLS;
         // (whole stages for every share but the last ones)
         const uint32_t stages = k / TK + (k % TK != 0u ? 1u : 0u), share = p.splits > 1u ? (stages + p.splits - 1u) / p.splits : stages;
         w.kFirst = (p.splits > 1u ? blockIdx.y * share : 0u) * TK;
@@ -100,42 +100,58 @@ namespace
         return true;
     }
 
-    // EW neighbouring elements of type E, as floats, from and to a buffer
-    template <typename E, uint32_t EW>
-    __device__ __forceinline__ void loadRow(__amdgpu_buffer_rsrc_t from, uint32_t offset, float (&v)[EW])
+    // Eight neighbouring elements of type E as they come from a buffer.  `whole`: all of them are there, and move as vectors whatever their alignment (the memory
+    // pipeline takes that).  Otherwise the lane's offset is outside, and with `some` (uniform: there are columns behind the last eight) its `left` < 8 elements move one by one.
+    template <typename E>
+    struct Eight
     {
-        if constexpr(EW == 1u && sizeof(E) == 2u)
-            v[0] = static_cast<float>(__builtin_bit_cast(E, static_cast<uint16_t>(__builtin_amdgcn_raw_buffer_load_b16(from, offset, 0, 0))));
-        else if constexpr(EW == 1u)
-            v[0] = __builtin_bit_cast(E, __builtin_amdgcn_raw_buffer_load_b32(from, offset, 0, 0));
-        else
+        static constexpr uint32_t PER = 16u / sizeof(E);
+        vec<E, PER>               w[8u / PER];
+        __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t from, uint32_t offset, bool whole, bool some, uint32_t left)
+        {
 #pragma unroll
-            for(uint32_t part = 0; part < EW * sizeof(E) / 16u; ++part)
-            {
-                const auto w = __builtin_bit_cast(vec<E, 16 / sizeof(E)>, __builtin_amdgcn_raw_buffer_load_b128(from, offset + part * 16u, 0, 0));
+            for(uint32_t part = 0; part < 8u / PER; ++part)
+                w[part] = __builtin_bit_cast(vec<E, PER>, __builtin_amdgcn_raw_buffer_load_b128(from, whole ? offset + part * 16u : OUTSIDE, 0, 0));
+            if(some && !whole)
 #pragma unroll
-                for(uint32_t e = 0; e < 16u / sizeof(E); ++e)
-                    v[part * (16u / sizeof(E)) + e] = static_cast<float>(w[e]);
-            }
-    }
-    template <typename E, uint32_t EW>
-    __device__ __forceinline__ void storeRow(__amdgpu_buffer_rsrc_t to, uint32_t offset, const float (&v)[EW])
+                for(uint32_t e = 0; e < 7u; ++e)
+                {
+                    const uint32_t at = e < left ? offset + e * static_cast<uint32_t>(sizeof(E)) : OUTSIDE;
+                    if constexpr(sizeof(E) == 2u)
+                        w[e / PER][e % PER] = __builtin_bit_cast(E, static_cast<uint16_t>(__builtin_amdgcn_raw_buffer_load_b16(from, at, 0, 0)));
+                    else
+                        w[e / PER][e % PER] = __builtin_bit_cast(E, __builtin_amdgcn_raw_buffer_load_b32(from, at, 0, 0));
+                }
+        }
+        __device__ __forceinline__ float operator[](uint32_t e) const
+        {
+            return static_cast<float>(w[e / PER][e % PER]);
+        }
+    };
+    template <typename E>
+    __device__ __forceinline__ void storeRow(__amdgpu_buffer_rsrc_t to, uint32_t offset, bool whole, bool some, uint32_t left, const float (&v)[8])
     {
-        constexpr int NT = 2; // nontemporal: written once
-        if constexpr(EW == 1u && sizeof(E) == 2u)
-            __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, static_cast<E>(v[0])), to, offset, 0, 0);
-        else if constexpr(EW == 1u)
-            __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, static_cast<E>(v[0])), to, offset, 0, 0);
-        else
+        constexpr int      NT  = 2; // nontemporal: written once
+        constexpr uint32_t PER = 16u / sizeof(E);
 #pragma unroll
-            for(uint32_t part = 0; part < EW * sizeof(E) / 16u; ++part)
+        for(uint32_t part = 0; part < 8u / PER; ++part)
+        {
+            vec<E, PER> w;
+#pragma unroll
+            for(uint32_t e = 0; e < PER; ++e)
+                w[e] = static_cast<E>(v[part * PER + e]);
+            // (the offset in the lane's register: gemm_tiled.hip says why)
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, w), to, whole ? offset + part * 16u : OUTSIDE, 0, NT);
+        }
+        if(some && !whole)
+#pragma unroll
+            for(uint32_t e = 0; e < 7u; ++e)
             {
-                vec<E, 16 / sizeof(E)> w;
-#pragma unroll
-                for(uint32_t e = 0; e < 16u / sizeof(E); ++e)
-                    w[e] = static_cast<E>(v[part * (16u / sizeof(E)) + e]);
-                // (the offset in the lane's register: gemm_tiled.hip says why)
-                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, w), to, offset + part * 16u, 0, NT);
+                const uint32_t at = e < left ? offset + e * static_cast<uint32_t>(sizeof(E)) : OUTSIDE;
+                if constexpr(sizeof(E) == 2u)
+                    __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, static_cast<E>(v[e])), to, at, 0, 0);
+                else
+                    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, static_cast<E>(v[e])), to, at, 0, 0);
             }
     }
 
@@ -147,135 +163,135 @@ namespace
         return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<char*>(addr), 0, static_cast<int>(__builtin_amdgcn_readfirstlane(records)), 0x00020000);
     }
 
-    // Results of one wave's tile of 16 WB x 16 WB, rows row0 .. and columns col0 .. of Y, `rows` x `cols` of them there: staged in f32 through the wave's own LDS, so that an
+    // Results of one wave's tile of 16 WM x 16 WN, rows row0 .. and columns col0 .. of Y, `rows` x `cols` of them there: staged in f32 through the wave's own LDS, so that an
     // access covers whole rows of the wave's tile and the epilogue is taken of sums that nothing has rounded.
     //   z = sum + bias;  y = act(z) gate + c     (FULL; otherwise y = sum + c)
     // each rounded once.  Rows and columns that are not there lie outside the buffers: no branch around an access.
-    template <uint32_t WB, uint32_t EW, bool FULL, typename Out>
-    __device__ __forceinline__ void storeWave(f32x4 (&acc)[WB][WB], const LinearParams& p, const Work& w, uint32_t rowIn, uint32_t colIn, uint32_t lane, char* scratch)
+    template <uint32_t WM, uint32_t WN, bool FULL, typename Out>
+    __device__ __forceinline__ void storeWave(f32x4 (&acc)[WM][WN], const LinearParams& p, const Work& w, uint32_t rowIn, uint32_t colIn, uint32_t lane, char* scratch)
     {
-        constexpr uint32_t WT = 16u * WB, ROW = WT * 4u, PASS = WT < 64u ? WT : 64u; // LDS bytes of a row, rows at a time
-        constexpr uint32_t SWZ = WB * 4u < 16u ? WB * 4u - 1u : 15u;
-        constexpr uint32_t LANES = WT / EW < 64u ? WT / EW : 64u, ACROSS = WT / EW / LANES, RPI = 64u / LANES; // lanes and accesses of a row, rows an access
-        constexpr uint32_t ITERS = PASS / RPI, BATCH = ITERS < 4u ? ITERS : 4u, OS = sizeof(Out);
+        constexpr uint32_t WT = 16u * WN, ROW = WT * 4u, PASS = 16u * WM < 64u ? 16u * WM : 64u; // LDS bytes of a row, rows at a time
+        constexpr uint32_t SWZ = WN * 4u < 16u ? WN * 4u - 1u : 15u;
+        constexpr uint32_t LANES = WT / 8u, RPI = 64u / LANES, ITERS = PASS / RPI; // lanes of a row, rows an access, accesses
+        constexpr uint32_t OS = sizeof(Out), MOST = OS == 4u ? 2u : 4u, BATCH = ITERS / 2u < MOST ? ITERS / 2u : MOST; // (more would not fit the registers)
         if(rowIn >= w.rowsLeft || colIn >= w.colsLeft)
             return; // (uniform)
-        const uint32_t rows = w.rowsLeft - rowIn < WT ? w.rowsLeft - rowIn : WT, cols = w.colsLeft - colIn < WT ? w.colsLeft - colIn : WT;
+        const uint32_t rows = w.rowsLeft - rowIn < 16u * WM ? w.rowsLeft - rowIn : 16u * WM, cols = w.colsLeft - colIn < WT ? w.colsLeft - colIn : WT;
         const uint64_t row0 = (uint64_t)w.first + rowIn;
-        const uint32_t col0 = w.col0 + colIn, r16 = lane & 15u, quad = lane >> 4, rowLane = lane / LANES, at = lane % LANES;
+        const uint32_t col0 = w.col0 + colIn, r16 = lane & 15u, quad = lane >> 4, rowLane = lane / LANES, col = lane % LANES * 8u;
+        const uint32_t left = col < cols ? cols - col : 0u; // columns of the lane
+        const bool     whole = left >= 8u, some = cols % 8u != 0u;
         // a share of a split sum goes to the workspace: [split][group, row of Y][column]
-        char* const y = p.y + (uint64_t)w.group * p.strideY + (p.splits > 1u ? (uint64_t)blockIdx.y * (p.groups * (uint64_t)p.m) * p.n * 4u : 0u);
+        char* const y = p.y + (uint64_t)w.group * p.strideY + (p.splits > 1u ? (uint64_t)blockIdx.y * p.strideSplit : 0u);
         const char* c = p.c ? p.c + (uint64_t)w.group * p.strideC : nullptr;
 
-        float bias[ACROSS][EW];
+        Eight<T> bias;
         if constexpr(FULL)
-        {
-            const auto from = rowsBuffer(p.bias, w.group, col0, p.n, p.bias ? 1u : 0u, cols, 2u);
+            bias.load(rowsBuffer(p.bias, w.group, col0, p.n, p.bias ? 1u : 0u, cols, 2u), col * 2u, whole, some, left);
 #pragma unroll
-            for(uint32_t h = 0; h < ACROSS; ++h)
-                loadRow<T, EW>(from, (at + h * LANES) * EW < cols ? (at + h * LANES) * EW * 2u : OUTSIDE, bias[h]);
-        }
-#pragma unroll
-        for(uint32_t pass = 0; pass < WT / PASS; ++pass)
+        for(uint32_t pass = 0; pass < 16u * WM / PASS; ++pass)
         {
-            const uint32_t left = pass * PASS < rows ? rows - pass * PASS : 0u, here = left < PASS ? left : PASS;
-            const uint64_t row  = row0 + pass * PASS;
+            const uint32_t under = pass * PASS < rows ? rows - pass * PASS : 0u, here = under < PASS ? under : PASS;
+            const uint64_t row   = row0 + pass * PASS;
+            const auto toY = rowsBuffer(y, row, col0, p.ldy, here, cols, OS);
+            const auto fromC = rowsBuffer(c, row, col0, p.ldc, c ? here : 0u, cols, OS);
+            const auto toZ = rowsBuffer(p.z, row, col0, p.ldz, FULL && p.z ? here : 0u, cols, 2u), fromG = rowsBuffer(p.gate, row, col0, p.ldg, FULL && p.gate ? here : 0u, cols, 2u);
+            // two batches of accesses in turn: what one reads is under way while the other is worked on
+            Eight<T>   gate[2][BATCH];
+            Eight<Out> add[2][BATCH];
+            auto request = [&](auto which, uint32_t b) __attribute__((always_inline)) {
+                constexpr uint32_t W = decltype(which)::value;
+                if(FULL && p.gate)
+#pragma unroll
+                    for(uint32_t u = 0; u < BATCH; ++u)
+                        gate[W][u].load(fromG, (((b + u) * RPI + rowLane) * p.ldg + col) * 2u, whole, some, left);
+                if(c)
+#pragma unroll
+                    for(uint32_t u = 0; u < BATCH; ++u)
+                        add[W][u].load(fromC, (((b + u) * RPI + rowLane) * p.ldc + col) * OS, whole, some, left);
+            };
+            auto finish = [&](auto which, uint32_t b) __attribute__((always_inline)) {
+                constexpr uint32_t W = decltype(which)::value;
+                float              sum[BATCH][8];
+#pragma unroll
+                for(uint32_t u = 0; u < BATCH; ++u)
+                {
+                    const uint32_t r = (b + u) * RPI + rowLane;
+#pragma unroll
+                    for(uint32_t part = 0; part < 2u; ++part)
+                    {
+                        const f32x4 v = *reinterpret_cast<const f32x4*>(scratch + r * ROW + (((col / 4u + part) ^ (r & SWZ)) * CHUNK));
+#pragma unroll
+                        for(uint32_t e = 0; e < 4u; ++e)
+                            sum[u][part * 4u + e] = v[e];
+                    }
+                }
+                if constexpr(FULL)
+                {
+#pragma unroll
+                    for(uint32_t u = 0; u < BATCH; ++u)
+#pragma unroll
+                        for(uint32_t e = 0; e < 8u; ++e)
+                            sum[u][e] += bias[e];
+                    if(p.z)
+#pragma unroll
+                        for(uint32_t u = 0; u < BATCH; ++u)
+                            storeRow<T>(toZ, (((b + u) * RPI + rowLane) * p.ldz + col) * 2u, whole, some, left, sum[u]);
+                    r355::withActivation(p.activation, [&](auto act) __attribute__((always_inline)) {
+#pragma unroll
+                        for(uint32_t u = 0; u < BATCH; ++u)
+#pragma unroll
+                            for(uint32_t e = 0; e < 8u; ++e)
+                                sum[u][e] = r355::activate<decltype(act)::value>(sum[u][e]);
+                    });
+                    if(p.gate)
+#pragma unroll
+                        for(uint32_t u = 0; u < BATCH; ++u)
+#pragma unroll
+                            for(uint32_t e = 0; e < 8u; ++e)
+                                sum[u][e] *= gate[W][u][e];
+                }
+                if(c)
+#pragma unroll
+                    for(uint32_t u = 0; u < BATCH; ++u)
+#pragma unroll
+                        for(uint32_t e = 0; e < 8u; ++e)
+                            sum[u][e] += add[W][u][e];
+#pragma unroll
+                for(uint32_t u = 0; u < BATCH; ++u)
+                    storeRow<Out>(toY, (((b + u) * RPI + rowLane) * p.ldy + col) * OS, whole, some, left, sum[u]);
+            };
+            constexpr std::integral_constant<uint32_t, 0> even;
+            constexpr std::integral_constant<uint32_t, 1> odd;
+            request(even, 0u);
 #pragma unroll
             for(uint32_t i = 0; i < PASS / 16u; ++i)
 #pragma unroll
-                for(uint32_t j = 0; j < WB; ++j)
+                for(uint32_t j = 0; j < WN; ++j)
                 {
                     const uint32_t r = 16u * i + r16;
                     *reinterpret_cast<f32x4*>(scratch + r * ROW + (((4u * j + quad) ^ (r & SWZ)) * CHUNK)) = acc[pass * (PASS / 16u) + i][j];
                 }
             __builtin_amdgcn_wave_barrier(); // the same wave reads back what it wrote (LDS is in order per wave)
-            const auto toY = rowsBuffer(y, row, col0, p.ldy, here, cols, OS);
-            const auto fromC = rowsBuffer(c, row, col0, p.ldc, c ? here : 0u, cols, OS);
-            const auto toZ = rowsBuffer(p.z, row, col0, p.ldz, FULL && p.z ? here : 0u, cols, 2u), fromG = rowsBuffer(p.gate, row, col0, p.ldg, FULL && p.gate ? here : 0u, cols, 2u);
-#pragma unroll
-            for(uint32_t h = 0; h < ACROSS; ++h)
-            {
-                const uint32_t col = (at + h * LANES) * EW;
-                const bool     in  = col < cols;
 #pragma unroll 1
-                for(uint32_t b = 0; b < ITERS; b += BATCH)
-                {
-                    if(b * RPI >= here)
-                        break; // (uniform)
-                    float gate[BATCH][EW], add[BATCH][EW], sum[BATCH][EW];
-                    if(FULL && p.gate)
-#pragma unroll
-                        for(uint32_t u = 0; u < BATCH; ++u)
-                            loadRow<T, EW>(fromG, in ? (((b + u) * RPI + rowLane) * p.ldg + col) * 2u : OUTSIDE, gate[u]);
-                    if(c)
-#pragma unroll
-                        for(uint32_t u = 0; u < BATCH; ++u)
-                            loadRow<Out, EW>(fromC, in ? (((b + u) * RPI + rowLane) * p.ldc + col) * OS : OUTSIDE, add[u]);
-#pragma unroll
-                    for(uint32_t u = 0; u < BATCH; ++u)
-                    {
-                        const uint32_t r = (b + u) * RPI + rowLane;
-                        if constexpr(EW == 1u)
-                            sum[u][0] = *reinterpret_cast<const float*>(scratch + r * ROW + (((col >> 2) ^ (r & SWZ)) * CHUNK) + (col & 3u) * 4u);
-                        else
-#pragma unroll
-                            for(uint32_t part = 0; part < EW / 4u; ++part)
-                            {
-                                const f32x4 v = *reinterpret_cast<const f32x4*>(scratch + r * ROW + (((col / 4u + part) ^ (r & SWZ)) * CHUNK));
-#pragma unroll
-                                for(uint32_t e = 0; e < 4u; ++e)
-                                    sum[u][part * 4u + e] = v[e];
-                            }
-                    }
-                    if constexpr(FULL)
-                    {
-#pragma unroll
-                        for(uint32_t u = 0; u < BATCH; ++u)
-#pragma unroll
-                            for(uint32_t e = 0; e < EW; ++e)
-                                sum[u][e] += bias[h][e];
-                        if(p.z)
-#pragma unroll
-                            for(uint32_t u = 0; u < BATCH; ++u)
-                                storeRow<T, EW>(toZ, in ? (((b + u) * RPI + rowLane) * p.ldz + col) * 2u : OUTSIDE, sum[u]);
-                        if(p.activation != R355_ACT_NONE)
-#pragma unroll
-                            for(uint32_t u = 0; u < BATCH; ++u)
-#pragma unroll
-                                for(uint32_t e = 0; e < EW; ++e)
-                                    sum[u][e] = r355::activate(p.activation, sum[u][e]);
-                        if(p.gate)
-#pragma unroll
-                            for(uint32_t u = 0; u < BATCH; ++u)
-#pragma unroll
-                                for(uint32_t e = 0; e < EW; ++e)
-                                    sum[u][e] *= gate[u][e];
-                    }
-                    if(c)
-#pragma unroll
-                        for(uint32_t u = 0; u < BATCH; ++u)
-#pragma unroll
-                            for(uint32_t e = 0; e < EW; ++e)
-                                sum[u][e] += add[u][e];
-#pragma unroll
-                    for(uint32_t u = 0; u < BATCH; ++u)
-                        storeRow<Out, EW>(toY, in ? (((b + u) * RPI + rowLane) * p.ldy + col) * OS : OUTSIDE, sum[u]);
-                }
+            for(uint32_t b = 0; b < ITERS && b * RPI < here; b += 2u * BATCH) // (uniform)
+            {
+                request(odd, b + BATCH);
+                finish(even, b);
+                if(b + 2u * BATCH < ITERS)
+                    request(even, b + 2u * BATCH);
+                finish(odd, b + BATCH);
             }
             __builtin_amdgcn_wave_barrier();
         }
     }
-    template <uint32_t WB, bool FULL>
-    __device__ __forceinline__ void storeTile(f32x4 (&acc)[WB][WB], const LinearParams& p, const Work& w, uint32_t rowIn, uint32_t colIn, uint32_t lane, char* scratch)
+    template <uint32_t WM, uint32_t WN, bool FULL>
+    __device__ __forceinline__ void storeTile(f32x4 (&acc)[WM][WN], const LinearParams& p, const Work& w, uint32_t rowIn, uint32_t colIn, uint32_t lane, char* scratch)
     {
-        if(p.wide && p.outF32)
-            storeWave<WB, 8, FULL, float>(acc, p, w, rowIn, colIn, lane, scratch);
-        else if(p.wide)
-            storeWave<WB, 8, FULL, T>(acc, p, w, rowIn, colIn, lane, scratch);
-        else if(p.outF32)
-            storeWave<WB, 1, FULL, float>(acc, p, w, rowIn, colIn, lane, scratch);
+        if(p.outF32)
+            storeWave<WM, WN, FULL, float>(acc, p, w, rowIn, colIn, lane, scratch);
         else
-            storeWave<WB, 1, FULL, T>(acc, p, w, rowIn, colIn, lane, scratch);
+            storeWave<WM, WN, FULL, T>(acc, p, w, rowIn, colIn, lane, scratch);
     }
 
     // A stage of an operand that has `valid` bytes of the sum left per row: past its end the loads write zeros (K-contiguous: by tailOffset, otherwise the buffer ends there)
@@ -286,29 +302,31 @@ namespace
                      0x00020000};
     }
 
-    template <bool AK, bool BK, uint32_t WB>
+    template <bool AK, bool BK, uint32_t WM, uint32_t WN>
     __device__ __forceinline__ void linearTile(const LinearParams& p)
     {
-        static_assert(WB == 8 || WB == 4 || WB == 2, "wave tiles of 128, 64 or 32");
-        constexpr uint32_t TILE = 32u * WB, WT = 16u * WB, OPER = TILE * STAGE_KB; // macro and wave tile; bytes of an operand's stage
-        constexpr uint32_t NS = WB * WB, XS = 2u * WB, QS = WB / 2u, LOAD_Q = QS > 2u ? 2u : QS - 1u;
+        constexpr uint32_t SIZE_A = 32u * WM * STAGE_KB, SIZE_B = 32u * WN * STAGE_KB; // bytes of the operands' stages
+        constexpr uint32_t FIRST_B = 2u * SIZE_A, LAST_B = FIRST_B + 2u * SIZE_B, LDS = FIRST_B + 3u * SIZE_B;
+        constexpr uint32_t NS = WM * WN, XS = WM + WN, BOTH = 2u * (WM < WN ? WM : WN); // matrix instructions and operand blocks of half a stage
         // the large tile's loads are dealt out over the whole stage, B two stages ahead; the small tiles', whose stages are a quarter as long and less, come in the
         // second half, B three stages ahead (gemm_tiled.hip has both measured)
-        constexpr bool     SPREAD = WB == 8u;
+        constexpr bool     SPREAD  = WM == 8u || WN == 8u;
         constexpr uint32_t B_AHEAD = SPREAD ? 2u : 3u;
-        __shared__ __attribute__((aligned(1024))) char lds[5u * OPER]; // A at 0 and OPER, B at 2, 3 and 4 OPER
+        constexpr uint32_t SCRATCH = 64u * WN * (16u * WM < 64u ? 16u * WM : 64u); // of a wave's part of the epilogue
+        static_assert(LDS <= 160u * 1024u && 4u * SCRATCH <= LDS, "what a CU has");
+        __shared__ __attribute__((aligned(1024))) char lds[LDS];
 
         Work w;
-        if(!workOf<AK, TILE>(p, w))
+        if(!workOf<AK, 32u * WM, 32u * WN>(p, w))
             return;
         const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1u;
         const uint32_t ldsBase = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
         const uint32_t dma     = ldsBase + wave * 64u * CHUNK;
 
-        uint32_t offA[WB], offB[WB], stepA, stepB, kByteA, kByteB;
+        uint32_t offA[WM], offB[WN], stepA, stepB, kByteA, kByteB;
         uint64_t stageA, stageB;
-        laneOffsets8<AK, WB, 2>(tid, p.lda, w.rowsLeft, offA, stepA, stageA, kByteA);
-        laneOffsets8<BK, WB, 2>(tid, p.ldb, w.colsLeft, offB, stepB, stageB, kByteB);
+        laneOffsets8<AK, WM, 2>(tid, p.lda, w.rowsLeft, offA, stepA, stageA, kByteA);
+        laneOffsets8<BK, WN, 2>(tid, p.ldb, w.colsLeft, offB, stepB, stageB, kByteB);
         uint64_t fromA, fromB;
         if constexpr(AK)
         {
@@ -316,7 +334,7 @@ namespace
             {
                 const uint32_t r = tid >> 3, slot = tid & 7u;
 #pragma unroll
-                for(uint32_t j = 0; j < WB; ++j)
+                for(uint32_t j = 0; j < WM; ++j)
                 {
                     const uint32_t row = r + 32u * j < w.rowsLeft ? r + 32u * j : w.rowsLeft - 1u, from = static_cast<uint32_t>(p.source[(uint64_t)w.first + row]);
                     offA[j]            = from < p.sourceRows ? from * p.lda * 2u + ((slot ^ swzK8(r)) * CHUNK) : OUTSIDE;
@@ -340,106 +358,122 @@ namespace
         auto issueA = [&](uint32_t s, uint32_t at) {
             const uint32_t valid = validOf(s);
 #pragma unroll
-            for(uint32_t j = 0; j < WB; ++j)
+            for(uint32_t j = 0; j < WM; ++j)
                 loadToLds(stageBuffer<AK>(addrA(s), valid, p.lda), tailA(j, valid), j * stepA, dma + at + j * THREADS * CHUNK);
         };
         auto issueB = [&](uint32_t s, uint32_t at) {
             const uint32_t valid = validOf(s);
 #pragma unroll
-            for(uint32_t j = 0; j < WB; ++j)
+            for(uint32_t j = 0; j < WN; ++j)
                 loadToLds(stageBuffer<BK>(addrB(s), valid, p.ldb), tailB(j, valid), j * stepB, dma + at + j * THREADS * CHUNK);
         };
 
         uint32_t rdA[8], rdB[8];
-        readOffsets8<AK, WB, 2>(wm, lane, rdA);
-        readOffsets8<BK, WB, 2>(wn, lane, rdB);
-        f32x4 acc[WB][WB];
+        readOffsets8<AK, WM, 2>(wm, lane, rdA);
+        readOffsets8<BK, WN, 2>(wn, lane, rdB);
+        f32x4 acc[WM][WN];
 #pragma unroll
-        for(uint32_t i = 0; i < WB; ++i)
+        for(uint32_t i = 0; i < WM; ++i)
 #pragma unroll
-            for(uint32_t j = 0; j < WB; ++j)
+            for(uint32_t j = 0; j < WN; ++j)
                 acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        i32x4 fa[2][WB], fb[2][WB];
-        // matrix instruction n of half a stage, in shells around block (0, 0), as the operand blocks A0 B0 A1 B1 ... come; the operands swapped: a lane holds four
-        // neighbouring columns of a row
+        i32x4 fa[2][WM], fb[2][WN];
+        // matrix instruction n of half a stage, in shells around block (0, 0) as the operand blocks come, A0 B0 A1 B1 ... and then the rest of the longer operand; the
+        // operands swapped: a lane holds four neighbouring columns of a row
         auto multiplyAt = [&](uint32_t half, uint32_t n) {
-            uint32_t d = 0;
-            while((d + 1u) * (d + 1u) <= n)
+            constexpr uint32_t LESS = BOTH / 2u;
+            uint32_t           d    = 0;
+            while(d < LESS && (d + 1u) * (d + 1u) <= n)
                 ++d;
-            const uint32_t r = n - d * d, i = r <= d ? d : r - d - 1u, j = r <= d ? r : d;
+            const uint32_t r = n - d * d, past = n - LESS * LESS;
+            const uint32_t i = n < LESS * LESS ? (r <= d ? d : r - d - 1u) : WM > WN ? LESS + past / LESS : past % LESS;
+            const uint32_t j = n < LESS * LESS ? (r <= d ? r : d) : WM > WN ? past % LESS : LESS + past / LESS;
             multiply(acc[i][j], fb[half][j], fa[half][i]);
         };
         auto readAt = [&](uint32_t atA, uint32_t atB, uint32_t half, uint32_t x, uint32_t part) {
-            if(x & 1u)
-                readBlock8<BK, WB, 2>(lds + atB, rdB, x >> 1, half, part, fb[half][x >> 1], 0u);
+            const bool     ofB = x < BOTH ? (x & 1u) != 0u : WN > WM;
+            const uint32_t i   = x < BOTH ? x >> 1 : x - BOTH / 2u;
+            if(ofB)
+                readBlock8<BK, WN, 2>(lds + atB, rdB, i, half, part, fb[half][i], 0u);
             else
-                readBlock8<AK, WB, 2>(lds + atA, rdA, x >> 1, half, part, fa[half][x >> 1], 0u);
+                readBlock8<AK, WM, 2>(lds + atA, rdA, i, half, part, fa[half][i], 0u);
         };
-        auto after = [](uint32_t at) { return at == 4u * OPER ? 2u * OPER : at + OPER; }; // B's buffers go round
+        auto after = [](uint32_t at) { return at == LAST_B ? FIRST_B : at + SIZE_B; }; // B's buffers go round
+        // matrix instructions firstOf(x) .. firstOf(x + 1) - 1 of half a stage go with operand block x, two at least; a load with the third of them, or the last
+        auto firstOf = [](uint32_t x) { return x * NS / XS; };
+        auto loadsAt = [&](uint32_t x, uint32_t n) {
+            const uint32_t q = n - firstOf(x), of = firstOf(x + 1u) - firstOf(x);
+            return q == (of > 2u ? 2u : of - 1u);
+        };
 
         // prologue: stages 0 and 1 (and B of stage 2) requested in the order that the loop keeps
         if constexpr(SPREAD)
         {
-            issueB(0u, 2u * OPER), issueA(0u, 0u), issueB(1u, 3u * OPER), issueA(1u, OPER);
-            waitVmcnt<2u * WB>();
+            issueB(0u, FIRST_B), issueA(0u, 0u), issueB(1u, FIRST_B + SIZE_B), issueA(1u, SIZE_A);
+            waitVmcnt<WM + WN>();
         }
         else
         {
-            issueA(0u, 0u), issueB(0u, 2u * OPER), issueA(1u, OPER), issueB(1u, 3u * OPER), issueB(2u, 4u * OPER);
-            waitVmcnt<3u * WB>();
+            issueA(0u, 0u), issueB(0u, FIRST_B), issueA(1u, SIZE_A), issueB(1u, FIRST_B + SIZE_B), issueB(2u, LAST_B);
+            waitVmcnt<WM + 2u * WN>();
         }
         ldsBarrier();
 #pragma unroll
         for(uint32_t x = 0; x < XS; ++x)
         {
-            readAt(0u, 2u * OPER, 0, x, 0);
-            readAt(0u, 2u * OPER, 0, x, 1);
+            readAt(0u, FIRST_B, 0, x, 0);
+            readAt(0u, FIRST_B, 0, x, 1);
         }
-        uint32_t aCur = 0u, bCur = 2u * OPER;
+        uint32_t aCur = 0u, bCur = FIRST_B;
         // One stage, its first half in registers: the second half arrives under the first's matrix instructions, then the first half of the next stage under the second's.
         // FULL: all that this stage requests lies inside the sum.
         auto stage = [&](auto full, uint32_t kt) {
             constexpr bool FULL = decltype(full)::value;
-            const uint32_t aNxt = aCur ^ OPER, bNxt = after(bCur), bTo = SPREAD ? after(bNxt) : bCur;
+            const uint32_t aNxt = SIZE_A - aCur, bNxt = after(bCur), bTo = SPREAD ? after(bNxt) : bCur;
             const uint32_t vB   = FULL ? STAGE_KB : validOf(kt + B_AHEAD);
             const i32x4    bufB = stageBuffer<BK>(addrB(kt + B_AHEAD), vB, p.ldb);
+            auto loadA = [&](i32x4 buf, uint32_t valid, uint32_t j) { loadToLds(buf, FULL ? offA[j] : tailA(j, valid), j * stepA, dma + aCur + j * THREADS * CHUNK); };
+            auto loadB = [&](uint32_t j) { loadToLds(bufB, FULL ? offB[j] : tailB(j, vB), j * stepB, dma + bTo + j * THREADS * CHUNK); };
 #pragma unroll
             for(uint32_t x = 0; x < XS; ++x)
 #pragma unroll
-                for(uint32_t q = 0; q < QS; ++q)
+                for(uint32_t n = firstOf(x); n < firstOf(x + 1u); ++n)
                 {
-                    multiplyAt(0, x * QS + q);
-                    if(q < 2u)
-                        readAt(aCur, bCur, 1, x, q);
-                    if constexpr(QS == 1u)
+                    multiplyAt(0, n);
+                    if(n - firstOf(x) < 2u)
+                        readAt(aCur, bCur, 1, x, n - firstOf(x));
+                    if constexpr(NS == XS)
                         readAt(aCur, bCur, 1, x, 1);
-                    if(SPREAD && q == LOAD_Q && (x & 1u))
-                        loadToLds(bufB, FULL ? offB[x >> 1] : tailB(x >> 1, vB), (x >> 1) * stepB, dma + bTo + (x >> 1) * THREADS * CHUNK);
+                    if(SPREAD && loadsAt(x, n))
+                        if(const uint32_t j = x * WN / XS; (x + 1u) * WN / XS > j)
+                            loadB(j);
                     __builtin_amdgcn_sched_barrier(0);
                 }
-            waitVmcnt<WB>(); // all but the youngest loads, B of stage kt + 2
+            waitVmcnt<WN>(); // all but the youngest loads, B of stage kt + 2
             ldsBarrier();
             const uint32_t vA   = FULL ? STAGE_KB : validOf(kt + 2u);
             const i32x4    bufA = stageBuffer<AK>(addrA(kt + 2u), vA, p.lda);
 #pragma unroll
             for(uint32_t x = 0; x < XS; ++x)
 #pragma unroll
-                for(uint32_t q = 0; q < QS; ++q)
+                for(uint32_t n = firstOf(x); n < firstOf(x + 1u); ++n)
                 {
-                    multiplyAt(1, x * QS + q);
-                    if(q < 2u)
-                        readAt(aNxt, bNxt, 0, x, q);
-                    if constexpr(QS == 1u)
+                    multiplyAt(1, n);
+                    if(n - firstOf(x) < 2u)
+                        readAt(aNxt, bNxt, 0, x, n - firstOf(x));
+                    if constexpr(NS == XS)
                         readAt(aNxt, bNxt, 0, x, 1);
-                    if(q == LOAD_Q)
+                    if(loadsAt(x, n))
                     {
-                        if(SPREAD ? (x & 1u) != 0u : x < WB)
+                        if constexpr(SPREAD)
                         {
-                            const uint32_t j = SPREAD ? x >> 1 : x;
-                            loadToLds(bufA, FULL ? offA[j] : tailA(j, vA), j * stepA, dma + aCur + j * THREADS * CHUNK);
+                            if(const uint32_t j = x * WM / XS; (x + 1u) * WM / XS > j)
+                                loadA(bufA, vA, j);
                         }
-                        else if(!SPREAD)
-                            loadToLds(bufB, FULL ? offB[x - WB] : tailB(x - WB, vB), (x - WB) * stepB, dma + bTo + (x - WB) * THREADS * CHUNK);
+                        else if(x < WM)
+                            loadA(bufA, vA, x);
+                        else
+                            loadB(x - WM);
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
@@ -457,24 +491,34 @@ namespace
         asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
         waitVmcnt<0>();
         ldsBarrier();
-        storeTile<WB, AK && BK>(acc, p, w, wm * WT, wn * WT, lane, lds + wave * (WB * 4096u));
+        storeTile<WM, WN, AK && BK>(acc, p, w, wm * 16u * WM, wn * 16u * WN, lane, lds + wave * SCRATCH);
     }
 
     // (a kernel per tile: the attribute cannot depend on a template parameter)
     template <bool AK, bool BK>
     __global__ void __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(1, 1))) linearTiles256(LinearParams p)
     {
-        linearTile<AK, BK, 8>(p);
+        linearTile<AK, BK, 8, 8>(p);
+    }
+    template <bool AK, bool BK>
+    __global__ void __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(1, 1))) linearTiles256x128(LinearParams p)
+    {
+        linearTile<AK, BK, 8, 4>(p);
+    }
+    template <bool AK, bool BK>
+    __global__ void __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(1, 1))) linearTiles128x256(LinearParams p)
+    {
+        linearTile<AK, BK, 4, 8>(p);
     }
     template <bool AK, bool BK>
     __global__ void __launch_bounds__(THREADS, 2) linearTiles128(LinearParams p)
     {
-        linearTile<AK, BK, 4>(p);
+        linearTile<AK, BK, 4, 4>(p);
     }
     template <bool AK, bool BK>
     __global__ void __launch_bounds__(THREADS, 4) linearTiles64(LinearParams p)
     {
-        linearTile<AK, BK, 2>(p);
+        linearTile<AK, BK, 2, 2>(p);
     }
 
     // The same on tiles of 64 x 64 for operands of any alignment, lengths and leading dimensions: loaded element by element through registers, 32 of the sum at a time.
@@ -485,7 +529,7 @@ namespace
         __shared__ __attribute__((aligned(16))) T   image[2][TILE * PITCH];
         __shared__ __attribute__((aligned(16))) char scratch[4u * 2u * 4096u];
         Work w;
-        if(!workOf<AK, TILE>(p, w))
+        if(!workOf<AK, TILE, TILE>(p, w))
             return;
         const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1u;
         // a thread's eight elements of a step: neighbours along the sum, or along the rows of Y (columns, for B)
@@ -554,34 +598,32 @@ namespace
                 for(uint32_t j = 0; j < 2u; ++j)
                     acc[i][j] = r355::mfma32<T>(fb[j], fa[i], acc[i][j]);
         }
-        storeTile<2, AK && BK>(acc, p, w, wm * 32u, wn * 32u, lane, scratch + wave * 8192u);
+        storeTile<2, 2, AK && BK>(acc, p, w, wm * 32u, wn * 32u, lane, scratch + wave * 8192u);
     }
 
     template <bool AK, bool BK>
-    void launch(const LinearParams& p, uint32_t tile, bool any, uint32_t workgroups, hipStream_t s)
+    void launch(const LinearParams& p, r355::LinearTile tile, uint32_t workgroups, hipStream_t s)
     {
-        const dim3 grid(workgroups, p.splits), block(THREADS);
-        if(any)
-            hipLaunchKernelGGL((linearAny<AK, BK>), grid, block, 0, s, p);
-        else if(tile == 256u)
-            hipLaunchKernelGGL((linearTiles256<AK, BK>), grid, block, 0, s, p);
-        else if(tile == 128u)
-            hipLaunchKernelGGL((linearTiles128<AK, BK>), grid, block, 0, s, p);
-        else
-            hipLaunchKernelGGL((linearTiles64<AK, BK>), grid, block, 0, s, p);
+        const auto kernel = tile == r355::TILE_256       ? linearTiles256<AK, BK>
+                            : tile == r355::TILE_256_128 ? linearTiles256x128<AK, BK>
+                            : tile == r355::TILE_128_256 ? linearTiles128x256<AK, BK>
+                            : tile == r355::TILE_128     ? linearTiles128<AK, BK>
+                            : tile == r355::TILE_64      ? linearTiles64<AK, BK>
+                                                         : linearAny<AK, BK>;
+        hipLaunchKernelGGL(kernel, dim3(workgroups, p.splits), dim3(THREADS), 0, s, p);
     }
 } // namespace
 
 #ifdef R355_LINEAR_BF16
-void r355::linearTilesBF16(const LinearParams& p, bool aK, bool bK, uint32_t tile, bool any, uint32_t workgroups, hipStream_t s)
+void r355::linearTilesBF16(const LinearParams& p, bool aK, bool bK, LinearTile tile, uint32_t workgroups, hipStream_t s)
 #else
-void r355::linearTilesF16(const LinearParams& p, bool aK, bool bK, uint32_t tile, bool any, uint32_t workgroups, hipStream_t s)
+void r355::linearTilesF16(const LinearParams& p, bool aK, bool bK, LinearTile tile, uint32_t workgroups, hipStream_t s)
 #endif
 {
     if(aK && bK)
-        launch<true, true>(p, tile, any, workgroups, s);
+        launch<true, true>(p, tile, workgroups, s);
     else if(aK)
-        launch<true, false>(p, tile, any, workgroups, s);
+        launch<true, false>(p, tile, workgroups, s);
     else
-        launch<false, false>(p, tile, any, workgroups, s);
+        launch<false, false>(p, tile, workgroups, s);
 }
