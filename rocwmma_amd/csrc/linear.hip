@@ -422,7 +422,7 @@ namespace
     Plan planOf(const LinearParams& p, bool aK, bool any, uint64_t workspaceBytes)
     {
         using namespace r355;
-        // (of ragged groups on average: half a tile of each is empty; a weights' gradient has their rows for its sum)
+        // (of ragged groups on average: half a tile of each is empty, of the largest tile, whose last one is as high as it has to be, a fifth; a weights' gradient has their rows for its sum)
         const double   stages = aK ? static_cast<double>(tilesOf(p.k, 64u)) : p.offsets ? static_cast<double>(p.rows) / p.groups / 64.0 + 0.5 : static_cast<double>(tilesOf(p.rows, 64u));
         const uint64_t rowsY  = aK ? p.rows : (uint64_t)p.m * p.groups;
         auto tiles = [&](uint32_t tile, uint64_t rows) {
@@ -432,7 +432,7 @@ namespace
             if(!p.offsets)
                 return static_cast<double>(tilesOf(rows, LINEAR_ROWS[tile])) * across;
             const double met = p.groups < rows ? p.groups : static_cast<double>(rows);
-            return (static_cast<double>(rows) / LINEAR_ROWS[tile] + 0.5 * met) * across;
+            return (static_cast<double>(rows) / LINEAR_ROWS[tile] + (tile == TILE_256 ? 0.2 : 0.5) * met) * across;
         };
         Plan best{any ? TILE_ANY : TILE_64, TILE_64, 1u, 0u, 1e30};
         for(uint32_t tile = any ? TILE_ANY : TILE_256; tile < (any ? LINEAR_TILES : TILE_ANY); ++tile)

@@ -100,59 +100,89 @@ namespace
         return true;
     }
 
-    // Eight neighbouring elements of type E as they come from a buffer.  `whole`: all of them are there, and move as vectors whatever their alignment (the memory
-    // pipeline takes that).  Otherwise the lane's offset is outside, and with `some` (uniform: there are columns behind the last eight) its `left` < 8 elements move one by one.
-    template <typename E>
+    // Where a lane's eight columns of a row lie: RUN = 8 neighbours, or two runs of 4, half of the row's width apart.  A run that is there as a whole moves as a vector, whatever its alignment
+    // (the memory pipeline takes that); one that is not lies outside the buffer, and with `some` (uniform: the last columns are not a whole run) its `left` elements move one by one.
+    template <uint32_t RUN>
+    struct Columns
+    {
+        uint32_t at[8 / RUN], left[8 / RUN];
+        bool     some;
+    };
+
+    // A lane's eight elements of type E of a row.
+    template <typename E, uint32_t RUN>
     struct Eight
     {
-        static constexpr uint32_t PER = 16u / sizeof(E);
+        static constexpr uint32_t PER = 16u / sizeof(E) < RUN ? 16u / sizeof(E) : RUN; // elements an access
         vec<E, PER>               w[8u / PER];
-        __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t from, uint32_t offset, bool whole, bool some, uint32_t left)
+        __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t from, uint32_t row, const Columns<RUN>& c) // row: byte offset
         {
 #pragma unroll
-            for(uint32_t part = 0; part < 8u / PER; ++part)
-                w[part] = __builtin_bit_cast(vec<E, PER>, __builtin_amdgcn_raw_buffer_load_b128(from, whole ? offset + part * 16u : OUTSIDE, 0, 0));
-            if(some && !whole)
+            for(uint32_t r = 0; r < 8u / RUN; ++r)
+            {
+                const uint32_t offset = row + c.at[r] * static_cast<uint32_t>(sizeof(E));
+                const bool     whole  = c.left[r] >= RUN;
 #pragma unroll
-                for(uint32_t e = 0; e < 7u; ++e)
+                for(uint32_t i = 0; i < RUN / PER; ++i)
                 {
-                    const uint32_t at = e < left ? offset + e * static_cast<uint32_t>(sizeof(E)) : OUTSIDE;
-                    if constexpr(sizeof(E) == 2u)
-                        w[e / PER][e % PER] = __builtin_bit_cast(E, static_cast<uint16_t>(__builtin_amdgcn_raw_buffer_load_b16(from, at, 0, 0)));
+                    const uint32_t at = whole ? offset + i * 16u : OUTSIDE;
+                    if constexpr(PER * sizeof(E) == 16u)
+                        w[r * (RUN / PER) + i] = __builtin_bit_cast(vec<E, PER>, __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, 0));
                     else
-                        w[e / PER][e % PER] = __builtin_bit_cast(E, __builtin_amdgcn_raw_buffer_load_b32(from, at, 0, 0));
+                        w[r * (RUN / PER) + i] = __builtin_bit_cast(vec<E, PER>, __builtin_amdgcn_raw_buffer_load_b64(from, at, 0, 0));
                 }
+                if(c.some && !whole)
+#pragma unroll
+                    for(uint32_t e = 0; e + 1u < RUN; ++e)
+                    {
+                        const uint32_t at = e < c.left[r] ? offset + e * static_cast<uint32_t>(sizeof(E)) : OUTSIDE, of = r * RUN + e;
+                        if constexpr(sizeof(E) == 2u)
+                            w[of / PER][of % PER] = __builtin_bit_cast(E, static_cast<uint16_t>(__builtin_amdgcn_raw_buffer_load_b16(from, at, 0, 0)));
+                        else
+                            w[of / PER][of % PER] = __builtin_bit_cast(E, __builtin_amdgcn_raw_buffer_load_b32(from, at, 0, 0));
+                    }
+            }
         }
         __device__ __forceinline__ float operator[](uint32_t e) const
         {
             return static_cast<float>(w[e / PER][e % PER]);
         }
     };
-    template <typename E>
-    __device__ __forceinline__ void storeRow(__amdgpu_buffer_rsrc_t to, uint32_t offset, bool whole, bool some, uint32_t left, const float (&v)[8])
+    template <typename E, uint32_t RUN>
+    __device__ __forceinline__ void storeRow(__amdgpu_buffer_rsrc_t to, uint32_t row, const Columns<RUN>& c, const float (&v)[8])
     {
         constexpr int      NT  = 2; // nontemporal: written once
-        constexpr uint32_t PER = 16u / sizeof(E);
+        constexpr uint32_t PER = Eight<E, RUN>::PER;
 #pragma unroll
-        for(uint32_t part = 0; part < 8u / PER; ++part)
+        for(uint32_t r = 0; r < 8u / RUN; ++r)
         {
-            vec<E, PER> w;
+            const uint32_t offset = row + c.at[r] * static_cast<uint32_t>(sizeof(E));
+            const bool     whole  = c.left[r] >= RUN;
 #pragma unroll
-            for(uint32_t e = 0; e < PER; ++e)
-                w[e] = static_cast<E>(v[part * PER + e]);
-            // (the offset in the lane's register: gemm_tiled.hip says why)
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, w), to, whole ? offset + part * 16u : OUTSIDE, 0, NT);
-        }
-        if(some && !whole)
-#pragma unroll
-            for(uint32_t e = 0; e < 7u; ++e)
+            for(uint32_t i = 0; i < RUN / PER; ++i)
             {
-                const uint32_t at = e < left ? offset + e * static_cast<uint32_t>(sizeof(E)) : OUTSIDE;
-                if constexpr(sizeof(E) == 2u)
-                    __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, static_cast<E>(v[e])), to, at, 0, 0);
+                vec<E, PER> w;
+#pragma unroll
+                for(uint32_t e = 0; e < PER; ++e)
+                    w[e] = static_cast<E>(v[r * RUN + i * PER + e]);
+                // (the offset in the lane's register: gemm_tiled.hip says why)
+                const uint32_t at = whole ? offset + i * 16u : OUTSIDE;
+                if constexpr(PER * sizeof(E) == 16u)
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, w), to, at, 0, NT);
                 else
-                    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, static_cast<E>(v[e])), to, at, 0, 0);
+                    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, w), to, at, 0, NT);
             }
+            if(c.some && !whole)
+#pragma unroll
+                for(uint32_t e = 0; e + 1u < RUN; ++e)
+                {
+                    const uint32_t at = e < c.left[r] ? offset + e * static_cast<uint32_t>(sizeof(E)) : OUTSIDE;
+                    if constexpr(sizeof(E) == 2u)
+                        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, static_cast<E>(v[r * RUN + e])), to, at, 0, 0);
+                    else
+                        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, static_cast<E>(v[r * RUN + e])), to, at, 0, 0);
+                }
+        }
     }
 
     // The buffer of `rows` rows of `cols` elements from (row, col) on, `bytes` an element: it ends with the last one
@@ -170,24 +200,28 @@ namespace
     template <uint32_t WM, uint32_t WN, bool FULL, typename Out>
     __device__ __forceinline__ void storeWave(f32x4 (&acc)[WM][WN], const LinearParams& p, const Work& w, uint32_t rowIn, uint32_t colIn, uint32_t lane, char* scratch)
     {
-        constexpr uint32_t WT = 16u * WN, ROW = WT * 4u, PASS = 16u * WM < 64u ? 16u * WM : 64u; // LDS bytes of a row, rows at a time
+        constexpr uint32_t WT = 16u * WN, ROW = WT * 4u, PASS = WM % 4u == 0u ? 64u : 32u; // LDS bytes of a row, rows at a time
         constexpr uint32_t SWZ = WN * 4u < 16u ? WN * 4u - 1u : 15u;
         constexpr uint32_t LANES = WT / 8u, RPI = 64u / LANES, ITERS = PASS / RPI; // lanes of a row, rows an access, accesses
+        constexpr uint32_t RUN = sizeof(Out) == 4u ? 4u : 8u; // (f32 in runs of 8 would leave every other 16 bytes to the next store: 16 products of 4096 x 1536 225 us, 199 so)
         constexpr uint32_t OS = sizeof(Out), MOST = OS == 4u ? 2u : 4u, BATCH = ITERS / 2u < MOST ? ITERS / 2u : MOST; // (more would not fit the registers)
         if(rowIn >= w.rowsLeft || colIn >= w.colsLeft)
             return; // (uniform)
         const uint32_t rows = w.rowsLeft - rowIn < 16u * WM ? w.rowsLeft - rowIn : 16u * WM, cols = w.colsLeft - colIn < WT ? w.colsLeft - colIn : WT;
         const uint64_t row0 = (uint64_t)w.first + rowIn;
-        const uint32_t col0 = w.col0 + colIn, r16 = lane & 15u, quad = lane >> 4, rowLane = lane / LANES, col = lane % LANES * 8u;
-        const uint32_t left = col < cols ? cols - col : 0u; // columns of the lane
-        const bool     whole = left >= 8u, some = cols % 8u != 0u;
+        const uint32_t col0 = w.col0 + colIn, r16 = lane & 15u, quad = lane >> 4, rowLane = lane / LANES;
+        Columns<RUN>   at;
+        at.some = cols % RUN != 0u;
+#pragma unroll
+        for(uint32_t r = 0; r < 8u / RUN; ++r)
+            at.at[r] = lane % LANES * RUN + r * LANES * RUN, at.left[r] = at.at[r] < cols ? cols - at.at[r] : 0u;
         // a share of a split sum goes to the workspace: [split][group, row of Y][column]
         char* const y = p.y + (uint64_t)w.group * p.strideY + (p.splits > 1u ? (uint64_t)blockIdx.y * p.strideSplit : 0u);
         const char* c = p.c ? p.c + (uint64_t)w.group * p.strideC : nullptr;
 
-        Eight<T> bias;
+        Eight<T, RUN> bias;
         if constexpr(FULL)
-            bias.load(rowsBuffer(p.bias, w.group, col0, p.n, p.bias ? 1u : 0u, cols, 2u), col * 2u, whole, some, left);
+            bias.load(rowsBuffer(p.bias, w.group, col0, p.n, p.bias ? 1u : 0u, cols, 2u), 0u, at);
 #pragma unroll
         for(uint32_t pass = 0; pass < 16u * WM / PASS; ++pass)
         {
@@ -197,18 +231,18 @@ namespace
             const auto fromC = rowsBuffer(c, row, col0, p.ldc, c ? here : 0u, cols, OS);
             const auto toZ = rowsBuffer(p.z, row, col0, p.ldz, FULL && p.z ? here : 0u, cols, 2u), fromG = rowsBuffer(p.gate, row, col0, p.ldg, FULL && p.gate ? here : 0u, cols, 2u);
             // two batches of accesses in turn: what one reads is under way while the other is worked on
-            Eight<T>   gate[2][BATCH];
-            Eight<Out> add[2][BATCH];
+            Eight<T, RUN>   gate[2][BATCH];
+            Eight<Out, RUN> add[2][BATCH];
             auto request = [&](auto which, uint32_t b) __attribute__((always_inline)) {
                 constexpr uint32_t W = decltype(which)::value;
                 if(FULL && p.gate)
 #pragma unroll
                     for(uint32_t u = 0; u < BATCH; ++u)
-                        gate[W][u].load(fromG, (((b + u) * RPI + rowLane) * p.ldg + col) * 2u, whole, some, left);
+                        gate[W][u].load(fromG, ((b + u) * RPI + rowLane) * p.ldg * 2u, at);
                 if(c)
 #pragma unroll
                     for(uint32_t u = 0; u < BATCH; ++u)
-                        add[W][u].load(fromC, (((b + u) * RPI + rowLane) * p.ldc + col) * OS, whole, some, left);
+                        add[W][u].load(fromC, ((b + u) * RPI + rowLane) * p.ldc * OS, at);
             };
             auto finish = [&](auto which, uint32_t b) __attribute__((always_inline)) {
                 constexpr uint32_t W = decltype(which)::value;
@@ -220,7 +254,8 @@ namespace
 #pragma unroll
                     for(uint32_t part = 0; part < 2u; ++part)
                     {
-                        const f32x4 v = *reinterpret_cast<const f32x4*>(scratch + r * ROW + (((col / 4u + part) ^ (r & SWZ)) * CHUNK));
+                        const uint32_t chunk = RUN == 8u ? at.at[0] / 4u + part : at.at[part % (8u / RUN)] / 4u;
+                        const f32x4    v     = *reinterpret_cast<const f32x4*>(scratch + r * ROW + ((chunk ^ (r & SWZ)) * CHUNK));
 #pragma unroll
                         for(uint32_t e = 0; e < 4u; ++e)
                             sum[u][part * 4u + e] = v[e];
@@ -236,7 +271,7 @@ namespace
                     if(p.z)
 #pragma unroll
                         for(uint32_t u = 0; u < BATCH; ++u)
-                            storeRow<T>(toZ, (((b + u) * RPI + rowLane) * p.ldz + col) * 2u, whole, some, left, sum[u]);
+                            storeRow<T>(toZ, ((b + u) * RPI + rowLane) * p.ldz * 2u, at, sum[u]);
                     r355::withActivation(p.activation, [&](auto act) __attribute__((always_inline)) {
 #pragma unroll
                         for(uint32_t u = 0; u < BATCH; ++u)
@@ -259,7 +294,7 @@ namespace
                             sum[u][e] += add[W][u][e];
 #pragma unroll
                 for(uint32_t u = 0; u < BATCH; ++u)
-                    storeRow<Out>(toY, (((b + u) * RPI + rowLane) * p.ldy + col) * OS, whole, some, left, sum[u]);
+                    storeRow<Out>(toY, ((b + u) * RPI + rowLane) * p.ldy * OS, at, sum[u]);
             };
             constexpr std::integral_constant<uint32_t, 0> even;
             constexpr std::integral_constant<uint32_t, 1> odd;
@@ -302,23 +337,24 @@ namespace
                      0x00020000};
     }
 
+    // bytes of LDS of a tile
+    constexpr uint32_t ldsOf(uint32_t wm, uint32_t wn)
+    {
+        return (2u * wm + 3u * wn) * 32u * STAGE_KB;
+    }
+
     template <bool AK, bool BK, uint32_t WM, uint32_t WN>
-    __device__ __forceinline__ void linearTile(const LinearParams& p)
+    __device__ __forceinline__ void linearTile(const LinearParams& p, const Work& w, char* lds)
     {
         constexpr uint32_t SIZE_A = 32u * WM * STAGE_KB, SIZE_B = 32u * WN * STAGE_KB; // bytes of the operands' stages
-        constexpr uint32_t FIRST_B = 2u * SIZE_A, LAST_B = FIRST_B + 2u * SIZE_B, LDS = FIRST_B + 3u * SIZE_B;
+        constexpr uint32_t FIRST_B = 2u * SIZE_A, LAST_B = FIRST_B + 2u * SIZE_B; // two buffers of A, three of B
         constexpr uint32_t NS = WM * WN, XS = WM + WN, BOTH = 2u * (WM < WN ? WM : WN); // matrix instructions and operand blocks of half a stage
         // the large tile's loads are dealt out over the whole stage, B two stages ahead; the small tiles', whose stages are a quarter as long and less, come in the
         // second half, B three stages ahead (gemm_tiled.hip has both measured)
         constexpr bool     SPREAD  = WM == 8u || WN == 8u;
         constexpr uint32_t B_AHEAD = SPREAD ? 2u : 3u;
-        constexpr uint32_t SCRATCH = 64u * WN * (16u * WM < 64u ? 16u * WM : 64u); // of a wave's part of the epilogue
-        static_assert(LDS <= 160u * 1024u && 4u * SCRATCH <= LDS, "what a CU has");
-        __shared__ __attribute__((aligned(1024))) char lds[LDS];
-
-        Work w;
-        if(!workOf<AK, 32u * WM, 32u * WN>(p, w))
-            return;
+        constexpr uint32_t SCRATCH = 64u * WN * (WM % 4u == 0u ? 64u : 32u); // of a wave's part of the epilogue
+        static_assert(ldsOf(WM, WN) <= 160u * 1024u && 4u * SCRATCH <= ldsOf(WM, WN), "what a CU has");
         const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1u;
         const uint32_t ldsBase = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
         const uint32_t dma     = ldsBase + wave * 64u * CHUNK;
@@ -399,8 +435,14 @@ namespace
                 readBlock8<AK, WM, 2>(lds + atA, rdA, i, half, part, fa[half][i], 0u);
         };
         auto after = [](uint32_t at) { return at == LAST_B ? FIRST_B : at + SIZE_B; }; // B's buffers go round
-        // matrix instructions firstOf(x) .. firstOf(x + 1) - 1 of half a stage go with operand block x, two at least; a load with the third of them, or the last
+        // matrix instructions firstOf(x) .. firstOf(x + 1) - 1 of half a stage go with operand block x, one at least: with the first two its reads, with the third, or the last, a load
         auto firstOf = [](uint32_t x) { return x * NS / XS; };
+        auto readsAt = [&](uint32_t atA, uint32_t atB, uint32_t half, uint32_t x, uint32_t n) {
+            if(n == firstOf(x))
+                readAt(atA, atB, half, x, 0);
+            if(n == firstOf(x) + 1u || firstOf(x + 1u) == firstOf(x) + 1u)
+                readAt(atA, atB, half, x, 1);
+        };
         auto loadsAt = [&](uint32_t x, uint32_t n) {
             const uint32_t q = n - firstOf(x), of = firstOf(x + 1u) - firstOf(x);
             return q == (of > 2u ? 2u : of - 1u);
@@ -440,10 +482,7 @@ namespace
                 for(uint32_t n = firstOf(x); n < firstOf(x + 1u); ++n)
                 {
                     multiplyAt(0, n);
-                    if(n - firstOf(x) < 2u)
-                        readAt(aCur, bCur, 1, x, n - firstOf(x));
-                    if constexpr(NS == XS)
-                        readAt(aCur, bCur, 1, x, 1);
+                    readsAt(aCur, bCur, 1, x, n);
                     if(SPREAD && loadsAt(x, n))
                         if(const uint32_t j = x * WN / XS; (x + 1u) * WN / XS > j)
                             loadB(j);
@@ -459,10 +498,7 @@ namespace
                 for(uint32_t n = firstOf(x); n < firstOf(x + 1u); ++n)
                 {
                     multiplyAt(1, n);
-                    if(n - firstOf(x) < 2u)
-                        readAt(aNxt, bNxt, 0, x, n - firstOf(x));
-                    if constexpr(NS == XS)
-                        readAt(aNxt, bNxt, 0, x, 1);
+                    readsAt(aNxt, bNxt, 0, x, n);
                     if(loadsAt(x, n))
                     {
                         if constexpr(SPREAD)
@@ -495,30 +531,57 @@ namespace
     }
 
     // (a kernel per tile: the attribute cannot depend on a template parameter)
+    // Of ragged rows, the last tile of a group takes a form as high as its rows (64 groups of 64 rows, 2048 x 2048: 112 -> 47 us with the weights at hand, 130 with those of each group from memory).
     template <bool AK, bool BK>
     __global__ void __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(1, 1))) linearTiles256(LinearParams p)
     {
-        linearTile<AK, BK, 8, 8>(p);
+        __shared__ __attribute__((aligned(1024))) char lds[ldsOf(8, 8)];
+        Work                                           w;
+        if(!workOf<AK, 256, 256>(p, w))
+            return;
+        if(!AK || w.rowsLeft > 192u)
+            linearTile<AK, BK, 8, 8>(p, w, lds);
+        else if constexpr(AK)
+        {
+            if(w.rowsLeft > 128u)
+                linearTile<AK, BK, 6, 8>(p, w, lds);
+            else if(w.rowsLeft > 64u)
+                linearTile<AK, BK, 4, 8>(p, w, lds);
+            else
+                linearTile<AK, BK, 2, 8>(p, w, lds);
+        }
     }
     template <bool AK, bool BK>
     __global__ void __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(1, 1))) linearTiles256x128(LinearParams p)
     {
-        linearTile<AK, BK, 8, 4>(p);
+        __shared__ __attribute__((aligned(1024))) char lds[ldsOf(8, 4)];
+        Work                                           w;
+        if(workOf<AK, 256, 128>(p, w))
+            linearTile<AK, BK, 8, 4>(p, w, lds);
     }
     template <bool AK, bool BK>
     __global__ void __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(1, 1))) linearTiles128x256(LinearParams p)
     {
-        linearTile<AK, BK, 4, 8>(p);
+        __shared__ __attribute__((aligned(1024))) char lds[ldsOf(4, 8)];
+        Work                                           w;
+        if(workOf<AK, 128, 256>(p, w))
+            linearTile<AK, BK, 4, 8>(p, w, lds);
     }
     template <bool AK, bool BK>
     __global__ void __launch_bounds__(THREADS, 2) linearTiles128(LinearParams p)
     {
-        linearTile<AK, BK, 4, 4>(p);
+        __shared__ __attribute__((aligned(1024))) char lds[ldsOf(4, 4)];
+        Work                                           w;
+        if(workOf<AK, 128, 128>(p, w))
+            linearTile<AK, BK, 4, 4>(p, w, lds);
     }
     template <bool AK, bool BK>
     __global__ void __launch_bounds__(THREADS, 4) linearTiles64(LinearParams p)
     {
-        linearTile<AK, BK, 2, 2>(p);
+        __shared__ __attribute__((aligned(1024))) char lds[ldsOf(2, 2)];
+        Work                                           w;
+        if(workOf<AK, 64, 64>(p, w))
+            linearTile<AK, BK, 2, 2>(p, w, lds);
     }
 
     // The same on tiles of 64 x 64 for operands of any alignment, lengths and leading dimensions: loaded element by element through registers, 32 of the sum at a time.

@@ -78,6 +78,15 @@ def test_groups(dtype, sizes):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("k", [64, 200, 328])
+def test_groups_on_large_tiles(k):
+    """Last tiles of 1 to 255 rows beside whole ones"""
+    sizes = [2300, 1, 64, 0, 65, 128, 129, 192, 193, 255, 256, 300, 100, 1500]
+    _run("bf16", "bf16", sum(sizes), 4000, k, act="silu", bias=True, gate=True, groups=len(sizes), offsets=_offsets(sizes))
+    _run("f16", "f32", sum(sizes), 4001, k, c=True, keep=True, groups=len(sizes), offsets=_offsets(sizes), source=[(13 * r + 5) % 999 for r in range(sum(sizes))], x_rows=999)
+
+
+@pytest.mark.gpu
 def test_groups_of_some_rows():
     """Offsets that begin after the first row and end before the last; a slice of the offsets is some of the experts"""
     _run("bf16", "bf16", 500, 72, 64, bias=True, groups=3, offsets=[17, 100, 100, 450], c=True, in_place=True)

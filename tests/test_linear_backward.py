@@ -64,6 +64,15 @@ def test_groups(dtype, sizes):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [64, 200, 328])
+def test_groups_on_large_tiles(n):
+    """Last tiles of 1 to 255 rows beside whole ones"""
+    sizes = [2300, 1, 64, 0, 65, 128, 129, 192, 193, 255, 256, 300, 100, 1500]
+    _run("bf16", "bf16", sum(sizes), n, 4000, act="silu", groups=len(sizes), offsets=_offsets(sizes), want=("dx",))
+    _run("f16", "f32", sum(sizes), n, 3000, groups=len(sizes), offsets=_offsets(sizes), workspace=_scratch())
+
+
+@pytest.mark.gpu
 def test_groups_of_some_rows():
     _run("bf16", "bf16", 500, 72, 64, act="relu", groups=3, offsets=[17, 100, 100, 450])
 
