@@ -114,6 +114,15 @@ class TreeAttentionArgs(ctypes.Structure):
 _TREE_ARGS = struct.Struct("=iIIIIIIIQQQQQqqqqqqqqQIIIiQQQIidQQ")
 
 
+# ... and for the calls of a feed-forward half (a call for a few rows takes about as long as what Python does for it: 9.5 us with structures, 5 so)
+_LINEAR_ARGS = struct.Struct("=iiiIIIIIQQQQQQQQQIIIIIIqQQ")
+_LINEAR_BACKWARD_ARGS = struct.Struct("=iiiiIIIIQQQQQQQQQQQIIIIIIIIIiqqQQ")
+_ROUTE_ARGS = struct.Struct("=iiiIIIIiQQQQQQQdQQ")
+_ROUTE_BACKWARD_ARGS = struct.Struct("=iiiIIIIIQQQQd")
+_COMBINE_ARGS = struct.Struct("=iIIIIiQQQQQIIIi")
+_DISPATCH_ARGS = struct.Struct("=iIIIIiQQQQQQIIIi")
+
+
 class LinearArgs(ctypes.Structure):
     _fields_ = [
         ("in_type", ctypes.c_int32), ("out_type", ctypes.c_int32), ("activation", ctypes.c_int32),
@@ -219,15 +228,15 @@ def lib():
         L.r355_rope_turns.argtypes = [u32, ctypes.c_double, ctypes.c_double, u32, ctypes.c_double, ctypes.c_double, vp]
         L.r355_tree_attention.argtypes = [ctypes.POINTER(TreeAttentionArgs), vp]
         L.r355_tree_attention_workspace_bytes.argtypes = [ctypes.POINTER(TreeAttentionArgs)]
-        L.r355_linear.argtypes = [ctypes.POINTER(LinearArgs), vp]
-        L.r355_linear_workspace_bytes.argtypes = [ctypes.POINTER(LinearArgs)]
-        L.r355_linear_backward.argtypes = [ctypes.POINTER(LinearBackwardArgs), vp]
-        L.r355_linear_backward_workspace_bytes.argtypes = [ctypes.POINTER(LinearBackwardArgs)]
-        L.r355_route.argtypes = [ctypes.POINTER(RouteArgs), vp]
+        L.r355_linear.argtypes = [vp, vp]
+        L.r355_linear_workspace_bytes.argtypes = [vp]
+        L.r355_linear_backward.argtypes = [vp, vp]
+        L.r355_linear_backward_workspace_bytes.argtypes = [vp]
+        L.r355_route.argtypes = [vp, vp]
         L.r355_route_workspace_bytes.argtypes = [u32, u32, u32]
-        L.r355_route_backward.argtypes = [ctypes.POINTER(RouteBackwardArgs), vp]
-        L.r355_combine.argtypes = [ctypes.POINTER(CombineArgs), vp]
-        L.r355_dispatch.argtypes = [ctypes.POINTER(DispatchArgs), vp]
+        L.r355_route_backward.argtypes = [vp, vp]
+        L.r355_combine.argtypes = [vp, vp]
+        L.r355_dispatch.argtypes = [vp, vp]
         L.r355_get_device_info.argtypes = [ctypes.POINTER(DeviceInfo)]
         L.r355_last_error.argtypes = []
         L.r355_version.argtypes = []
@@ -597,29 +606,35 @@ def tree_attention_workspace_bytes(a):
     return lib().r355_tree_attention_workspace_bytes(ctypes.byref(a))
 
 
-def _workspace(workspace, workspace_bytes):
-    """Address and bytes of a workspace"""
-    if workspace_bytes is None:
-        workspace_bytes = workspace.numel() * workspace.element_size() if hasattr(workspace, "numel") else 0
-    return _ptr(workspace), workspace_bytes
+def _workspace_size(workspace, workspace_bytes):
+    if workspace is None or workspace_bytes is not None:
+        return workspace_bytes or 0
+    return workspace.numel() * workspace.element_size() if hasattr(workspace, "numel") else 0
+
+
+def _linear_bytes(in_type, out_type, rows, n, k, x, w, y, bias, activation, gate, c, z, groups, offsets, source, x_rows, ldx, ldw, ldg, ldc, ldy, ldz, w_stride, workspace,
+                  workspace_bytes):
+    if ldw is None:
+        ldw = k
+    return _LINEAR_ARGS.pack(in_type, out_type, activation, rows, n, k, groups, rows if x_rows is None else x_rows, _ptr(x) or 0, _ptr(w) or 0, _ptr(bias) or 0, _ptr(gate) or 0,
+                             _ptr(c) or 0, _ptr(y) or 0, _ptr(z) or 0, _index("linear: offsets", offsets, 4, groups + 1) or 0, _index("linear: source", source, 4, rows) or 0,
+                             k if ldx is None else ldx, ldw, n if ldg is None else ldg, n if ldc is None else ldc, n if ldy is None else ldy, n if ldz is None else ldz,
+                             n * ldw if w_stride is None else w_stride, _ptr(workspace) or 0, _workspace_size(workspace, workspace_bytes))
 
 
 def linear_args(in_type, out_type, rows, n, k, x, w, y, bias=None, activation=ACT_NONE, gate=None, c=None, z=None, groups=1, offsets=None, source=None, x_rows=None, ldx=None,
                 ldw=None, ldg=None, ldc=None, ldy=None, ldz=None, w_stride=None, workspace=None, workspace_bytes=None):
-    ldw = k if ldw is None else ldw
-    at, size = _workspace(workspace, workspace_bytes)
-    return LinearArgs(in_type, out_type, activation, rows, n, k, groups, rows if x_rows is None else x_rows, _ptr(x), _ptr(w), _ptr(bias), _ptr(gate), _ptr(c), _ptr(y), _ptr(z),
-                      _index("linear: offsets", offsets, 4, groups + 1), _index("linear: source", source, 4, rows), k if ldx is None else ldx, ldw, n if ldg is None else ldg,
-                      n if ldc is None else ldc, n if ldy is None else ldy, n if ldz is None else ldz, n * ldw if w_stride is None else w_stride, at, size)
+    return LinearArgs.from_buffer_copy(_linear_bytes(in_type, out_type, rows, n, k, x, w, y, bias, activation, gate, c, z, groups, offsets, source, x_rows, ldx, ldw, ldg, ldc, ldy,
+                                                     ldz, w_stride, workspace, workspace_bytes))
 
 
 def linear(in_type, out_type, rows, n, k, x, w, y, bias=None, activation=ACT_NONE, gate=None, c=None, z=None, groups=1, offsets=None, source=None, x_rows=None, ldx=None,
            ldw=None, ldg=None, ldc=None, ldy=None, ldz=None, w_stride=None, workspace=None, workspace_bytes=None, stream=None):
     """y = activation(x W^T + bias) * gate + c for w [groups][n][k] (include/r355_wmma.h); rows offsets[e] .. offsets[e + 1] - 1 use group e, row r is row source[r] of x (of
     x_rows; default: rows) where source is given.  z: where the activation's argument is kept for linear_backward()."""
-    a = linear_args(in_type, out_type, rows, n, k, x, w, y, bias, activation, gate, c, z, groups, offsets, source, x_rows, ldx, ldw, ldg, ldc, ldy, ldz, w_stride, workspace,
-                    workspace_bytes)
-    rc = lib().r355_linear(ctypes.byref(a), None if stream is None else _stream_handle(stream))
+    a = _linear_bytes(in_type, out_type, rows, n, k, x, w, y, bias, activation, gate, c, z, groups, offsets, source, x_rows, ldx, ldw, ldg, ldc, ldy, ldz, w_stride, workspace,
+                      workspace_bytes)
+    rc = lib().r355_linear(a, None if stream is None else _stream_handle(stream))
     if rc != 0:
         _check(rc)
 
@@ -629,15 +644,22 @@ def linear_workspace_bytes(a):
     return lib().r355_linear_workspace_bytes(ctypes.byref(a))
 
 
+def _linear_backward_bytes(in_type, grad_type, rows, n, k, dy, x, w, dx, dw, dbias, z, activation, gate, dgate, dz, accumulate, groups, offsets, lddy, ldx, ldw, ldz, ldg, lddz, lddg,
+                           lddx, lddw, w_stride, dw_stride, workspace, workspace_bytes):
+    ldw, lddw = k if ldw is None else ldw, k if lddw is None else lddw
+    return _LINEAR_BACKWARD_ARGS.pack(
+        in_type, grad_type, activation, accumulate, rows, n, k, groups, _ptr(dy) or 0, _ptr(x) or 0, _ptr(w) or 0, _ptr(z) or 0, _ptr(gate) or 0, _ptr(dz) or 0, _ptr(dgate) or 0,
+        _ptr(dx) or 0, _ptr(dw) or 0, _floats("linear_backward: dbias", dbias, groups * n) or 0, _index("linear_backward: offsets", offsets, 4, groups + 1) or 0,
+        n if lddy is None else lddy, k if ldx is None else ldx, ldw, n if ldz is None else ldz, n if ldg is None else ldg, n if lddz is None else lddz, n if lddg is None else lddg,
+        k if lddx is None else lddx, lddw, 0, n * ldw if w_stride is None else w_stride, n * lddw if dw_stride is None else dw_stride, _ptr(workspace) or 0,
+        _workspace_size(workspace, workspace_bytes))
+
+
 def linear_backward_args(in_type, grad_type, rows, n, k, dy, x, w, dx=None, dw=None, dbias=None, z=None, activation=ACT_NONE, gate=None, dgate=None, dz=None, accumulate=False,
                          groups=1, offsets=None, lddy=None, ldx=None, ldw=None, ldz=None, ldg=None, lddz=None, lddg=None, lddx=None, lddw=None, w_stride=None, dw_stride=None,
                          workspace=None, workspace_bytes=None):
-    of_n, of_k = lambda ld: n if ld is None else ld, lambda ld: k if ld is None else ld  # noqa: E731
-    at, size = _workspace(workspace, workspace_bytes)
-    return LinearBackwardArgs(in_type, grad_type, activation, accumulate, rows, n, k, groups, _ptr(dy), _ptr(x), _ptr(w), _ptr(z), _ptr(gate), _ptr(dz), _ptr(dgate), _ptr(dx),
-                              _ptr(dw), _ptr(dbias), _index("linear_backward: offsets", offsets, 4, groups + 1), of_n(lddy), of_k(ldx), of_k(ldw), of_n(ldz), of_n(ldg),
-                              of_n(lddz), of_n(lddg), of_k(lddx), of_k(lddw), n * of_k(ldw) if w_stride is None else w_stride,
-                              n * of_k(lddw) if dw_stride is None else dw_stride, at, size)
+    return LinearBackwardArgs.from_buffer_copy(_linear_backward_bytes(in_type, grad_type, rows, n, k, dy, x, w, dx, dw, dbias, z, activation, gate, dgate, dz, accumulate, groups,
+                                                                      offsets, lddy, ldx, ldw, ldz, ldg, lddz, lddg, lddx, lddw, w_stride, dw_stride, workspace, workspace_bytes))
 
 
 def linear_backward(in_type, grad_type, rows, n, k, dy, x, w, dx=None, dw=None, dbias=None, z=None, activation=ACT_NONE, gate=None, dgate=None, dz=None, accumulate=False,
@@ -645,9 +667,9 @@ def linear_backward(in_type, grad_type, rows, n, k, dy, x, w, dx=None, dw=None, 
                     workspace=None, workspace_bytes=None, stream=None):
     """The gradients of linear() for dy (include/r355_wmma.h): those of dx, dw (grad_type), dbias (f32) and dgate that are given.  z: what linear() kept; dz: room for the gradient
     of that, needed with an activation or a gate; accumulate: dw and dbias are added to what is there."""
-    a = linear_backward_args(in_type, grad_type, rows, n, k, dy, x, w, dx, dw, dbias, z, activation, gate, dgate, dz, accumulate, groups, offsets, lddy, ldx, ldw, ldz, ldg, lddz,
-                             lddg, lddx, lddw, w_stride, dw_stride, workspace, workspace_bytes)
-    rc = lib().r355_linear_backward(ctypes.byref(a), None if stream is None else _stream_handle(stream))
+    a = _linear_backward_bytes(in_type, grad_type, rows, n, k, dy, x, w, dx, dw, dbias, z, activation, gate, dgate, dz, accumulate, groups, offsets, lddy, ldx, ldw, ldz, ldg, lddz,
+                               lddg, lddx, lddw, w_stride, dw_stride, workspace, workspace_bytes)
+    rc = lib().r355_linear_backward(a, None if stream is None else _stream_handle(stream))
     if rc != 0:
         _check(rc)
 
@@ -657,14 +679,25 @@ def linear_backward_workspace_bytes(a):
     return lib().r355_linear_backward_workspace_bytes(ctypes.byref(a))
 
 
+_F32_TYPES = set()  # the types of 32-bit floating numbers that have been met
+
+
 def _floats(name, t, count):
     """Address of `count` 32-bit floating numbers one after the other (a raw address is taken as it is)"""
-    if t is None or not hasattr(t, "dtype"):
+    if t is None:
+        return None
+    try:
+        if t.dtype in _F32_TYPES and t.is_cuda and t.is_contiguous() and t.numel() >= count:
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    if not hasattr(t, "dtype"):
         return t
     if str(t.dtype) not in ("torch.float32", "float32"):
         raise ValueError("%s must hold 32-bit floating numbers, got %s" % (name, t.dtype))
-    if not getattr(t, "is_cuda", False):
-        raise ValueError("%s must lie in device memory" % name)
+    _F32_TYPES.add(t.dtype)
+    if not hasattr(t, "is_cuda") or not (t.is_cuda or t.is_pinned()):
+        raise ValueError("%s must lie in device memory or in pinned host memory" % name)
     if not t.is_contiguous() or t.numel() < count:
         raise ValueError("%s must be %d contiguous elements, got %s with strides %s" % (name, count, tuple(t.shape), t.stride()))
     return t.data_ptr()
@@ -680,38 +713,41 @@ def route(dtype, tokens, experts, top, logits, weights, chosen, place, source, o
     """The `top` experts of each token by logits [tokens][experts] (plus bias, for the choice), their weights, and the rows in order of experts (include/r355_wmma.h): chosen, place
     [tokens][top], source [tokens * top], offsets [experts + 1], what linear(), dispatch() and combine() take."""
     slots = tokens * top
-    at, size = _workspace(workspace, workspace_bytes)
-    a = RouteArgs(dtype, score, chosen_only, tokens, experts, top, experts if ldl is None else ldl, _ptr(logits), _floats("route: bias", bias, experts),
-                  _floats("route: weights", weights, slots), _index("route: chosen", chosen, 4, slots), _index("route: place", place, 4, slots),
-                  _index("route: source", source, 4, slots), _index("route: offsets", offsets, 4, experts + 1), scale, at, size)
-    rc = lib().r355_route(ctypes.byref(a), None if stream is None else _stream_handle(stream))
+    a = _ROUTE_ARGS.pack(dtype, score, chosen_only, tokens, experts, top, experts if ldl is None else ldl, 0, _ptr(logits) or 0, _floats("route: bias", bias, experts) or 0,
+                         _floats("route: weights", weights, slots) or 0, _index("route: chosen", chosen, 4, slots) or 0, _index("route: place", place, 4, slots) or 0,
+                         _index("route: source", source, 4, slots) or 0, _index("route: offsets", offsets, 4, experts + 1) or 0, scale, _ptr(workspace) or 0,
+                         _workspace_size(workspace, workspace_bytes))
+    rc = lib().r355_route(a, None if stream is None else _stream_handle(stream))
     if rc != 0:
         _check(rc)
 
 
 def route_backward(dtype, tokens, experts, top, logits, chosen, dweights, dlogits, score=ROUTE_SOFTMAX, chosen_only=False, scale=1.0, ldl=None, ldd=None, stream=None):
     """dlogits [tokens][experts] for the gradient of the weights that route() gave to the experts chosen."""
-    a = RouteBackwardArgs(dtype, score, chosen_only, tokens, experts, top, experts if ldl is None else ldl, experts if ldd is None else ldd, _ptr(logits),
-                          _index("route_backward: chosen", chosen, 4, tokens * top), _floats("route_backward: dweights", dweights, tokens * top), _ptr(dlogits), scale)
-    rc = lib().r355_route_backward(ctypes.byref(a), None if stream is None else _stream_handle(stream))
+    a = _ROUTE_BACKWARD_ARGS.pack(dtype, score, chosen_only, tokens, experts, top, experts if ldl is None else ldl, experts if ldd is None else ldd, _ptr(logits) or 0,
+                                  _index("route_backward: chosen", chosen, 4, tokens * top) or 0, _floats("route_backward: dweights", dweights, tokens * top) or 0,
+                                  _ptr(dlogits) or 0, scale)
+    rc = lib().r355_route_backward(a, None if stream is None else _stream_handle(stream))
     if rc != 0:
         _check(rc)
 
 
 def combine(dtype, tokens, top, width, values, rows, place, y, weights=None, c=None, ldv=None, ldc=None, ldy=None, stream=None):
     """y[t] = sum_j weights[t][j] values[place[t][j]] + c[t] over the `rows` rows of values; weights: default ones."""
-    a = CombineArgs(dtype, tokens, top, width, rows, _ptr(values), _index("combine: place", place, 4, tokens * top), _floats("combine: weights", weights, tokens * top), _ptr(c),
-                    _ptr(y), width if ldv is None else ldv, width if ldc is None else ldc, width if ldy is None else ldy)
-    rc = lib().r355_combine(ctypes.byref(a), None if stream is None else _stream_handle(stream))
+    a = _COMBINE_ARGS.pack(dtype, tokens, top, width, rows, 0, _ptr(values) or 0, _index("combine: place", place, 4, tokens * top) or 0,
+                           _floats("combine: weights", weights, tokens * top) or 0, _ptr(c) or 0, _ptr(y) or 0, width if ldv is None else ldv, width if ldc is None else ldc,
+                           width if ldy is None else ldy, 0)
+    rc = lib().r355_combine(a, None if stream is None else _stream_handle(stream))
     if rc != 0:
         _check(rc)
 
 
 def dispatch(dtype, tokens, top, width, x, out, rows, place, weights=None, values=None, dweights=None, ldx=None, ldv=None, ldo=None, stream=None):
     """out[place[t][j]] = weights[t][j] x[t] (default: x[t]), of `rows` rows; with dweights also x[t] . values[place[t][j]], so that it is the gradient of combine() for x = dy."""
-    a = DispatchArgs(dtype, tokens, top, width, rows, _ptr(x), _index("dispatch: place", place, 4, tokens * top), _floats("dispatch: weights", weights, tokens * top), _ptr(values),
-                     _ptr(out), _floats("dispatch: dweights", dweights, tokens * top), width if ldx is None else ldx, width if ldv is None else ldv, width if ldo is None else ldo)
-    rc = lib().r355_dispatch(ctypes.byref(a), None if stream is None else _stream_handle(stream))
+    a = _DISPATCH_ARGS.pack(dtype, tokens, top, width, rows, 0, _ptr(x) or 0, _index("dispatch: place", place, 4, tokens * top) or 0,
+                            _floats("dispatch: weights", weights, tokens * top) or 0, _ptr(values) or 0, _ptr(out) or 0, _floats("dispatch: dweights", dweights, tokens * top) or 0,
+                            width if ldx is None else ldx, width if ldv is None else ldv, width if ldo is None else ldo, 0)
+    rc = lib().r355_dispatch(a, None if stream is None else _stream_handle(stream))
     if rc != 0:
         _check(rc)
 

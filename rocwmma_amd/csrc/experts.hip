@@ -57,7 +57,7 @@ namespace
         const float*   dweights;
         char*          dlogits;
         uint32_t       tokens, experts, top, ldl, ldd, blocks, perBlock;
-        int32_t        score, chosenOnly;
+        int32_t        score, chosenOnly, even; // even: rows of logits on the boundaries of what a lane reads of them
         float          scale;
     };
 
@@ -76,46 +76,53 @@ namespace
         return in ? __expf(v - (most == -INFINITY ? 0.0f : most)) : 0.0f;
     }
 
-    // One token a wave: expert lane + 64 i in v[i] of the lane.  `top` rounds of the largest key; a key orders numbers as integers, NaN below them.
+    // One token a wave: expert V lane + i in x[i] of the lane.  A key orders numbers as integers, NaN below them; every lane sorts its keys, and `top` rounds take the largest of
+    // the lanes' first ones, of the lowest lane that has it, which then moves up.  Bound by the vector instructions (some 15 a round).
     // What is returned lies in lane j for the j-th choice: its expert and its logit.
     template <uint32_t V>
     __device__ __forceinline__ void choose(const RouteParams& p, const float (&x)[V], uint32_t lane, uint32_t& expert, float& logit)
     {
-        uint32_t key[V];
+        uint32_t key[V], of[V]; // keys, and which of the lane's experts they are of
 #pragma unroll
         for(uint32_t i = 0; i < V; ++i)
         {
-            const uint32_t e  = lane + 64u * i;
+            const uint32_t e  = lane * V + i;
             const float    by = e < p.experts ? (p.bias ? x[i] + p.bias[e] : x[i]) + 0.0f : 0.0f; // (-0 counts as 0)
             const uint32_t b  = __float_as_uint(by);
             key[i] = e >= p.experts ? 0u : by != by ? 1u : (b & 0x80000000u) ? ~b : b | 0x80000000u; // (-infinity: 0x007FFFFF)
+            of[i]  = i;
         }
-        expert = 0u, logit = 0.0f;
+        // (neighbours change places only if the later one is larger: equal ones stay in the order of their experts)
+#pragma unroll
+        for(uint32_t end = V - 1u; end > 0u; --end)
+#pragma unroll
+            for(uint32_t i = 0; i < end; ++i)
+            {
+                const bool     swap = key[i + 1u] > key[i];
+                const uint32_t k = key[i], o = of[i];
+                key[i] = swap ? key[i + 1u] : k, key[i + 1u] = swap ? k : key[i + 1u];
+                of[i] = swap ? of[i + 1u] : o, of[i + 1u] = swap ? o : of[i + 1u];
+            }
+        expert = 0u;
         for(uint32_t j = 0; j < p.top; ++j)
         {
-            uint32_t best = key[0];
+            const uint32_t best = largest(key[0]);
+            const uint32_t l    = static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(__ballot(key[0] == best)))) - 1u;
+            const uint32_t e    = l * V + __builtin_amdgcn_readlane(of[0], l);
+            expert              = lane == j ? e : expert;
+            const bool moves    = lane == l;
 #pragma unroll
-            for(uint32_t i = 1; i < V; ++i)
-                best = best > key[i] ? best : key[i];
-            best = largest(best);
-            // the lowest expert that has it
-            bool     found = false;
-            uint32_t who = 0u;
-            float    of = 0.0f;
+            for(uint32_t i = 0; i + 1u < V; ++i)
+                key[i] = moves ? key[i + 1u] : key[i], of[i] = moves ? of[i + 1u] : of[i];
+            key[V - 1u] = moves ? 0u : key[V - 1u];
+        }
+        // the logit of the lane's choice lies with lane expert / V
+        logit = 0.0f;
 #pragma unroll
-            for(uint32_t i = 0; i < V; ++i)
-            {
-                const uint64_t have = __ballot(key[i] == best);
-                if(!found && have != 0u) // (uniform)
-                {
-                    const uint32_t l = static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(have))) - 1u;
-                    found = true, who = l + 64u * i;
-                    of = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x[i]), l));
-                    key[i] = lane == l ? 0u : key[i];
-                }
-            }
-            if(lane == j)
-                expert = who, logit = of;
+        for(uint32_t i = 0; i < V; ++i)
+        {
+            const float v = __uint_as_float(__builtin_amdgcn_ds_bpermute(static_cast<int>(expert / V * 4u), static_cast<int>(__float_as_uint(x[i]))));
+            logit         = expert % V == i ? v : logit;
         }
     }
 
@@ -135,22 +142,62 @@ namespace
         float most = -INFINITY, all = 0.0f;
 #pragma unroll
         for(uint32_t i = 0; i < V; ++i)
-            most = fmaxf(most, lane + 64u * i < p.experts ? x[i] : -INFINITY);
+            most = fmaxf(most, lane * V + i < p.experts ? x[i] : -INFINITY);
         most = largest(most);
 #pragma unroll
         for(uint32_t i = 0; i < V; ++i)
-            all += exponentials(x[i], lane + 64u * i < p.experts, most);
+            all += exponentials(x[i], lane * V + i < p.experts, most);
         all = sum(all);
         return all == 0.0f ? 0.0f : exponentials(logit, in, most) / all * p.scale;
     }
 
+    // experts V lane .. V lane + V - 1 of a token: as vectors where the rows are even (a rule of the host's)
     template <typename T, uint32_t V>
     __device__ __forceinline__ void readLogits(const RouteParams& p, uint32_t token, uint32_t lane, float (&x)[V])
     {
-        const T* from = reinterpret_cast<const T*>(p.logits) + (uint64_t)token * p.ldl;
+        const T* from = reinterpret_cast<const T*>(p.logits) + (uint64_t)token * p.ldl + lane * V;
+        if(V > 1u && p.even)
+        {
+            constexpr uint32_t PER = V * sizeof(T) > 16u ? 16u / sizeof(T) : V;
 #pragma unroll
-        for(uint32_t i = 0; i < V; ++i)
-            x[i] = lane + 64u * i < p.experts ? static_cast<float>(from[lane + 64u * i]) : 0.0f;
+            for(uint32_t i = 0; i < V; i += PER)
+            {
+                vec<T, PER> v{};
+                if(lane * V + i < p.experts)
+                    v = *reinterpret_cast<const vec<T, PER>*>(from + i);
+#pragma unroll
+                for(uint32_t e = 0; e < PER; ++e)
+                    x[i + e] = static_cast<float>(v[e]);
+            }
+        }
+        else
+#pragma unroll
+            for(uint32_t i = 0; i < V; ++i)
+                x[i] = lane * V + i < p.experts ? static_cast<float>(from[i]) : 0.0f;
+    }
+    template <typename T, uint32_t V>
+    __device__ __forceinline__ void writeLogits(const RouteParams& p, uint32_t token, uint32_t lane, const float (&d)[V])
+    {
+        T* to = reinterpret_cast<T*>(p.dlogits) + (uint64_t)token * p.ldd + lane * V;
+        if(V > 1u && p.even)
+        {
+            constexpr uint32_t PER = V * sizeof(T) > 16u ? 16u / sizeof(T) : V;
+#pragma unroll
+            for(uint32_t i = 0; i < V; i += PER)
+            {
+                vec<T, PER> v;
+#pragma unroll
+                for(uint32_t e = 0; e < PER; ++e)
+                    v[e] = static_cast<T>(d[i + e]);
+                if(lane * V + i < p.experts)
+                    *reinterpret_cast<vec<T, PER>*>(to + i) = v;
+            }
+        }
+        else
+#pragma unroll
+            for(uint32_t i = 0; i < V; ++i)
+                if(lane * V + i < p.experts)
+                    to[i] = static_cast<T>(d[i]);
     }
 
     // The block's slots (token, choice) in order, a contiguous run of them for each wave: row = base[expert] + how many slots before have the same expert.
@@ -243,12 +290,19 @@ namespace
         __syncthreads();
         const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const uint32_t from = blockIdx.x * p.perBlock, left = p.tokens - from, here = left < p.perBlock ? left : p.perBlock;
+        float next[V]; // the following token's, read ahead
+        if(wave < here)
+            readLogits<T, V>(p, from + wave, lane, next);
         for(uint32_t i = wave; i < here; i += WAVES)
         {
             const uint32_t token = from + i;
             float          x[V], logit;
             uint32_t       expert;
-            readLogits<T, V>(p, token, lane, x);
+#pragma unroll
+            for(uint32_t e = 0; e < V; ++e)
+                x[e] = next[e];
+            if(i + WAVES < here)
+                readLogits<T, V>(p, token + WAVES, lane, next);
             choose<V>(p, x, lane, expert, logit);
             const float weight = weightOf<V>(p, x, lane, logit);
             if(lane < p.top)
@@ -272,23 +326,37 @@ namespace
                 p.counts[(uint64_t)e * p.blocks + blockIdx.x] = counts[e];
     }
 
-    // Of one expert: how many rows the blocks before each have, and the total; a wave
+    // Of one expert: how many rows the blocks before each have, and the total; a wave, a run of 16 blocks a lane at a time
     __global__ void __launch_bounds__(64) routeCounts(RouteParams p)
     {
-        uint32_t* const counts = p.counts + (uint64_t)blockIdx.x * p.blocks;
-        uint32_t        before = 0u;
-        for(uint32_t b0 = 0; b0 < p.blocks; b0 += 64u)
+        constexpr uint32_t RUN    = 16u;
+        uint32_t* const    counts = p.counts + (uint64_t)blockIdx.x * p.blocks;
+        uint32_t           before = 0u;
+        for(uint32_t b0 = 0; b0 < p.blocks; b0 += 64u * RUN)
         {
-            const uint32_t b = b0 + threadIdx.x, mine = b < p.blocks ? counts[b] : 0u;
-            uint32_t       upto = mine;
+            const uint32_t b = b0 + threadIdx.x * RUN;
+            uint32_t       mine[RUN], all = 0u;
+#pragma unroll
+            for(uint32_t i = 0; i < RUN; ++i)
+                mine[i] = b + i < p.blocks ? counts[b + i] : 0u;
+#pragma unroll
+            for(uint32_t i = 0; i < RUN; ++i)
+                all += mine[i];
+            uint32_t upto = all;
 #pragma unroll
             for(uint32_t d = 1u; d < 64u; d <<= 1)
             {
                 const uint32_t below = __shfl_up(upto, d);
                 upto += threadIdx.x >= d ? below : 0u;
             }
-            if(b < p.blocks)
-                counts[b] = before + upto - mine;
+            uint32_t at = before + upto - all;
+#pragma unroll
+            for(uint32_t i = 0; i < RUN; ++i)
+            {
+                if(b + i < p.blocks)
+                    counts[b + i] = at;
+                at += mine[i];
+            }
             before += __builtin_amdgcn_readlane(upto, 63);
         }
         if(threadIdx.x == 0u)
@@ -346,11 +414,11 @@ namespace
         {
 #pragma unroll
             for(uint32_t i = 0; i < V; ++i)
-                most = fmaxf(most, lane + 64u * i < p.experts ? x[i] : -INFINITY);
+                most = fmaxf(most, lane * V + i < p.experts ? x[i] : -INFINITY);
             most = largest(most);
 #pragma unroll
             for(uint32_t i = 0; i < V; ++i)
-                all += exponentials(x[i], lane + 64u * i < p.experts, most);
+                all += exponentials(x[i], lane * V + i < p.experts, most);
             all = sum(all);
             g   = in && all != 0.0f ? dw * p.scale * exponentials(logit, true, most) / all : 0.0f;
             off = all == 0.0f ? 0.0f : sum(g) / all;
@@ -360,20 +428,16 @@ namespace
         float d[V];
 #pragma unroll
         for(uint32_t i = 0; i < V; ++i)
-            d[i] = off == 0.0f ? 0.0f : -off * exponentials(x[i], lane + 64u * i < p.experts, most);
+            d[i] = off == 0.0f ? 0.0f : -off * exponentials(x[i], lane * V + i < p.experts, most);
         for(uint32_t j = 0; j < p.top; ++j) // (one after the other: an expert given twice gets both)
         {
             const uint32_t e = __builtin_amdgcn_readlane(expert, j);
             const float    v = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(g), j));
 #pragma unroll
             for(uint32_t i = 0; i < V; ++i)
-                d[i] += lane + 64u * i == e ? v : 0.0f;
+                d[i] += lane * V + i == e ? v : 0.0f;
         }
-        T* to = reinterpret_cast<T*>(p.dlogits) + (uint64_t)token * p.ldd;
-#pragma unroll
-        for(uint32_t i = 0; i < V; ++i)
-            if(lane + 64u * i < p.experts)
-                to[lane + 64u * i] = static_cast<T>(d[i]);
+        writeLogits<T, V>(p, token, lane, d);
     }
 
     // ---- rows to the experts and back
@@ -569,9 +633,18 @@ namespace
     {
         hipLaunchKernelGGL((routeGrad<T, V>), dim3((p.tokens + WAVES - 1u) / WAVES), dim3(THREADS), 0, s, p);
     }
+    // rows whose lanes read vectors: those of V elements, up to 16 bytes, begin on their boundaries and end with one
     template <typename T>
-    void launchRouteType(const RouteParams& p, bool gradient, hipStream_t s)
+    bool evenRows(const void* at, uint32_t ld, uint32_t experts)
     {
+        const uint32_t v = experts <= 64u ? 1u : experts <= 128u ? 2u : experts <= 256u ? 4u : 16u, per = v * sizeof(T) > 16u ? 16u / sizeof(T) : v;
+        return !at || (r355::aligned(at, per * sizeof(T)) && ld % per == 0u && experts % per == 0u);
+    }
+
+    template <typename T>
+    void launchRouteType(RouteParams p, bool gradient, hipStream_t s)
+    {
+        p.even = evenRows<T>(p.logits, p.ldl, p.experts) && evenRows<T>(p.dlogits, p.ldd, p.experts);
         if(p.experts <= 64u)
             gradient ? launchRouteGrad<T, 1>(p, s) : launchRoute<T, 1>(p, s);
         else if(p.experts <= 128u)

@@ -25,9 +25,208 @@ namespace
 
     constexpr uint32_t WAVES = 8u;
 
+    // ---- One or two rows of each group: dot products.  A wave takes 16 weight rows, each lane 16 bytes of every row at a time, so that an access is 1 KiB of one row (the matrix instructions'
+    // operands are 64 bytes of each of 16 rows: 16 experts of 4096 x 4096 105 us instead of 84).  Pieces of 512 of the sum go to WK waves in turn, other
+    // waves have other rows.  Bound by HBM.
+    //
+    // A lane's 16 T sums become one sum of the wave in each lane: of a pair of sums each half of the lanes keeps one and adds the other half's part of it, and so on by halves,
+    // about 16 T additions instead of 6 for each sum.  After the steps over lanes 32, 16, 8 and 4 apart lane l has sum 8 (l / 4 % 2) + 4 (l / 8 % 2) + 2 (l / 16 % 2) + l / 32 of 16.
+    __device__ __forceinline__ float other(float v, uint32_t distance) // the lane's that is so far away
+    {
+        if(distance == 8u)
+            return __uint_as_float(static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(__float_as_uint(v)), 0x128, 0xF, 0xF, true))); // row_ror:8
+        if(distance == 2u)
+            return __uint_as_float(static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(__float_as_uint(v)), 0x4E, 0xF, 0xF, true))); // quad_perm [2, 3, 0, 1]
+        if(distance == 1u)
+            return __uint_as_float(static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(__float_as_uint(v)), 0xB1, 0xF, 0xF, true))); // quad_perm [1, 0, 3, 2]
+        return __shfl_xor(v, static_cast<int>(distance));
+    }
+    template <uint32_t N>
+    __device__ __forceinline__ void halve(float (&v)[N], uint32_t lane)
+    {
+        static_assert(N == 16u || N == 32u, "one or two rows");
+        auto step = [&](auto countOf, auto distanceOf) __attribute__((always_inline)) {
+            constexpr uint32_t COUNT = decltype(countOf)::value, D = decltype(distanceOf)::value;
+#pragma unroll
+            for(uint32_t i = 0; i < COUNT; ++i)
+            {
+                const uint32_t a = __float_as_uint(v[2u * i]), b = __float_as_uint(v[2u * i + 1u]);
+                if constexpr(D == 32u)
+                {
+                    const auto s = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+                    v[i]         = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+                }
+                else if constexpr(D == 16u)
+                {
+                    const auto s = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+                    v[i]         = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+                }
+                else
+                {
+                    const bool  high = (lane & D) != 0u;
+                    const float keep = high ? v[2u * i + 1u] : v[2u * i], give = high ? v[2u * i] : v[2u * i + 1u];
+                    v[i]             = keep + other(give, D);
+                }
+            }
+        };
+        using std::integral_constant;
+        step(integral_constant<uint32_t, N / 2u>{}, integral_constant<uint32_t, 32>{});
+        step(integral_constant<uint32_t, N / 4u>{}, integral_constant<uint32_t, 16>{});
+        step(integral_constant<uint32_t, N / 8u>{}, integral_constant<uint32_t, 8>{});
+        step(integral_constant<uint32_t, N / 16u>{}, integral_constant<uint32_t, 4>{});
+        if constexpr(N == 32u)
+            step(integral_constant<uint32_t, 1>{}, integral_constant<uint32_t, 2>{});
+        else
+            v[0] += other(v[0], 2u);
+        v[0] += other(v[0], 1u);
+    }
+    // the sum that a lane has after halve()
+    __device__ __forceinline__ uint32_t sumOf(uint32_t lane)
+    {
+        return __brev(lane) >> 26;
+    }
+
+    // acc + a0 b0 + ... + a7 b7
+    template <typename T>
+    __device__ __forceinline__ float dot8(u32x4 a, u32x4 b, float acc)
+    {
+#pragma unroll
+        for(uint32_t i = 0; i < 4u; ++i)
+        {
+            const uint32_t x = a[i], y = b[i]; // (a cast of a vector's element itself takes the first one's bits)
+            if constexpr(__is_same(T, __bf16))
+                acc = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(vec<__bf16, 2>, x), __builtin_bit_cast(vec<__bf16, 2>, y), acc, false);
+            else
+                acc = __builtin_amdgcn_fdot2(__builtin_bit_cast(vec<_Float16, 2>, x), __builtin_bit_cast(vec<_Float16, 2>, y), acc, false);
+        }
+        return acc;
+    }
+
+    // y of one row and column, from its sum: z = sum + bias; y = act(z) gate + c
+    template <typename T>
+    __device__ __forceinline__ void finishOne(const LinearParams& p, uint32_t group, uint64_t row, uint32_t col, float sum)
+    {
+        float gate = 1.0f, add = 0.0f; // (asked for before anything waits)
+        if(p.gate)
+            gate = static_cast<float>(reinterpret_cast<const T*>(p.gate)[row * p.ldg + col]);
+        if(p.c)
+            add = p.outF32 ? reinterpret_cast<const float*>(p.c)[row * p.ldc + col] : static_cast<float>(reinterpret_cast<const T*>(p.c)[row * p.ldc + col]);
+        if(p.bias)
+            sum += static_cast<float>(reinterpret_cast<const T*>(p.bias)[(uint64_t)group * p.n + col]);
+        if(p.z)
+            reinterpret_cast<T*>(p.z)[row * p.ldz + col] = static_cast<T>(sum);
+        r355::withActivation(p.activation, [&](auto act) { sum = r355::activate<decltype(act)::value>(sum); });
+        if(p.gate)
+            sum *= gate;
+        if(p.c)
+            sum += add;
+        if(p.outF32)
+            reinterpret_cast<float*>(p.y)[row * p.ldy + col] = sum;
+        else
+            reinterpret_cast<T*>(p.y)[row * p.ldy + col] = static_cast<T>(sum);
+    }
+
+    // the sums of ROWS rows (count of them there) and a wave's 16 columns: sums[16 t + column]
+    template <typename T, uint32_t ROWS, bool STREAM>
+    __device__ __forceinline__ void dotWave(const LinearParams& p, const GroupTile& t, uint32_t col0, uint32_t waveK, uint32_t wavesK, float* sums)
+    {
+        const uint32_t lane = threadIdx.x & 63u, pieces = (p.k + 511u) / 512u;
+        const uint32_t last = p.n - col0 < 16u ? p.n - col0 - 1u : 15u; // (columns past the last read it again)
+        const auto bufW = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p.b) + (uint64_t)t.group * p.strideB + (uint64_t)col0 * p.ldb * 2u, 0,
+                                                            static_cast<int>((last * p.ldb + p.k) * 2u), 0x00020000);
+        const char* x[ROWS];
+        bool        in[ROWS];
+#pragma unroll
+        for(uint32_t r = 0; r < ROWS; ++r)
+        {
+            uint64_t row = t.first + (r < t.count ? r : t.count - 1u);
+            in[r]        = true;
+            if(p.source)
+            {
+                row   = static_cast<uint32_t>(p.source[row]);
+                in[r] = row < p.sourceRows;
+            }
+            x[r] = p.a + (in[r] ? row * p.lda * 2u : 0u);
+        }
+        float acc[16u * ROWS];
+#pragma unroll
+        for(uint32_t i = 0; i < 16u * ROWS; ++i)
+            acc[i] = 0.0f;
+        u32x4 w[16], xs[ROWS];
+        auto  offset = [&](uint32_t piece) { return piece * 512u + lane * 8u < p.k ? lane * 16u : OUTSIDE; };
+        auto  loadX = [&](uint32_t piece) __attribute__((always_inline)) {
+#pragma unroll
+            for(uint32_t r = 0; r < ROWS; ++r)
+                xs[r] = in[r] && piece * 512u + lane * 8u < p.k ? *reinterpret_cast<const u32x4*>(x[r] + ((uint64_t)piece * 512u + lane * 8u) * 2u) : u32x4{0u, 0u, 0u, 0u};
+        };
+        auto loadW = [&](uint32_t piece, uint32_t c) __attribute__((always_inline)) {
+            return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(bufW, offset(piece), (c < last ? c : last) * p.ldb * 2u + piece * 1024u, STREAM ? 2 : 0));
+        };
+        if(waveK < pieces)
+        {
+#pragma unroll
+            for(uint32_t c = 0; c < 16u; ++c)
+                w[c] = loadW(waveK, c);
+            loadX(waveK);
+        }
+        for(uint32_t piece = waveK; piece < pieces; piece += wavesK)
+        {
+            const uint32_t next = piece + wavesK;
+#pragma unroll
+            for(uint32_t c = 0; c < 16u; ++c)
+            {
+#pragma unroll
+                for(uint32_t r = 0; r < ROWS; ++r)
+                    acc[16u * r + c] = dot8<T>(w[c], xs[r], acc[16u * r + c]);
+                if(next < pieces) // (uniform)
+                    w[c] = loadW(next, c);
+            }
+            if(next < pieces)
+                loadX(next);
+        }
+        halve<16u * ROWS>(acc, lane);
+        constexpr uint32_t SAME = 64u / (16u * ROWS); // lanes that have the same sum
+        if((lane & (SAME - 1u)) == 0u)
+            sums[sumOf(lane) & (16u * ROWS - 1u)] = acc[0];
+    }
+
+    // ROWS: of a tile.  Workgroups of wavesK x (waves / wavesK) waves.
+    template <typename T, uint32_t ROWS, bool STREAM>
+    __global__ void __launch_bounds__(64 * WAVES, 2) linearDots(LinearParams p, uint32_t wavesK)
+    {
+        __shared__ float sums[WAVES][16u * ROWS];
+        GroupTiles<ROWS> tiles{p};
+        const uint32_t   tilesM = tiles.total(), count = tilesM * p.tilesN, perXcd = (count + 7u) / 8u;
+        const uint32_t   id = blockIdx.x % 8u * perXcd + blockIdx.x / 8u;
+        if(blockIdx.x / 8u >= perXcd || id >= count)
+            return;
+        GroupTile t = tiles.at(id % tilesM);
+        t.group = __builtin_amdgcn_readfirstlane(t.group), t.first = __builtin_amdgcn_readfirstlane(t.first), t.count = __builtin_amdgcn_readfirstlane(t.count);
+        const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), sets = (blockDim.x >> 6) / wavesK, set = wave / wavesK;
+        const uint32_t col0 = id / tilesM * 16u * sets, mine = col0 + set * 16u;
+        if(mine < p.n)
+        {
+            if(ROWS == 1u || t.count == 1u)
+                dotWave<T, 1, STREAM>(p, t, mine, wave % wavesK, wavesK, sums[wave]);
+            else
+                dotWave<T, ROWS, STREAM>(p, t, mine, wave % wavesK, wavesK, sums[wave]);
+        }
+        __syncthreads();
+        for(uint32_t i = threadIdx.x; i < 16u * sets * t.count; i += blockDim.x)
+        {
+            const uint32_t row = i / (16u * sets), col = i % (16u * sets), of = col / 16u * wavesK;
+            if(col0 + col >= p.n)
+                continue;
+            float sum = 0.0f;
+            for(uint32_t v = 0; v < wavesK; ++v)
+                sum += sums[of + v][row * 16u + col % 16u];
+            finishOne<T>(p, t.group, (uint64_t)t.first + row, col0 + col, sum);
+        }
+    }
+
     // ---- Few rows of each group.  A workgroup's eight waves share 16 RB weight rows x 16 CB rows of x and take pieces of 64 of the sum in turn, both
     // straight from global memory; their sums meet in LDS in the order of the waves.  The weights are the first operand: a lane then holds four of them of one row of x.
-    template <typename T, uint32_t RB, uint32_t CB, uint32_t DEPTH>
+    template <typename T, uint32_t RB, uint32_t CB, uint32_t DEPTH, bool STREAM>
     __global__ void __launch_bounds__(64 * WAVES, 2) linearFew(LinearParams p)
     {
         constexpr uint32_t ROWS = 16u * CB, COLS = 16u * RB, PITCH = COLS + 4u;
@@ -85,7 +284,7 @@ namespace
                 const bool in = piece * 64u + i * 32u + quad * 8u < p.k; // (what lies past the sum's end is another row's)
 #pragma unroll
                 for(uint32_t r = 0; r < RB; ++r)
-                    s.w[r][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(bufW, in ? offW[r] + i * 64u : OUTSIDE, piece * 128u, 0));
+                    s.w[r][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(bufW, in ? offW[r] + i * 64u : OUTSIDE, piece * 128u, STREAM ? 2 : 0));
 #pragma unroll
                 for(uint32_t c = 0; c < CB; ++c)
                     s.x[c][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(bufX, in ? offX[c] + i * 64u : OUTSIDE, piece * 128u, 0));
@@ -130,18 +329,7 @@ namespace
 #pragma unroll
             for(uint32_t v = 0; v < WAVES; ++v)
                 sum += sums[(v * ROWS + row) * PITCH + col];
-            const uint64_t at = (uint64_t)first + row;
-            if(p.bias)
-                sum += static_cast<float>(reinterpret_cast<const T*>(p.bias)[(uint64_t)group * p.n + col0 + col]);
-            if(p.z)
-                reinterpret_cast<T*>(p.z)[at * p.ldz + col0 + col] = static_cast<T>(sum);
-            r355::withActivation(p.activation, [&](auto act) { sum = r355::activate<decltype(act)::value>(sum); });
-            if(p.gate)
-                sum *= static_cast<float>(reinterpret_cast<const T*>(p.gate)[at * p.ldg + col0 + col]);
-            if(p.outF32)
-                reinterpret_cast<float*>(p.y)[at * p.ldy + col0 + col] = p.c ? sum + reinterpret_cast<const float*>(p.c)[at * p.ldc + col0 + col] : sum;
-            else
-                reinterpret_cast<T*>(p.y)[at * p.ldy + col0 + col] = static_cast<T>(p.c ? sum + static_cast<float>(reinterpret_cast<const T*>(p.c)[at * p.ldc + col0 + col]) : sum);
+            finishOne<T>(p, group, (uint64_t)first + row, col0 + col, sum);
         }
     }
 
@@ -463,12 +651,36 @@ namespace
         return best;
     }
 
+    // Weights that no cache keeps from one call to the next are read nontemporally (16 experts of 4096 x 4096 95 -> 85 us, 8192 x 8192 29.8 -> 26.0; three matrices of
+    // 2048 x 8192 in turn, which the 256 MiB of the memory-side cache hold: 8.1 -> 9.1).
+    bool streams(const LinearParams& p)
+    {
+        const uint64_t met = p.offsets && p.groups < p.rows ? p.groups : p.offsets ? p.rows : 1u;
+        return met * p.n * p.k * 2u > (uint64_t{96} << 20);
+    }
+
+    template <typename T, uint32_t ROWS>
+    void launchDots(LinearParams p, hipStream_t s)
+    {
+        // Few waves along the sum, each with a long stretch of 16 rows, as long as there are enough workgroups (32 experts of 4096 x 4096, 16 of them met, one, two, four, eight waves: 84, 95, 93, 105 us;
+        // 16384 x 4096 29, 27, 25, 27; 8192 x 8192 38, 28, 26, 26); of small layers one set of them a workgroup.
+        const uint32_t pieces = static_cast<uint32_t>(tilesOf(p.k, 512u)), enough = r355::computeUnits() * 5u / 4u;
+        uint32_t       wavesK = 1u;
+        while(wavesK < WAVES && 2u * wavesK <= pieces && tilesOf(p.n, 16u * (WAVES / wavesK)) * mostTiles(p, ROWS) < enough)
+            wavesK *= 2u;
+        const uint32_t sets = tilesOf(p.n, 16u * (WAVES / wavesK)) * mostTiles(p, ROWS) >= enough ? WAVES / wavesK : 1u;
+        p.tilesN              = static_cast<uint32_t>(tilesOf(p.n, 16u * sets));
+        const uint64_t groups = (mostTiles(p, ROWS) * p.tilesN + 7u) / 8u * 8u;
+        const auto     kernel = streams(p) ? linearDots<T, ROWS, true> : linearDots<T, ROWS, false>;
+        hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(groups)), dim3(64 * wavesK * sets), 0, s, p, wavesK);
+    }
     template <typename T>
     void launchFew(LinearParams p, hipStream_t s)
     {
         p.tilesN             = static_cast<uint32_t>(tilesOf(p.n, 16u));
         const uint64_t groups = (mostTiles(p, 16u) * p.tilesN + 7u) / 8u * 8u;
-        hipLaunchKernelGGL((linearFew<T, 1, 1, 4>), dim3(static_cast<uint32_t>(groups)), dim3(64 * WAVES), 0, s, p);
+        const auto     kernel = streams(p) ? linearFew<T, 1, 1, 4, true> : linearFew<T, 1, 1, 4, false>;
+        hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(groups)), dim3(64 * WAVES), 0, s, p);
     }
 
     int tooMany(const char* what)
@@ -593,9 +805,22 @@ namespace
     {
         return a.k % 8u == 0u && evenRows(a.x, a.ldx, 2) && evenRows(a.w, a.ldw, 2) && (a.groups == 1u || a.w_stride % 8 == 0);
     }
-    bool fewRows(const r355_linear_args& a)
+    // The kernel of a forward product by its rows: us of dot products, of the kernel for few rows and of tiles for 4096 x 4096: one row 7.3, 8.0, 14; two 7.8, 8.2, 14; four 8.8, 8.3, 14; sixteen
+    // -, 10, 15; 24 -, 17, 14.  Of experts with about one row each (32 of 4096 x 4096, 128 of 1024 x 1024) 84, 105, 115 and 49, 75, 50; with two 265, 179, 192; four of 1024 x 1024 -, 96, 57 (a workgroup
+    // of the kernel for few rows has 16 columns, little work with a short sum); eight of 2048 x 2048 -, 117, 124, sixteen -, 166, 125.
+    enum class Kernel
     {
-        return a.rows / a.groups <= 16u;
+        DOTS,
+        FEW,
+        TILES
+    };
+    Kernel kernelOf(const r355_linear_args& a, bool even)
+    {
+        if(!even)
+            return Kernel::TILES;
+        if(a.groups == 1u)
+            return a.rows <= 2u ? Kernel::DOTS : a.rows <= 16u ? Kernel::FEW : Kernel::TILES;
+        return a.rows <= a.groups ? Kernel::DOTS : a.rows / a.groups < 9u && a.k >= 2048u ? Kernel::FEW : Kernel::TILES;
     }
     LinearParams inputParams(const r355_linear_backward_args& a, const char* dz, uint32_t lddz)
     {
@@ -671,20 +896,27 @@ extern "C" int r355_linear(const r355_linear_args* args, void* stream)
     const bool         even = evenForward(a);
     const hipStream_t  s    = static_cast<hipStream_t>(stream);
     r355::beginCall();
-    if(even && fewRows(a))
+    const bool         f16  = a.in_type == R355_F16;
+    const Kernel       kernel = kernelOf(a, even);
+    if(kernel != Kernel::TILES && mostTiles(p, kernel == Kernel::DOTS ? 1u : 16u) * tilesOf(p.n, 16u) > r355::MAX_GROUPS / 2u)
+        return tooMany(what);
+    switch(kernel)
     {
-        if(mostTiles(p, 16u) * tilesOf(p.n, 16u) > r355::MAX_GROUPS / 2u)
-            return tooMany(what);
-        a.in_type == R355_F16 ? launchFew<_Float16>(p, s) : launchFew<__bf16>(p, s);
+    case Kernel::DOTS:
+        if(a.rows == 1u)
+            f16 ? launchDots<_Float16, 1>(p, s) : launchDots<__bf16, 1>(p, s);
+        else
+            f16 ? launchDots<_Float16, 2>(p, s) : launchDots<__bf16, 2>(p, s);
+        break;
+    case Kernel::FEW: f16 ? launchFew<_Float16>(p, s) : launchFew<__bf16>(p, s); break;
+    default: R355_TRY(launchTiles(a.in_type, p, true, true, !even, a.workspace, a.workspace_bytes, s, what));
     }
-    else
-        R355_TRY(launchTiles(a.in_type, p, true, true, !even, a.workspace, a.workspace_bytes, s, what));
     return r355::checkLaunch(what);
 }
 
 extern "C" size_t r355_linear_workspace_bytes(const r355_linear_args* args)
 {
-    if(!args || args->rows == 0 || args->n == 0 || args->k == 0 || args->groups == 0 || (evenForward(*args) && fewRows(*args)))
+    if(!args || args->rows == 0 || args->n == 0 || args->k == 0 || args->groups == 0 || kernelOf(*args, evenForward(*args)) != Kernel::TILES)
         return 0;
     return splitBytes(forwardParams(*args), true, !evenForward(*args));
 }

@@ -395,5 +395,16 @@ def test_argument_structures(tmp_path):
                        (R.LinearBackwardArgs, "linear_backward")):
         names = [f for f, _ in kind._fields_]
         layout, size = B._layout(tmp_path, "r355_%s_args" % name, names)
-        assert ctypes.sizeof(kind) == size
+        packed = getattr(R, "_%s_ARGS" % name.upper())
+        assert ctypes.sizeof(kind) == size == packed.size
+        # every value that is packed, made one at a time not zero, is the structure's field of that place; what is left over is padding
+        fields = iter(names)
+        letters = packed.format.lstrip("=")
+        for i, letter in enumerate(letters):
+            values = [0.0 if c == "d" else 0 for c in letters]
+            values[i] = 1.5 if letter == "d" else 3
+            a = kind.from_buffer_copy(packed.pack(*values))
+            held = [f for f in names if getattr(a, f)]
+            assert held == ([next(fields)] if held else []) and (not held or getattr(a, held[0]) == values[i]), (name, i)
+        assert next(fields, None) is None
         assert {n: (getattr(kind, n).offset, getattr(kind, n).size) for n in names} == layout
