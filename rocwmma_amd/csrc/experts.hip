@@ -76,6 +76,17 @@ namespace
         return in ? __expf(v - (most == -INFINITY ? 0.0f : most)) : 0.0f;
     }
 
+    __device__ __forceinline__ uint32_t maskOf(bool is)
+    {
+        uint32_t m = is ? ~0u : 0u;
+        asm("" : "+v"(m)); // (kept from the compiler, which would take it for a condition again)
+        return m;
+    }
+    __device__ __forceinline__ uint32_t either(uint32_t mask, uint32_t a, uint32_t b)
+    {
+        return (a & mask) | (b & ~mask);
+    }
+
     // One token a wave: expert V lane + i in x[i] of the lane.  A key orders numbers as integers, NaN below them; every lane sorts its keys, and `top` rounds take the largest of
     // the lanes' first ones, of the lowest lane that has it, which then moves up.  Bound by the vector instructions (some 15 a round).
     // What is returned lies in lane j for the j-th choice: its expert and its logit.
@@ -92,16 +103,16 @@ namespace
             key[i] = e >= p.experts ? 0u : by != by ? 1u : (b & 0x80000000u) ? ~b : b | 0x80000000u; // (-infinity: 0x007FFFFF)
             of[i]  = i;
         }
-        // (neighbours change places only if the later one is larger: equal ones stay in the order of their experts)
+        // (Neighbours change places only if the later one is larger: equal ones stay in the order of their experts.  Choices by masks, one instruction each: of conditions the
+        // compiler makes branches and indices, twice as many.)
 #pragma unroll
         for(uint32_t end = V - 1u; end > 0u; --end)
 #pragma unroll
             for(uint32_t i = 0; i < end; ++i)
             {
-                const bool     swap = key[i + 1u] > key[i];
-                const uint32_t k = key[i], o = of[i];
-                key[i] = swap ? key[i + 1u] : k, key[i + 1u] = swap ? k : key[i + 1u];
-                of[i] = swap ? of[i + 1u] : o, of[i + 1u] = swap ? o : of[i + 1u];
+                const uint32_t k = key[i], l = key[i + 1u], o = of[i], swap = maskOf(l > k);
+                key[i] = k > l ? k : l, key[i + 1u] = k > l ? l : k;
+                of[i] = either(swap, of[i + 1u], o), of[i + 1u] = either(swap, o, of[i + 1u]);
             }
         expert = 0u;
         for(uint32_t j = 0; j < p.top; ++j)
@@ -110,11 +121,11 @@ namespace
             const uint32_t l    = static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(__ballot(key[0] == best)))) - 1u;
             const uint32_t e    = l * V + __builtin_amdgcn_readlane(of[0], l);
             expert              = lane == j ? e : expert;
-            const bool moves    = lane == l;
+            const uint32_t moves = maskOf(lane == l);
 #pragma unroll
             for(uint32_t i = 0; i + 1u < V; ++i)
-                key[i] = moves ? key[i + 1u] : key[i], of[i] = moves ? of[i + 1u] : of[i];
-            key[V - 1u] = moves ? 0u : key[V - 1u];
+                key[i] = either(moves, key[i + 1u], key[i]), of[i] = either(moves, of[i + 1u], of[i]);
+            key[V - 1u] &= ~moves;
         }
         // the logit of the lane's choice lies with lane expert / V
         logit = 0.0f;
@@ -453,19 +464,28 @@ namespace
         uint32_t       ldx, ldv, ldo, pieces; // pieces: of EW elements of a row
     };
 
-    template <typename T, uint32_t EW>
+    // STREAM: nontemporally, as what lies beyond the caches (a rule of the host's)
+    template <typename T, uint32_t EW, bool STREAM>
     __device__ __forceinline__ vec<T, EW> readPiece(const char* base, uint64_t row, uint32_t ld, uint32_t col)
     {
-        return *reinterpret_cast<const vec<T, EW>*>(reinterpret_cast<const T*>(base) + row * ld + col);
+        const vec<T, EW>* at = reinterpret_cast<const vec<T, EW>*>(reinterpret_cast<const T*>(base) + row * ld + col);
+        if constexpr(STREAM)
+            return __builtin_nontemporal_load(at);
+        else
+            return *at;
     }
-    template <typename T, uint32_t EW>
+    template <typename T, uint32_t EW, bool STREAM>
     __device__ __forceinline__ void writePiece(char* base, uint64_t row, uint32_t ld, uint32_t col, vec<T, EW> v)
     {
-        *reinterpret_cast<vec<T, EW>*>(reinterpret_cast<T*>(base) + row * ld + col) = v;
+        vec<T, EW>* at = reinterpret_cast<vec<T, EW>*>(reinterpret_cast<T*>(base) + row * ld + col);
+        if constexpr(STREAM)
+            __builtin_nontemporal_store(v, at);
+        else
+            *at = v;
     }
 
     // A thread per piece of a token's row; the rows of up to eight of its choices are under way at once.
-    template <typename T, uint32_t EW>
+    template <typename T, uint32_t EW, bool STREAM>
     __global__ void __launch_bounds__(THREADS) combineRows(RowsParams p)
     {
         const uint32_t at = blockIdx.x * THREADS + threadIdx.x, token = at / p.pieces; // (a launch has less than 2^32 threads)
@@ -490,7 +510,7 @@ namespace
                     in[u]               = row < p.rows;
                     w[u]                = p.weights ? p.weights[slot] : 1.0f;
                     if(in[u])
-                        v[u] = readPiece<T, EW>(p.values, row, p.ldv, col);
+                        v[u] = readPiece<T, EW, STREAM>(p.values, row, p.ldv, col);
                 }
 #pragma unroll
             for(uint32_t u = 0; u < 8u; ++u)
@@ -501,7 +521,7 @@ namespace
         }
         if(p.x)
         {
-            const vec<T, EW> c = readPiece<T, EW>(p.x, token, p.ldx, col);
+            const vec<T, EW> c = readPiece<T, EW, STREAM>(p.x, token, p.ldx, col);
 #pragma unroll
             for(uint32_t e = 0; e < EW; ++e)
                 total[e] += static_cast<float>(c[e]);
@@ -510,11 +530,11 @@ namespace
 #pragma unroll
         for(uint32_t e = 0; e < EW; ++e)
             y[e] = static_cast<T>(total[e]);
-        writePiece<T, EW>(p.out, token, p.ldo, col, y);
+        writePiece<T, EW, STREAM>(p.out, token, p.ldo, col, y);
     }
 
     // SHARE waves per token take its pieces in turn, 64 at a time; the dot products of up to eight choices at once, joined in the order of the waves.
-    template <typename T, uint32_t EW, uint32_t SHARE, bool DOTS>
+    template <typename T, uint32_t EW, uint32_t SHARE, bool DOTS, bool STREAM>
     __global__ void __launch_bounds__(THREADS) dispatchRows(RowsParams p)
     {
         __shared__ float meet[WAVES][8];
@@ -537,13 +557,13 @@ namespace
                 for(uint32_t at = part * 64u + lane; at < p.pieces; at += SHARE * 64u)
                 {
                     const uint32_t   col = at * EW;
-                    const vec<T, EW> x   = readPiece<T, EW>(p.x, token, p.ldx, col);
+                    const vec<T, EW> x   = readPiece<T, EW, false>(p.x, token, p.ldx, col);
                     vec<T, EW>       v[DOTS ? 8 : 1];
                     if constexpr(DOTS)
 #pragma unroll
                         for(uint32_t u = 0; u < 8u; ++u)
                             if(row[u] < p.rows)
-                                v[u] = readPiece<T, EW>(p.values, row[u], p.ldv, col);
+                                v[u] = readPiece<T, EW, STREAM>(p.values, row[u], p.ldv, col);
 #pragma unroll
                     for(uint32_t u = 0; u < 8u; ++u)
                         if(row[u] < p.rows)
@@ -557,7 +577,7 @@ namespace
                                     dot[u] = fmaf(static_cast<float>(x[e]), static_cast<float>(v[u][e]), dot[u]);
                             }
                             if(p.out)
-                                writePiece<T, EW>(p.out, row[u], p.ldo, col, y);
+                                writePiece<T, EW, false>(p.out, row[u], p.ldo, col, y);
                         }
                 }
             if constexpr(DOTS)
@@ -691,6 +711,12 @@ namespace
             return r355::fail(R355_ERR_BAD_SIZE, "%s: at most 2^30 rows of 2^24 elements, got %u tokens, %u choices, %u rows and %u elements", what, tokens, top, rows, width);
         return R355_OK;
     }
+    // Whether the experts' rows are more than the caches keep.  Combined: 8192 x 8 x 4096 133 -> 112 us nontemporally, 512 x 8 x 4096 7.9 -> 9.7; dispatched, the reads for the weights' gradient: 8192 x 8 x
+    // 4096 233 -> 220, 4099 x 2 x 2832 23.9 -> 28.1.
+    bool streams(uint32_t tokens, uint32_t top, uint32_t width)
+    {
+        return (uint64_t)tokens * top * width * 2u > (uint64_t{96} << 20);
+    }
     bool pieces16(const void* at, uint32_t ld)
     {
         return !at || (r355::aligned(at, 16) && ld % 8u == 0u);
@@ -782,7 +808,12 @@ extern "C" int r355_combine(const r355_combine_args* args, void* stream)
     if(groups > r355::MAX_GROUPS)
         return r355::fail(R355_ERR_BAD_SIZE, "combine: %u tokens of %u elements are too many for a launch", a.tokens, a.width);
     const bool f16    = a.type == R355_F16;
-    const auto kernel = wide ? (f16 ? combineRows<_Float16, 8> : combineRows<__bf16, 8>) : (f16 ? combineRows<_Float16, 1> : combineRows<__bf16, 1>);
+    const bool nontemporal = streams(a.tokens, a.top, a.width);
+    auto       pick   = [&](auto type) {
+        using T = decltype(type);
+        return wide ? (nontemporal ? combineRows<T, 8, true> : combineRows<T, 8, false>) : combineRows<T, 1, false>;
+    };
+    const auto kernel = f16 ? pick(_Float16{}) : pick(__bf16{});
     r355::beginCall();
     hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(groups)), dim3(THREADS), 0, static_cast<hipStream_t>(stream), p);
     return r355::checkLaunch("combine");
@@ -817,7 +848,10 @@ extern "C" int r355_dispatch(const r355_dispatch_args* args, void* stream)
     auto pick = [&](auto type, auto dots) {
         using T             = decltype(type);
         constexpr bool DOTS = decltype(dots)::value;
-        return wide ? (share ? dispatchRows<T, 8, 4, DOTS> : dispatchRows<T, 8, 1, DOTS>) : (share ? dispatchRows<T, 1, 4, DOTS> : dispatchRows<T, 1, 1, DOTS>);
+        if constexpr(DOTS)
+            if(wide && share && streams(a.tokens, a.top, a.width))
+                return dispatchRows<T, 8, 4, DOTS, true>;
+        return wide ? (share ? dispatchRows<T, 8, 4, DOTS, false> : dispatchRows<T, 8, 1, DOTS, false>) : (share ? dispatchRows<T, 1, 4, DOTS, false> : dispatchRows<T, 1, 1, DOTS, false>);
     };
     const bool f16    = a.type == R355_F16;
     const auto kernel = a.dweights ? (f16 ? pick(_Float16{}, std::true_type{}) : pick(__bf16{}, std::true_type{})) : (f16 ? pick(_Float16{}, std::false_type{}) : pick(__bf16{}, std::false_type{}));

@@ -569,10 +569,10 @@ namespace
         return most < p.rows ? most : p.rows;
     }
 
-    // How a product on macro tiles is launched: `splits` workgroups along the sum; the first `tall` rows alone where the rest goes to other tiles.
+    // How a product on macro tiles is launched: `splits` workgroups along the sum; the first `tall` rows alone where the rest goes out by a plan of its own.
     struct Plan
     {
-        r355::LinearTile tile, rest;
+        r355::LinearTile tile;
         uint32_t         splits, tall;
         double           us;
     };
@@ -584,8 +584,8 @@ namespace
         uint32_t held;
         double   ends, stage[4];
     };
-    constexpr TileTimes TILE_TIMES[r355::LINEAR_TILES] = {{1u, 11.0, {1.05, 1.34}}, {1u, 6.0, {0.63, 0.80}}, {1u, 6.0, {0.63, 0.80}}, {2u, 4.5, {0.45, 0.88}}, {4u, 3.0, {0.37, 0.42, 0.56, 0.70}},
-                                                          {2u, 2.0, {1.40, 2.60}}};
+    constexpr TileTimes TILE_TIMES[r355::LINEAR_TILES] = {{1u, 11.0, {1.05, 1.34}}, {1u, 9.0, {0.85, 1.10}}, {1u, 6.0, {0.63, 0.80}}, {1u, 5.0, {0.55, 0.68}}, {1u, 6.0, {0.63, 0.80}}, {2u, 4.5, {0.45, 0.88}},
+                                                          {4u, 3.0, {0.37, 0.42, 0.56, 0.70}}, {2u, 2.0, {1.40, 2.60}}};
     double launchTime(uint32_t tile, double tiles, double stages)
     {
         const TileTimes& t    = TILE_TIMES[tile];
@@ -622,7 +622,7 @@ namespace
             const double met = p.groups < rows ? p.groups : static_cast<double>(rows);
             return (static_cast<double>(rows) / LINEAR_ROWS[tile] + (tile == TILE_256 ? 0.2 : 0.5) * met) * across;
         };
-        Plan best{any ? TILE_ANY : TILE_64, TILE_64, 1u, 0u, 1e30};
+        Plan best{any ? TILE_ANY : TILE_64, 1u, 0u, 1e30};
         for(uint32_t tile = any ? TILE_ANY : TILE_256; tile < (any ? LINEAR_TILES : TILE_ANY); ++tile)
         {
             const double all = tiles(tile, p.rows);
@@ -633,19 +633,20 @@ namespace
                     break;
                 const double us = launchTime(tile, all * splits, stages / splits) + (splits > 1u ? 5.0 + static_cast<double>(rowsY) * p.n * 4.0 * (2u * splits + 1u) / 5e6 : 0.0);
                 if(us < best.us)
-                    best = Plan{static_cast<LinearTile>(tile), TILE_64, splits, 0u, us};
+                    best = Plan{static_cast<LinearTile>(tile), splits, 0u, us};
             }
-            // whole rounds of large tiles, the rest on other ones
+            // whole rounds of large tiles, then the rest
             if(tile == TILE_256 && aK && !p.offsets)
             {
                 const uint64_t across = tilesOf(p.n, 256u), rounds = static_cast<uint64_t>(all) / computeUnits(), tall = rounds * computeUnits() / across * 256u;
                 if(tall > 0u && tall < p.rows)
-                    for(uint32_t rest = TILE_256_128; rest <= TILE_64; ++rest)
-                    {
-                        const double us = launchTime(TILE_256, tiles(TILE_256, tall), stages) + launchTime(rest, tiles(rest, p.rows - tall), stages);
-                        if(us < best.us)
-                            best = Plan{TILE_256, static_cast<LinearTile>(rest), 1u, static_cast<uint32_t>(tall), us};
-                    }
+                {
+                    LinearParams rest = p;
+                    rest.rows         = static_cast<uint32_t>(p.rows - tall);
+                    const double us   = launchTime(TILE_256, tiles(TILE_256, tall), stages) + planOf(rest, aK, any, workspaceBytes).us;
+                    if(us < best.us)
+                        best = Plan{TILE_256, 1u, static_cast<uint32_t>(tall), us};
+                }
             }
         }
         return best;
@@ -743,7 +744,7 @@ namespace
         rest.c = p.c ? p.c + by * p.ldc * outBytes : nullptr, rest.gate = p.gate ? p.gate + by * p.ldg * 2u : nullptr, rest.z = p.z ? p.z + by * p.ldz * 2u : nullptr;
         if(const int rc = launchTile(type, first, aK, bK, plan.tile, s, what))
             return rc;
-        return launchTile(type, rest, aK, bK, plan.rest, s, what);
+        return launchTiles(type, rest, aK, bK, any, workspace, workspaceBytes, s, what);
     }
 
     bool evenRows(const void* at, uint32_t ld, uint32_t bytes) // rows on 16-byte boundaries
@@ -848,10 +849,15 @@ namespace
         return evenRows(dz, lddz, 2) && evenRows(a.x, a.ldx, 2);
     }
     // what the sums of a split product take
-    size_t splitBytes(const LinearParams& p, bool aK, bool any)
+    size_t splitBytes(LinearParams p, bool aK, bool any)
     {
-        const uint32_t splits = planOf(p, aK, any, ~0ull).splits;
-        return splits > 1u ? static_cast<size_t>((aK ? p.rows : (uint64_t)p.m * p.groups) * pitchOf(p.n) * 4u * splits) : 0u;
+        Plan plan = planOf(p, aK, any, ~0ull);
+        while(plan.tall != 0u) // (the rest may be split)
+        {
+            p.rows -= plan.tall;
+            plan = planOf(p, aK, any, ~0ull);
+        }
+        return plan.splits > 1u ? static_cast<size_t>((aK ? p.rows : (uint64_t)p.m * p.groups) * pitchOf(p.n) * 4u * plan.splits) : 0u;
     }
 } // namespace
 

@@ -210,13 +210,15 @@ namespace r355
     enum LinearTile : uint32_t
     {
         TILE_256 = 0,
+        TILE_192_256,
         TILE_256_128,
+        TILE_192_128,
         TILE_128_256,
         TILE_128,
         TILE_64,
         TILE_ANY
     };
-    constexpr uint32_t LINEAR_TILES = 6u, LINEAR_ROWS[LINEAR_TILES] = {256u, 256u, 128u, 128u, 64u, 64u}, LINEAR_COLS[LINEAR_TILES] = {256u, 128u, 256u, 128u, 64u, 64u};
+    constexpr uint32_t LINEAR_TILES = 8u, LINEAR_ROWS[LINEAR_TILES] = {256u, 192u, 256u, 192u, 128u, 128u, 64u, 64u}, LINEAR_COLS[LINEAR_TILES] = {256u, 256u, 128u, 128u, 256u, 128u, 64u, 64u};
     // the forms, one set of kernels per type; aK, bK: A, B contiguous along the sum
     void linearTilesF16(const LinearParams& p, bool aK, bool bK, LinearTile tile, uint32_t workgroups, hipStream_t s);
     void linearTilesBF16(const LinearParams& p, bool aK, bool bK, LinearTile tile, uint32_t workgroups, hipStream_t s);

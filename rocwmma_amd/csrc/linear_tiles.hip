@@ -552,6 +552,22 @@ namespace
         }
     }
     template <bool AK, bool BK>
+    __global__ void __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(1, 1))) linearTiles192x256(LinearParams p)
+    {
+        __shared__ __attribute__((aligned(1024))) char lds[ldsOf(6, 8)];
+        Work                                           w;
+        if(workOf<AK, 192, 256>(p, w))
+            linearTile<AK, BK, 6, 8>(p, w, lds);
+    }
+    template <bool AK, bool BK>
+    __global__ void __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(1, 1))) linearTiles192x128(LinearParams p)
+    {
+        __shared__ __attribute__((aligned(1024))) char lds[ldsOf(6, 4)];
+        Work                                           w;
+        if(workOf<AK, 192, 128>(p, w))
+            linearTile<AK, BK, 6, 4>(p, w, lds);
+    }
+    template <bool AK, bool BK>
     __global__ void __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(1, 1))) linearTiles256x128(LinearParams p)
     {
         __shared__ __attribute__((aligned(1024))) char lds[ldsOf(8, 4)];
@@ -584,7 +600,23 @@ namespace
             linearTile<AK, BK, 2, 2>(p, w, lds);
     }
 
-    // The same on tiles of 64 x 64 for operands of any alignment, lengths and leading dimensions: loaded element by element through registers, 32 of the sum at a time.
+    // Eight elements of any alignment, `left` of them there: at once, or at the ends one by one
+    __device__ __forceinline__ vec<T, 8> piece(const T* at, uint32_t left)
+    {
+        typedef T Unaligned __attribute__((ext_vector_type(8), aligned(2)));
+        vec<T, 8> v{};
+        if(left >= 8u)
+            v = *reinterpret_cast<const Unaligned*>(at);
+        else
+#pragma unroll
+            for(uint32_t e = 0; e < 7u; ++e)
+                if(e < left)
+                    v[e] = at[e];
+        return v;
+    }
+
+    // The same on tiles of 64 x 64 for operands of any alignment, lengths and leading dimensions: through registers, 32 of the sum at a time (1500 x 1500 x 4096 backward, both
+    // products, 460 us with single elements; even rows take 60).
     template <bool AK, bool BK>
     __global__ void __launch_bounds__(THREADS) linearAny(LinearParams p)
     {
@@ -625,15 +657,10 @@ namespace
                 acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         for(uint32_t k0 = 0; k0 < w.k; k0 += STEP)
         {
-            vec<T, 8> va, vb;
-#pragma unroll
-            for(uint32_t e = 0; e < 8u; ++e)
-            {
-                const bool inA = AK ? there && k0 + kA + e < w.k : rowA + e < w.rowsLeft && k0 + kA < w.k;
-                const bool inB = BK ? rowB < w.colsLeft && k0 + kB + e < w.k : rowB + e < w.colsLeft && k0 + kB < w.k;
-                va[e] = inA ? (AK ? a[k0 + kA + e] : a[(uint64_t)(k0 + kA) * p.lda + e]) : T(0.0f);
-                vb[e] = inB ? (BK ? b[k0 + kB + e] : b[(uint64_t)(k0 + kB) * p.ldb + e]) : T(0.0f);
-            }
+            const uint32_t  leftK = w.k - k0; // of the sum
+            const vec<T, 8> va = piece(a + (AK ? (uint64_t)k0 + kA : (uint64_t)(k0 + kA) * p.lda), AK ? (there && kA < leftK ? leftK - kA : 0u) : (kA < leftK && rowA < w.rowsLeft ? w.rowsLeft - rowA : 0u));
+            const vec<T, 8> vb = piece(b + (BK ? (uint64_t)k0 + kB : (uint64_t)(k0 + kB) * p.ldb),
+                                       BK ? (rowB < w.colsLeft && kB < leftK ? leftK - kB : 0u) : (kB < leftK && rowB < w.colsLeft ? w.colsLeft - rowB : 0u));
             __syncthreads();
             if constexpr(AK)
                 *reinterpret_cast<vec<T, 8>*>(&image[0][rowA * PITCH + kA]) = va;
@@ -668,7 +695,9 @@ namespace
     void launch(const LinearParams& p, r355::LinearTile tile, uint32_t workgroups, hipStream_t s)
     {
         const auto kernel = tile == r355::TILE_256       ? linearTiles256<AK, BK>
+                            : tile == r355::TILE_192_256 ? linearTiles192x256<AK, BK>
                             : tile == r355::TILE_256_128 ? linearTiles256x128<AK, BK>
+                            : tile == r355::TILE_192_128 ? linearTiles192x128<AK, BK>
                             : tile == r355::TILE_128_256 ? linearTiles128x256<AK, BK>
                             : tile == r355::TILE_128     ? linearTiles128<AK, BK>
                             : tile == r355::TILE_64      ? linearTiles64<AK, BK>
