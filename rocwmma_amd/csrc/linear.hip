@@ -689,8 +689,16 @@ namespace
         return r355::fail(R355_ERR_BAD_SIZE, "%s: more than 2^24 tiles of the result", what);
     }
 
+    // whether rows begin with a cache line
+    bool lines(const void* at, uint32_t ld, uint32_t bytes)
+    {
+        return r355::aligned(at, 128) && (uint64_t)ld * bytes % 128u == 0u;
+    }
+
     int launchTile(int32_t type, LinearParams p, bool aK, bool bK, r355::LinearTile tile, hipStream_t s, const char* what)
     {
+        // (shares of a split sum are read again at once)
+        p.linesY = p.splits == 1u && lines(p.y, p.ldy, p.outF32 ? 4u : 2u), p.linesZ = lines(p.z, p.ldz, 2u);
         const uint32_t rows = r355::LINEAR_ROWS[tile];
         p.tilesN = static_cast<uint32_t>(tilesOf(p.n, r355::LINEAR_COLS[tile])), p.tilesM = static_cast<uint32_t>(tilesOf(p.m, rows));
         const uint64_t tiles = (aK ? mostTiles(p, rows) : (uint64_t)p.tilesM * p.groups) * p.tilesN;

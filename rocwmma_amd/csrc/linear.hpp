@@ -37,7 +37,7 @@ namespace r355
         uint32_t       tilesM, tilesN; // tilesM: of a group's Y (weights' gradient)
         uint32_t       splits; // workgroups along the sum, each writes its own f32 sums (workspace [splits][rows of Y][n]); 1: none
         int32_t        activation;
-        uint32_t       outF32;
+        uint32_t       outF32, linesY, linesZ; // lines: rows begin with a cache line
     };
 
     constexpr uint32_t OUTSIDE = 0x80000000u; // a lane's offset past the end of any buffer here: loads zeros, stores nothing

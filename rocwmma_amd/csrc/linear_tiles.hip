@@ -148,10 +148,9 @@ namespace
             return static_cast<float>(w[e / PER][e % PER]);
         }
     };
-    template <typename E, uint32_t RUN>
+    template <typename E, int POLICY, uint32_t RUN>
     __device__ __forceinline__ void storeRow(__amdgpu_buffer_rsrc_t to, uint32_t row, const Columns<RUN>& c, const float (&v)[8])
     {
-        constexpr int      NT  = 2; // nontemporal: written once
         constexpr uint32_t PER = Eight<E, RUN>::PER;
 #pragma unroll
         for(uint32_t r = 0; r < 8u / RUN; ++r)
@@ -168,9 +167,9 @@ namespace
                 // (the offset in the lane's register: gemm_tiled.hip says why)
                 const uint32_t at = whole ? offset + i * 16u : OUTSIDE;
                 if constexpr(PER * sizeof(E) == 16u)
-                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, w), to, at, 0, NT);
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, w), to, at, 0, POLICY);
                 else
-                    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, w), to, at, 0, NT);
+                    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, w), to, at, 0, POLICY);
             }
             if(c.some && !whole)
 #pragma unroll
@@ -182,6 +181,25 @@ namespace
                     else
                         __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, static_cast<E>(v[r * RUN + e])), to, at, 0, 0);
                 }
+        }
+    }
+
+    // Nontemporally where rows begin with a cache line, as what is written once; otherwise the L2 puts the lines together that neighbouring tiles write parts of
+    // (8 gradients of 8144 x 5544 in f32 569 -> 277 us; of 4096 x 1536 102 instead of 76).
+    template <typename E, uint32_t BATCH, uint32_t RUN>
+    __device__ __forceinline__ void storeRows(bool lines, __amdgpu_buffer_rsrc_t to, uint32_t first, uint32_t step, const Columns<RUN>& c, const float (&v)[BATCH][8])
+    {
+        if(lines) // (uniform)
+        {
+#pragma unroll
+            for(uint32_t u = 0; u < BATCH; ++u)
+                storeRow<E, 2>(to, first + u * step, c, v[u]);
+        }
+        else
+        {
+#pragma unroll
+            for(uint32_t u = 0; u < BATCH; ++u)
+                storeRow<E, 0>(to, first + u * step, c, v[u]);
         }
     }
 
@@ -269,9 +287,7 @@ namespace
                         for(uint32_t e = 0; e < 8u; ++e)
                             sum[u][e] += bias[e];
                     if(p.z)
-#pragma unroll
-                        for(uint32_t u = 0; u < BATCH; ++u)
-                            storeRow<T>(toZ, ((b + u) * RPI + rowLane) * p.ldz * 2u, at, sum[u]);
+                        storeRows<T>(p.linesZ != 0u, toZ, (b * RPI + rowLane) * p.ldz * 2u, RPI * p.ldz * 2u, at, sum);
                     r355::withActivation(p.activation, [&](auto act) __attribute__((always_inline)) {
 #pragma unroll
                         for(uint32_t u = 0; u < BATCH; ++u)
@@ -292,9 +308,7 @@ namespace
 #pragma unroll
                         for(uint32_t e = 0; e < 8u; ++e)
                             sum[u][e] += add[W][u][e];
-#pragma unroll
-                for(uint32_t u = 0; u < BATCH; ++u)
-                    storeRow<Out>(toY, ((b + u) * RPI + rowLane) * p.ldy * OS, at, sum[u]);
+                storeRows<Out>(p.linesY != 0u, toY, (b * RPI + rowLane) * p.ldy * OS, RPI * p.ldy * OS, at, sum);
             };
             constexpr std::integral_constant<uint32_t, 0> even;
             constexpr std::integral_constant<uint32_t, 1> odd;
