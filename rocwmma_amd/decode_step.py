@@ -4,7 +4,8 @@ sequence's cache and its ancestors in the draft, and a second 4-bit product that
 
     python -m rocwmma_amd.decode_step [--sequences 8] [--drafted 48] [--cached 4000] [--hidden 4096] [--heads 32] [--kv-heads 8] [--head-dim 128]
 
-times such a step over random weights and a random cache, launched one by one and replayed from a graph."""
+times such a step over random weights and a random cache, launched one by one and replayed from a graph.  With --experts (and --top, --width) the feed-forward
+half follows, expert_layer.py's."""
 import argparse
 
 
@@ -137,6 +138,9 @@ def main():
     ap.add_argument("--head-dim", type=int, default=128)
     ap.add_argument("--page-size", type=int, default=16)
     ap.add_argument("--steps", type=int, default=200)
+    ap.add_argument("--experts", type=int, default=0, help="a feed-forward half of so many experts (0: none)")
+    ap.add_argument("--top", type=int, default=4, help="experts of a token")
+    ap.add_argument("--width", type=int, default=1024, help="of an expert")
     args = ap.parse_args()
 
     import torch
@@ -150,13 +154,23 @@ def main():
     tokens = args.sequences * args.drafted
     layer.reserve(tokens, args.drafted, args.drafted + args.cached, args.sequences, step["table"].shape[1])
     x = torch.randn(tokens, args.hidden, device="cuda").to(layer.torch_type)
-    layer.step(x, **step)
+    whole = layer.step
+    if args.experts:
+        from rocwmma_amd.expert_layer import ExpertLayer
+
+        experts = ExpertLayer(args.hidden, args.width, args.experts, args.top)
+        experts.reserve(tokens)
+
+        def whole(x, stream=None, **step):
+            return experts.forward(layer.step(x, stream=stream, **step), stream=stream)
+
+    whole(x, **step)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph, stream=side):
-        layer.step(x, **step, stream=torch.cuda.current_stream())
-    for name, fn in (("launched", lambda: layer.step(x, **step)), ("replayed", graph.replay)):
+        whole(x, **step, stream=torch.cuda.current_stream())
+    for name, fn in (("launched", lambda: whole(x, **step)), ("replayed", graph.replay)):
         for _ in range(20):
             fn()
         begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
