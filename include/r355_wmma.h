@@ -401,7 +401,7 @@ typedef enum
  * groups = 1, offsets = NULL: one matrix of weights.  Otherwise rows offsets[e] .. offsets[e + 1] - 1 use weights and bias of group e; offsets is device memory, not read by the host;
  * rows in no group are left as they were, and what offsets holds beyond the rows is cut off.  (A slice of the offsets with w from its first group on: some of the experts.)
  * source (device memory, or NULL): row r is row source[r] of x, which has x_rows of them; a number that is none of them reads as zeros.
- * c may be y.  Any sizes up to 2^30 rows, n and k of 2^22 - 8 and 1024 groups; any leading dimension and alignment of an element, fastest (several times) with rows of x and w on
+ * c may be y (of the same leading dimension); any other overlap of y or z with what is read is undefined.  Any sizes up to 2^30 rows, n and k of 2^22 - 8 and 1024 groups; any leading dimension and alignment of an element, fastest (several times) with rows of x and w on
  * 16-byte boundaries and k a multiple of 8; then with n a multiple of 8 and the other rows on 16-byte boundaries.  With source, x_rows times ldx up to 2^31 bytes.
  * workspace (16-byte aligned, contents irrelevant): with it the sum is split over workgroups where the result has few tiles; r355_linear_workspace_bytes says how much is made use of.
  * Calls that overlap need one each.  The result depends on the sizes and the workspace offered, not on scheduling.
@@ -431,7 +431,7 @@ size_t r355_linear_workspace_bytes(const r355_linear_args* args);
  * The gradients of r355_linear for dy = dL / dy [rows][n]:
  *   dz = dy * gate * act'(z);  dgate = dy * act(z);  dx = dz W;  dw = dz^T x;  dbias = sum of dz over a group's rows      (of c: dy itself)
  * z: as the forward call wrote it; gate, z: NULL where there is none or no activation.  dgate, dx, dw, dbias: NULL where not wanted.  dz (in_type, written) is needed with an
- * activation or a gate; without either dz is dy.  It is rounded to in_type for the two products; dbias (f32) is summed before that rounding.  dw: grad_type (in_type
+ * activation or a gate, and may be dy or z (of the same leading dimension); without either dz is dy.  It is rounded to in_type for the two products; dbias (f32) is summed before that rounding.  dw: grad_type (in_type
  * or R355_F32), [groups][n][k]; of a group without rows zeros.  accumulate: dw and dbias are added to what is there.  All else is of in_type.
  * x and dx are by rows, as dy is (rows taken by source: their gradient is the sum over the rows that took them, r355_combine).  Groups, sizes and strides as above; fastest with
  * rows on 16-byte boundaries and, for dx, n a multiple of 8.  workspace: as above, and for the shares of dbias.

@@ -75,13 +75,15 @@ namespace r355
         uint32_t group, first, count;
     };
     // Walks the groups' tiles of TM rows, 64 groups at a time, a group a lane: total() counts them, at() finds one.  The host does not know the groups' sizes;
-    // a launch has as many workgroups as any division of the rows could need, and those without a tile end at once.
+    // a launch has as many workgroups as any division of the rows could need, and those without a tile end at once.  (Offsets that are no division of the rows can name more tiles than
+    // that: the count stops at MOST, which keeps it from passing 32 bits, and tiles past the launch's workgroups are left out.)
     template <uint32_t TM>
     struct GroupTiles
     {
-        const LinearParams& p;
-        uint32_t            base = 0u, tiles = 0u, upto = 0u, all = 0u;
-        Rows                rows{0u, 0u};
+        static constexpr uint32_t MOST = 1u << 31; // (64 groups have 2^30 tiles at most: 2^30 rows, TM >= 64 or few rows)
+        const LinearParams&       p;
+        uint32_t                  base = 0u, tiles = 0u, upto = 0u, all = 0u;
+        Rows                      rows{0u, 0u};
 
         __device__ __forceinline__ void block(uint32_t first, uint32_t before)
         {
@@ -91,6 +93,11 @@ namespace r355
             base             = first;
             upto             = before + lanesUpTo(tiles);
         }
+        __device__ __forceinline__ uint32_t upToHere() const
+        {
+            const uint32_t n = __builtin_amdgcn_readlane(upto, 63);
+            return n < MOST ? n : MOST;
+        }
         __device__ __forceinline__ uint32_t total()
         {
             if(!p.offsets)
@@ -99,7 +106,7 @@ namespace r355
             for(uint32_t first = 0; first < p.groups; first += 64u)
             {
                 block(first, all);
-                all = __builtin_amdgcn_readlane(upto, 63);
+                all = upToHere();
             }
             return all;
         }
@@ -114,7 +121,7 @@ namespace r355
                 for(uint32_t first = 0, before = 0; first < p.groups; first += 64u)
                 {
                     block(first, before);
-                    before = __builtin_amdgcn_readlane(upto, 63);
+                    before = upToHere();
                     if(before > tile)
                         break;
                 }

@@ -111,6 +111,25 @@ def test_offsets_beyond_the_rows_are_cut_off(offsets, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,groups", [(200, 300), (2000, 300), (5000, 130)])
+def test_groups_that_are_no_division_of_the_rows(rows, groups):
+    """Every other group claims all rows: more tiles than a launch has workgroups for.  Every row that is written is one of the groups' results"""
+    import linearlib
+    import torch
+
+    n, k = 40, 64
+    x, w = torch.randint(-2, 3, (rows, k), device="cuda").half(), torch.randint(-2, 3, (1, n, k), device="cuda").half().expand(groups, n, k).contiguous()
+    offsets = torch.tensor([0, rows] * (groups // 2 + 1), dtype=torch.int32)[: groups + 1].cuda()
+    y, view = linearlib.matrix(torch.zeros(rows, n, device="cuda"), torch.float16, n + 4)
+    y.fill_(float("nan"))
+    R.linear(R.F16, R.F16, rows, n, k, x, w, y, groups=groups, offsets=offsets, ldy=n + 4)
+    assert torch.isnan(view[0, :, n:]).all() and torch.isnan(y[rows * (n + 4):]).all()
+    want = x.float() @ w[0].float().t()
+    got = view[0, :, :n].float()
+    assert (torch.isnan(got) | (got == want)).all() and (got == want).any()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows,k", [(6, 64), (300, 72), (30, 65)])
 def test_source_rows_that_are_not_there_read_as_zeros(rows, k):
     source = [(r * 7) % 11 for r in range(rows)]

@@ -94,6 +94,23 @@ def test_parts_of_the_gradient(want):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("over", ["dy", "z"])
+def test_dz_in_the_place_of_what_it_is_made_of(over):
+    import torch
+
+    rows, n, k = 100, 64, 72
+    make = lambda *shape: torch.randn(*shape, device="cuda").half()  # noqa: E731
+    x, w, dy, z, gate = make(rows, k), make(n, k), make(rows, n), make(rows, n), make(rows, n)
+    results = []
+    for dz in (torch.empty_like(dy), dy.clone() if over == "dy" else z.clone()):
+        dx, dw, db, dg = torch.empty_like(x), torch.empty_like(w), torch.empty(n, device="cuda"), torch.empty_like(dy)
+        here = dict(dy=dz if over == "dy" and results else dy, z=dz if over == "z" and results else z)
+        R.linear_backward(R.F16, R.F16, rows, n, k, here["dy"], x, w, dx=dx, dw=dw, dbias=db, z=here["z"], activation=R.ACT_SILU, gate=gate, dgate=dg, dz=dz)
+        results.append((dx, dw, db, dg, dz))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.gpu
 def test_the_result_does_not_depend_on_scheduling_and_little_on_the_workspace():
     import torch
 
