@@ -505,7 +505,8 @@ int r355_route_backward(const r355_route_backward_args* args, void* stream);
 
 /*
  * y[t] = sum_j weights[t][j] values[place[t][j]] + c[t]: the experts' rows put together, f32 sums, rounded once.  values: [rows][width] of type (R355_F16 or R355_BF16), as c and y;
- * weights: f32, or NULL for ones; c: NULL, or y itself.  A place outside [0, rows) is left out.  Any width, leading dimension and alignment of an element, fastest in multiples of 16 bytes.
+ * weights: f32, or NULL for ones; c: NULL, or y itself (of the same leading dimension).  A place outside [0, rows) is left out.  Any width, leading dimension and alignment of an element, fastest in multiples of 16 bytes.
+ * At most 2^30 rows and places, 2^24 elements a row and about 2^35 elements of y (2^32 where rows are not multiples of 16 bytes).
  */
 typedef struct
 {
@@ -523,7 +524,8 @@ int r355_combine(const r355_combine_args* args, void* stream);
 /*
  * out[place[t][j]] = weights[t][j] x[t] (weights NULL: x[t]): the tokens' rows to the experts, and the gradient of r355_combine with respect to its values; its weights'
  * gradient is dweights[t][j] = x[t] . values[place[t][j]] (f32 sums; dweights NULL: not wanted, values then not read; out NULL: only that).  A place outside [0, rows) is left out (its
- * dweights 0); rows that no place names are left as they were; no row is named twice.  out must not overlap x or values.  Sizes and types as above.
+ * dweights 0); rows that no place names are left as they were; no row is named twice.  out must not overlap x or values.  Sizes and types as above; at most 2^24 - 8 tokens
+ * (of 1024 elements and less: four times as many).
  */
 typedef struct
 {

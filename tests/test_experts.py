@@ -92,6 +92,26 @@ def test_route_numbers_of_tokens(tokens):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tokens,experts", [(3, 8), (70, 32), (40, 3)])
+def test_route_to_every_expert(tokens, experts):
+    import torch
+
+    for score in ("softmax", "sigmoid"):
+        _run(torch.randn(tokens, experts, device="cuda"), experts, "f16", score, True, bias=torch.randn(experts, device="cuda"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("experts", [1, 8, 1000])
+def test_route_of_no_tokens(experts):
+    """Every expert's rows begin and end at 0"""
+    import torch
+
+    offsets = torch.full((experts + 2,), -7, dtype=torch.int32, device="cuda")
+    R.route(R.F16, 0, experts, 1, None, None, None, None, None, offsets)
+    assert (offsets[:-1] == 0).all() and offsets[-1] == -7
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("tokens", [5, 200])
 @pytest.mark.parametrize("top", [2, 8])
 def test_route_ties_infinities_and_nan(tokens, top):
@@ -272,6 +292,30 @@ def test_each_is_the_others_gradient():
     R.dispatch(R.BF16, tokens, top, width, dy, dv, tokens * top, place, weights=w, values=v, dweights=dw)
     inner = (y.double() * dy.double()).sum()
     assert inner == (v.double() * dv.double()).sum() and inner == (w.double() * dw.double()).sum()
+
+
+@pytest.mark.gpu
+def test_more_rows_than_the_caches_keep():
+    """In values that 16 bits hold exactly"""
+    import torch
+
+    tokens, top, width = 3000, 8, 2104
+    rows = tokens * top
+    place = torch.randperm(rows, device="cuda").to(torch.int32).view(tokens, top)
+    place[5, 2], place[2999, 7] = -1, rows
+    small = lambda *shape: torch.randint(-3, 4, shape, device="cuda").bfloat16()  # noqa: E731
+    v, x, w = small(rows, width), small(tokens, width), torch.randint(-1, 2, (tokens, top), device="cuda").float()
+    y, out, dw = torch.empty_like(x), torch.full_like(v, float("nan")), torch.empty(tokens, top, device="cuda")
+    R.combine(R.BF16, tokens, top, width, v, rows, place, y, weights=w, c=x)
+    R.dispatch(R.BF16, tokens, top, width, x, out, rows, place, weights=w, values=v, dweights=dw)
+    there = (place >= 0) & (place < rows)
+    at = torch.where(there, place, 0).long()
+    total = x.float()
+    for j in range(top):
+        total += torch.where(there[:, j, None], v[at[:, j]].float() * w[:, j, None], 0.0)
+        assert torch.equal(out[at[:, j]][there[:, j]].float(), (x.float() * w[:, j, None])[there[:, j]])
+        assert torch.equal(dw[:, j], torch.where(there[:, j], (x.float() * v[at[:, j]].float()).sum(1), 0.0))
+    assert torch.equal(y.float(), total) and torch.isnan(out).any(1).sum() == 2
 
 
 @pytest.mark.gpu

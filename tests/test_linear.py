@@ -219,6 +219,84 @@ def test_streams_and_graph():
     assert linearlib.EPS
 
 
+def _workspace_bytes(rows, n, k, **kw):
+    return R.linear_workspace_bytes(R.linear_args(R.BF16, R.BF16, rows, n, k, 0x1000, 0x2000, 0x3000, **kw))
+
+
+def _scratch(nbytes):
+    import torch
+
+    return torch.full((nbytes,), 255, dtype=torch.uint8, device="cuda")  # (NaN, whatever is read of it before it is written)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n,k,pad", [(100, 200, 4096, 0), (65, 129, 2056, 3), (300, 70, 1999, 1), (17, 513, 8192, 0)])
+def test_sums_split_over_workgroups(rows, n, k, pad):
+    """With a workspace and few tiles: the whole epilogue after the shares are added, c in place, both types of the result, a workspace for fewer shares, one that is too small for any"""
+    need = _workspace_bytes(rows, n, k, ldx=k + pad)
+    assert need > 0
+    for size in (need, need // 2 // 16 * 16, 16):
+        _run("bf16", "bf16", rows, n, k, act="gelu", bias=True, gate=True, c=True, keep=True, pad=(pad, 0, pad, pad, pad, pad), workspace=_scratch(size))
+        _run("f16", "f32", rows, n, k, act="silu", bias=True, c=True, in_place=True, pad=(pad, 0, 0, 0, 0, 0), workspace=_scratch(size))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n,k", [(4099, 4096, 1544), (2600, 8192, 1600)])
+def test_rows_past_whole_rounds_of_tiles(rows, n, k):
+    """The rows that whole rounds of large tiles leave go out on tiles of their own, all operands with them, split along the sum where there is a workspace"""
+    _run("bf16", "bf16", rows, n, k, act="silu", bias=True, gate=True, c=True, keep=True, pad=(0, 0, 8, 16, 24, 32))
+    _run("f16", "f32", rows, n, k, c=True, in_place=True, source=[(13 * r + 5) % 2000 for r in range(rows)], x_rows=2000, workspace=_scratch(1 << 24))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sizes,n,k", [([1] * 32, 2048, 1024), ([4] * 16, 2048, 2048), ([5, 0, 0, 1, 0, 0, 0, 0, 2, 0], 80, 1032), ([3, 0, 9, 0, 20], 100, 2056), ([0, 1], 72, 64)])
+def test_few_rows_of_each_group(sizes, n, k):
+    """The kernels for few rows, with weights that the caches hold and that they do not, with several of their tiles to a group"""
+    _run("bf16", "bf16", sum(sizes), n, k, act="silu", bias=True, gate=True, groups=len(sizes), offsets=_offsets(sizes))
+    _run("f16", "f32", sum(sizes), n, k, c=True, keep=True, groups=len(sizes), offsets=_offsets(sizes), source=[(3 * r) % 5 for r in range(sum(sizes))], x_rows=5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [2, 12, 70, 900])
+def test_one_group_with_offsets(rows):
+    _run("bf16", "bf16", rows, 72, 128, bias=True, act="relu", groups=1, offsets=[rows // 3, rows - 1], c=True, in_place=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pad,offset", [(0, 0), (64, 0), (8, 0), (0, 32)])
+def test_rows_of_results_on_and_off_cache_lines(pad, offset):
+    """Results whose rows begin with a cache line are written past the caches, others not: what lies between the rows stays, in either case"""
+    _run("bf16", "bf16", 300, 256, 128, act="silu", keep=True, pad=(0, 0, 0, 0, pad, 64 - pad % 64), offset=offset)
+    _run("f16", "f32", 300, 256, 128, c=True, in_place=True, pad=(0, 0, 0, 0, pad, 0), offset=offset)
+
+
+@pytest.mark.gpu
+def test_two_calls_at_once():
+    """On two streams, each with a workspace of its own, against the same calls one after the other"""
+    import torch
+
+    rows, n, k = 100, 200, 4096
+    a = [torch.randn(rows, k, device="cuda").bfloat16() for _ in range(2)]
+    w = [torch.randn(n, k, device="cuda").bfloat16() for _ in range(2)]
+    streams, need = [torch.cuda.Stream() for _ in range(2)], _workspace_bytes(rows, n, k)
+    scratch = [_scratch(need) for _ in range(2)]
+    alone, both = ([torch.empty(rows, n, dtype=torch.bfloat16, device="cuda") for _ in range(2)] for _ in range(2))
+    for i in range(2):
+        R.linear(R.BF16, R.BF16, rows, n, k, a[i], w[i], alone[i], workspace=scratch[0])
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i in range(2):
+            R.linear(R.BF16, R.BF16, rows, n, k, a[i], w[i], both[i], workspace=scratch[i], stream=streams[i])
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(alone, both))
+
+
+def test_workspace_bytes():
+    assert _workspace_bytes(100, 200, 4096) >= 2 * 100 * 200 * 4
+    assert _workspace_bytes(2, 4096, 4096) == 0 and _workspace_bytes(4096, 4096, 4096) == 0 and _workspace_bytes(0, 8, 8) == 0
+    assert _workspace_bytes(100, 200, 4096, groups=2, offsets=0x4000) == 0  # (rows of no group are not to be written)
+
+
 def _args(**change):
     a = R.linear_args(R.BF16, R.BF16, 4, 8, 16, 0x1000, 0x2000, 0x3000)
     for name, value in change.items():

@@ -94,6 +94,101 @@ def test_parts_of_the_gradient(want):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("grad", ["bf16", "f32"])
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("rows,n,k,sizes,pad", [(4096, 72, 136, None, 0), (90, 4096, 72, None, 0), (3000, 100, 45, None, 1), (4000, 40, 72, [3000, 0, 1000], 0)])
+def test_sums_split_over_workgroups(rows, n, k, sizes, pad, accumulate, grad):
+    """With a workspace and few tiles, dx and dw: whole, for fewer shares, and too small for any"""
+    groups, offsets = (1, None) if sizes is None else (len(sizes), _offsets(sizes))
+    a = R.linear_backward_args(R.BF16, R.F32, rows, n, k, 0x1000, 0x2000, 0x3000, dx=0x4000, dw=0x5000, groups=groups, offsets=None if sizes is None else 0x6000)
+    need = R.linear_backward_workspace_bytes(a)
+    assert need > 0
+    for size in (need, need // 2 // 16 * 16, 16):
+        _run("bf16", grad, rows, n, k, act="gelu", groups=groups, offsets=offsets, accumulate=accumulate, pad=pad, workspace=_scratch(size))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("act", ["none", "silu"])
+@pytest.mark.parametrize("k", [72, 45])
+def test_no_rows(accumulate, act, k):
+    """The weights' and the bias's gradient are zeros, or what was there"""
+    import torch
+
+    dw, db = torch.full((40, k), 3.0, device="cuda"), torch.full((40,), 5.0, device="cuda")
+    R.linear_backward(R.F16, R.F32, 0, 40, k, None, None, None, dx=0x1000, dw=dw, dbias=db, activation=R.ACT_SILU if act == "silu" else R.ACT_NONE, dz=0x1000, accumulate=accumulate,
+                      workspace=_scratch())
+    assert (dw == (3.0 if accumulate else 0.0)).all() and (db == (5.0 if accumulate else 0.0)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [2, 70, 900])
+def test_one_group_with_offsets(rows):
+    _run("bf16", "f32", rows, 72, 136, act="relu", gate=True, groups=1, offsets=[rows // 3, rows - 1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n,k", [(4099, 1544, 4096)])
+def test_rows_past_whole_rounds_of_tiles(rows, n, k):
+    _run("bf16", "bf16", rows, n, k, act="silu", gate=True, pad=8, workspace=_scratch(1 << 24))
+
+
+@pytest.mark.gpu
+def test_infinities_and_nan_stay_in_their_rows_and_columns():
+    import torch
+
+    rows, n, k = 200, 72, 136
+    x, w, dy = torch.randn(rows, k, device="cuda").bfloat16(), torch.randn(n, k, device="cuda").bfloat16(), torch.randn(rows, n, device="cuda").bfloat16()
+    x[3, 5], w[7, 9], dy[rows - 1, n - 1] = float("nan"), float("inf"), float("nan")
+    dx, dw, db = torch.empty_like(x), torch.empty(n, k, device="cuda"), torch.empty(n, device="cuda")
+    R.linear_backward(R.BF16, R.F32, rows, n, k, dy, x, w, dx=dx, dw=dw, dbias=db)
+    bad = torch.zeros(rows, k, dtype=torch.bool, device="cuda")
+    bad[-1], bad[:, 9] = True, True
+    assert torch.equal(~torch.isfinite(dx), bad)
+    bad = torch.zeros(n, k, dtype=torch.bool, device="cuda")
+    bad[-1], bad[:, 5] = True, True
+    assert torch.equal(~torch.isfinite(dw), bad)
+    assert torch.equal(~torch.isfinite(db), torch.arange(n, device="cuda") == n - 1)
+
+
+@pytest.mark.gpu
+def test_graph():
+    """Recorded on a stream of its own with other values and offsets at every replay, the program's eager work between them"""
+    import torch
+
+    rows, n, k, groups = 300, 72, 136, 3
+    make = lambda *shape: torch.randn(*shape, device="cuda").bfloat16()  # noqa: E731
+    x, w, dy, z, gate = make(rows, k), make(groups, n, k), make(rows, n), make(rows, n), make(rows, n)
+    offsets = torch.zeros(groups + 1, dtype=torch.int32, device="cuda")
+    scratch = [_scratch() for _ in range(2)]
+
+    def results():
+        return [torch.zeros(rows, k, dtype=torch.bfloat16, device="cuda"), torch.zeros(groups, n, k, device="cuda"), torch.zeros(groups, n, device="cuda"),
+                torch.zeros_like(z), torch.zeros_like(z)]
+
+    def call(to, workspace, stream):
+        dx, dw, db, dg, dz = to
+        R.linear_backward(R.BF16, R.F32, rows, n, k, dy, x, w, dx=dx, dw=dw, dbias=db, z=z, activation=R.ACT_SILU, gate=gate, dgate=dg, dz=dz, accumulate=True, groups=groups,
+                          offsets=offsets, workspace=workspace, stream=stream)
+
+    recorded, eager = results(), results()
+    call(eager, scratch[1], None)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        call(recorded, scratch[0], torch.cuda.current_stream())
+    for at in ([0, 100, 100, 300], [0, 0, 0, 300], [10, 20, 250, 260]):
+        offsets.copy_(torch.tensor(at, dtype=torch.int32))
+        dy.copy_(torch.randn(rows, n, device="cuda"))
+        for a, b in zip(recorded, eager):
+            a.zero_(), b.zero_()
+        graph.replay()
+        call(eager, scratch[1], None)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(recorded, eager)) and eager[1].abs().sum() > 0
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("over", ["dy", "z"])
 def test_dz_in_the_place_of_what_it_is_made_of(over):
     import torch
@@ -123,8 +218,9 @@ def test_the_result_does_not_depend_on_scheduling_and_little_on_the_workspace():
 @pytest.mark.gpu
 @pytest.mark.parametrize("act", ["none", "relu", "gelu", "gelu_tanh", "silu"])
 def test_against_differences(act):
-    """dL of L = sum y r for steps of x, w, bias and gate along random directions, of calls in f32 results.  A central difference of a function whose second derivative along the step is
-    curved by less than 10 is off by h^2 10 / 6 at most; roundings of y in f32 and of the operands (the steps are made of 16-bit values) by 2^-24 sum |y r| / h.  dz is rounded to 16 bits."""
+    """dL of L = sum y r for steps of x, w, bias and gate along random directions, of calls in f32 results.  A central difference is off by
+    h^2 / 6 times the third derivative along the step, here |act'''| <= 1 times the cube of the argument's change; roundings of y in f32 and of the operands (the steps are made of
+    16-bit values) by 2^-24 sum |y r| / h.  dz is rounded to 16 bits."""
     import torch
 
     rows, n, k, h = 24, 32, 64, 2.0 ** -5
@@ -154,8 +250,7 @@ def test_against_differences(act):
         down, _ = loss(**{**values, name: at - h * step})
         analytic = (grad.double() * step.double()).sum().item()
         spread = (grad.double() * step.double()).abs().sum().item()
-        # curvature: |act''| <= 1.13 for each result, times the square of its change along the step; relu has a kink: a result whose argument passes zero on the way
-        # is off by half of its change
+        # curvature, as above (six times as much); relu has a kink: a result whose argument passes zero on the way is off by half of its change
         dzs = (x.double() @ step.double().t()) if name == "w" else (step.double() @ w.double().t()) if name == "x" else step.double().expand(rows, n) if name == "b" else torch.zeros(rows, n, device="cuda").double()
         rg = (r * gate).double().abs()
         curved = 0.0 if act == "none" else (rg * dzs.abs() * (z.double().abs() <= h * dzs.abs() + 2.0 ** -8)).sum().item() if act == "relu" else (rg * dzs.abs() ** 3).sum().item() * h * h
