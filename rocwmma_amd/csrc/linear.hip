@@ -334,13 +334,13 @@ namespace
     }
 
     // ---- Sums of a split product: [splits][rows][pitch] of f32, added in order, then the epilogue of linear_tiles.hip.  Result rows are `p.m` to a group (weights' gradient), or
-    // all one group's.  Four columns a thread; what is not four columns wide, or past a row's end, goes element by element.
+    // by offsets; those of no group are left.  Four columns a thread; what is not four columns wide, or past a row's end, goes element by element.
     template <typename T, typename Out>
     __global__ void __launch_bounds__(256) linearReduce(LinearParams p, const float* sums, uint64_t rows, uint32_t pitch)
     {
-        const uint32_t col = (blockIdx.x * 256u + threadIdx.x) * 4u, left = col < p.n ? p.n - col : 0u;
-        if(left == 0u)
-            return;
+        const uint32_t mine = (blockIdx.x * 256u + threadIdx.x) * 4u, left = mine < p.n ? p.n - mine : 0u, col = left ? mine : 0u;
+        if(__ballot(left != 0u) == 0u)
+            return; // (whole waves: the lanes find a row's group together)
         // (rows anywhere: vectors of an element's alignment)
         typedef T    TU __attribute__((ext_vector_type(4), aligned(2)));
         typedef Out  OutU __attribute__((ext_vector_type(4), aligned(sizeof(Out))));
@@ -371,12 +371,26 @@ namespace
                         to[e] = static_cast<E>(v[e]);
         };
         float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if(p.bias)
+        if(p.bias && !p.offsets)
             read(reinterpret_cast<const T*>(p.bias) + col, bias);
         const uint64_t share = rows * pitch;
         for(uint64_t row = blockIdx.y; row < rows; row += gridDim.y)
         {
             const uint64_t group = p.m ? row / p.m : 0u, in = p.m ? row % p.m : row;
+            if(p.m == 0u && p.offsets)
+            {
+                // a row's group is the last one that begins at or before it: as many offsets are no larger, less one
+                uint32_t begun = 0u;
+                for(uint32_t g = threadIdx.x & 63u; g - (threadIdx.x & 63u) <= p.groups; g += 64u)
+                    begun += static_cast<uint32_t>(__popcll(__ballot(g <= p.groups && p.offsets[g <= p.groups ? g : 0u] <= static_cast<int64_t>(row))));
+                if(begun == 0u || begun > p.groups)
+                    continue; // no group's
+                const Rows its = r355::rowsOf(p, begun - 1u);
+                if(row < its.first || row - its.first >= its.count)
+                    continue; // (offsets that are no division)
+                if(p.bias)
+                    read(reinterpret_cast<const T*>(p.bias) + (uint64_t)(begun - 1u) * p.n + col, bias);
+            }
             const float*   from = sums + row * pitch + col;
             float          sum[4], more[4];
             f32x4          all{0.0f, 0.0f, 0.0f, 0.0f};
@@ -628,8 +642,8 @@ namespace
             const double all = tiles(tile, p.rows);
             for(uint32_t splits = 1u; splits <= 64u; splits += splits < 4u ? 1u : splits / 2u)
             {
-                // (a sum is split in whole stages, four of them at least; rows of no group are not to be written)
-                if(splits > 1u && ((aK && p.offsets) || stages < 4.0 * splits || rowsY * pitchOf(p.n) * 4u * splits > workspaceBytes || all > computeUnits()))
+                // (a sum is split in whole stages, four of them at least)
+                if(splits > 1u && (stages < 4.0 * splits || rowsY * pitchOf(p.n) * 4u * splits > workspaceBytes || all > computeUnits()))
                     break;
                 const double us = launchTime(tile, all * splits, stages / splits) + (splits > 1u ? 5.0 + static_cast<double>(rowsY) * p.n * 4.0 * (2u * splits + 1u) / 5e6 : 0.0);
                 if(us < best.us)
@@ -701,7 +715,8 @@ namespace
         p.linesY = p.splits == 1u && lines(p.y, p.ldy, p.outF32 ? 4u : 2u), p.linesZ = lines(p.z, p.ldz, 2u);
         const uint32_t rows = r355::LINEAR_ROWS[tile];
         p.tilesN = static_cast<uint32_t>(tilesOf(p.n, r355::LINEAR_COLS[tile])), p.tilesM = static_cast<uint32_t>(tilesOf(p.m, rows));
-        const uint64_t tiles = (aK ? mostTiles(p, rows) : (uint64_t)p.tilesM * p.groups) * p.tilesN;
+        // (of a weights' gradient: an eighth of a group's tiles for each XCD may be a tile more)
+        const uint64_t tiles = aK ? mostTiles(p, rows) * p.tilesN : tilesOf((uint64_t)p.tilesM * p.tilesN, 8u) * 8u * p.groups;
         if(tiles > r355::MAX_GROUPS)
             return tooMany(what);
         const uint32_t workgroups = static_cast<uint32_t>((tiles + 7u) / 8u * 8u);

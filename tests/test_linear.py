@@ -241,6 +241,17 @@ def test_sums_split_over_workgroups(rows, n, k, pad):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("offsets,rows,n,k", [([0, 30, 30, 58, 60], 60, 200, 4096), ([3, 20, 50], 64, 1030, 2056), ([0] * 70 + [40] + [90] * 60, 97, 33, 1999), ([5, 90], 100, 72, 2048)])
+def test_sums_of_groups_split_over_workgroups(offsets, rows, n, k):
+    """Rows before, between and behind the groups are left as they were, also by what adds the shares"""
+    groups = len(offsets) - 1
+    need = _workspace_bytes(rows, n, k, groups=groups, offsets=0x4000)
+    assert need > 0
+    _run("bf16", "bf16", rows, n, k, act="gelu", bias=True, gate=True, keep=True, groups=groups, offsets=offsets, workspace=_scratch(need))
+    _run("f16", "f32", rows, n, k, bias=True, c=True, in_place=True, groups=groups, offsets=offsets, workspace=_scratch(need // 2 // 16 * 16))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows,n,k", [(4099, 4096, 1544), (2600, 8192, 1600)])
 def test_rows_past_whole_rounds_of_tiles(rows, n, k):
     """The rows that whole rounds of large tiles leave go out on tiles of their own, all operands with them, split along the sum where there is a workspace"""
@@ -294,7 +305,7 @@ def test_two_calls_at_once():
 def test_workspace_bytes():
     assert _workspace_bytes(100, 200, 4096) >= 2 * 100 * 200 * 4
     assert _workspace_bytes(2, 4096, 4096) == 0 and _workspace_bytes(4096, 4096, 4096) == 0 and _workspace_bytes(0, 8, 8) == 0
-    assert _workspace_bytes(100, 200, 4096, groups=2, offsets=0x4000) == 0  # (rows of no group are not to be written)
+    assert _workspace_bytes(100, 200, 4096, groups=2, offsets=0x4000) >= 2 * 100 * 200 * 4
 
 
 def _args(**change):
