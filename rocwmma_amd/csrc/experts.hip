@@ -33,9 +33,16 @@ namespace
     {
         return reduce(0u, v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
     }
-    __device__ __forceinline__ float largest(float v) // (a NaN counts as less than any number)
+    // numbers as integers in their order, infinities at their ends and NaN beyond them, and back
+    __device__ __forceinline__ uint32_t orderOf(float v)
     {
-        return __uint_as_float(reduce(0xFF800000u, __float_as_uint(v), [](uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }));
+        const uint32_t b = __float_as_uint(v);
+        return b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
+    }
+    __device__ __forceinline__ float largest(float v) // (of integers a step is one instruction, of floats it is four; where one is NaN so is all that is made of the result)
+    {
+        const uint32_t k = largest(orderOf(v));
+        return __uint_as_float(k ^ (~static_cast<uint32_t>(static_cast<int32_t>(k) >> 31) | 0x80000000u));
     }
     __device__ __forceinline__ float sum(float v)
     {
@@ -67,7 +74,8 @@ namespace
     // log of a score: the logit itself (softmax, up to what its sum takes off) or log sigma
     __device__ __forceinline__ float logScore(int32_t score, float x)
     {
-        return score == R355_ROUTE_SIGMOID ? fminf(x, 0.0f) - __logf(1.0f + __expf(-fabsf(x))) : x;
+        // (the logarithm's argument lies in [1, 2]: nothing to scale)
+        return score == R355_ROUTE_SIGMOID ? fminf(x, 0.0f) - 0.69314718056f * __builtin_amdgcn_logf(1.0f + __expf(-fabsf(x))) : x;
     }
 
     // e^(v - the largest) and their sum; a row of -infinity has zeros
@@ -87,21 +95,38 @@ namespace
         return (a & mask) | (b & ~mask);
     }
 
+    // What a lane keeps from token to token: its experts' biases (zeros without), and which of them there are
+    template <uint32_t V>
+    struct Lane
+    {
+        float    bias[V];
+        uint32_t there[V];
+        __device__ __forceinline__ Lane(const RouteParams& p, uint32_t lane)
+        {
+#pragma unroll
+            for(uint32_t i = 0; i < V; ++i)
+            {
+                const uint32_t e = lane * V + i;
+                bias[i]          = p.bias && e < p.experts ? p.bias[e] + 0.0f : 0.0f; // (never -0)
+                there[i]         = maskOf(e < p.experts);
+            }
+        }
+    };
+
     // One token a wave: expert V lane + i in x[i] of the lane.  A key orders numbers as integers, NaN below them; every lane sorts its keys, and `top` rounds take the largest of
-    // the lanes' first ones, of the lowest lane that has it, which then moves up.  Bound by the vector instructions (some 15 a round).
+    // the lanes' first ones, of the lowest lane that has it, which then moves up.  Bound by the vector instructions: of 256 experts
+    // and 8 choices 309 a token, 17 of them a round; 16384 tokens 16 us (8.6 of issuing).
     // What is returned lies in lane j for the j-th choice: its expert and its logit.
     template <uint32_t V>
-    __device__ __forceinline__ void choose(const RouteParams& p, const float (&x)[V], uint32_t lane, uint32_t& expert, float& logit)
+    __device__ __forceinline__ void choose(const RouteParams& p, const float (&x)[V], const Lane<V>& own, uint32_t lane, uint32_t& expert, float& logit)
     {
         uint32_t key[V], of[V]; // keys, and which of the lane's experts they are of
 #pragma unroll
         for(uint32_t i = 0; i < V; ++i)
         {
-            const uint32_t e  = lane * V + i;
-            const float    by = e < p.experts ? (p.bias ? x[i] + p.bias[e] : x[i]) + 0.0f : 0.0f; // (-0 counts as 0)
-            const uint32_t b  = __float_as_uint(by);
-            key[i] = e >= p.experts ? 0u : by != by ? 1u : (b & 0x80000000u) ? ~b : b | 0x80000000u; // (-infinity: 0x007FFFFF)
-            of[i]  = i;
+            const float by = x[i] + own.bias[i]; // (-0 counts as 0)
+            key[i]         = either(maskOf(by != by), 1u, orderOf(by)) & own.there[i]; // (-infinity: 0x007FFFFF)
+            of[i]          = i;
         }
         // (Neighbours change places only if the later one is larger: equal ones stay in the order of their experts.  Choices by masks, one instruction each: of conditions the
         // compiler makes branches and indices, twice as many.)
@@ -146,10 +171,10 @@ namespace
         {
             const float l = logScore(p.score, logit), most = largest(in ? l : -INFINITY);
             const float e = exponentials(l, in, most), all = sum(e);
-            return all == 0.0f ? 0.0f : e / all * p.scale;
+            return all == 0.0f ? 0.0f : e * __builtin_amdgcn_rcpf(all) * p.scale;
         }
         if(p.score == R355_ROUTE_SIGMOID)
-            return p.scale / (1.0f + __expf(-logit));
+            return p.scale * __builtin_amdgcn_rcpf(1.0f + __expf(-logit));
         float most = -INFINITY, all = 0.0f;
 #pragma unroll
         for(uint32_t i = 0; i < V; ++i)
@@ -159,7 +184,7 @@ namespace
         for(uint32_t i = 0; i < V; ++i)
             all += exponentials(x[i], lane * V + i < p.experts, most);
         all = sum(all);
-        return all == 0.0f ? 0.0f : exponentials(logit, in, most) / all * p.scale;
+        return all == 0.0f ? 0.0f : exponentials(logit, in, most) * __builtin_amdgcn_rcpf(all) * p.scale;
     }
 
     // experts V lane .. V lane + V - 1 of a token: as vectors where the rows are even (a rule of the host's)
@@ -301,7 +326,8 @@ namespace
         __syncthreads();
         const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const uint32_t from = blockIdx.x * p.perBlock, left = p.tokens - from, here = left < p.perBlock ? left : p.perBlock;
-        float next[V]; // the following token's, read ahead
+        const Lane<V>  own(p, lane);
+        float          next[V]; // the following token's, read ahead
         if(wave < here)
             readLogits<T, V>(p, from + wave, lane, next);
         for(uint32_t i = wave; i < here; i += WAVES)
@@ -314,7 +340,7 @@ namespace
                 x[e] = next[e];
             if(i + WAVES < here)
                 readLogits<T, V>(p, token + WAVES, lane, next);
-            choose<V>(p, x, lane, expert, logit);
+            choose<V>(p, x, own, lane, expert, logit);
             const float weight = weightOf<V>(p, x, lane, logit);
             if(lane < p.top)
             {

@@ -224,9 +224,11 @@ namespace
         }
     }
 
-    // ---- Few rows of each group.  A workgroup's eight waves share 16 RB weight rows x 16 CB rows of x and take pieces of 64 of the sum in turn, both
+    // ---- Few rows of each group.  A workgroup's eight waves share 16 RB weight rows x 16 CB rows of x and take DEPTH neighbouring pieces of 64 of the sum in turn, both
     // straight from global memory; their sums meet in LDS in the order of the waves.  The weights are the first operand: a lane then holds four of them of one row of x.
-    template <typename T, uint32_t RB, uint32_t CB, uint32_t DEPTH, bool STREAM>
+    // Bound by HBM: 64 rows of 16 experts of 4096 x 4096 105 us, 5.1 TB/s.  (Single pieces in turn: rows that do not begin with a cache line have lines of two waves, 30 rows of 8 experts
+    // of 8192 x 4104 167 instead of 162 us; and such lines come twice where they are read nontemporally, 162 instead of 125.)
+    template <typename T, uint32_t RB, uint32_t CB, uint32_t DEPTH>
     __global__ void __launch_bounds__(64 * WAVES, 2) linearFew(LinearParams p)
     {
         constexpr uint32_t ROWS = 16u * CB, COLS = 16u * RB, PITCH = COLS + 4u;
@@ -284,7 +286,7 @@ namespace
                 const bool in = piece * 64u + i * 32u + quad * 8u < p.k; // (what lies past the sum's end is another row's)
 #pragma unroll
                 for(uint32_t r = 0; r < RB; ++r)
-                    s.w[r][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(bufW, in ? offW[r] + i * 64u : OUTSIDE, piece * 128u, STREAM ? 2 : 0));
+                    s.w[r][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(bufW, in ? offW[r] + i * 64u : OUTSIDE, piece * 128u, 0));
 #pragma unroll
                 for(uint32_t c = 0; c < CB; ++c)
                     s.x[c][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(bufX, in ? offX[c] + i * 64u : OUTSIDE, piece * 128u, 0));
@@ -294,13 +296,13 @@ namespace
         Stage stage[DEPTH];
         each<DEPTH>([&](auto at) __attribute__((always_inline)) {
             constexpr uint32_t d = decltype(at)::value;
-            if(wave + d * WAVES < pieces)
-                stage[d] = load(wave + d * WAVES);
+            if(wave * DEPTH + d < pieces)
+                stage[d] = load(wave * DEPTH + d);
         });
-        for(uint32_t from = wave; from < pieces; from += DEPTH * WAVES)
+        for(uint32_t from = wave * DEPTH; from < pieces; from += DEPTH * WAVES)
             each<DEPTH>([&](auto at) __attribute__((always_inline)) {
                 constexpr uint32_t d     = decltype(at)::value;
-                const uint32_t     piece = from + d * WAVES;
+                const uint32_t     piece = from + d;
                 if(piece < pieces)
                 {
 #pragma unroll
@@ -666,7 +668,7 @@ namespace
         return best;
     }
 
-    // Weights that no cache keeps from one call to the next are read nontemporally (16 experts of 4096 x 4096 95 -> 85 us, 8192 x 8192 29.8 -> 26.0; three matrices of
+    // One or two rows: weights that no cache keeps from one call to the next are read nontemporally (16 experts of 4096 x 4096 95 -> 85 us, 8192 x 8192 29.8 -> 26.0; three matrices of
     // 2048 x 8192 in turn, which the 256 MiB of the memory-side cache hold: 8.1 -> 9.1).
     bool streams(const LinearParams& p)
     {
@@ -694,8 +696,7 @@ namespace
     {
         p.tilesN             = static_cast<uint32_t>(tilesOf(p.n, 16u));
         const uint64_t groups = (mostTiles(p, 16u) * p.tilesN + 7u) / 8u * 8u;
-        const auto     kernel = streams(p) ? linearFew<T, 1, 1, 4, true> : linearFew<T, 1, 1, 4, false>;
-        hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(groups)), dim3(64 * WAVES), 0, s, p);
+        hipLaunchKernelGGL((linearFew<T, 1, 1, 4>), dim3(static_cast<uint32_t>(groups)), dim3(64 * WAVES), 0, s, p);
     }
 
     int tooMany(const char* what)
@@ -830,8 +831,9 @@ namespace
         return a.k % 8u == 0u && evenRows(a.x, a.ldx, 2) && evenRows(a.w, a.ldw, 2) && (a.groups == 1u || a.w_stride % 8 == 0);
     }
     // The kernel of a forward product by its rows: us of dot products, of the kernel for few rows and of tiles for 4096 x 4096: one row 7.3, 8.0, 14; two 7.8, 8.2, 14; four 8.8, 8.3, 14; sixteen
-    // -, 10, 15; 24 -, 17, 14.  Of experts with about one row each (32 of 4096 x 4096, 128 of 1024 x 1024) 84, 105, 115 and 49, 75, 50; with two 265, 179, 192; four of 1024 x 1024 -, 96, 57 (a workgroup
-    // of the kernel for few rows has 16 columns, little work with a short sum); eight of 2048 x 2048 -, 117, 124, sixteen -, 166, 125.
+    // -, 10, 15; 24 -, 17, 14.  Of experts with about one row each (32 of 4096 x 4096, 128 of 1024 x 1024) 84, 105, 115 and 49, 75, 50; with four (8, 32, 64 experts of 2048 x 2048) 21, 15, 21; 79,
+    // 54, 70 and 143, 105, 138; with twelve 37, 21, 18; 166, 73, 75 and 321, 143, 124.  A workgroup of the kernel for few rows has 16 columns, little work with a short sum: 64 experts of 1024 x 1024
+    // with four 43, 30, 23; only where the CUs hold all of them at once it wins (4 of 1024 x 1024 5.6, 4.9, 6.7, 8 8.8, 6.1, 7.6).
     enum class Kernel
     {
         DOTS,
@@ -844,7 +846,7 @@ namespace
             return Kernel::TILES;
         if(a.groups == 1u)
             return a.rows <= 2u ? Kernel::DOTS : a.rows <= 16u ? Kernel::FEW : Kernel::TILES;
-        return a.rows <= a.groups ? Kernel::DOTS : a.rows / a.groups < 9u && a.k >= 2048u ? Kernel::FEW : Kernel::TILES;
+        return a.rows <= a.groups ? Kernel::DOTS : a.rows / a.groups < 9u && (a.k >= 2048u || tilesOf(a.n, 16u) * a.groups <= 2u * r355::computeUnits()) ? Kernel::FEW : Kernel::TILES;
     }
     LinearParams inputParams(const r355_linear_backward_args& a, const char* dz, uint32_t lddz)
     {
