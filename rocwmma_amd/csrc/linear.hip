@@ -710,7 +710,8 @@ namespace
         return r355::aligned(at, 128) && (uint64_t)ld * bytes % 128u == 0u;
     }
 
-    int launchTile(int32_t type, LinearParams p, bool aK, bool bK, r355::LinearTile tile, hipStream_t s, const char* what)
+    // The tiles of a launch: sets them in p, returns the workgroups
+    uint64_t tilesOfLaunch(LinearParams& p, bool aK, r355::LinearTile tile)
     {
         // (shares of a split sum are read again at once)
         p.linesY = p.splits == 1u && lines(p.y, p.ldy, p.outF32 ? 4u : 2u), p.linesZ = lines(p.z, p.ldz, 2u);
@@ -718,13 +719,17 @@ namespace
         p.tilesN = static_cast<uint32_t>(tilesOf(p.n, r355::LINEAR_COLS[tile])), p.tilesM = static_cast<uint32_t>(tilesOf(p.m, rows));
         // (of a weights' gradient: an eighth of a group's tiles for each XCD may be a tile more)
         const uint64_t tiles = aK ? mostTiles(p, rows) * p.tilesN : tilesOf((uint64_t)p.tilesM * p.tilesN, 8u) * 8u * p.groups;
-        if(tiles > r355::MAX_GROUPS)
+        return (tiles + 7u) / 8u * 8u;
+    }
+    int launchTile(int32_t type, LinearParams p, bool aK, bool bK, r355::LinearTile tile, hipStream_t s, const char* what)
+    {
+        const uint64_t workgroups = tilesOfLaunch(p, aK, tile);
+        if(workgroups > r355::MAX_GROUPS)
             return tooMany(what);
-        const uint32_t workgroups = static_cast<uint32_t>((tiles + 7u) / 8u * 8u);
         if(type == R355_F16)
-            r355::linearTilesF16(p, aK, bK, tile, workgroups, s);
+            r355::linearTilesF16(p, aK, bK, tile, static_cast<uint32_t>(workgroups), s);
         else
-            r355::linearTilesBF16(p, aK, bK, tile, workgroups, s);
+            r355::linearTilesBF16(p, aK, bK, tile, static_cast<uint32_t>(workgroups), s);
         return R355_OK;
     }
 
@@ -733,26 +738,42 @@ namespace
         return workspace && r355::aligned(workspace, 16) ? bytes : 0u;
     }
 
-    // one product on macro tiles
-    int launchTiles(int32_t type, const LinearParams& p, bool aK, bool bK, bool any, void* workspace, uint64_t workspaceBytes, hipStream_t s, const char* what)
+    uint64_t rowsOfResult(const LinearParams& p, bool aK)
     {
-        const Plan plan = planOf(p, aK, any, usable(workspace, workspaceBytes));
+        return aK ? p.rows : (uint64_t)p.m * p.groups;
+    }
+    uint64_t sumsBytes(const LinearParams& p, bool aK, uint32_t splits) // of a split product
+    {
+        return splits > 1u ? rowsOfResult(p, aK) * pitchOf(p.n) * 4u * splits : 0u;
+    }
+    // a product whose shares of the sum go to `sums`
+    LinearParams sharesOf(const LinearParams& p, bool aK, uint32_t splits, void* sums)
+    {
+        const uint32_t pitch = pitchOf(p.n);
+        LinearParams   d     = p;
+        d.splits = splits, d.y = static_cast<char*>(sums), d.ldy = pitch, d.strideY = (uint64_t)p.m * pitch * 4u, d.strideSplit = rowsOfResult(p, aK) * pitch * 4u, d.outF32 = 1u;
+        d.bias = d.gate = d.c = nullptr, d.z = nullptr, d.activation = R355_ACT_NONE;
+        return d;
+    }
+    void launchReduce(int32_t type, const LinearParams& p, bool aK, uint32_t splits, const void* sums, hipStream_t s)
+    {
+        const uint64_t rowsY = rowsOfResult(p, aK);
+        LinearParams   r     = p;
+        r.splits             = splits;
+        const dim3 grid(static_cast<uint32_t>(tilesOf(p.n, 1024u)), static_cast<uint32_t>(rowsY < 32768u ? rowsY : 32768u));
+        const auto kernel = type == R355_F16 ? (p.outF32 ? linearReduce<_Float16, float> : linearReduce<_Float16, _Float16>)
+                                             : (p.outF32 ? linearReduce<__bf16, float> : linearReduce<__bf16, __bf16>);
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, r, static_cast<const float*>(sums), rowsY, pitchOf(p.n));
+    }
+
+    // one product on macro tiles, by its plan
+    int launchTiles(int32_t type, const LinearParams& p, bool aK, bool bK, bool any, const Plan& plan, void* workspace, uint64_t workspaceBytes, hipStream_t s, const char* what)
+    {
         if(plan.splits > 1u)
         {
-            const uint64_t rowsY = aK ? p.rows : (uint64_t)p.m * p.groups;
-            const uint32_t pitch = pitchOf(p.n);
-            LinearParams   d     = p;
-            d.splits = plan.splits, d.y = static_cast<char*>(workspace), d.ldy = pitch, d.strideY = (uint64_t)p.m * pitch * 4u, d.strideSplit = rowsY * pitch * 4u, d.outF32 = 1u;
-            d.bias = d.gate = d.c = nullptr, d.z = nullptr, d.activation = R355_ACT_NONE;
-            if(const int rc = launchTile(type, d, aK, bK, plan.tile, s, what))
+            if(const int rc = launchTile(type, sharesOf(p, aK, plan.splits, workspace), aK, bK, plan.tile, s, what))
                 return rc;
-            LinearParams r = p;
-            r.splits       = plan.splits;
-            const dim3   grid(static_cast<uint32_t>(tilesOf(p.n, 1024u)), static_cast<uint32_t>(rowsY < 32768u ? rowsY : 32768u));
-            const float* sums   = static_cast<const float*>(workspace);
-            const auto   kernel = type == R355_F16 ? (p.outF32 ? linearReduce<_Float16, float> : linearReduce<_Float16, _Float16>)
-                                                   : (p.outF32 ? linearReduce<__bf16, float> : linearReduce<__bf16, __bf16>);
-            hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, r, sums, rowsY, pitch);
+            launchReduce(type, p, aK, plan.splits, workspace, s);
             return R355_OK;
         }
         if(plan.tall == 0u)
@@ -768,7 +789,40 @@ namespace
         rest.c = p.c ? p.c + by * p.ldc * outBytes : nullptr, rest.gate = p.gate ? p.gate + by * p.ldg * 2u : nullptr, rest.z = p.z ? p.z + by * p.ldz * 2u : nullptr;
         if(const int rc = launchTile(type, first, aK, bK, plan.tile, s, what))
             return rc;
-        return launchTiles(type, rest, aK, bK, any, workspace, workspaceBytes, s, what);
+        return launchTiles(type, rest, aK, bK, any, planOf(rest, aK, any, usable(workspace, workspaceBytes)), workspace, workspaceBytes, s, what);
+    }
+
+    // Both gradients in one launch of small tiles: how their sums are split, and what it takes (as launchTime(), with tiles of two lengths).
+    struct PlanBoth
+    {
+        uint32_t splitsX, splitsW;
+        double   us;
+    };
+    PlanBoth planBoth(const LinearParams& px, const LinearParams& pw, uint64_t workspaceBytes)
+    {
+        using namespace r355;
+        const TileTimes& t    = TILE_TIMES[TILE_64];
+        const double     cus  = computeUnits(), stagesX = static_cast<double>(tilesOf(px.k, 64u)), last = t.stage[3];
+        const double     stagesW = pw.offsets ? static_cast<double>(pw.rows) / pw.groups / 64.0 + 0.5 : static_cast<double>(tilesOf(pw.rows, 64u));
+        const double     met = px.groups < px.rows ? px.groups : px.rows;
+        const double     tilesX = (px.offsets ? px.rows / 64.0 + 0.5 * met : static_cast<double>(tilesOf(px.rows, 64u))) * static_cast<double>(tilesOf(px.n, 64u));
+        const double     tilesW = static_cast<double>(tilesOf(pw.m, 64u) * tilesOf(pw.n, 64u)) * pw.groups;
+        PlanBoth         best{1u, 1u, 1e30};
+        auto reduced = [](const LinearParams& p, bool aK, uint32_t splits) { return splits > 1u ? 5.0 + static_cast<double>(rowsOfResult(p, aK)) * p.n * 4.0 * (2u * splits + 1u) / 5e6 : 0.0; };
+        for(uint32_t sx = 1u; sx <= 16u && (sx == 1u || (stagesX >= 4.0 * sx && tilesX <= cus)); sx *= 2u)
+            for(uint32_t sw = 1u; sw <= 16u && (sw == 1u || (stagesW >= 4.0 * sw && tilesW <= cus)); sw *= 2u)
+            {
+                if(sumsBytes(px, true, sx) + sumsBytes(pw, false, sw) > workspaceBytes)
+                    continue;
+                const double nx = tilesX * sx, nw = tilesW * sw, lx = stagesX / sx, lw = stagesW / sw, n = nx + nw, longer = lx > lw ? nx : nw, shorter = lx < lw ? lx : lw, rest = (lx > lw ? lx : lw) - shorter;
+                auto         stage = [&](double tiles) { return t.stage[tiles > 3.0 * cus ? 3u : tiles > 2.0 * cus ? 2u : tiles > cus ? 1u : 0u]; };
+                const double us = 2.0 + reduced(px, true, sx) + reduced(pw, false, sw)
+                                  + (n <= 4.0 * cus ? t.ends + shorter * stage(n) + rest * stage(longer)
+                                                    : (nx * (t.ends + lx * last) + nw * (t.ends + lw * last)) / (4.0 * cus) + 0.5 * (t.ends + (shorter + rest) * last));
+                if(us < best.us)
+                    best = PlanBoth{sx, sw, us};
+            }
+        return best;
     }
 
     bool evenRows(const void* at, uint32_t ld, uint32_t bytes) // rows on 16-byte boundaries
@@ -882,7 +936,7 @@ namespace
             p.rows -= plan.tall;
             plan = planOf(p, aK, any, ~0ull);
         }
-        return plan.splits > 1u ? static_cast<size_t>((aK ? p.rows : (uint64_t)p.m * p.groups) * pitchOf(p.n) * 4u * plan.splits) : 0u;
+        return static_cast<size_t>(sumsBytes(p, aK, plan.splits));
     }
 } // namespace
 
@@ -940,7 +994,7 @@ extern "C" int r355_linear(const r355_linear_args* args, void* stream)
             f16 ? launchDots<_Float16, 2>(p, s) : launchDots<__bf16, 2>(p, s);
         break;
     case Kernel::FEW: f16 ? launchFew<_Float16>(p, s) : launchFew<__bf16>(p, s); break;
-    default: R355_TRY(launchTiles(a.in_type, p, true, true, !even, a.workspace, a.workspace_bytes, s, what));
+    default: R355_TRY(launchTiles(a.in_type, p, true, true, !even, planOf(p, true, !even, usable(a.workspace, a.workspace_bytes)), a.workspace, a.workspace_bytes, s, what));
     }
     return r355::checkLaunch(what);
 }
@@ -964,16 +1018,19 @@ extern "C" size_t r355_linear_backward_workspace_bytes(const r355_linear_backwar
     const bool     element = a.activation != R355_ACT_NONE || a.gate;
     const char*    dz      = static_cast<const char*>(element ? a.dz : a.dy);
     const uint32_t lddz    = element ? a.lddz : a.lddy;
-    if(a.dx)
+    const bool     anyX = !evenInput(a, dz, lddz), anyW = !evenWeight(a, dz, lddz);
+    const LinearParams px = inputParams(a, dz, lddz), pw = weightParams(a, dz, lddz);
+    if(a.dx && a.dw && !anyX && !anyW)
     {
-        const size_t bytes = splitBytes(inputParams(a, dz, lddz), true, !evenInput(a, dz, lddz));
-        most               = most > bytes ? most : bytes;
+        const PlanBoth both = planBoth(px, pw, ~0ull);
+        if(both.us < planOf(px, true, anyX, ~0ull).us + planOf(pw, false, anyW, ~0ull).us)
+        {
+            const size_t bytes = static_cast<size_t>(sumsBytes(px, true, both.splitsX) + sumsBytes(pw, false, both.splitsW));
+            return most > bytes ? most : bytes;
+        }
     }
-    if(a.dw)
-    {
-        const size_t bytes = splitBytes(weightParams(a, dz, lddz), false, !evenWeight(a, dz, lddz));
-        most               = most > bytes ? most : bytes;
-    }
+    for(size_t bytes : {a.dx ? splitBytes(px, true, anyX) : size_t{0}, a.dw ? splitBytes(pw, false, anyW) : size_t{0}})
+        most = most > bytes ? most : bytes;
     return most;
 }
 
@@ -1037,13 +1094,32 @@ extern "C" int r355_linear_backward(const r355_linear_backward_args* args, void*
     }
     const char*    dz   = static_cast<const char*>(element ? a.dz : a.dy);
     const uint32_t lddz = element ? a.lddz : a.lddy;
-    if(a.dx && a.rows)
+    const bool         wantX = a.dx && a.rows, wantW = a.dw != nullptr, anyX = !evenInput(a, dz, lddz), anyW = !evenWeight(a, dz, lddz);
+    const LinearParams px = inputParams(a, dz, lddz), pw = weightParams(a, dz, lddz);
+    const uint64_t     room  = usable(a.workspace, a.workspace_bytes);
+    const Plan         planX = wantX ? planOf(px, true, anyX, room) : Plan{}, planW = wantW ? planOf(pw, false, anyW, room) : Plan{};
+    if(wantX && wantW && !anyX && !anyW)
     {
-        R355_TRY(launchTiles(a.in_type, inputParams(a, dz, lddz), true, false, !evenInput(a, dz, lddz), a.workspace, a.workspace_bytes, s, what));
+        const PlanBoth both = planBoth(px, pw, room);
+        if(both.us < planX.us + planW.us)
+        {
+            char* const    sums  = static_cast<char*>(a.workspace);
+            const uint64_t sumsX = sumsBytes(px, true, both.splitsX);
+            LinearParams   x = both.splitsX > 1u ? sharesOf(px, true, both.splitsX, sums) : px, w = both.splitsW > 1u ? sharesOf(pw, false, both.splitsW, sums + sumsX) : pw;
+            const uint64_t workgroupsX = tilesOfLaunch(x, true, r355::TILE_64), workgroupsW = tilesOfLaunch(w, false, r355::TILE_64);
+            if(workgroupsX * both.splitsX + workgroupsW * both.splitsW > r355::MAX_GROUPS)
+                return tooMany(what);
+            (a.in_type == R355_F16 ? r355::linearBothF16 : r355::linearBothBF16)(x, w, static_cast<uint32_t>(workgroupsX), static_cast<uint32_t>(workgroupsW), s);
+            if(both.splitsX > 1u)
+                launchReduce(a.in_type, px, true, both.splitsX, sums, s);
+            if(both.splitsW > 1u)
+                launchReduce(a.in_type, pw, false, both.splitsW, sums + sumsX, s);
+            return r355::checkLaunch(what);
+        }
     }
-    if(a.dw)
-    {
-        R355_TRY(launchTiles(a.in_type, weightParams(a, dz, lddz), false, false, !evenWeight(a, dz, lddz), a.workspace, a.workspace_bytes, s, what));
-    }
+    if(wantX)
+        R355_TRY(launchTiles(a.in_type, px, true, false, anyX, planX, a.workspace, a.workspace_bytes, s, what));
+    if(wantW)
+        R355_TRY(launchTiles(a.in_type, pw, false, false, anyW, planW, a.workspace, a.workspace_bytes, s, what));
     return r355::checkLaunch(what);
 }

@@ -229,6 +229,9 @@ namespace r355
     // the forms, one set of kernels per type; aK, bK: A, B contiguous along the sum
     void linearTilesF16(const LinearParams& p, bool aK, bool bK, LinearTile tile, uint32_t workgroups, hipStream_t s);
     void linearTilesBF16(const LinearParams& p, bool aK, bool bK, LinearTile tile, uint32_t workgroups, hipStream_t s);
+    // both gradients, input's and weights', on tiles of 64 x 64 in one launch
+    void linearBothF16(const LinearParams& px, const LinearParams& pw, uint32_t workgroupsX, uint32_t workgroupsW, hipStream_t s);
+    void linearBothBF16(const LinearParams& px, const LinearParams& pw, uint32_t workgroupsX, uint32_t workgroupsW, hipStream_t s);
 } // namespace r355
 
 #endif // R355_LINEAR_HPP

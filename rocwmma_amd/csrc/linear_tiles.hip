@@ -59,19 +59,20 @@ namespace
     // What a workgroup multiplies: Y rows first .. first + rowsLeft, columns col0 .. col0 + colsLeft, of group `group`; the sum's share [kFirst, kFirst + k).
     struct Work
     {
-        uint32_t group, first, rowsLeft, col0, colsLeft, k, kFirst;
+        uint32_t group, first, rowsLeft, col0, colsLeft, k, kFirst, share;
         uint64_t sumRow; // weights' gradient: first row of the group
     };
 
+    // of workgroup `id` of those that have share `share` of the sums (an XCD has those of the same id % 8)
     template <bool AK, uint32_t ROWS, uint32_t COLS>
-    __device__ __forceinline__ bool workOf(const LinearParams& p, Work& w)
+    __device__ __forceinline__ bool workOf(const LinearParams& p, Work& w, uint32_t id, uint32_t share)
     {
         uint32_t tm, tn, k;
         if constexpr(AK)
         {
             GroupTiles<ROWS> tiles{p};
             const uint32_t   tilesM = tiles.total();
-            if(!r355::tileCoordRange(blockIdx.x, tilesM, p.tilesN, 0u, tilesM * p.tilesN, false, tm, tn))
+            if(!r355::tileCoordRange(id, tilesM, p.tilesN, 0u, tilesM * p.tilesN, false, tm, tn))
                 return false;
             const GroupTile t = tiles.at(tm);
             w.group = t.group, w.first = t.first, w.rowsLeft = t.count, w.sumRow = 0u, k = p.k;
@@ -82,16 +83,16 @@ namespace
             // more, whole groups, whose operands one XCD alone then reads (16 of 4096 x 1536 264 us, in eighths 315).
             if(p.groups > 1u && p.groups < 16u)
             {
-                const uint32_t share = (p.tilesM * p.tilesN + 7u) / 8u, slot = blockIdx.x / 8u;
-                w.group              = slot / share;
-                const uint32_t tile  = (blockIdx.x + w.group) % 8u * share + slot % share;
+                const uint32_t eighth = (p.tilesM * p.tilesN + 7u) / 8u, slot = id / 8u;
+                w.group               = slot / eighth;
+                const uint32_t tile   = (id + w.group) % 8u * eighth + slot % eighth;
                 if(w.group >= p.groups || tile >= p.tilesM * p.tilesN)
                     return false;
                 r355::tileOfId(tile, p.tilesM, p.tilesN, tm, tn);
             }
             else
             {
-                if(!r355::tileCoordRange(blockIdx.x, p.groups * p.tilesM, p.tilesN, 0u, p.groups * p.tilesM * p.tilesN, false, tm, tn))
+                if(!r355::tileCoordRange(id, p.groups * p.tilesM, p.tilesN, 0u, p.groups * p.tilesM * p.tilesN, false, tm, tn))
                     return false;
                 w.group = tm / p.tilesM, tm %= p.tilesM;
             }
@@ -103,10 +104,11 @@ namespace
         w.col0     = tn * COLS;
         w.colsLeft = p.n - w.col0 < COLS ? p.n - w.col0 : COLS;
         // (whole stages for every share but the last ones)
-        const uint32_t stages = k / TK + (k % TK != 0u ? 1u : 0u), share = p.splits > 1u ? (stages + p.splits - 1u) / p.splits : stages;
-        w.kFirst = (p.splits > 1u ? blockIdx.y * share : 0u) * TK;
+        const uint32_t stages = k / TK + (k % TK != 0u ? 1u : 0u), part = p.splits > 1u ? (stages + p.splits - 1u) / p.splits : stages;
+        w.share  = share;
+        w.kFirst = share * part * TK;
         w.kFirst = w.kFirst < k ? w.kFirst : k;
-        w.k      = k - w.kFirst < share * TK ? k - w.kFirst : share * TK;
+        w.k      = k - w.kFirst < part * TK ? k - w.kFirst : part * TK;
         // (uniform, which the compiler does not see through the lanes' part in finding it)
         w.group = __builtin_amdgcn_readfirstlane(w.group), w.first = __builtin_amdgcn_readfirstlane(w.first), w.rowsLeft = __builtin_amdgcn_readfirstlane(w.rowsLeft);
         w.col0 = __builtin_amdgcn_readfirstlane(w.col0), w.colsLeft = __builtin_amdgcn_readfirstlane(w.colsLeft);
@@ -248,7 +250,7 @@ namespace
         for(uint32_t r = 0; r < 8u / RUN; ++r)
             at.at[r] = lane % LANES * RUN + r * LANES * RUN, at.left[r] = at.at[r] < cols ? cols - at.at[r] : 0u;
         // a share of a split sum goes to the workspace: [split][group, row of Y][column]
-        char* const y = p.y + (uint64_t)w.group * p.strideY + (p.splits > 1u ? (uint64_t)blockIdx.y * p.strideSplit : 0u);
+        char* const y = p.y + (uint64_t)w.group * p.strideY + (p.splits > 1u ? (uint64_t)w.share * p.strideSplit : 0u);
         const char* c = p.c ? p.c + (uint64_t)w.group * p.strideC : nullptr;
 
         Eight<T, RUN> bias;
@@ -565,7 +567,7 @@ namespace
     {
         __shared__ __attribute__((aligned(1024))) char lds[ldsOf(8, 8)];
         Work                                           w;
-        if(!workOf<AK, 256, 256>(p, w))
+        if(!workOf<AK, 256, 256>(p, w, blockIdx.x, blockIdx.y))
             return;
         if(!AK || w.rowsLeft > 192u)
             linearTile<AK, BK, 8, 8>(p, w, lds);
@@ -584,7 +586,7 @@ namespace
     {
         __shared__ __attribute__((aligned(1024))) char lds[ldsOf(6, 8)];
         Work                                           w;
-        if(workOf<AK, 192, 256>(p, w))
+        if(workOf<AK, 192, 256>(p, w, blockIdx.x, blockIdx.y))
             linearTile<AK, BK, 6, 8>(p, w, lds);
     }
     template <bool AK, bool BK>
@@ -592,7 +594,7 @@ namespace
     {
         __shared__ __attribute__((aligned(1024))) char lds[ldsOf(6, 4)];
         Work                                           w;
-        if(workOf<AK, 192, 128>(p, w))
+        if(workOf<AK, 192, 128>(p, w, blockIdx.x, blockIdx.y))
             linearTile<AK, BK, 6, 4>(p, w, lds);
     }
     template <bool AK, bool BK>
@@ -600,7 +602,7 @@ namespace
     {
         __shared__ __attribute__((aligned(1024))) char lds[ldsOf(8, 4)];
         Work                                           w;
-        if(workOf<AK, 256, 128>(p, w))
+        if(workOf<AK, 256, 128>(p, w, blockIdx.x, blockIdx.y))
             linearTile<AK, BK, 8, 4>(p, w, lds);
     }
     template <bool AK, bool BK>
@@ -608,7 +610,7 @@ namespace
     {
         __shared__ __attribute__((aligned(1024))) char lds[ldsOf(4, 8)];
         Work                                           w;
-        if(workOf<AK, 128, 256>(p, w))
+        if(workOf<AK, 128, 256>(p, w, blockIdx.x, blockIdx.y))
             linearTile<AK, BK, 4, 8>(p, w, lds);
     }
     template <bool AK, bool BK>
@@ -616,7 +618,7 @@ namespace
     {
         __shared__ __attribute__((aligned(1024))) char lds[ldsOf(4, 4)];
         Work                                           w;
-        if(workOf<AK, 128, 128>(p, w))
+        if(workOf<AK, 128, 128>(p, w, blockIdx.x, blockIdx.y))
             linearTile<AK, BK, 4, 4>(p, w, lds);
     }
     template <bool AK, bool BK>
@@ -624,8 +626,24 @@ namespace
     {
         __shared__ __attribute__((aligned(1024))) char lds[ldsOf(2, 2)];
         Work                                           w;
-        if(workOf<AK, 64, 64>(p, w))
+        if(workOf<AK, 64, 64>(p, w, blockIdx.x, blockIdx.y))
             linearTile<AK, BK, 2, 2>(p, w, lds);
+    }
+
+    // Both gradients of a small layer in one launch: the input's by the first workgroups, the weights' by the others, on small tiles, four workgroups a CU (992 x 1008 x 1232 24.1 -> 17.3 us,
+    // 100 x 512 x 512 11.1 -> 8.4, 2048 x 1024 x 1024 26.1 -> 18.9; of larger layers separate launches of larger tiles take less, by planBoth()).
+    __global__ void __launch_bounds__(THREADS, 4) linearBoth64(LinearParams px, LinearParams pw, uint32_t workgroupsX, uint32_t workgroupsW)
+    {
+        __shared__ __attribute__((aligned(1024))) char lds[ldsOf(2, 2)];
+        Work                                           w;
+        const uint32_t                                 first = workgroupsX * px.splits;
+        if(blockIdx.x < first)
+        {
+            if(workOf<true, 64, 64>(px, w, blockIdx.x % workgroupsX, blockIdx.x / workgroupsX))
+                linearTile<true, false, 2, 2>(px, w, lds);
+        }
+        else if(workOf<false, 64, 64>(pw, w, (blockIdx.x - first) % workgroupsW, (blockIdx.x - first) / workgroupsW))
+            linearTile<false, false, 2, 2>(pw, w, lds);
     }
 
     // Eight elements of any alignment, `left` of them there: at once, or at the ends one by one
@@ -652,7 +670,7 @@ namespace
         __shared__ __attribute__((aligned(16))) T   image[2][TILE * PITCH];
         __shared__ __attribute__((aligned(16))) char scratch[4u * 2u * 4096u];
         Work w;
-        if(!workOf<AK, TILE, TILE>(p, w))
+        if(!workOf<AK, TILE, TILE>(p, w, blockIdx.x, blockIdx.y))
             return;
         const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1u;
         // a thread's eight elements of a step: neighbours along the sum, or along the rows of Y (columns, for B)
@@ -746,4 +764,13 @@ void r355::linearTilesF16(const LinearParams& p, bool aK, bool bK, LinearTile ti
         launch<true, false>(p, tile, workgroups, s);
     else
         launch<false, false>(p, tile, workgroups, s);
+}
+
+#ifdef R355_LINEAR_BF16
+void r355::linearBothBF16(const LinearParams& px, const LinearParams& pw, uint32_t workgroupsX, uint32_t workgroupsW, hipStream_t s)
+#else
+void r355::linearBothF16(const LinearParams& px, const LinearParams& pw, uint32_t workgroupsX, uint32_t workgroupsW, hipStream_t s)
+#endif
+{
+    hipLaunchKernelGGL(linearBoth64, dim3(workgroupsX * px.splits + workgroupsW * pw.splits), dim3(THREADS), 0, s, px, pw, workgroupsX, workgroupsW);
 }
