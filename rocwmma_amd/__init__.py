@@ -1,4 +1,5 @@
-"""rocwmma_amd: MI355X (gfx950) matrix-fragment hot path -- GEMM, DLRM dot interaction, GEMV, and the operators of a decoding step.
+"""rocwmma_amd: MI355X (gfx950) matrix-fragment hot path -- GEMM, DLRM dot interaction, GEMV, the operators of a decoding step,
+and those of a layer's feed-forward half: products with an epilogue and their gradients, by expert too, the router, the rows' way to the experts and back.
 
 The device code lives in csrc/ (hand-written HIP) and include/rocwmma/ (the header-only
 fragment API, same names as the reference's rocwmma.hpp).  This module is the thin host

@@ -27,7 +27,7 @@ namespace
 
     // ---- One or two rows of each group: dot products.  A wave takes 16 weight rows, each lane 16 bytes of every row at a time, so that an access is 1 KiB of one row (the matrix instructions'
     // operands are 64 bytes of each of 16 rows: 16 experts of 4096 x 4096 105 us instead of 84).  Pieces of 512 of the sum go to WK waves in turn, other
-    // waves have other rows.  Bound by HBM.
+    // waves have other rows.  Bound by HBM: 16 rows of 16 experts of 4096 x 4096 83 us, 6.5 TB/s; 1024 x 2048 4.0, a launch and two accesses' latency.
     //
     // A lane's 16 T sums become one sum of the wave in each lane: of a pair of sums each half of the lanes keeps one and adds the other half's part of it, and so on by halves,
     // about 16 T additions instead of 6 for each sum.  After the steps over lanes 32, 16, 8 and 4 apart lane l has sum 8 (l / 4 % 2) + 4 (l / 8 % 2) + 2 (l / 16 % 2) + l / 32 of 16.
@@ -336,7 +336,7 @@ namespace
     }
 
     // ---- Sums of a split product: [splits][rows][pitch] of f32, added in order, then the epilogue of linear_tiles.hip.  Result rows are `p.m` to a group (weights' gradient), or
-    // by offsets; those of no group are left.  Four columns a thread; what is not four columns wide, or past a row's end, goes element by element.
+    // by offsets; those of no group are left.  Four columns a thread; what is not four columns wide, or past a row's end, goes element by element.  4 to 5 us: a launch, and the shares out of the caches.
     template <typename T, typename Out>
     __global__ void __launch_bounds__(256) linearReduce(LinearParams p, const float* sums, uint64_t rows, uint32_t pitch)
     {
@@ -427,7 +427,8 @@ namespace
         }
     }
 
-    // ---- The gradient's part element by element: dz, dgate and the bias's gradient, one pass over dy, z and gate.
+    // ---- The gradient's part element by element: dz, dgate and the bias's gradient, one pass over dy, z and gate.  Bound by HBM: three operands and two results of 4099 x 4096 in bf16 31 us,
+    // 5.4 TB/s.  (Made once and read by both products: in their loads it would be made anew for each tile that a row is part of, and dz would have to lie somewhere for the transposed reads anyway.)
     struct GradParams
     {
         const char*    dy;
@@ -570,6 +571,42 @@ namespace
         }
     }
 
+    // ---- An operand whose rows do not begin on 16-byte boundaries, or end inside 16 bytes, laid out in the workspace so that they do, with zeros behind them; the macro tiles' loads
+    // are 16 bytes.  A thread moves 16 of them.  Bound by memory.
+    struct Copy
+    {
+        const char* from; // NULL: there is nothing to do
+        uint64_t    stride; // bytes from group to group
+        uint32_t    groups, rows, cols, ld;
+        uint32_t    toRows, toCols;
+
+        uint64_t bytes() const
+        {
+            return from ? (uint64_t)groups * toRows * toCols * 2u : 0u;
+        }
+    };
+    __global__ void __launch_bounds__(256) linearEven(Copy c, char* to)
+    {
+        typedef uint16_t Unaligned __attribute__((ext_vector_type(8), aligned(2)));
+        const uint64_t at = (uint64_t)blockIdx.x * 256u + threadIdx.x;
+        const uint32_t pieces = c.toCols / 8u;
+        const uint64_t row = at / pieces, group = row / c.toRows;
+        if(group >= c.groups)
+            return;
+        const uint32_t  in = static_cast<uint32_t>(row % c.toRows), col = static_cast<uint32_t>(at % pieces) * 8u, left = in < c.rows && col < c.cols ? c.cols - col : 0u;
+        const uint16_t* from = reinterpret_cast<const uint16_t*>(c.from + group * c.stride) + (uint64_t)in * c.ld + col;
+        Unaligned       v{};
+        if(left >= 8u)
+            v = *reinterpret_cast<const Unaligned*>(from);
+        else
+#pragma unroll
+            for(uint32_t e = 0; e < 7u; ++e)
+                if(e < left)
+                    v[e] = from[e];
+        *reinterpret_cast<u32x4*>(to + at * 16u) = __builtin_bit_cast(u32x4, v);
+    }
+
+    constexpr uint64_t FAR = 0x7FFFFFF0u; // bytes of a buffer that rows are taken from by their numbers
     constexpr uint32_t MOST_ROWS = 1u << 30, MOST_LENGTH = (1u << 22) - 8u, MOST_GROUPS = 1024u;
 
     uint64_t tilesOf(uint64_t n, uint32_t edge)
@@ -927,6 +964,70 @@ namespace
     {
         return evenRows(dz, lddz, 2) && evenRows(a.x, a.ldx, 2);
     }
+    // Operands to be laid out anew in a workspace, one after the other, and what that takes
+    struct Copies
+    {
+        Copy     copy[3] = {};
+        uint32_t count   = 0u;
+        uint64_t bytes   = 0u;
+        double   us      = 0.0;
+
+        // where `what` will lie
+        const char* add(const Copy& what, const void* workspace)
+        {
+            const char* at = static_cast<const char*>(workspace) + bytes;
+            copy[count++]  = what;
+            bytes += what.bytes();
+            us += 3.0 + 2.0 * static_cast<double>(what.bytes()) / 4.5e6;
+            return at;
+        }
+        void launch(void* workspace, hipStream_t s) const
+        {
+            char* at = static_cast<char*>(workspace);
+            for(uint32_t i = 0; i < count; ++i)
+            {
+                hipLaunchKernelGGL(linearEven, dim3(static_cast<uint32_t>((copy[i].bytes() / 16u + 255u) / 256u)), dim3(256), 0, s, copy[i], at);
+                at += copy[i].bytes();
+            }
+        }
+        bool fit(uint64_t room) const // (and a launch holds the largest)
+        {
+            return bytes <= room && bytes / 4096u < r355::MAX_GROUPS;
+        }
+    };
+    uint32_t eights(uint32_t n)
+    {
+        return (n + 7u) / 8u * 8u;
+    }
+    // The forward product with even operands.  (Both gradients of 1500 x 1500 x 1496, whose rows of 1500 are 3000 bytes: 152 us on tiles of single elements, 42 so, 35 of 1504.)
+    Copies evened(const r355_linear_args& a, const void* workspace, LinearParams& p)
+    {
+        Copies         c;
+        const uint32_t rows = a.source ? a.x_rows : a.rows;
+        if(a.k % 8u != 0u || !evenRows(a.x, a.ldx, 2))
+            p.a = c.add(Copy{p.a, 0u, 1u, rows, a.k, a.ldx, rows, eights(a.k)}, workspace), p.lda = eights(a.k);
+        if(a.k % 8u != 0u || !evenRows(a.w, a.ldw, 2) || (a.groups > 1u && a.w_stride % 8 != 0))
+            p.b = c.add(Copy{p.b, p.strideB, a.groups, a.n, a.k, a.ldw, a.n, eights(a.k)}, workspace), p.ldb = eights(a.k), p.strideB = (uint64_t)a.n * eights(a.k) * 2u;
+        p.k = eights(a.k);
+        if(a.source && (uint64_t)rows * p.lda * 2u > FAR)
+            c.bytes = ~0ull; // (rows taken by their numbers must lie within a buffer's reach)
+        return c;
+    }
+    // Both gradients with even operands: dz (with zeros behind its rows, and as many rows of zeros behind those of w: the sum of dx goes over them), w, x
+    Copies evened(const r355_linear_backward_args& a, const char* dz, uint32_t lddz, bool wantX, bool wantW, const void* workspace, LinearParams& px, LinearParams& pw)
+    {
+        Copies         c;
+        const uint32_t n8 = eights(a.n), k8 = eights(a.k);
+        if((wantX && a.n % 8u != 0u) || !evenRows(dz, lddz, 2))
+            px.a = pw.a = c.add(Copy{dz, 0u, 1u, a.rows, a.n, lddz, a.rows, n8}, workspace), px.lda = pw.lda = n8;
+        if(wantX && (a.n % 8u != 0u || !evenRows(a.w, a.ldw, 2) || (a.groups > 1u && a.w_stride % 8 != 0)))
+            px.b = c.add(Copy{px.b, px.strideB, a.groups, a.n, a.k, a.ldw, n8, k8}, workspace), px.ldb = k8, px.strideB = (uint64_t)n8 * k8 * 2u;
+        if(wantW && !evenRows(a.x, a.ldx, 2))
+            pw.b = c.add(Copy{pw.b, 0u, 1u, a.rows, a.k, a.ldx, a.rows, k8}, workspace), pw.ldb = k8;
+        px.k = n8;
+        return c;
+    }
+
     // what the sums of a split product take
     size_t splitBytes(LinearParams p, bool aK, bool any)
     {
@@ -937,6 +1038,34 @@ namespace
             plan = planOf(p, aK, any, ~0ull);
         }
         return static_cast<size_t>(sumsBytes(p, aK, plan.splits));
+    }
+
+    // How the products of the gradients go out
+    struct BackwardPlan
+    {
+        Plan     x, w;
+        PlanBoth both;
+        bool     together;
+        double   us;
+    };
+    BackwardPlan planBackward(const LinearParams& px, const LinearParams& pw, bool wantX, bool wantW, bool anyX, bool anyW, uint64_t room)
+    {
+        BackwardPlan plan{wantX ? planOf(px, true, anyX, room) : Plan{}, wantW ? planOf(pw, false, anyW, room) : Plan{}, {}, false, 0.0};
+        plan.us = plan.x.us + plan.w.us;
+        if(wantX && wantW && !anyX && !anyW)
+        {
+            plan.both     = planBoth(px, pw, room);
+            plan.together = plan.both.us < plan.us;
+            plan.us       = plan.together ? plan.both.us : plan.us;
+        }
+        return plan;
+    }
+    size_t backwardBytes(const BackwardPlan& plan, const LinearParams& px, const LinearParams& pw, bool wantX, bool wantW, bool anyX, bool anyW)
+    {
+        if(plan.together)
+            return static_cast<size_t>(sumsBytes(px, true, plan.both.splitsX) + sumsBytes(pw, false, plan.both.splitsW));
+        const size_t x = wantX ? splitBytes(px, true, anyX) : 0u, w = wantW ? splitBytes(pw, false, anyW) : 0u;
+        return x > w ? x : w;
     }
 } // namespace
 
@@ -974,7 +1103,7 @@ extern "C" int r355_linear(const r355_linear_args* args, void* stream)
     {
         if(!r355::aligned(a.source, 4))
             return r355::fail(R355_ERR_MISALIGNED, "linear: source needs the alignment of its elements");
-        if(a.x_rows == 0 || (uint64_t)a.x_rows * a.ldx * 2u > 0x7FFFFFF0u)
+        if(a.x_rows == 0 || (uint64_t)a.x_rows * a.ldx * 2u > FAR)
             return r355::fail(R355_ERR_BAD_SIZE, "linear: rows taken by their numbers must be of 1 to 2^31 bytes of x, got %u rows %u elements apart", a.x_rows, a.ldx);
     }
     const LinearParams p    = forwardParams(a);
@@ -994,7 +1123,24 @@ extern "C" int r355_linear(const r355_linear_args* args, void* stream)
             f16 ? launchDots<_Float16, 2>(p, s) : launchDots<__bf16, 2>(p, s);
         break;
     case Kernel::FEW: f16 ? launchFew<_Float16>(p, s) : launchFew<__bf16>(p, s); break;
-    default: R355_TRY(launchTiles(a.in_type, p, true, true, !even, planOf(p, true, !even, usable(a.workspace, a.workspace_bytes)), a.workspace, a.workspace_bytes, s, what));
+    default:
+    {
+        const uint64_t room = usable(a.workspace, a.workspace_bytes);
+        const Plan     plan = planOf(p, true, !even, room);
+        if(!even)
+        {
+            LinearParams q      = p;
+            const Copies copies = evened(a, a.workspace, q);
+            if(copies.fit(room))
+                if(const Plan other = planOf(q, true, false, room - copies.bytes); other.us + copies.us < plan.us)
+                {
+                    copies.launch(a.workspace, s);
+                    R355_TRY(launchTiles(a.in_type, q, true, true, false, other, static_cast<char*>(a.workspace) + copies.bytes, room - copies.bytes, s, what));
+                    break;
+                }
+        }
+        R355_TRY(launchTiles(a.in_type, p, true, true, !even, plan, a.workspace, a.workspace_bytes, s, what));
+    }
     }
     return r355::checkLaunch(what);
 }
@@ -1003,7 +1149,16 @@ extern "C" size_t r355_linear_workspace_bytes(const r355_linear_args* args)
 {
     if(!args || args->rows == 0 || args->n == 0 || args->k == 0 || args->groups == 0 || kernelOf(*args, evenForward(*args)) != Kernel::TILES)
         return 0;
-    return splitBytes(forwardParams(*args), true, !evenForward(*args));
+    const LinearParams p    = forwardParams(*args);
+    const bool         even = evenForward(*args);
+    if(!even)
+    {
+        LinearParams q      = p;
+        const Copies copies = evened(*args, nullptr, q);
+        if(copies.fit(~0ull) && planOf(q, true, false, ~0ull).us + copies.us < planOf(p, true, true, ~0ull).us)
+            return static_cast<size_t>(copies.bytes) + splitBytes(q, true, false);
+    }
+    return splitBytes(p, true, !even);
 }
 
 extern "C" size_t r355_linear_backward_workspace_bytes(const r355_linear_backward_args* args)
@@ -1018,19 +1173,19 @@ extern "C" size_t r355_linear_backward_workspace_bytes(const r355_linear_backwar
     const bool     element = a.activation != R355_ACT_NONE || a.gate;
     const char*    dz      = static_cast<const char*>(element ? a.dz : a.dy);
     const uint32_t lddz    = element ? a.lddz : a.lddy;
-    const bool     anyX = !evenInput(a, dz, lddz), anyW = !evenWeight(a, dz, lddz);
+    const bool         wantX = a.dx != nullptr, wantW = a.dw != nullptr, anyX = wantX && !evenInput(a, dz, lddz), anyW = wantW && !evenWeight(a, dz, lddz);
     const LinearParams px = inputParams(a, dz, lddz), pw = weightParams(a, dz, lddz);
-    if(a.dx && a.dw && !anyX && !anyW)
+    const BackwardPlan plan  = planBackward(px, pw, wantX, wantW, anyX, anyW, ~0ull);
+    size_t             bytes = backwardBytes(plan, px, pw, wantX, wantW, anyX, anyW);
+    if(anyX || anyW)
     {
-        const PlanBoth both = planBoth(px, pw, ~0ull);
-        if(both.us < planOf(px, true, anyX, ~0ull).us + planOf(pw, false, anyW, ~0ull).us)
-        {
-            const size_t bytes = static_cast<size_t>(sumsBytes(px, true, both.splitsX) + sumsBytes(pw, false, both.splitsW));
-            return most > bytes ? most : bytes;
-        }
+        LinearParams       x = px, w = pw;
+        const Copies       copies = evened(a, dz, lddz, wantX, wantW, nullptr, x, w);
+        const BackwardPlan other  = planBackward(x, w, wantX, wantW, false, false, ~0ull);
+        if(copies.fit(~0ull) && other.us + copies.us < plan.us)
+            bytes = static_cast<size_t>(copies.bytes) + backwardBytes(other, x, w, wantX, wantW, false, false);
     }
-    for(size_t bytes : {a.dx ? splitBytes(px, true, anyX) : size_t{0}, a.dw ? splitBytes(pw, false, anyW) : size_t{0}})
-        most = most > bytes ? most : bytes;
+    most = most > bytes ? most : bytes;
     return most;
 }
 
@@ -1094,32 +1249,42 @@ extern "C" int r355_linear_backward(const r355_linear_backward_args* args, void*
     }
     const char*    dz   = static_cast<const char*>(element ? a.dz : a.dy);
     const uint32_t lddz = element ? a.lddz : a.lddy;
-    const bool         wantX = a.dx && a.rows, wantW = a.dw != nullptr, anyX = !evenInput(a, dz, lddz), anyW = !evenWeight(a, dz, lddz);
-    const LinearParams px = inputParams(a, dz, lddz), pw = weightParams(a, dz, lddz);
-    const uint64_t     room  = usable(a.workspace, a.workspace_bytes);
-    const Plan         planX = wantX ? planOf(px, true, anyX, room) : Plan{}, planW = wantW ? planOf(pw, false, anyW, room) : Plan{};
-    if(wantX && wantW && !anyX && !anyW)
+    const bool     wantX = a.dx && a.rows, wantW = a.dw != nullptr;
+    bool           anyX = wantX && !evenInput(a, dz, lddz), anyW = wantW && !evenWeight(a, dz, lddz);
+    LinearParams   px = inputParams(a, dz, lddz), pw = weightParams(a, dz, lddz);
+    uint64_t       room = usable(a.workspace, a.workspace_bytes);
+    char*          work = static_cast<char*>(a.workspace);
+    BackwardPlan   plan = planBackward(px, pw, wantX, wantW, anyX, anyW, room);
+    if((anyX || anyW) && a.rows)
     {
-        const PlanBoth both = planBoth(px, pw, room);
-        if(both.us < planX.us + planW.us)
-        {
-            char* const    sums  = static_cast<char*>(a.workspace);
-            const uint64_t sumsX = sumsBytes(px, true, both.splitsX);
-            LinearParams   x = both.splitsX > 1u ? sharesOf(px, true, both.splitsX, sums) : px, w = both.splitsW > 1u ? sharesOf(pw, false, both.splitsW, sums + sumsX) : pw;
-            const uint64_t workgroupsX = tilesOfLaunch(x, true, r355::TILE_64), workgroupsW = tilesOfLaunch(w, false, r355::TILE_64);
-            if(workgroupsX * both.splitsX + workgroupsW * both.splitsW > r355::MAX_GROUPS)
-                return tooMany(what);
-            (a.in_type == R355_F16 ? r355::linearBothF16 : r355::linearBothBF16)(x, w, static_cast<uint32_t>(workgroupsX), static_cast<uint32_t>(workgroupsW), s);
-            if(both.splitsX > 1u)
-                launchReduce(a.in_type, px, true, both.splitsX, sums, s);
-            if(both.splitsW > 1u)
-                launchReduce(a.in_type, pw, false, both.splitsW, sums + sumsX, s);
-            return r355::checkLaunch(what);
-        }
+        LinearParams x = px, w = pw;
+        const Copies copies = evened(a, dz, lddz, wantX, wantW, work, x, w);
+        if(copies.fit(room))
+            if(const BackwardPlan other = planBackward(x, w, wantX, wantW, false, false, room - copies.bytes); other.us + copies.us < plan.us)
+            {
+                copies.launch(work, s);
+                px = x, pw = w, plan = other, anyX = anyW = false;
+                work += copies.bytes, room -= copies.bytes;
+            }
+    }
+    if(plan.together)
+    {
+        const PlanBoth& both  = plan.both;
+        const uint64_t  sumsX = sumsBytes(px, true, both.splitsX);
+        LinearParams    x = both.splitsX > 1u ? sharesOf(px, true, both.splitsX, work) : px, w = both.splitsW > 1u ? sharesOf(pw, false, both.splitsW, work + sumsX) : pw;
+        const uint64_t  workgroupsX = tilesOfLaunch(x, true, r355::TILE_64), workgroupsW = tilesOfLaunch(w, false, r355::TILE_64);
+        if(workgroupsX * both.splitsX + workgroupsW * both.splitsW > r355::MAX_GROUPS)
+            return tooMany(what);
+        (a.in_type == R355_F16 ? r355::linearBothF16 : r355::linearBothBF16)(x, w, static_cast<uint32_t>(workgroupsX), static_cast<uint32_t>(workgroupsW), s);
+        if(both.splitsX > 1u)
+            launchReduce(a.in_type, px, true, both.splitsX, work, s);
+        if(both.splitsW > 1u)
+            launchReduce(a.in_type, pw, false, both.splitsW, work + sumsX, s);
+        return r355::checkLaunch(what);
     }
     if(wantX)
-        R355_TRY(launchTiles(a.in_type, px, true, false, anyX, planX, a.workspace, a.workspace_bytes, s, what));
+        R355_TRY(launchTiles(a.in_type, px, true, false, anyX, plan.x, work, room, s, what));
     if(wantW)
-        R355_TRY(launchTiles(a.in_type, pw, false, false, anyW, planW, a.workspace, a.workspace_bytes, s, what));
+        R355_TRY(launchTiles(a.in_type, pw, false, false, anyW, plan.w, work, room, s, what));
     return r355::checkLaunch(what);
 }

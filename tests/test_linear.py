@@ -241,6 +241,24 @@ def test_sums_split_over_workgroups(rows, n, k, pad):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,n,k,groups,pad,offset,gather", [(700, 1000, 999, 1, 0, 0, False), (600, 1100, 1024, 1, 3, 1, True), (1000, 600, 1003, 3, 1, 1, True), (1500, 700, 520, 4, 4, 0, False)])
+def test_operands_laid_out_anew(rows, n, k, groups, pad, offset, gather):
+    """Rows off 16-byte boundaries, or that end inside 16 bytes, with a workspace that holds them evenly; NaN behind every row and beside the operands"""
+    offsets = None if groups == 1 else _offsets([rows // 2, 0] + [rows // 8] * (groups - 2))
+    a = R.linear_args(R.BF16, R.BF16, rows, n, k, 0x1000 + 2 * offset, 0x2000 + 2 * offset, 0x3000, groups=groups, offsets=0x4000 if groups > 1 else None, ldx=k + pad, ldw=k + pad,
+                      source=0x5000 if gather else None, x_rows=rows // 3 if gather else None)
+    eights = (k + 7) // 8 * 8
+    need = R.linear_workspace_bytes(a)
+    assert need >= 2 * eights * groups * n
+    kw = dict(groups=groups, offsets=offsets, pad=(pad, pad, 0, 0, 0, 0), offset=offset)
+    if gather:
+        kw.update(source=[(13 * r + 5) % (rows // 3) for r in range(rows)], x_rows=rows // 3)
+    for size in (need, 2 * eights * groups * n // 2):
+        _run("bf16", "bf16", rows, n, k, act="silu", bias=True, gate=True, keep=True, workspace=_scratch(size), **kw)
+        _run("f16", "f32", rows, n, k, c=True, workspace=_scratch(size), **kw)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("offsets,rows,n,k", [([0, 30, 30, 58, 60], 60, 200, 4096), ([3, 20, 50], 64, 1030, 2056), ([0] * 70 + [40] + [90] * 60, 97, 33, 1999), ([5, 90], 100, 72, 2048)])
 def test_sums_of_groups_split_over_workgroups(offsets, rows, n, k):
     """Rows before, between and behind the groups are left as they were, also by what adds the shares"""

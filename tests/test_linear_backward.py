@@ -108,6 +108,22 @@ def test_sums_split_over_workgroups(rows, n, k, sizes, pad, accumulate, grad):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("act", ["none", "silu"])
+@pytest.mark.parametrize("rows,n,k,sizes,pad,offset", [(1100, 1003, 520, None, 0, 0), (900, 1000, 603, None, 0, 1), (1000, 700, 999, [500, 0, 300, 150], 1, 0), (1200, 1001, 512, [200, 1000], 7, 1)])
+def test_operands_laid_out_anew(rows, n, k, sizes, pad, offset, act):
+    """Rows off 16-byte boundaries, or that end inside 16 bytes, with a workspace that holds them evenly; NaN behind every row and beside the operands"""
+    groups, offsets = (1, None) if sizes is None else (len(sizes), _offsets(sizes))
+    a = R.linear_backward_args(R.BF16, R.BF16, rows, n, k, 0x1000 + 2 * offset, 0x2000 + 2 * offset, 0x3000 + 2 * offset, dx=0x4000, dw=0x5000, groups=groups,
+                               offsets=None if sizes is None else 0x6000, lddy=n + pad, ldx=k + pad, ldw=k + pad)
+    need, eights = R.linear_backward_workspace_bytes(a), (n + 7) // 8 * 8
+    assert need >= 2 * eights * (groups * k + rows)
+    for size in (need, need // 3 // 16 * 16):
+        _run("bf16", "bf16", rows, n, k, act=act, groups=groups, offsets=offsets, pad=pad, offset=offset, workspace=_scratch(size))
+    _run("f16", "f32", rows, n, k, act=act, groups=groups, offsets=offsets, pad=pad, offset=offset, accumulate=True, workspace=_scratch(need), want=("dw",))
+    _run("f16", "f16", rows, n, k, act=act, groups=groups, offsets=offsets, pad=pad, offset=offset, workspace=_scratch(need), want=("dx", "dbias"))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("accumulate", [False, True])
 @pytest.mark.parametrize("act", ["none", "silu"])
 @pytest.mark.parametrize("k", [72, 45])
