@@ -403,7 +403,8 @@ typedef enum
  * source (device memory, or NULL): row r is row source[r] of x, which has x_rows of them; a number that is none of them reads as zeros.
  * c may be y (of the same leading dimension); any other overlap of y or z with what is read is undefined.  Any sizes up to 2^30 rows, n and k of 2^22 - 8 and 1024 groups; any leading dimension and alignment of an element, fastest (several times) with rows of x and w on
  * 16-byte boundaries and k a multiple of 8; then with n a multiple of 8 and the other rows on 16-byte boundaries.  With source, x_rows times ldx up to 2^31 bytes.
- * workspace (16-byte aligned, contents irrelevant): with it the sum is split over workgroups where the result has few tiles; r355_linear_workspace_bytes says how much is made use of.
+ * workspace (16-byte aligned, contents irrelevant): with it the sum is split over workgroups where the result has few tiles, and operands off 16-byte boundaries are laid out evenly
+ * first where that pays; r355_linear_workspace_bytes says how much is made use of.
  * Calls that overlap need one each.  The result depends on the sizes and the workspace offered, not on scheduling.
  */
 typedef struct
