@@ -653,6 +653,16 @@ namespace
         return us;
     }
 
+    // What tiles of groups, each with weights of its own, take to read them from memory (those of a group's other rows find them in the caches): 5.8 TB/s in whole rounds, of fewer tiles as much
+    // as each has under way, 24 bytes a ns of 256 columns, 22 of 128 with two tiles on a CU, otherwise 12 (96 tiles of 256 columns of 6520 119 us, 176 of 128 74, 336 of 64 71).
+    double weightsTime(uint32_t tile, double tiles, double k)
+    {
+        const uint32_t held = TILE_TIMES[tile].held;
+        const double   round = static_cast<double>(r355::computeUnits()) * held, bytes = r355::LINEAR_COLS[tile] * k * 2.0, full = static_cast<double>(static_cast<uint64_t>(tiles / round)),
+                     rest = tiles - full * round, each = held == 2u ? 22e3 : held == 4u || r355::LINEAR_COLS[tile] < 256u ? 12e3 : 24e3;
+        return full * round * bytes / 5.8e6 + (rest > 0.0 ? bytes / (each * rest < 5.8e6 ? each : 5.8e6 / rest) : 0.0);
+    }
+
     // floats between the rows of the sums of a split product
     uint32_t pitchOf(uint32_t n)
     {
@@ -675,16 +685,25 @@ namespace
             const double met = p.groups < rows ? p.groups : static_cast<double>(rows);
             return (static_cast<double>(rows) / LINEAR_ROWS[tile] + (tile == TILE_256 ? 0.2 : 0.5) * met) * across;
         };
-        Plan best{any ? TILE_ANY : TILE_64, 1u, 0u, 1e30};
+        // (A sum that finds its rows' groups again costs more than one that does not.)
+        const double sums = aK && p.offsets ? 10.0 : 5.0;
+        // (the largest tile is as high as its rows, by quarters: of groups with few rows a quarter high, which takes half the time)
+        const double rowsMet = aK && p.offsets ? static_cast<double>(p.rows) / (p.groups < p.rows ? p.groups : p.rows) : 256.0, height = rowsMet < 40.0 ? 0.5 : rowsMet < 80.0 ? 0.75 : 1.0;
+        Plan         best{any ? TILE_ANY : TILE_64, 1u, 0u, 1e30};
         for(uint32_t tile = any ? TILE_ANY : TILE_256; tile < (any ? LINEAR_TILES : TILE_ANY); ++tile)
         {
-            const double all = tiles(tile, p.rows);
+            // (each group that is met has a tile, whatever part of it is there)
+            const double all = tiles(tile, p.rows), least = aK && p.offsets ? static_cast<double>(p.groups < p.rows ? p.groups : p.rows) * static_cast<double>(tilesOf(p.n, LINEAR_COLS[tile])) : 0.0,
+                         there = all > least ? all : least;
             for(uint32_t splits = 1u; splits <= 64u; splits += splits < 4u ? 1u : splits / 2u)
             {
                 // (a sum is split in whole stages, four of them at least)
-                if(splits > 1u && (stages < 4.0 * splits || rowsY * pitchOf(p.n) * 4u * splits > workspaceBytes || all > computeUnits()))
+                if(splits > 1u && (stages < 4.0 * splits || rowsY * pitchOf(p.n) * 4u * splits > workspaceBytes || there > computeUnits()))
                     break;
-                const double us = launchTime(tile, all * splits, stages / splits) + (splits > 1u ? 5.0 + static_cast<double>(rowsY) * p.n * 4.0 * (2u * splits + 1u) / 5e6 : 0.0);
+                const double launch = launchTime(tile, all * splits, stages / splits) * (tile == TILE_256 ? height : 1.0);
+                // (a third more where many groups have rows of a second tile, which does not find all of the weights in the caches)
+                const double again = 0.5 + rowsMet / LINEAR_ROWS[tile], reads = aK && p.offsets ? weightsTime(tile, there * splits, static_cast<double>(p.k) / splits * least / there) * (again < 1.0 ? 1.0 : again < 1.3 ? again : 1.3) : 0.0;
+                const double us     = (launch > reads ? launch : reads) + (splits > 1u ? sums + static_cast<double>(rowsY) * p.n * 4.0 * (2u * splits + 1u) / 5e6 : 0.0);
                 if(us < best.us)
                     best = Plan{static_cast<LinearTile>(tile), splits, 0u, us};
             }
@@ -922,22 +941,25 @@ namespace
         return a.k % 8u == 0u && evenRows(a.x, a.ldx, 2) && evenRows(a.w, a.ldw, 2) && (a.groups == 1u || a.w_stride % 8 == 0);
     }
     // The kernel of a forward product by its rows: us of dot products, of the kernel for few rows and of tiles for 4096 x 4096: one row 7.3, 8.0, 14; two 7.8, 8.2, 14; four 8.8, 8.3, 14; sixteen
-    // -, 10, 15; 24 -, 17, 14.  Of experts with about one row each (32 of 4096 x 4096, 128 of 1024 x 1024) 84, 105, 115 and 49, 75, 50; with four (8, 32, 64 experts of 2048 x 2048) 21, 15, 21; 79,
-    // 54, 70 and 143, 105, 138; with twelve 37, 21, 18; 166, 73, 75 and 321, 143, 124.  A workgroup of the kernel for few rows has 16 columns, little work with a short sum: 64 experts of 1024 x 1024
-    // with four 43, 30, 23; only where the CUs hold all of them at once it wins (4 of 1024 x 1024 5.6, 4.9, 6.7, 8 8.8, 6.1, 7.6).
+    // -, 10, 15; 24 -, 17, 14.  Of experts with about one row each (32 of 4096 x 4096, 128 of 1024 x 1024) 84, 105, 115 and 49, 75, 50; with four (8, 32, 64 experts of 2048 x 2048) 21, 15, 16; 79,
+    // 54, 48 and 143, 105, 95; with twelve 37, 21, 17; 166, 73, 48 and 321, 143, 95: the kernel for few rows reads the weights at 5.7 TB/s, and once more for every 20 rows or so, after 4 us, whatever their
+    // lengths; where the tiles' plan takes more, as of few groups, it wins (4 of 1024 x 1024 with four 5.6, 4.9, 6.7; 16 of 1326 x 6520 with two -, 51, 71).
     enum class Kernel
     {
         DOTS,
         FEW,
         TILES
     };
-    Kernel kernelOf(const r355_linear_args& a, bool even)
+    Kernel kernelOf(const r355_linear_args& a, bool even, uint64_t room)
     {
         if(!even)
             return Kernel::TILES;
         if(a.groups == 1u)
             return a.rows <= 2u ? Kernel::DOTS : a.rows <= 16u ? Kernel::FEW : Kernel::TILES;
-        return a.rows <= a.groups ? Kernel::DOTS : a.rows / a.groups < 9u && (a.k >= 2048u || tilesOf(a.n, 16u) * a.groups <= 2u * r355::computeUnits()) ? Kernel::FEW : Kernel::TILES;
+        if(a.rows <= a.groups)
+            return Kernel::DOTS;
+        const double few = 4.0 + static_cast<double>(a.groups) * a.n * a.k * 2.0 / 5.7e6 * (1.0 + 0.05 * a.rows / a.groups);
+        return a.rows / a.groups < 9u && few < planOf(forwardParams(a), true, false, room).us ? Kernel::FEW : Kernel::TILES;
     }
     LinearParams inputParams(const r355_linear_backward_args& a, const char* dz, uint32_t lddz)
     {
@@ -1111,7 +1133,7 @@ extern "C" int r355_linear(const r355_linear_args* args, void* stream)
     const hipStream_t  s    = static_cast<hipStream_t>(stream);
     r355::beginCall();
     const bool         f16  = a.in_type == R355_F16;
-    const Kernel       kernel = kernelOf(a, even);
+    const Kernel       kernel = kernelOf(a, even, usable(a.workspace, a.workspace_bytes));
     if(kernel != Kernel::TILES && mostTiles(p, kernel == Kernel::DOTS ? 1u : 16u) * tilesOf(p.n, 16u) > r355::MAX_GROUPS / 2u)
         return tooMany(what);
     switch(kernel)
@@ -1147,7 +1169,7 @@ extern "C" int r355_linear(const r355_linear_args* args, void* stream)
 
 extern "C" size_t r355_linear_workspace_bytes(const r355_linear_args* args)
 {
-    if(!args || args->rows == 0 || args->n == 0 || args->k == 0 || args->groups == 0 || kernelOf(*args, evenForward(*args)) != Kernel::TILES)
+    if(!args || args->rows == 0 || args->n == 0 || args->k == 0 || args->groups == 0 || kernelOf(*args, evenForward(*args), ~0ull) != Kernel::TILES)
         return 0;
     const LinearParams p    = forwardParams(*args);
     const bool         even = evenForward(*args);

@@ -259,12 +259,14 @@ def test_operands_laid_out_anew(rows, n, k, groups, pad, offset, gather):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("offsets,rows,n,k", [([0, 30, 30, 58, 60], 60, 200, 4096), ([3, 20, 50], 64, 1030, 2056), ([0] * 70 + [40] + [90] * 60, 97, 33, 1999), ([5, 90], 100, 72, 2048)])
+@pytest.mark.parametrize("offsets,rows,n,k", [([0, 30, 30, 58, 60], 60, 200, 4096), ([3, 20, 50], 64, 1030, 2056), ([0] * 70 + [40] + [90] * 60, 97, 33, 1999), ([5, 90], 100, 72, 2048),
+                                                ([3, 20, 50], 64, 1030, 8200), ([5, 90], 100, 72, 8192), ([0] * 70 + [40] + [90] * 60, 97, 33, 5999)])
 def test_sums_of_groups_split_over_workgroups(offsets, rows, n, k):
     """Rows before, between and behind the groups are left as they were, also by what adds the shares"""
     groups = len(offsets) - 1
     need = _workspace_bytes(rows, n, k, groups=groups, offsets=0x4000)
-    assert need > 0
+    assert need > 0 or k < 4096  # (short sums are left whole)
+    need = need or 1 << 16
     _run("bf16", "bf16", rows, n, k, act="gelu", bias=True, gate=True, keep=True, groups=groups, offsets=offsets, workspace=_scratch(need))
     _run("f16", "f32", rows, n, k, bias=True, c=True, in_place=True, groups=groups, offsets=offsets, workspace=_scratch(need // 2 // 16 * 16))
 
