@@ -226,7 +226,7 @@ namespace
 
     // ---- Few rows of each group.  A workgroup's eight waves share 16 RB weight rows x 16 CB rows of x and take DEPTH neighbouring pieces of 64 of the sum in turn, both
     // straight from global memory; their sums meet in LDS in the order of the waves.  The weights are the first operand: a lane then holds four of them of one row of x.
-    // Bound by HBM: 64 rows of 16 experts of 4096 x 4096 105 us, 5.1 TB/s.  (Single pieces in turn: rows that do not begin with a cache line have lines of two waves, 30 rows of 8 experts
+    // Bound by HBM: two rows of each of 16 experts of 1326 x 6520 50 us, 5.5 TB/s.  (Single pieces in turn: rows that do not begin with a cache line have lines of two waves, 30 rows of 8 experts
     // of 8192 x 4104 167 instead of 162 us; and such lines come twice where they are read nontemporally, 162 instead of 125.)
     template <typename T, uint32_t RB, uint32_t CB, uint32_t DEPTH>
     __global__ void __launch_bounds__(64 * WAVES, 2) linearFew(LinearParams p)
@@ -941,7 +941,7 @@ namespace
         return a.k % 8u == 0u && evenRows(a.x, a.ldx, 2) && evenRows(a.w, a.ldw, 2) && (a.groups == 1u || a.w_stride % 8 == 0);
     }
     // The kernel of a forward product by its rows: us of dot products, of the kernel for few rows and of tiles for 4096 x 4096: one row 7.3, 8.0, 14; two 7.8, 8.2, 14; four 8.8, 8.3, 14; sixteen
-    // -, 10, 15; 24 -, 17, 14.  Of experts with about one row each (32 of 4096 x 4096, 128 of 1024 x 1024) 84, 105, 115 and 49, 75, 50; with four (8, 32, 64 experts of 2048 x 2048) 21, 15, 16; 79,
+    // -, 10, 15; 24 -, 17, 14.  Of experts with about one row each (32 of 4096 x 4096, 128 of 1024 x 1024) the first two 84, 105 and 49, 75; with four (8, 32, 64 experts of 2048 x 2048) 21, 15, 16; 79,
     // 54, 48 and 143, 105, 95; with twelve 37, 21, 17; 166, 73, 48 and 321, 143, 95: the kernel for few rows reads the weights at 5.7 TB/s, and once more for every 20 rows or so, after 4 us, whatever their
     // lengths; where the tiles' plan takes more, as of few groups, it wins (4 of 1024 x 1024 with four 5.6, 4.9, 6.7; 16 of 1326 x 6520 with two -, 51, 71).
     enum class Kernel
