@@ -371,31 +371,40 @@ namespace
                      0x00020000};
     }
 
-    // bytes of LDS of a tile
-    constexpr uint32_t ldsOf(uint32_t wm, uint32_t wn)
+    // Blocks of 32 rows of A's image.  Of an operand that is not contiguous along the sum there are images of 2, 4 and 8 (a load brings whole rows of the sum, whose swizzle stays
+    // inside them): 192 rows of one lie in an image of 256, whose last quarter no wave reads (dW of 4096 x 2880 x 2880 71 us, on tiles of 256 rows 87; 8840 rows over 4 groups of 536 x 3552
+    // 40 and 75).
+    constexpr uint32_t imageOf(bool aK, uint32_t wm)
     {
-        return (2u * wm + 3u * wn) * 32u * STAGE_KB;
+        return aK || wm != 6u ? wm : 8u;
+    }
+    // bytes of LDS of a tile
+    constexpr uint32_t ldsOf(bool aK, uint32_t wm, uint32_t wn)
+    {
+        return (2u * imageOf(aK, wm) + 3u * wn) * 32u * STAGE_KB;
     }
 
     template <bool AK, bool BK, uint32_t WM, uint32_t WN>
     __device__ __forceinline__ void linearTile(const LinearParams& p, const Work& w, char* lds)
     {
-        constexpr uint32_t SIZE_A = 32u * WM * STAGE_KB, SIZE_B = 32u * WN * STAGE_KB; // bytes of the operands' stages
+        constexpr uint32_t IA = imageOf(AK, WM);
+        constexpr uint32_t SIZE_A = 32u * IA * STAGE_KB, SIZE_B = 32u * WN * STAGE_KB; // bytes of the operands' stages
         constexpr uint32_t FIRST_B = 2u * SIZE_A, LAST_B = FIRST_B + 2u * SIZE_B; // two buffers of A, three of B
         constexpr uint32_t NS = WM * WN, XS = WM + WN, BOTH = 2u * (WM < WN ? WM : WN); // matrix instructions and operand blocks of half a stage
         // the large tile's loads are dealt out over the whole stage, B two stages ahead; the small tiles', whose stages are a quarter as long and less, come in the
-        // second half, B three stages ahead (gemm_tiled.hip has both measured)
-        constexpr bool     SPREAD  = WM == 8u || WN == 8u;
+        // second half, B three stages ahead (gemm_tiled.hip has both measured), where there is room for all of them
+        constexpr bool     SPREAD  = IA == 8u || WN == 8u;
         constexpr uint32_t B_AHEAD = SPREAD ? 2u : 3u;
         constexpr uint32_t SCRATCH = 64u * WN * (WM % 4u == 0u ? 64u : 32u); // of a wave's part of the epilogue
-        static_assert(ldsOf(WM, WN) <= 160u * 1024u && 4u * SCRATCH <= ldsOf(WM, WN), "what a CU has");
+        static_assert(ldsOf(AK, WM, WN) <= 160u * 1024u && 4u * SCRATCH <= ldsOf(AK, WM, WN), "what a CU has");
+        static_assert(SPREAD ? IA <= XS && WN <= XS : IA == WM, "one load an operand block at most");
         const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1u;
         const uint32_t ldsBase = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
         const uint32_t dma     = ldsBase + wave * 64u * CHUNK;
 
-        uint32_t offA[WM], offB[WN], stepA, stepB, kByteA, kByteB;
+        uint32_t offA[IA], offB[WN], stepA, stepB, kByteA, kByteB;
         uint64_t stageA, stageB;
-        laneOffsets8<AK, WM, 2>(tid, p.lda, w.rowsLeft, offA, stepA, stageA, kByteA);
+        laneOffsets8<AK, IA, 2>(tid, p.lda, w.rowsLeft, offA, stepA, stageA, kByteA);
         laneOffsets8<BK, WN, 2>(tid, p.ldb, w.colsLeft, offB, stepB, stageB, kByteB);
         uint64_t fromA, fromB;
         if constexpr(AK)
@@ -440,7 +449,7 @@ namespace
         auto issueA = [&](uint32_t s, uint32_t at) {
             const uint32_t valid = validOf(s);
 #pragma unroll
-            for(uint32_t j = 0; j < WM; ++j)
+            for(uint32_t j = 0; j < IA; ++j)
                 loadToLds(stageBuffer<AK>(addrA(s), valid, p.lda), tailA(j, valid), j * stepA, dma + at + j * THREADS * CHUNK);
         };
         auto issueB = [&](uint32_t s, uint32_t at) {
@@ -451,7 +460,7 @@ namespace
         };
 
         uint32_t rdA[8], rdB[8];
-        readOffsets8<AK, WM, 2>(wm, lane, rdA);
+        readOffsets8<AK, IA, 2, WM>(wm, lane, rdA);
         readOffsets8<BK, WN, 2>(wn, lane, rdB);
         f32x4 acc[WM][WN];
 #pragma unroll
@@ -478,7 +487,7 @@ namespace
             if(ofB)
                 readBlock8<BK, WN, 2>(lds + atB, rdB, i, half, part, fb[half][i], 0u);
             else
-                readBlock8<AK, WM, 2>(lds + atA, rdA, i, half, part, fa[half][i], 0u);
+                readBlock8<AK, IA, 2>(lds + atA, rdA, i, half, part, fa[half][i], 0u);
         };
         auto after = [](uint32_t at) { return at == LAST_B ? FIRST_B : at + SIZE_B; }; // B's buffers go round
         // matrix instructions firstOf(x) .. firstOf(x + 1) - 1 of half a stage go with operand block x, one at least: with the first two its reads, with the third, or the last, a load
@@ -498,12 +507,12 @@ namespace
         if constexpr(SPREAD)
         {
             issueB(0u, FIRST_B), issueA(0u, 0u), issueB(1u, FIRST_B + SIZE_B), issueA(1u, SIZE_A);
-            waitVmcnt<WM + WN>();
+            waitVmcnt<IA + WN>();
         }
         else
         {
             issueA(0u, 0u), issueB(0u, FIRST_B), issueA(1u, SIZE_A), issueB(1u, FIRST_B + SIZE_B), issueB(2u, LAST_B);
-            waitVmcnt<WM + 2u * WN>();
+            waitVmcnt<IA + 2u * WN>();
         }
         ldsBarrier();
 #pragma unroll
@@ -549,7 +558,7 @@ namespace
                     {
                         if constexpr(SPREAD)
                         {
-                            if(const uint32_t j = x * WM / XS; (x + 1u) * WM / XS > j)
+                            if(const uint32_t j = x * IA / XS; (x + 1u) * IA / XS > j)
                                 loadA(bufA, vA, j);
                         }
                         else if(x < WM)
@@ -581,7 +590,7 @@ namespace
     template <bool AK, bool BK>
     __global__ void __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(1, 1))) linearTiles256(LinearParams p)
     {
-        __shared__ __attribute__((aligned(1024))) char lds[ldsOf(8, 8)];
+        __shared__ __attribute__((aligned(1024))) char lds[ldsOf(AK, 8, 8)];
         Work                                           w;
         if(!workOf<AK, 256, 256>(p, w, blockIdx.x, blockIdx.y))
             return;
@@ -600,7 +609,7 @@ namespace
     template <bool AK, bool BK>
     __global__ void __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(1, 1))) linearTiles192x256(LinearParams p)
     {
-        __shared__ __attribute__((aligned(1024))) char lds[ldsOf(6, 8)];
+        __shared__ __attribute__((aligned(1024))) char lds[ldsOf(AK, 6, 8)];
         Work                                           w;
         if(workOf<AK, 192, 256>(p, w, blockIdx.x, blockIdx.y))
             linearTile<AK, BK, 6, 8>(p, w, lds);
@@ -608,7 +617,7 @@ namespace
     template <bool AK, bool BK>
     __global__ void __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(1, 1))) linearTiles192x128(LinearParams p)
     {
-        __shared__ __attribute__((aligned(1024))) char lds[ldsOf(6, 4)];
+        __shared__ __attribute__((aligned(1024))) char lds[ldsOf(AK, 6, 4)];
         Work                                           w;
         if(workOf<AK, 192, 128>(p, w, blockIdx.x, blockIdx.y))
             linearTile<AK, BK, 6, 4>(p, w, lds);
@@ -616,7 +625,7 @@ namespace
     template <bool AK, bool BK>
     __global__ void __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(1, 1))) linearTiles256x128(LinearParams p)
     {
-        __shared__ __attribute__((aligned(1024))) char lds[ldsOf(8, 4)];
+        __shared__ __attribute__((aligned(1024))) char lds[ldsOf(AK, 8, 4)];
         Work                                           w;
         if(workOf<AK, 256, 128>(p, w, blockIdx.x, blockIdx.y))
             linearTile<AK, BK, 8, 4>(p, w, lds);
@@ -624,7 +633,7 @@ namespace
     template <bool AK, bool BK>
     __global__ void __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(1, 1))) linearTiles128x256(LinearParams p)
     {
-        __shared__ __attribute__((aligned(1024))) char lds[ldsOf(4, 8)];
+        __shared__ __attribute__((aligned(1024))) char lds[ldsOf(AK, 4, 8)];
         Work                                           w;
         if(workOf<AK, 128, 256>(p, w, blockIdx.x, blockIdx.y))
             linearTile<AK, BK, 4, 8>(p, w, lds);
@@ -632,7 +641,7 @@ namespace
     template <bool AK, bool BK>
     __global__ void __launch_bounds__(THREADS, 2) linearTiles128(LinearParams p)
     {
-        __shared__ __attribute__((aligned(1024))) char lds[ldsOf(4, 4)];
+        __shared__ __attribute__((aligned(1024))) char lds[ldsOf(AK, 4, 4)];
         Work                                           w;
         if(workOf<AK, 128, 128>(p, w, blockIdx.x, blockIdx.y))
             linearTile<AK, BK, 4, 4>(p, w, lds);
@@ -640,7 +649,7 @@ namespace
     template <bool AK, bool BK>
     __global__ void __launch_bounds__(THREADS, 4) linearTiles64(LinearParams p)
     {
-        __shared__ __attribute__((aligned(1024))) char lds[ldsOf(2, 2)];
+        __shared__ __attribute__((aligned(1024))) char lds[ldsOf(AK, 2, 2)];
         Work                                           w;
         if(workOf<AK, 64, 64>(p, w, blockIdx.x, blockIdx.y))
             linearTile<AK, BK, 2, 2>(p, w, lds);
@@ -650,7 +659,7 @@ namespace
     // 100 x 512 x 512 11.1 -> 8.4, 2048 x 1024 x 1024 26.1 -> 18.9; of larger layers separate launches of larger tiles take less, by planBoth()).
     __global__ void __launch_bounds__(THREADS, 4) linearBoth64(LinearParams px, LinearParams pw, uint32_t workgroupsX, uint32_t workgroupsW)
     {
-        __shared__ __attribute__((aligned(1024))) char lds[ldsOf(2, 2)];
+        __shared__ __attribute__((aligned(1024))) char lds[ldsOf(false, 2, 2)];
         Work                                           w;
         const uint32_t                                 first = workgroupsX * px.splits;
         if(blockIdx.x < first)

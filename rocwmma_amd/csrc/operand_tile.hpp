@@ -78,6 +78,7 @@ namespace r355
             else
             {
                 constexpr uint32_t SLOTS = 2u * WB * ES, KROWS = THREADS / SLOTS; // chunks per k-row, k-rows per load
+                static_assert(THREADS % SLOTS == 0u, "a load brings whole k-rows, and a k-row's swizzle stays inside it");
                 const uint32_t     r = tid / SLOTS, slot = tid % SLOTS; // k-row KROWS j + r (the swizzle may alternate with j)
     #pragma unroll
                 for(uint32_t j = 0; j < WB; ++j)
@@ -97,6 +98,7 @@ namespace r355
         __device__ __forceinline__ void readOffsets8(uint32_t w, uint32_t lane, uint32_t (&rd)[8])
         {
             static_assert(WT == WB || ES <= 2, "narrower wave tiles: 8- and 16-bit operands");
+            static_assert(KCONTIG || (WB & (WB - 1u)) == 0u, "a k-row's swizzle stays inside it");
             const uint32_t t = lane & 15u, g = lane >> 4;
     #pragma unroll
             for(uint32_t i = 0; i < 8; ++i)
