@@ -428,6 +428,24 @@ typedef struct
 int    r355_linear(const r355_linear_args* args, void* stream);
 size_t r355_linear_workspace_bytes(const r355_linear_args* args);
 
+/* What a call with exactly these arguments launches (on the host; nothing is launched): the kernel, and of tiles their size, the workgroups along the sum, how many rows go out in such
+ * tiles while the rest has a plan of its own (0: all of them), how many operands are laid out evenly first, and whether both gradients are one launch.  Zeros where there is nothing
+ * to do.  A call that is refused has no plan: the same error. */
+typedef enum
+{
+    R355_LINEAR_NONE     = 0,
+    R355_LINEAR_DOTS     = 1, /* one or two rows: dot products */
+    R355_LINEAR_FEW      = 2, /* few rows: matrix instructions straight from memory */
+    R355_LINEAR_TILES    = 3, /* macro tiles */
+    R355_LINEAR_ELEMENTS = 4  /* macro tiles of operands of any alignment */
+} r355_linear_kernel;
+typedef struct
+{
+    int32_t  kernel;
+    uint32_t tile_rows, tile_cols, splits, first_rows, copies, together;
+} r355_linear_plan;
+int    r355_linear_launch_plan(const r355_linear_args* args, r355_linear_plan* plan);
+
 /*
  * The gradients of r355_linear for dy = dL / dy [rows][n]:
  *   dz = dy * gate * act'(z);  dgate = dy * act(z);  dx = dz W;  dw = dz^T x;  dbias = sum of dz over a group's rows      (of c: dy itself)
@@ -459,6 +477,7 @@ typedef struct
 } r355_linear_backward_args;
 int    r355_linear_backward(const r355_linear_backward_args* args, void* stream);
 size_t r355_linear_backward_workspace_bytes(const r355_linear_backward_args* args);
+int    r355_linear_backward_launch_plan(const r355_linear_backward_args* args, r355_linear_plan* dx, r355_linear_plan* dw);
 
 /*
  * The router: for each token the `top` experts of the largest logit (plus bias [experts], where given: in f32, for the choice alone), the lowest expert of equal ones first, NaN behind

@@ -31,6 +31,8 @@ ROPE_HALF, ROPE_INTERLEAVED = 0, 1
 
 # r355_activation
 ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = range(5)
+# r355_linear_kernel
+LINEAR_NONE, LINEAR_DOTS, LINEAR_FEW, LINEAR_TILES, LINEAR_ELEMENTS = range(5)
 # r355_route_score
 ROUTE_SOFTMAX, ROUTE_SIGMOID = 0, 1
 
@@ -40,7 +42,7 @@ EXPORTS = [
     "r355_gemm", "r355_gemm_noalloc", "r355_gemm_query", "r355_gemm_launch_plan", "r355_gemm_timed", "r355_dlrm_fwd", "r355_dlrm_fwd_timed",
     "r355_dlrm_bwd", "r355_dlrm_kernel", "r355_gemv", "r355_gemv_timed", "r355_dgemv", "r355_gemv_workspace_bytes", "r355_gemv_ws", "r355_dgemv_ws", "r355_compress_24", "r355_decompress_24", "r355_compress_24_16", "r355_decompress_24_16",
     "r355_w4_matmul", "r355_w4_packed_bytes", "r355_w4_pack", "r355_rope", "r355_rope_turns", "r355_tree_attention", "r355_tree_attention_workspace_bytes",
-    "r355_linear", "r355_linear_workspace_bytes", "r355_linear_backward", "r355_linear_backward_workspace_bytes",
+    "r355_linear", "r355_linear_workspace_bytes", "r355_linear_launch_plan", "r355_linear_backward", "r355_linear_backward_workspace_bytes", "r355_linear_backward_launch_plan",
     "r355_route", "r355_route_workspace_bytes", "r355_route_backward", "r355_combine", "r355_dispatch",
     "r355_get_device_info", "r355_last_error", "r355_version",
 ]
@@ -147,6 +149,10 @@ class LinearBackwardArgs(ctypes.Structure):
     ]
 
 
+class LinearPlan(ctypes.Structure):
+    _fields_ = [("kernel", ctypes.c_int32)] + [(name, ctypes.c_uint32) for name in ("tile_rows", "tile_cols", "splits", "first_rows", "copies", "together")]
+
+
 class RouteArgs(ctypes.Structure):
     _fields_ = [
         ("type", ctypes.c_int32), ("score", ctypes.c_int32), ("chosen_only", ctypes.c_int32),
@@ -231,8 +237,10 @@ def lib():
         L.r355_tree_attention_workspace_bytes.argtypes = [ctypes.POINTER(TreeAttentionArgs)]
         L.r355_linear.argtypes = [vp, vp]
         L.r355_linear_workspace_bytes.argtypes = [vp]
+        L.r355_linear_launch_plan.argtypes = [vp, vp]
         L.r355_linear_backward.argtypes = [vp, vp]
         L.r355_linear_backward_workspace_bytes.argtypes = [vp]
+        L.r355_linear_backward_launch_plan.argtypes = [vp, vp, vp]
         L.r355_route.argtypes = [vp, vp]
         L.r355_route_workspace_bytes.argtypes = [u32, u32, u32]
         L.r355_route_backward.argtypes = [vp, vp]
@@ -645,6 +653,13 @@ def linear_workspace_bytes(a):
     return lib().r355_linear_workspace_bytes(ctypes.byref(a))
 
 
+def linear_launch_plan(a):
+    """The LinearPlan of what r355_linear launches for exactly these LinearArgs (on the host)."""
+    plan = LinearPlan()
+    _check(lib().r355_linear_launch_plan(ctypes.byref(a), ctypes.byref(plan)))
+    return plan
+
+
 def _linear_backward_bytes(in_type, grad_type, rows, n, k, dy, x, w, dx, dw, dbias, z, activation, gate, dgate, dz, accumulate, groups, offsets, lddy, ldx, ldw, ldz, ldg, lddz, lddg,
                            lddx, lddw, w_stride, dw_stride, workspace, workspace_bytes):
     ldw, lddw = k if ldw is None else ldw, k if lddw is None else lddw
@@ -678,6 +693,13 @@ def linear_backward(in_type, grad_type, rows, n, k, dy, x, w, dx=None, dw=None, 
 def linear_backward_workspace_bytes(a):
     """Bytes of workspace that r355_linear_backward makes use of for LinearBackwardArgs (0: none)."""
     return lib().r355_linear_backward_workspace_bytes(ctypes.byref(a))
+
+
+def linear_backward_launch_plan(a):
+    """The LinearPlans of dx and dw of what r355_linear_backward launches for exactly these LinearBackwardArgs (on the host)."""
+    dx, dw = LinearPlan(), LinearPlan()
+    _check(lib().r355_linear_backward_launch_plan(ctypes.byref(a), ctypes.byref(dx), ctypes.byref(dw)))
+    return dx, dw
 
 
 _F32_TYPES = set()  # the types of 32-bit floating numbers that have been met

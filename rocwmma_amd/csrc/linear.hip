@@ -11,6 +11,14 @@
 
 #include "linear.hpp"
 
+#define R355_TRY(call)          \
+    do                          \
+    {                           \
+        const int rc_ = (call); \
+        if(rc_ != R355_OK)      \
+            return rc_;         \
+    } while(0)
+
 namespace
 {
     using r355::each;
@@ -1089,15 +1097,131 @@ namespace
         const size_t x = wantX ? splitBytes(px, true, anyX) : 0u, w = wantW ? splitBytes(pw, false, anyW) : 0u;
         return x > w ? x : w;
     }
-} // namespace
 
-#define R355_TRY(call)          \
-    do                          \
-    {                           \
-        const int rc_ = (call); \
-        if(rc_ != R355_OK)      \
-            return rc_;         \
-    } while(0)
+    // What a call launches, by its arguments and the workspace offered; the entry points launch it, the queries report it.
+    struct ForwardChoice
+    {
+        Kernel       kernel;
+        bool         any; // element by element
+        LinearParams p;
+        Plan         plan; // TILES
+        Copies       copies;
+    };
+    ForwardChoice chooseForward(const r355_linear_args& a, const void* workspace, uint64_t room)
+    {
+        ForwardChoice c{};
+        const bool    even = evenForward(a);
+        c.p = forwardParams(a), c.kernel = kernelOf(a, even, room);
+        if(c.kernel != Kernel::TILES)
+            return c;
+        c.any = !even, c.plan = planOf(c.p, true, c.any, room);
+        if(!even)
+        {
+            LinearParams q      = c.p;
+            const Copies copies = evened(a, workspace, q);
+            if(copies.fit(room))
+                if(const Plan other = planOf(q, true, false, room - copies.bytes); other.us + copies.us < c.plan.us)
+                    c.p = q, c.plan = other, c.copies = copies, c.any = false;
+        }
+        return c;
+    }
+    struct BackwardChoice
+    {
+        bool         element, wantX, wantW, anyX, anyW; // element: dz is made first
+        LinearParams px, pw;
+        BackwardPlan plan;
+        Copies       copies;
+    };
+    BackwardChoice chooseBackward(const r355_linear_backward_args& a, const void* workspace, uint64_t room)
+    {
+        BackwardChoice c{};
+        c.element              = a.activation != R355_ACT_NONE || a.gate;
+        const char*    dz      = static_cast<const char*>(c.element ? a.dz : a.dy);
+        const uint32_t lddz    = c.element ? a.lddz : a.lddy;
+        c.wantX = a.dx && a.rows, c.wantW = a.dw != nullptr, c.anyX = c.wantX && !evenInput(a, dz, lddz), c.anyW = c.wantW && !evenWeight(a, dz, lddz);
+        c.px = inputParams(a, dz, lddz), c.pw = weightParams(a, dz, lddz);
+        c.plan = planBackward(c.px, c.pw, c.wantX, c.wantW, c.anyX, c.anyW, room);
+        if((c.anyX || c.anyW) && a.rows)
+        {
+            LinearParams x = c.px, w = c.pw;
+            const Copies copies = evened(a, dz, lddz, c.wantX, c.wantW, workspace, x, w);
+            if(copies.fit(room))
+                if(const BackwardPlan other = planBackward(x, w, c.wantX, c.wantW, false, false, room - copies.bytes); other.us + copies.us < c.plan.us)
+                    c.px = x, c.pw = w, c.plan = other, c.copies = copies, c.anyX = c.anyW = false;
+        }
+        return c;
+    }
+
+    r355_linear_plan reported(Kernel kernel, bool any, const Plan& plan, const Copies& copies)
+    {
+        r355_linear_plan r{};
+        r.kernel = kernel == Kernel::DOTS ? R355_LINEAR_DOTS : kernel == Kernel::FEW ? R355_LINEAR_FEW : any ? R355_LINEAR_ELEMENTS : R355_LINEAR_TILES;
+        if(kernel == Kernel::TILES)
+            r.tile_rows = r355::LINEAR_ROWS[plan.tile], r.tile_cols = r355::LINEAR_COLS[plan.tile], r.splits = plan.splits, r.first_rows = plan.tall, r.copies = copies.count;
+        return r;
+    }
+
+    int checkForward(const r355_linear_args& a)
+    {
+        constexpr const char* what = "linear";
+        R355_TRY(checkCommon(what, a.in_type, a.activation, a.rows, a.n, a.k, a.groups, a.offsets));
+        if(a.out_type != a.in_type && a.out_type != R355_F32)
+            return r355::fail(R355_ERR_UNSUPPORTED, "linear: the result has the type of x or is f32");
+        if(a.rows == 0)
+            return R355_OK; // (nothing is read or written)
+        if(!a.x || !a.w || !a.y)
+            return r355::fail(R355_ERR_BAD_ARG, "linear: null pointer");
+        const uint32_t outBytes = r355::dtypeBytes(a.out_type);
+        R355_TRY(checkMatrix(what, "x", a.x, a.ldx, a.k, 2));
+        R355_TRY(checkMatrix(what, "w", a.w, a.ldw, a.k, 2));
+        R355_TRY(checkMatrix(what, "bias", a.bias, a.n, a.n, 2));
+        R355_TRY(checkMatrix(what, "gate", a.gate, a.ldg, a.n, 2));
+        R355_TRY(checkMatrix(what, "z", a.z, a.ldz, a.n, 2));
+        R355_TRY(checkMatrix(what, "c", a.c, a.ldc, a.n, outBytes));
+        R355_TRY(checkMatrix(what, "y", a.y, a.ldy, a.n, outBytes));
+        R355_TRY(checkStride(what, "w_stride", a.w_stride, a.groups, (uint64_t)(a.n - 1u) * a.ldw + a.k));
+        if(a.source)
+        {
+            if(!r355::aligned(a.source, 4))
+                return r355::fail(R355_ERR_MISALIGNED, "linear: source needs the alignment of its elements");
+            if(a.x_rows == 0 || (uint64_t)a.x_rows * a.ldx * 2u > FAR)
+                return r355::fail(R355_ERR_BAD_SIZE, "linear: rows taken by their numbers must be of 1 to 2^31 bytes of x, got %u rows %u elements apart", a.x_rows, a.ldx);
+        }
+        return R355_OK;
+    }
+    int checkBackward(const r355_linear_backward_args& a)
+    {
+        constexpr const char* what = "linear_backward";
+        R355_TRY(checkCommon(what, a.in_type, a.activation, a.rows, a.n, a.k, a.groups, a.offsets));
+        if(a.grad_type != a.in_type && a.grad_type != R355_F32)
+            return r355::fail(R355_ERR_UNSUPPORTED, "linear_backward: dw has the type of x or is f32");
+        const bool slope = a.activation != R355_ACT_NONE, element = slope || a.gate;
+        if(a.rows != 0 && (!a.dy || (a.dx && !a.w) || (a.dw && !a.x)))
+            return r355::fail(R355_ERR_BAD_ARG, "linear_backward: null pointer");
+        if(a.rows != 0 && slope && !a.z)
+            return r355::fail(R355_ERR_BAD_ARG, "linear_backward: an activation's gradient needs z");
+        if(a.dgate && (!a.gate || !a.z))
+            return r355::fail(R355_ERR_BAD_ARG, "linear_backward: dgate needs gate and z");
+        if(element && !a.dz)
+            return r355::fail(R355_ERR_BAD_ARG, "linear_backward: with an activation or a gate dz is needed");
+        const uint32_t gradBytes = r355::dtypeBytes(a.grad_type);
+        R355_TRY(checkMatrix(what, "dy", a.dy, a.lddy, a.n, 2));
+        R355_TRY(checkMatrix(what, "x", a.x, a.ldx, a.k, 2));
+        R355_TRY(checkMatrix(what, "w", a.w, a.ldw, a.k, 2));
+        R355_TRY(checkMatrix(what, "z", a.z, a.ldz, a.n, 2));
+        R355_TRY(checkMatrix(what, "gate", a.gate, a.ldg, a.n, 2));
+        R355_TRY(checkMatrix(what, "dz", element ? a.dz : nullptr, a.lddz, a.n, 2));
+        R355_TRY(checkMatrix(what, "dgate", a.dgate, a.lddg, a.n, 2));
+        R355_TRY(checkMatrix(what, "dx", a.dx, a.lddx, a.k, 2));
+        R355_TRY(checkMatrix(what, "dw", a.dw, a.lddw, a.k, gradBytes));
+        R355_TRY(checkMatrix(what, "dbias", a.dbias, a.n, a.n, 4));
+        if(a.dx)
+            R355_TRY(checkStride(what, "w_stride", a.w_stride, a.groups, (uint64_t)(a.n - 1u) * a.ldw + a.k));
+        if(a.dw)
+            R355_TRY(checkStride(what, "dw_stride", a.dw_stride, a.groups, (uint64_t)(a.n - 1u) * a.lddw + a.k));
+        return R355_OK;
+    }
+} // namespace
 
 extern "C" int r355_linear(const r355_linear_args* args, void* stream)
 {
@@ -1105,82 +1229,51 @@ extern "C" int r355_linear(const r355_linear_args* args, void* stream)
     if(!args)
         return r355::fail(R355_ERR_BAD_ARG, "linear: null arguments");
     const r355_linear_args& a = *args;
-    R355_TRY(checkCommon(what, a.in_type, a.activation, a.rows, a.n, a.k, a.groups, a.offsets));
-    if(a.out_type != a.in_type && a.out_type != R355_F32)
-        return r355::fail(R355_ERR_UNSUPPORTED, "linear: the result has the type of x or is f32");
+    R355_TRY(checkForward(a));
     if(a.rows == 0)
         return R355_OK;
-    if(!a.x || !a.w || !a.y)
-        return r355::fail(R355_ERR_BAD_ARG, "linear: null pointer");
-    const uint32_t outBytes = r355::dtypeBytes(a.out_type);
-    R355_TRY(checkMatrix(what, "x", a.x, a.ldx, a.k, 2));
-    R355_TRY(checkMatrix(what, "w", a.w, a.ldw, a.k, 2));
-    R355_TRY(checkMatrix(what, "bias", a.bias, a.n, a.n, 2));
-    R355_TRY(checkMatrix(what, "gate", a.gate, a.ldg, a.n, 2));
-    R355_TRY(checkMatrix(what, "z", a.z, a.ldz, a.n, 2));
-    R355_TRY(checkMatrix(what, "c", a.c, a.ldc, a.n, outBytes));
-    R355_TRY(checkMatrix(what, "y", a.y, a.ldy, a.n, outBytes));
-    R355_TRY(checkStride(what, "w_stride", a.w_stride, a.groups, (uint64_t)(a.n - 1u) * a.ldw + a.k));
-    if(a.source)
-    {
-        if(!r355::aligned(a.source, 4))
-            return r355::fail(R355_ERR_MISALIGNED, "linear: source needs the alignment of its elements");
-        if(a.x_rows == 0 || (uint64_t)a.x_rows * a.ldx * 2u > FAR)
-            return r355::fail(R355_ERR_BAD_SIZE, "linear: rows taken by their numbers must be of 1 to 2^31 bytes of x, got %u rows %u elements apart", a.x_rows, a.ldx);
-    }
-    const LinearParams p    = forwardParams(a);
-    const bool         even = evenForward(a);
-    const hipStream_t  s    = static_cast<hipStream_t>(stream);
+    const uint64_t      room = usable(a.workspace, a.workspace_bytes);
+    const ForwardChoice c    = chooseForward(a, a.workspace, room);
+    const hipStream_t   s    = static_cast<hipStream_t>(stream);
+    const bool          f16  = a.in_type == R355_F16;
     r355::beginCall();
-    const bool         f16  = a.in_type == R355_F16;
-    const Kernel       kernel = kernelOf(a, even, usable(a.workspace, a.workspace_bytes));
-    if(kernel != Kernel::TILES && mostTiles(p, kernel == Kernel::DOTS ? 1u : 16u) * tilesOf(p.n, 16u) > r355::MAX_GROUPS / 2u)
+    if(c.kernel != Kernel::TILES && mostTiles(c.p, c.kernel == Kernel::DOTS ? 1u : 16u) * tilesOf(c.p.n, 16u) > r355::MAX_GROUPS / 2u)
         return tooMany(what);
-    switch(kernel)
+    switch(c.kernel)
     {
     case Kernel::DOTS:
         if(a.rows == 1u)
-            f16 ? launchDots<_Float16, 1>(p, s) : launchDots<__bf16, 1>(p, s);
+            f16 ? launchDots<_Float16, 1>(c.p, s) : launchDots<__bf16, 1>(c.p, s);
         else
-            f16 ? launchDots<_Float16, 2>(p, s) : launchDots<__bf16, 2>(p, s);
+            f16 ? launchDots<_Float16, 2>(c.p, s) : launchDots<__bf16, 2>(c.p, s);
         break;
-    case Kernel::FEW: f16 ? launchFew<_Float16>(p, s) : launchFew<__bf16>(p, s); break;
+    case Kernel::FEW: f16 ? launchFew<_Float16>(c.p, s) : launchFew<__bf16>(c.p, s); break;
     default:
-    {
-        const uint64_t room = usable(a.workspace, a.workspace_bytes);
-        const Plan     plan = planOf(p, true, !even, room);
-        if(!even)
-        {
-            LinearParams q      = p;
-            const Copies copies = evened(a, a.workspace, q);
-            if(copies.fit(room))
-                if(const Plan other = planOf(q, true, false, room - copies.bytes); other.us + copies.us < plan.us)
-                {
-                    copies.launch(a.workspace, s);
-                    R355_TRY(launchTiles(a.in_type, q, true, true, false, other, static_cast<char*>(a.workspace) + copies.bytes, room - copies.bytes, s, what));
-                    break;
-                }
-        }
-        R355_TRY(launchTiles(a.in_type, p, true, true, !even, plan, a.workspace, a.workspace_bytes, s, what));
-    }
+        c.copies.launch(a.workspace, s);
+        R355_TRY(launchTiles(a.in_type, c.p, true, true, c.any, c.plan, static_cast<char*>(a.workspace) + c.copies.bytes, room - c.copies.bytes, s, what));
     }
     return r355::checkLaunch(what);
 }
 
+extern "C" int r355_linear_launch_plan(const r355_linear_args* args, r355_linear_plan* plan)
+{
+    if(!args || !plan)
+        return r355::fail(R355_ERR_BAD_ARG, "linear_launch_plan: null arguments");
+    R355_TRY(checkForward(*args));
+    *plan = r355_linear_plan{};
+    if(args->rows == 0)
+        return R355_OK;
+    const ForwardChoice c = chooseForward(*args, args->workspace, usable(args->workspace, args->workspace_bytes));
+    *plan                 = reported(c.kernel, c.any, c.plan, c.copies);
+    return R355_OK;
+}
+
 extern "C" size_t r355_linear_workspace_bytes(const r355_linear_args* args)
 {
-    if(!args || args->rows == 0 || args->n == 0 || args->k == 0 || args->groups == 0 || kernelOf(*args, evenForward(*args), ~0ull) != Kernel::TILES)
+    if(!args || args->rows == 0 || args->n == 0 || args->k == 0 || args->groups == 0)
         return 0;
-    const LinearParams p    = forwardParams(*args);
-    const bool         even = evenForward(*args);
-    if(!even)
-    {
-        LinearParams q      = p;
-        const Copies copies = evened(*args, nullptr, q);
-        if(copies.fit(~0ull) && planOf(q, true, false, ~0ull).us + copies.us < planOf(p, true, true, ~0ull).us)
-            return static_cast<size_t>(copies.bytes) + splitBytes(q, true, false);
-    }
-    return splitBytes(p, true, !even);
+    const ForwardChoice c = chooseForward(*args, nullptr, ~0ull);
+    return c.kernel == Kernel::TILES ? static_cast<size_t>(c.copies.bytes) + splitBytes(c.p, true, c.any) : 0u;
 }
 
 extern "C" size_t r355_linear_backward_workspace_bytes(const r355_linear_backward_args* args)
@@ -1192,23 +1285,25 @@ extern "C" size_t r355_linear_backward_workspace_bytes(const r355_linear_backwar
     if(a.dbias)
         if(const uint64_t parts = gradParts(a, static_cast<uint32_t>(tilesOf(a.n, 512u))); parts > 1u)
             most = static_cast<size_t>(parts * a.groups * a.n * 4u);
-    const bool     element = a.activation != R355_ACT_NONE || a.gate;
-    const char*    dz      = static_cast<const char*>(element ? a.dz : a.dy);
-    const uint32_t lddz    = element ? a.lddz : a.lddy;
-    const bool         wantX = a.dx != nullptr, wantW = a.dw != nullptr, anyX = wantX && !evenInput(a, dz, lddz), anyW = wantW && !evenWeight(a, dz, lddz);
-    const LinearParams px = inputParams(a, dz, lddz), pw = weightParams(a, dz, lddz);
-    const BackwardPlan plan  = planBackward(px, pw, wantX, wantW, anyX, anyW, ~0ull);
-    size_t             bytes = backwardBytes(plan, px, pw, wantX, wantW, anyX, anyW);
-    if(anyX || anyW)
+    const BackwardChoice c     = chooseBackward(a, nullptr, ~0ull);
+    const size_t         bytes = static_cast<size_t>(c.copies.bytes) + backwardBytes(c.plan, c.px, c.pw, c.wantX, c.wantW, c.anyX, c.anyW);
+    return most > bytes ? most : bytes;
+}
+
+extern "C" int r355_linear_backward_launch_plan(const r355_linear_backward_args* args, r355_linear_plan* dx, r355_linear_plan* dw)
+{
+    if(!args || !dx || !dw)
+        return r355::fail(R355_ERR_BAD_ARG, "linear_backward_launch_plan: null arguments");
+    R355_TRY(checkBackward(*args));
+    const BackwardChoice c = chooseBackward(*args, args->workspace, usable(args->workspace, args->workspace_bytes));
+    *dx = c.wantX ? reported(Kernel::TILES, c.anyX, c.plan.x, c.copies) : r355_linear_plan{};
+    *dw = c.wantW ? reported(Kernel::TILES, c.anyW, c.plan.w, c.copies) : r355_linear_plan{};
+    if(c.plan.together)
     {
-        LinearParams       x = px, w = pw;
-        const Copies       copies = evened(a, dz, lddz, wantX, wantW, nullptr, x, w);
-        const BackwardPlan other  = planBackward(x, w, wantX, wantW, false, false, ~0ull);
-        if(copies.fit(~0ull) && other.us + copies.us < plan.us)
-            bytes = static_cast<size_t>(copies.bytes) + backwardBytes(other, x, w, wantX, wantW, false, false);
+        dx->tile_rows = dx->tile_cols = dw->tile_rows = dw->tile_cols = 64u, dx->first_rows = 0u, dx->together = dw->together = 1u;
+        dx->splits = c.plan.both.splitsX, dw->splits = c.plan.both.splitsW;
     }
-    most = most > bytes ? most : bytes;
-    return most;
+    return R355_OK;
 }
 
 extern "C" int r355_linear_backward(const r355_linear_backward_args* args, void* stream)
@@ -1217,41 +1312,17 @@ extern "C" int r355_linear_backward(const r355_linear_backward_args* args, void*
     if(!args)
         return r355::fail(R355_ERR_BAD_ARG, "linear_backward: null arguments");
     const r355_linear_backward_args& a = *args;
-    R355_TRY(checkCommon(what, a.in_type, a.activation, a.rows, a.n, a.k, a.groups, a.offsets));
-    if(a.grad_type != a.in_type && a.grad_type != R355_F32)
-        return r355::fail(R355_ERR_UNSUPPORTED, "linear_backward: dw has the type of x or is f32");
-    const bool slope = a.activation != R355_ACT_NONE, element = slope || a.gate;
-    if(a.rows != 0 && (!a.dy || (a.dx && !a.w) || (a.dw && !a.x)))
-        return r355::fail(R355_ERR_BAD_ARG, "linear_backward: null pointer");
-    if(a.rows != 0 && slope && !a.z)
-        return r355::fail(R355_ERR_BAD_ARG, "linear_backward: an activation's gradient needs z");
-    if(a.dgate && (!a.gate || !a.z))
-        return r355::fail(R355_ERR_BAD_ARG, "linear_backward: dgate needs gate and z");
-    if(element && !a.dz)
-        return r355::fail(R355_ERR_BAD_ARG, "linear_backward: with an activation or a gate dz is needed");
-    const uint32_t gradBytes = r355::dtypeBytes(a.grad_type);
-    R355_TRY(checkMatrix(what, "dy", a.dy, a.lddy, a.n, 2));
-    R355_TRY(checkMatrix(what, "x", a.x, a.ldx, a.k, 2));
-    R355_TRY(checkMatrix(what, "w", a.w, a.ldw, a.k, 2));
-    R355_TRY(checkMatrix(what, "z", a.z, a.ldz, a.n, 2));
-    R355_TRY(checkMatrix(what, "gate", a.gate, a.ldg, a.n, 2));
-    R355_TRY(checkMatrix(what, "dz", element ? a.dz : nullptr, a.lddz, a.n, 2));
-    R355_TRY(checkMatrix(what, "dgate", a.dgate, a.lddg, a.n, 2));
-    R355_TRY(checkMatrix(what, "dx", a.dx, a.lddx, a.k, 2));
-    R355_TRY(checkMatrix(what, "dw", a.dw, a.lddw, a.k, gradBytes));
-    R355_TRY(checkMatrix(what, "dbias", a.dbias, a.n, a.n, 4));
-    if(a.dx)
-        R355_TRY(checkStride(what, "w_stride", a.w_stride, a.groups, (uint64_t)(a.n - 1u) * a.ldw + a.k));
-    if(a.dw)
-        R355_TRY(checkStride(what, "dw_stride", a.dw_stride, a.groups, (uint64_t)(a.n - 1u) * a.lddw + a.k));
-    const hipStream_t s = static_cast<hipStream_t>(stream);
+    R355_TRY(checkBackward(a));
+    uint64_t             room = usable(a.workspace, a.workspace_bytes);
+    const BackwardChoice c    = chooseBackward(a, a.workspace, room);
+    const hipStream_t    s    = static_cast<hipStream_t>(stream);
     r355::beginCall();
 
-    if(element || a.dbias)
+    if(c.element || a.dbias)
     {
         GradParams g{};
         g.dy = static_cast<const char*>(a.dy), g.z = static_cast<const char*>(a.z), g.gate = static_cast<const char*>(a.gate);
-        g.dz = element ? static_cast<char*>(a.dz) : nullptr, g.dgate = static_cast<char*>(a.dgate), g.offsets = a.offsets;
+        g.dz = c.element ? static_cast<char*>(a.dz) : nullptr, g.dgate = static_cast<char*>(a.dgate), g.offsets = a.offsets;
         g.rows = a.rows, g.n = a.n, g.groups = a.groups, g.lddy = a.lddy, g.ldz = a.ldz, g.ldg = a.ldg, g.lddz = a.lddz, g.lddg = a.lddg;
         g.activation = a.activation, g.accumulate = a.accumulate;
         const bool     wide   = a.n % 8u == 0u && evenRows(a.dy, a.lddy, 2) && evenRows(a.z, a.ldz, 2) && evenRows(a.gate, a.ldg, 2) && evenRows(g.dz, a.lddz, 2) && evenRows(a.dgate, a.lddg, 2);
@@ -1269,44 +1340,27 @@ extern "C" int r355_linear_backward(const r355_linear_backward_args* args, void*
             hipLaunchKernelGGL(linearGradSums, dim3(static_cast<uint32_t>(tilesOf(a.n, 64u)), a.groups), block, 0, s, static_cast<const float*>(a.workspace), a.dbias, g.parts, a.n,
                                a.accumulate);
     }
-    const char*    dz   = static_cast<const char*>(element ? a.dz : a.dy);
-    const uint32_t lddz = element ? a.lddz : a.lddy;
-    const bool     wantX = a.dx && a.rows, wantW = a.dw != nullptr;
-    bool           anyX = wantX && !evenInput(a, dz, lddz), anyW = wantW && !evenWeight(a, dz, lddz);
-    LinearParams   px = inputParams(a, dz, lddz), pw = weightParams(a, dz, lddz);
-    uint64_t       room = usable(a.workspace, a.workspace_bytes);
-    char*          work = static_cast<char*>(a.workspace);
-    BackwardPlan   plan = planBackward(px, pw, wantX, wantW, anyX, anyW, room);
-    if((anyX || anyW) && a.rows)
+    char* work = static_cast<char*>(a.workspace);
+    c.copies.launch(work, s);
+    work += c.copies.bytes, room -= c.copies.bytes;
+    if(c.plan.together)
     {
-        LinearParams x = px, w = pw;
-        const Copies copies = evened(a, dz, lddz, wantX, wantW, work, x, w);
-        if(copies.fit(room))
-            if(const BackwardPlan other = planBackward(x, w, wantX, wantW, false, false, room - copies.bytes); other.us + copies.us < plan.us)
-            {
-                copies.launch(work, s);
-                px = x, pw = w, plan = other, anyX = anyW = false;
-                work += copies.bytes, room -= copies.bytes;
-            }
-    }
-    if(plan.together)
-    {
-        const PlanBoth& both  = plan.both;
-        const uint64_t  sumsX = sumsBytes(px, true, both.splitsX);
-        LinearParams    x = both.splitsX > 1u ? sharesOf(px, true, both.splitsX, work) : px, w = both.splitsW > 1u ? sharesOf(pw, false, both.splitsW, work + sumsX) : pw;
+        const PlanBoth& both  = c.plan.both;
+        const uint64_t  sumsX = sumsBytes(c.px, true, both.splitsX);
+        LinearParams    x = both.splitsX > 1u ? sharesOf(c.px, true, both.splitsX, work) : c.px, w = both.splitsW > 1u ? sharesOf(c.pw, false, both.splitsW, work + sumsX) : c.pw;
         const uint64_t  workgroupsX = tilesOfLaunch(x, true, r355::TILE_64), workgroupsW = tilesOfLaunch(w, false, r355::TILE_64);
         if(workgroupsX * both.splitsX + workgroupsW * both.splitsW > r355::MAX_GROUPS)
             return tooMany(what);
         (a.in_type == R355_F16 ? r355::linearBothF16 : r355::linearBothBF16)(x, w, static_cast<uint32_t>(workgroupsX), static_cast<uint32_t>(workgroupsW), s);
         if(both.splitsX > 1u)
-            launchReduce(a.in_type, px, true, both.splitsX, work, s);
+            launchReduce(a.in_type, c.px, true, both.splitsX, work, s);
         if(both.splitsW > 1u)
-            launchReduce(a.in_type, pw, false, both.splitsW, work + sumsX, s);
+            launchReduce(a.in_type, c.pw, false, both.splitsW, work + sumsX, s);
         return r355::checkLaunch(what);
     }
-    if(wantX)
-        R355_TRY(launchTiles(a.in_type, px, true, false, anyX, plan.x, work, room, s, what));
-    if(wantW)
-        R355_TRY(launchTiles(a.in_type, pw, false, false, anyW, plan.w, work, room, s, what));
+    if(c.wantX)
+        R355_TRY(launchTiles(a.in_type, c.px, true, false, c.anyX, c.plan.x, work, room, s, what));
+    if(c.wantW)
+        R355_TRY(launchTiles(a.in_type, c.pw, false, false, c.anyW, c.plan.w, work, room, s, what));
     return r355::checkLaunch(what);
 }
