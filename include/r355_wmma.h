@@ -401,7 +401,8 @@ typedef enum
  * groups = 1, offsets = NULL: one matrix of weights.  Otherwise rows offsets[e] .. offsets[e + 1] - 1 use weights and bias of group e; offsets is device memory, not read by the host;
  * rows in no group are left as they were, and what offsets holds beyond the rows is cut off.  (A slice of the offsets with w from its first group on: some of the experts.)
  * source (device memory, or NULL): row r is row source[r] of x, which has x_rows of them; a number that is none of them reads as zeros.
- * c may be y (of the same leading dimension); any other overlap of y or z with what is read is undefined.  Any sizes up to 2^30 rows, n and k of 2^22 - 8 and 1024 groups; any leading dimension and alignment of an element, fastest (several times) with rows of x and w on
+ * c may be y (of the same leading dimension); any other overlap of y or z with what is read is undefined.  Any sizes up to 2^30 rows, n and k of 2^22 - 8 and 1024 groups
+ * as far as fewer than 2^24 tiles cover the result, of 256 x 256, or of 64 x 64 where operands are not on 16-byte boundaries (more are refused); any leading dimension and alignment of an element, fastest (several times) with rows of x and w on
  * 16-byte boundaries and k a multiple of 8; then with n a multiple of 8 and the other rows on 16-byte boundaries.  With source, x_rows times ldx up to 2^31 bytes.
  * workspace (16-byte aligned, contents irrelevant): with it the sum is split over workgroups where the result has few tiles, and operands off 16-byte boundaries are laid out evenly
  * first where that pays; r355_linear_workspace_bytes says how much is made use of.

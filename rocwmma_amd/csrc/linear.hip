@@ -630,6 +630,14 @@ namespace
         return most < p.rows ? most : p.rows;
     }
 
+    // Workgroups of a product on macro tiles (of a share of the sum): every XCD has as many
+    uint64_t workgroupsOf(const LinearParams& p, bool aK, uint32_t tile)
+    {
+        const uint64_t across = tilesOf(p.n, r355::LINEAR_COLS[tile]);
+        // (of a weights' gradient: an eighth of a group's tiles for each XCD may be a tile more)
+        return aK ? tilesOf(mostTiles(p, r355::LINEAR_ROWS[tile]) * across, 8u) * 8u : tilesOf(tilesOf(p.m, r355::LINEAR_ROWS[tile]) * across, 8u) * 8u * p.groups;
+    }
+
     // How a product on macro tiles is launched: `splits` workgroups along the sum; the first `tall` rows alone where the rest goes out by a plan of its own.
     struct Plan
     {
@@ -677,7 +685,9 @@ namespace
         return (n + 3u) / 4u * 4u;
     }
 
-    // The plan that takes the least by launchTime(), with as many splits as the workspace holds.
+    constexpr double NEVER = 1e30; // us of a plan that there is none of
+
+    // The plan that takes the least by launchTime() of those that a launch holds (none: NEVER), with as many splits as the workspace holds.
     Plan planOf(const LinearParams& p, bool aK, bool any, uint64_t workspaceBytes)
     {
         using namespace r355;
@@ -697,9 +707,11 @@ namespace
         const double sums = aK && p.offsets ? 10.0 : 5.0;
         // (the largest tile is as high as its rows, by quarters: of groups with few rows a quarter high, which takes half the time)
         const double rowsMet = aK && p.offsets ? static_cast<double>(p.rows) / (p.groups < p.rows ? p.groups : p.rows) : 256.0, height = rowsMet < 40.0 ? 0.5 : rowsMet < 80.0 ? 0.75 : 1.0;
-        Plan         best{any ? TILE_ANY : TILE_64, 1u, 0u, 1e30};
+        Plan         best{any ? TILE_ANY : TILE_64, 1u, 0u, NEVER};
         for(uint32_t tile = any ? TILE_ANY : TILE_256; tile < (any ? LINEAR_TILES : TILE_ANY); ++tile)
         {
+            if(workgroupsOf(p, aK, tile) > MAX_GROUPS)
+                continue;
             // (each group that is met has a tile, whatever part of it is there)
             const double all = tiles(tile, p.rows), least = aK && p.offsets ? static_cast<double>(p.groups < p.rows ? p.groups : p.rows) * static_cast<double>(tilesOf(p.n, LINEAR_COLS[tile])) : 0.0,
                          there = all > least ? all : least;
@@ -775,26 +787,20 @@ namespace
     }
 
     // The tiles of a launch: sets them in p, returns the workgroups
-    uint64_t tilesOfLaunch(LinearParams& p, bool aK, r355::LinearTile tile)
+    uint32_t tilesOfLaunch(LinearParams& p, bool aK, r355::LinearTile tile)
     {
         // (shares of a split sum are read again at once)
         p.linesY = p.splits == 1u && lines(p.y, p.ldy, p.outF32 ? 4u : 2u), p.linesZ = lines(p.z, p.ldz, 2u);
-        const uint32_t rows = r355::LINEAR_ROWS[tile];
-        p.tilesN = static_cast<uint32_t>(tilesOf(p.n, r355::LINEAR_COLS[tile])), p.tilesM = static_cast<uint32_t>(tilesOf(p.m, rows));
-        // (of a weights' gradient: an eighth of a group's tiles for each XCD may be a tile more)
-        const uint64_t tiles = aK ? mostTiles(p, rows) * p.tilesN : tilesOf((uint64_t)p.tilesM * p.tilesN, 8u) * 8u * p.groups;
-        return (tiles + 7u) / 8u * 8u;
+        p.tilesN = static_cast<uint32_t>(tilesOf(p.n, r355::LINEAR_COLS[tile])), p.tilesM = static_cast<uint32_t>(tilesOf(p.m, r355::LINEAR_ROWS[tile]));
+        return static_cast<uint32_t>(workgroupsOf(p, aK, tile));
     }
-    int launchTile(int32_t type, LinearParams p, bool aK, bool bK, r355::LinearTile tile, hipStream_t s, const char* what)
+    void launchTile(int32_t type, LinearParams p, bool aK, bool bK, r355::LinearTile tile, hipStream_t s)
     {
-        const uint64_t workgroups = tilesOfLaunch(p, aK, tile);
-        if(workgroups > r355::MAX_GROUPS)
-            return tooMany(what);
+        const uint32_t workgroups = tilesOfLaunch(p, aK, tile);
         if(type == R355_F16)
-            r355::linearTilesF16(p, aK, bK, tile, static_cast<uint32_t>(workgroups), s);
+            r355::linearTilesF16(p, aK, bK, tile, workgroups, s);
         else
-            r355::linearTilesBF16(p, aK, bK, tile, static_cast<uint32_t>(workgroups), s);
-        return R355_OK;
+            r355::linearTilesBF16(p, aK, bK, tile, workgroups, s);
     }
 
     uint64_t usable(const void* workspace, uint64_t bytes)
@@ -831,17 +837,15 @@ namespace
     }
 
     // one product on macro tiles, by its plan
-    int launchTiles(int32_t type, const LinearParams& p, bool aK, bool bK, bool any, const Plan& plan, void* workspace, uint64_t workspaceBytes, hipStream_t s, const char* what)
+    void launchTiles(int32_t type, const LinearParams& p, bool aK, bool bK, bool any, const Plan& plan, void* workspace, uint64_t workspaceBytes, hipStream_t s)
     {
         if(plan.splits > 1u)
         {
-            if(const int rc = launchTile(type, sharesOf(p, aK, plan.splits, workspace), aK, bK, plan.tile, s, what))
-                return rc;
-            launchReduce(type, p, aK, plan.splits, workspace, s);
-            return R355_OK;
+            launchTile(type, sharesOf(p, aK, plan.splits, workspace), aK, bK, plan.tile, s);
+            return launchReduce(type, p, aK, plan.splits, workspace, s);
         }
         if(plan.tall == 0u)
-            return launchTile(type, p, aK, bK, plan.tile, s, what);
+            return launchTile(type, p, aK, bK, plan.tile, s);
         LinearParams first = p, rest = p;
         first.rows = plan.tall, rest.rows = p.rows - plan.tall;
         const uint64_t outBytes = p.outF32 ? 4u : 2u, by = plan.tall;
@@ -851,9 +855,8 @@ namespace
             rest.a += by * p.lda * 2u;
         rest.y += by * p.ldy * outBytes;
         rest.c = p.c ? p.c + by * p.ldc * outBytes : nullptr, rest.gate = p.gate ? p.gate + by * p.ldg * 2u : nullptr, rest.z = p.z ? p.z + by * p.ldz * 2u : nullptr;
-        if(const int rc = launchTile(type, first, aK, bK, plan.tile, s, what))
-            return rc;
-        return launchTiles(type, rest, aK, bK, any, planOf(rest, aK, any, usable(workspace, workspaceBytes)), workspace, workspaceBytes, s, what);
+        launchTile(type, first, aK, bK, plan.tile, s);
+        launchTiles(type, rest, aK, bK, any, planOf(rest, aK, any, usable(workspace, workspaceBytes)), workspace, workspaceBytes, s);
     }
 
     // Both gradients in one launch of small tiles: how their sums are split, and what it takes (as launchTime(), with tiles of two lengths).
@@ -871,12 +874,13 @@ namespace
         const double     met = px.groups < px.rows ? px.groups : px.rows;
         const double     tilesX = (px.offsets ? px.rows / 64.0 + 0.5 * met : static_cast<double>(tilesOf(px.rows, 64u))) * static_cast<double>(tilesOf(px.n, 64u));
         const double     tilesW = static_cast<double>(tilesOf(pw.m, 64u) * tilesOf(pw.n, 64u)) * pw.groups;
-        PlanBoth         best{1u, 1u, 1e30};
+        PlanBoth         best{1u, 1u, NEVER};
+        const uint64_t   workgroupsX = workgroupsOf(px, true, TILE_64), workgroupsW = workgroupsOf(pw, false, TILE_64);
         auto reduced = [](const LinearParams& p, bool aK, uint32_t splits) { return splits > 1u ? 5.0 + static_cast<double>(rowsOfResult(p, aK)) * p.n * 4.0 * (2u * splits + 1u) / 5e6 : 0.0; };
         for(uint32_t sx = 1u; sx <= 16u && (sx == 1u || (stagesX >= 4.0 * sx && tilesX <= cus)); sx *= 2u)
             for(uint32_t sw = 1u; sw <= 16u && (sw == 1u || (stagesW >= 4.0 * sw && tilesW <= cus)); sw *= 2u)
             {
-                if(sumsBytes(px, true, sx) + sumsBytes(pw, false, sw) > workspaceBytes)
+                if(sumsBytes(px, true, sx) + sumsBytes(pw, false, sw) > workspaceBytes || workgroupsX * sx + workgroupsW * sw > MAX_GROUPS)
                     continue;
                 const double nx = tilesX * sx, nw = tilesW * sw, lx = stagesX / sx, lw = stagesW / sw, n = nx + nw, longer = lx > lw ? nx : nw, shorter = lx < lw ? lx : lw, rest = (lx > lw ? lx : lw) - shorter;
                 auto         stage = [&](double tiles) { return t.stage[tiles > 3.0 * cus ? 3u : tiles > 2.0 * cus ? 2u : tiles > cus ? 1u : 0u]; };
@@ -960,14 +964,17 @@ namespace
     };
     Kernel kernelOf(const r355_linear_args& a, bool even, uint64_t room)
     {
+        const LinearParams p = forwardParams(a);
+        // (both have a workgroup of up to 512 threads for 16 columns of one row and more, of 16 rows and less: as many for every XCD as a launch holds)
+        auto held = [&](uint32_t rows) { return tilesOf(mostTiles(p, rows) * tilesOf(p.n, 16u), 8u) * 8u <= r355::MAX_GROUPS / 2u; };
         if(!even)
             return Kernel::TILES;
         if(a.groups == 1u)
-            return a.rows <= 2u ? Kernel::DOTS : a.rows <= 16u ? Kernel::FEW : Kernel::TILES;
-        if(a.rows <= a.groups)
+            return a.rows <= 2u ? Kernel::DOTS : a.rows <= 16u ? Kernel::FEW : Kernel::TILES; // (of 2^22 columns a launch holds them)
+        if(a.rows <= a.groups && held(1u))
             return Kernel::DOTS;
         const double few = 4.0 + static_cast<double>(a.groups) * a.n * a.k * 2.0 / 5.7e6 * (1.0 + 0.05 * a.rows / a.groups);
-        return a.rows / a.groups < 9u && few < planOf(forwardParams(a), true, false, room).us ? Kernel::FEW : Kernel::TILES;
+        return a.rows / a.groups < 9u && held(16u) && few < planOf(p, true, false, room).us ? Kernel::FEW : Kernel::TILES;
     }
     LinearParams inputParams(const r355_linear_backward_args& a, const char* dz, uint32_t lddz)
     {
@@ -1106,6 +1113,11 @@ namespace
         LinearParams p;
         Plan         plan; // TILES
         Copies       copies;
+
+        bool held() const // whether there are launches of as many tiles
+        {
+            return kernel != Kernel::TILES || plan.us < NEVER;
+        }
     };
     ForwardChoice chooseForward(const r355_linear_args& a, const void* workspace, uint64_t room)
     {
@@ -1131,6 +1143,11 @@ namespace
         LinearParams px, pw;
         BackwardPlan plan;
         Copies       copies;
+
+        bool held() const
+        {
+            return plan.us < NEVER;
+        }
     };
     BackwardChoice chooseBackward(const r355_linear_backward_args& a, const void* workspace, uint64_t room)
     {
@@ -1236,9 +1253,9 @@ extern "C" int r355_linear(const r355_linear_args* args, void* stream)
     const ForwardChoice c    = chooseForward(a, a.workspace, room);
     const hipStream_t   s    = static_cast<hipStream_t>(stream);
     const bool          f16  = a.in_type == R355_F16;
-    r355::beginCall();
-    if(c.kernel != Kernel::TILES && mostTiles(c.p, c.kernel == Kernel::DOTS ? 1u : 16u) * tilesOf(c.p.n, 16u) > r355::MAX_GROUPS / 2u)
+    if(!c.held())
         return tooMany(what);
+    r355::beginCall();
     switch(c.kernel)
     {
     case Kernel::DOTS:
@@ -1250,7 +1267,7 @@ extern "C" int r355_linear(const r355_linear_args* args, void* stream)
     case Kernel::FEW: f16 ? launchFew<_Float16>(c.p, s) : launchFew<__bf16>(c.p, s); break;
     default:
         c.copies.launch(a.workspace, s);
-        R355_TRY(launchTiles(a.in_type, c.p, true, true, c.any, c.plan, static_cast<char*>(a.workspace) + c.copies.bytes, room - c.copies.bytes, s, what));
+        launchTiles(a.in_type, c.p, true, true, c.any, c.plan, static_cast<char*>(a.workspace) + c.copies.bytes, room - c.copies.bytes, s);
     }
     return r355::checkLaunch(what);
 }
@@ -1264,7 +1281,9 @@ extern "C" int r355_linear_launch_plan(const r355_linear_args* args, r355_linear
     if(args->rows == 0)
         return R355_OK;
     const ForwardChoice c = chooseForward(*args, args->workspace, usable(args->workspace, args->workspace_bytes));
-    *plan                 = reported(c.kernel, c.any, c.plan, c.copies);
+    if(!c.held())
+        return tooMany("linear");
+    *plan = reported(c.kernel, c.any, c.plan, c.copies);
     return R355_OK;
 }
 
@@ -1296,6 +1315,8 @@ extern "C" int r355_linear_backward_launch_plan(const r355_linear_backward_args*
         return r355::fail(R355_ERR_BAD_ARG, "linear_backward_launch_plan: null arguments");
     R355_TRY(checkBackward(*args));
     const BackwardChoice c = chooseBackward(*args, args->workspace, usable(args->workspace, args->workspace_bytes));
+    if(!c.held())
+        return tooMany("linear_backward");
     *dx = c.wantX ? reported(Kernel::TILES, c.anyX, c.plan.x, c.copies) : r355_linear_plan{};
     *dw = c.wantW ? reported(Kernel::TILES, c.anyW, c.plan.w, c.copies) : r355_linear_plan{};
     if(c.plan.together)
@@ -1316,6 +1337,8 @@ extern "C" int r355_linear_backward(const r355_linear_backward_args* args, void*
     uint64_t             room = usable(a.workspace, a.workspace_bytes);
     const BackwardChoice c    = chooseBackward(a, a.workspace, room);
     const hipStream_t    s    = static_cast<hipStream_t>(stream);
+    if(!c.held())
+        return tooMany(what);
     r355::beginCall();
 
     if(c.element || a.dbias)
@@ -1348,10 +1371,8 @@ extern "C" int r355_linear_backward(const r355_linear_backward_args* args, void*
         const PlanBoth& both  = c.plan.both;
         const uint64_t  sumsX = sumsBytes(c.px, true, both.splitsX);
         LinearParams    x = both.splitsX > 1u ? sharesOf(c.px, true, both.splitsX, work) : c.px, w = both.splitsW > 1u ? sharesOf(c.pw, false, both.splitsW, work + sumsX) : c.pw;
-        const uint64_t  workgroupsX = tilesOfLaunch(x, true, r355::TILE_64), workgroupsW = tilesOfLaunch(w, false, r355::TILE_64);
-        if(workgroupsX * both.splitsX + workgroupsW * both.splitsW > r355::MAX_GROUPS)
-            return tooMany(what);
-        (a.in_type == R355_F16 ? r355::linearBothF16 : r355::linearBothBF16)(x, w, static_cast<uint32_t>(workgroupsX), static_cast<uint32_t>(workgroupsW), s);
+        const uint32_t  workgroupsX = tilesOfLaunch(x, true, r355::TILE_64), workgroupsW = tilesOfLaunch(w, false, r355::TILE_64);
+        (a.in_type == R355_F16 ? r355::linearBothF16 : r355::linearBothBF16)(x, w, workgroupsX, workgroupsW, s);
         if(both.splitsX > 1u)
             launchReduce(a.in_type, c.px, true, both.splitsX, work, s);
         if(both.splitsW > 1u)
@@ -1359,8 +1380,8 @@ extern "C" int r355_linear_backward(const r355_linear_backward_args* args, void*
         return r355::checkLaunch(what);
     }
     if(c.wantX)
-        R355_TRY(launchTiles(a.in_type, c.px, true, false, c.anyX, c.plan.x, work, room, s, what));
+        launchTiles(a.in_type, c.px, true, false, c.anyX, c.plan.x, work, room, s);
     if(c.wantW)
-        R355_TRY(launchTiles(a.in_type, c.pw, false, false, c.anyW, c.plan.w, work, room, s, what));
+        launchTiles(a.in_type, c.pw, false, false, c.anyW, c.plan.w, work, room, s);
     return r355::checkLaunch(what);
 }
