@@ -482,7 +482,8 @@ int    r355_linear_backward_launch_plan(const r355_linear_backward_args* args, r
 
 /*
  * The router: for each token the `top` experts of the largest logit (plus bias [experts], where given: in f32, for the choice alone), the lowest expert of equal ones first, NaN behind
- * every number.  weights [tokens][top]: softmax or sigmoid of the logits, over the chosen ones alone with chosen_only (their sum is then `scale`), times scale; an
+ * every number.  With R355_ROUTE_SCORE_BIAS and a bias: those of the largest score plus bias, the score (sigmoid of the logit, or its softmax over all experts) and the sum in f32: the bias
+ * that evens out the experts' load where it is learned beside scores; scores that f32 does not tell apart are equal.  weights [tokens][top]: softmax or sigmoid of the logits, over the chosen ones alone with chosen_only (their sum is then `scale`), times scale; an
  * expert at -infinity has weight 0.  The rows of the experts' products are the tokens' choices in order of (expert, token, choice): chosen [tokens][top], place [tokens][top]
  * (the row of a choice), source [tokens * top] (the token of a row), offsets [experts + 1] (an expert's first row).  logits: R355_F16, R355_BF16 or R355_F32, rows ldl elements apart.
  * Up to 1024 experts, 32 choices and 2^30 rows.  workspace (16-byte aligned, contents irrelevant): r355_route_workspace_bytes are needed, 0 for a few tokens, never less for more of them.  Calls that overlap need one each.
@@ -490,7 +491,8 @@ int    r355_linear_backward_launch_plan(const r355_linear_backward_args* args, r
 typedef enum
 {
     R355_ROUTE_SOFTMAX = 0,
-    R355_ROUTE_SIGMOID = 1
+    R355_ROUTE_SIGMOID = 1,
+    R355_ROUTE_SCORE_BIAS = 256 /* with either: the bias is added to the score, not to the logit */
 } r355_route_score;
 typedef struct
 {
@@ -510,7 +512,7 @@ typedef struct
 int    r355_route(const r355_route_args* args, void* stream);
 size_t r355_route_workspace_bytes(uint32_t tokens, uint32_t experts, uint32_t top);
 
-/* dlogits [tokens][experts] for dweights [tokens][top] of the experts chosen, score, chosen_only and scale as in r355_route; every element is written.  A number
+/* dlogits [tokens][experts] for dweights [tokens][top] of the experts chosen, score, chosen_only and scale as in r355_route (a bias has no part in it); every element is written.  A number
  * in chosen that is no expert's is left out; one that is there twice counts twice. */
 typedef struct
 {

@@ -34,7 +34,7 @@ ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = range(5)
 # r355_linear_kernel
 LINEAR_NONE, LINEAR_DOTS, LINEAR_FEW, LINEAR_TILES, LINEAR_ELEMENTS = range(5)
 # r355_route_score
-ROUTE_SOFTMAX, ROUTE_SIGMOID = 0, 1
+ROUTE_SOFTMAX, ROUTE_SIGMOID, ROUTE_SCORE_BIAS = 0, 1, 256
 
 DTYPE_BYTES = {F16: 2, BF16: 2, E4M3: 1, I8: 1, F32: 4, I32: 4, F64: 8, E5M2: 1}
 
@@ -733,7 +733,7 @@ def route_workspace_bytes(tokens, experts, top):
 
 def route(dtype, tokens, experts, top, logits, weights, chosen, place, source, offsets, score=ROUTE_SOFTMAX, chosen_only=False, scale=1.0, bias=None, ldl=None, workspace=None,
           workspace_bytes=None, stream=None):
-    """The `top` experts of each token by logits [tokens][experts] (plus bias, for the choice), their weights, and the rows in order of experts (include/r355_wmma.h): chosen, place
+    """The `top` experts of each token by logits [tokens][experts] (plus bias, for the choice; score=ROUTE_SIGMOID | ROUTE_SCORE_BIAS: by scores plus bias), their weights, and the rows in order of experts (include/r355_wmma.h): chosen, place
     [tokens][top], source [tokens * top], offsets [experts + 1], what linear(), dispatch() and combine() take."""
     slots = tokens * top
     a = _ROUTE_ARGS.pack(dtype, score, chosen_only, tokens, experts, top, experts if ldl is None else ldl, 0, _ptr(logits) or 0, _floats("route: bias", bias, experts) or 0,

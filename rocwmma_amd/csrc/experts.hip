@@ -1,6 +1,6 @@
 // The router of a layer with experts, and the rows' way to the experts and back, with the gradients of both.  No counterpart in the reference.
 //
-//   route      the `top` experts of each token by logit (plus bias), their weights, and the rows in order of experts: place[t][j], source[row], offsets[e]
+//   route      the `top` experts of each token by logit (plus bias) or by score plus bias, their weights, and the rows in order of experts: place[t][j], source[row], offsets[e]
 //   combine    y_t = sum_j w_tj rows[place_tj] + c_t
 //   dispatch   rows[place_tj] = w_tj x_t;  dw_tj = x_t . values[place_tj]      (the gradient of combine; without weights that of its own, and the way to the experts)
 #include <hip/hip_runtime.h>
@@ -65,6 +65,7 @@ namespace
         char*          dlogits;
         uint32_t       tokens, experts, top, ldl, ldd, blocks, perBlock;
         int32_t        score, chosenOnly, even; // even: rows of logits on the boundaries of what a lane reads of them
+        int32_t        scoreBias; // the bias is added to the score, otherwise to the logit
         float          scale;
     };
 
@@ -82,6 +83,21 @@ namespace
     __device__ __forceinline__ float exponentials(float v, bool in, float most)
     {
         return in ? __expf(v - (most == -INFINITY ? 0.0f : most)) : 0.0f;
+    }
+
+    // the largest of a token's logits, and the sum of the exponentials
+    template <uint32_t V>
+    __device__ __forceinline__ void ofAll(const RouteParams& p, const float (&x)[V], uint32_t lane, float& most, float& all)
+    {
+        most = -INFINITY, all = 0.0f;
+#pragma unroll
+        for(uint32_t i = 0; i < V; ++i)
+            most = fmaxf(most, lane * V + i < p.experts ? x[i] : -INFINITY);
+        most = largest(most);
+#pragma unroll
+        for(uint32_t i = 0; i < V; ++i)
+            all += exponentials(x[i], lane * V + i < p.experts, most);
+        all = sum(all);
     }
 
     __device__ __forceinline__ uint32_t maskOf(bool is)
@@ -121,13 +137,24 @@ namespace
     __device__ __forceinline__ void choose(const RouteParams& p, const float (&x)[V], const Lane<V>& own, uint32_t lane, uint32_t& expert, float& logit)
     {
         uint32_t key[V], of[V]; // keys, and which of the lane's experts they are of
-#pragma unroll
-        for(uint32_t i = 0; i < V; ++i)
+        auto setKey = [&](uint32_t i, float by) __attribute__((always_inline)) {
+            key[i] = either(maskOf(by != by), 1u, orderOf(by)) & own.there[i]; // (-infinity: 0x007FFFFF)
+            of[i]  = i;
+        };
+        if(p.scoreBias) // (uniform)
         {
-            const float by = x[i] + own.bias[i]; // (-0 counts as 0)
-            key[i]         = either(maskOf(by != by), 1u, orderOf(by)) & own.there[i]; // (-infinity: 0x007FFFFF)
-            of[i]          = i;
+            // (divisions: equal logits aside, what a score is off by decides between experts)
+            float most = 0.0f, all = 1.0f;
+            if(p.score != R355_ROUTE_SIGMOID)
+                ofAll<V>(p, x, lane, most, all);
+#pragma unroll
+            for(uint32_t i = 0; i < V; ++i)
+                setKey(i, (p.score == R355_ROUTE_SIGMOID ? 1.0f / (1.0f + __expf(-x[i])) : all == 0.0f ? 0.0f : exponentials(x[i], true, most) / all) + own.bias[i]);
         }
+        else
+#pragma unroll
+            for(uint32_t i = 0; i < V; ++i)
+                setKey(i, x[i] + own.bias[i]); // (-0 counts as 0)
         // (Neighbours change places only if the later one is larger: equal ones stay in the order of their experts.  Choices by masks, one instruction each: of conditions the
         // compiler makes branches and indices, twice as many.)
 #pragma unroll
@@ -175,15 +202,8 @@ namespace
         }
         if(p.score == R355_ROUTE_SIGMOID)
             return p.scale * __builtin_amdgcn_rcpf(1.0f + __expf(-logit));
-        float most = -INFINITY, all = 0.0f;
-#pragma unroll
-        for(uint32_t i = 0; i < V; ++i)
-            most = fmaxf(most, lane * V + i < p.experts ? x[i] : -INFINITY);
-        most = largest(most);
-#pragma unroll
-        for(uint32_t i = 0; i < V; ++i)
-            all += exponentials(x[i], lane * V + i < p.experts, most);
-        all = sum(all);
+        float most, all;
+        ofAll<V>(p, x, lane, most, all);
         return all == 0.0f ? 0.0f : exponentials(logit, in, most) * __builtin_amdgcn_rcpf(all) * p.scale;
     }
 
@@ -451,14 +471,7 @@ namespace
             g = in ? dw * p.scale / (1.0f + __expf(-logit)) : 0.0f;
         else
         {
-#pragma unroll
-            for(uint32_t i = 0; i < V; ++i)
-                most = fmaxf(most, lane * V + i < p.experts ? x[i] : -INFINITY);
-            most = largest(most);
-#pragma unroll
-            for(uint32_t i = 0; i < V; ++i)
-                all += exponentials(x[i], lane * V + i < p.experts, most);
-            all = sum(all);
+            ofAll<V>(p, x, lane, most, all);
             g   = in && all != 0.0f ? dw * p.scale * exponentials(logit, true, most) / all : 0.0f;
             off = all == 0.0f ? 0.0f : sum(g) / all;
         }
@@ -714,11 +727,15 @@ namespace
             launchRouteType<float>(p, gradient, s);
     }
 
+    int32_t scoreOf(int32_t score)
+    {
+        return score & ~R355_ROUTE_SCORE_BIAS;
+    }
     int checkRoute(const char* what, int32_t type, int32_t score, uint32_t tokens, uint32_t experts, uint32_t top, const void* logits, uint32_t ldl)
     {
         if(type != R355_F16 && type != R355_BF16 && type != R355_F32)
             return r355::fail(R355_ERR_UNSUPPORTED, "%s: logits are f16, bf16 or f32", what);
-        if(score != R355_ROUTE_SOFTMAX && score != R355_ROUTE_SIGMOID)
+        if(scoreOf(score) != R355_ROUTE_SOFTMAX && scoreOf(score) != R355_ROUTE_SIGMOID)
             return r355::fail(R355_ERR_BAD_ARG, "%s: unknown score %d", what, score);
         if(experts == 0 || top == 0 || top > experts)
             return r355::fail(R355_ERR_BAD_ARG, "%s: of %u experts %u cannot be chosen", what, experts, top);
@@ -779,7 +796,8 @@ extern "C" int r355_route(const r355_route_args* args, void* stream)
         return r355::fail(R355_ERR_MISALIGNED, "route: the workspace needs 16-byte alignment");
     RouteParams p{};
     p.logits = static_cast<const char*>(a.logits), p.bias = a.bias, p.weights = a.weights, p.chosen = a.chosen, p.place = a.place, p.source = a.source, p.offsets = a.offsets;
-    p.tokens = a.tokens, p.experts = a.experts, p.top = a.top, p.ldl = a.ldl, p.score = a.score, p.chosenOnly = a.chosen_only, p.scale = static_cast<float>(a.scale);
+    p.tokens = a.tokens, p.experts = a.experts, p.top = a.top, p.ldl = a.ldl, p.score = scoreOf(a.score), p.chosenOnly = a.chosen_only, p.scale = static_cast<float>(a.scale);
+    p.scoreBias = a.bias && (a.score & R355_ROUTE_SCORE_BIAS); // (without a bias the order of the scores is that of the logits)
     p.perBlock = need ? tokensPerBlock(a.tokens, a.top) : a.tokens;
     p.blocks   = need ? (a.tokens - 1u) / p.perBlock + 1u : 1u;
     p.counts   = static_cast<uint32_t*>(a.workspace);
@@ -808,7 +826,7 @@ extern "C" int r355_route_backward(const r355_route_backward_args* args, void* s
         return r355::fail(R355_ERR_BAD_SIZE, "route_backward: at most %u tokens, got %u", r355::MAX_GROUPS * WAVES, a.tokens);
     RouteParams p{};
     p.logits = static_cast<const char*>(a.logits), p.given = a.chosen, p.dweights = a.dweights, p.dlogits = static_cast<char*>(a.dlogits);
-    p.tokens = a.tokens, p.experts = a.experts, p.top = a.top, p.ldl = a.ldl, p.ldd = a.ldd, p.score = a.score, p.chosenOnly = a.chosen_only, p.scale = static_cast<float>(a.scale);
+    p.tokens = a.tokens, p.experts = a.experts, p.top = a.top, p.ldl = a.ldl, p.ldd = a.ldd, p.score = scoreOf(a.score), p.chosenOnly = a.chosen_only, p.scale = static_cast<float>(a.scale);
     r355::beginCall();
     launchRouteAny(a.type, p, true, static_cast<hipStream_t>(stream));
     return r355::checkLaunch("route_backward");
