@@ -28,16 +28,17 @@ class ExpertLayer:
         self.router = weights(experts, hidden)
         self.gate, self.up, self.down = weights(experts, width, hidden), weights(experts, width, hidden), weights(experts, hidden, width)
         self.tokens = self.trained = 0
+        self.kept = None  # tokens of the pass whose buffers backward() can take
 
     def reserve(self, tokens, training=False):
-        """The buffers of passes of up to that many tokens, kept for all of them."""
+        """The buffers of passes of up to that many tokens, kept for all of them (a pass that was kept is gone)."""
         import torch
 
         import rocwmma_amd as R
 
         empty = lambda *shape, dtype=self.torch_type: torch.empty(shape, dtype=dtype, device="cuda")  # noqa: E731
         rows, i32, f32 = tokens * self.top, torch.int32, torch.float32
-        self.tokens, self.trained = tokens, tokens if training else 0
+        self.tokens, self.trained, self.kept = tokens, tokens if training else 0, None
         self.logits, self.y = empty(tokens, self.experts), empty(tokens, self.hidden)
         self.weights, self.chosen, self.place = empty(tokens, self.top, dtype=f32), empty(tokens, self.top, dtype=i32), empty(tokens, self.top, dtype=i32)
         self.source, self.offsets = empty(rows, dtype=i32), empty(self.experts + 1, dtype=i32)
@@ -68,11 +69,12 @@ class ExpertLayer:
         return tokens, tokens * self.top
 
     def forward(self, x, keep=False, stream=None):
-        """x [tokens][hidden] -> y.  keep: what backward() needs stays in the buffers (reserved with training=True)."""
+        """x [tokens][hidden] -> y.  keep: what backward() needs stays in the buffers (reserved with training=True) until the next pass."""
         import rocwmma_amd as R
 
         t, e = self.dtype, self.experts
         tokens, rows = self._rows(x, self.trained if keep else self.tokens)
+        self.kept = None  # (every pass writes to the buffers of the last one)
         grouped = dict(groups=e, offsets=self.offsets, workspace=self.workspace, stream=stream)
         R.linear(t, t, tokens, e, self.hidden, x, self.router, self.logits, workspace=self.workspace, stream=stream)
         R.route(t, tokens, e, self.top, self.logits, self.weights, self.chosen, self.place, self.source, self.offsets, score=self.score, chosen_only=True, workspace=self.workspace,
@@ -81,16 +83,21 @@ class ExpertLayer:
         R.linear(t, t, rows, self.width, self.hidden, x, self.gate, self.h, activation=R.ACT_SILU, gate=self.u, z=self.z if keep else None, source=self.source, x_rows=tokens, **grouped)
         R.linear(t, t, rows, self.hidden, self.width, self.h, self.down, self.out, **grouped)
         R.combine(t, tokens, self.top, self.hidden, self.out, rows, self.place, self.y, weights=self.weights, c=x, stream=stream)
+        self.kept = tokens if keep else None
         return self.y[:tokens]
 
     def backward(self, x, dy, stream=None):
-        """dL/dx for dL/dy of the last forward(x, keep=True); the weights' gradients are left in self.gradients."""
+        """dL/dx for dL/dy of the forward(x, keep=True) before it, with no other pass between (of recorded passes a replay is one, which is not seen here); the weights' gradients are left
+        in self.gradients."""
         import rocwmma_amd as R
 
         t, e, g = self.dtype, self.experts, self.gradients
         tokens, rows = self._rows(x, self.trained)
         if dy.shape != x.shape or dy.dtype != x.dtype or not dy.is_contiguous():
             raise ValueError("ExpertLayer: dy must be as x, got %s of %s" % (tuple(dy.shape), dy.dtype))
+        if self.kept != tokens:
+            raise ValueError("ExpertLayer: backward() of %d tokens needs the forward(keep=True) of them just before, %s" % (
+                tokens, "the buffers hold none" if self.kept is None else "it was of %d" % self.kept))
         grouped = dict(groups=e, offsets=self.offsets, workspace=self.workspace, stream=stream)
         R.dispatch(t, tokens, self.top, self.hidden, dy, self.dout, rows, self.place, weights=self.weights, values=self.out, dweights=self.dweights, stream=stream)
         R.dispatch(t, tokens, self.top, self.hidden, x, self.xs, rows, self.place, stream=stream)
