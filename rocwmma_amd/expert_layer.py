@@ -7,6 +7,15 @@ times a forward pass, launched call by call and replayed from a graph, and a for
 import argparse
 
 
+def _on(stream):
+    """torch's own kernels on the stream that a call of the library takes (None: the default stream)"""
+    import torch
+
+    if stream is None:
+        stream = torch.cuda.default_stream()
+    return torch.cuda.stream(stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(stream))
+
+
 class ExpertLayer:
     """y = x + sum over the chosen experts e of w_e (silu(x G_e^T) * (x U_e^T)) D_e^T.  forward() and backward() only launch kernels into the buffers of reserve(), so they
     can be recorded into a graph."""
@@ -50,10 +59,13 @@ class ExpertLayer:
                                                                    offsets=self.offsets if groups > 1 else None)))
         if training:
             self.z, self.xs = empty(rows, self.width), empty(rows, self.hidden)
-            self.dout, self.dxs, self.dxs2 = empty(rows, self.hidden), empty(rows, self.hidden), empty(rows, self.hidden)
+            self.dout = empty(rows, self.hidden)
+            # the parts of dx: the rows of both products and the router's; and which of them are of which token, so that one sum rounds them once
+            self.parts, self.terms = empty(2 * rows + tokens, self.hidden), empty(tokens, 2 * self.top + 1, dtype=i32)
+            self.dxs, self.dxs2, self.dx_router = self.parts[:rows], self.parts[rows: 2 * rows], self.parts[2 * rows:]
+            self.terms[:, -1] = torch.arange(2 * rows, 2 * rows + tokens, dtype=i32, device="cuda")
             self.dh, self.dz, self.du = empty(rows, self.width), empty(rows, self.width), empty(rows, self.width)
             self.dweights, self.dlogits, self.dx = empty(tokens, self.top, dtype=f32), empty(tokens, self.experts), empty(tokens, self.hidden)
-            self.dx_router, self.itself = empty(tokens, self.hidden), torch.arange(tokens, dtype=i32, device="cuda")
             self.gradients = {name: torch.empty_like(getattr(self, name)) for name in ("router", "gate", "up", "down")}
             for n, k, groups, m in ((self.hidden, self.width, self.experts, rows), (self.width, self.hidden, self.experts, rows), (self.experts, self.hidden, 1, tokens)):
                 a = R.linear_backward_args(self.dtype, self.dtype, m, n, k, self.xs, self.xs, self.xs, dx=self.xs, dw=self.xs, groups=groups, offsets=self.offsets if groups > 1 else None)
@@ -89,6 +101,8 @@ class ExpertLayer:
     def backward(self, x, dy, stream=None):
         """dL/dx for dL/dy of the forward(x, keep=True) before it, with no other pass between (of recorded passes a replay is one, which is not seen here); the weights' gradients are left
         in self.gradients."""
+        import torch
+
         import rocwmma_amd as R
 
         t, e, g = self.dtype, self.experts, self.gradients
@@ -108,9 +122,11 @@ class ExpertLayer:
         R.route_backward(t, tokens, e, self.top, self.logits, self.chosen, self.dweights, self.dlogits, score=self.score, chosen_only=True, stream=stream)
         R.linear_backward(t, t, tokens, e, self.hidden, self.dlogits, x, self.router, dx=self.dx_router, dw=g["router"], workspace=self.workspace, stream=stream)
         # the residual's gradient, the rows' of both products, the router's
-        R.combine(t, tokens, self.top, self.hidden, self.dxs, rows, self.place, self.dx, c=dy, stream=stream)
-        R.combine(t, tokens, self.top, self.hidden, self.dxs2, rows, self.place, self.dx, c=self.dx, stream=stream)
-        R.combine(t, tokens, 1, self.hidden, self.dx_router, tokens, self.itself, self.dx, c=self.dx, stream=stream)
+        with _on(stream):
+            place, terms = self.place[:tokens], self.terms[:tokens]
+            terms[:, : self.top].copy_(place)
+            torch.add(place, len(self.dxs), out=terms[:, self.top: 2 * self.top])
+        R.combine(t, tokens, 2 * self.top + 1, self.hidden, self.parts, len(self.parts), self.terms, self.dx, c=dy, stream=stream)
         return self.dx[:tokens]
 
 
