@@ -390,7 +390,7 @@ typedef enum
 {
     R355_ACT_NONE      = 0,
     R355_ACT_RELU      = 1,
-    R355_ACT_GELU      = 2, /* z (1 + erf(z / sqrt 2)) / 2 */
+    R355_ACT_GELU      = 2, /* z (1 + erf(z / sqrt 2)) / 2; off by (1.5 z^2 + 16) 2^-24 of itself at most, below zero too */
     R355_ACT_GELU_TANH = 3, /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
     R355_ACT_SILU      = 4  /* z / (1 + exp(-z)) */
 } r355_activation;
