@@ -583,14 +583,14 @@ namespace
     // are 16 bytes.  A thread moves 16 of them.  Bound by memory.
     struct Copy
     {
-        const char* from; // NULL: there is nothing to do
+        const char* from;
         uint64_t    stride; // bytes from group to group
         uint32_t    groups, rows, cols, ld;
         uint32_t    toRows, toCols;
 
         uint64_t bytes() const
         {
-            return from ? (uint64_t)groups * toRows * toCols * 2u : 0u;
+            return (uint64_t)groups * toRows * toCols * 2u;
         }
     };
     __global__ void __launch_bounds__(256) linearEven(Copy c, char* to)
@@ -898,6 +898,12 @@ namespace
         return !at || (r355::aligned(at, 16) && (uint64_t)ld * bytes % 16u == 0u);
     }
 
+    // ... of a product's operand, whose rows are there whatever their address says (a query may come before there is one)
+    bool evenOperand(const void* at, uint32_t ld)
+    {
+        return r355::aligned(at, 16) && ld % 8u == 0u;
+    }
+
     int checkCommon(const char* what, int32_t type, int32_t activation, uint32_t rows, uint32_t n, uint32_t k, uint32_t groups, const int32_t* offsets)
     {
         if(type != R355_F16 && type != R355_BF16)
@@ -950,7 +956,7 @@ namespace
     }
     bool evenForward(const r355_linear_args& a)
     {
-        return a.k % 8u == 0u && evenRows(a.x, a.ldx, 2) && evenRows(a.w, a.ldw, 2) && (a.groups == 1u || a.w_stride % 8 == 0);
+        return a.k % 8u == 0u && evenOperand(a.x, a.ldx) && evenOperand(a.w, a.ldw) && (a.groups == 1u || a.w_stride % 8 == 0);
     }
     // The kernel of a forward product by its rows: us of dot products, of the kernel for few rows and of tiles for 4096 x 4096: one row 7.3, 8.0, 14; two 7.8, 8.2, 14; four 8.8, 8.3, 14; sixteen
     // -, 10, 15; 24 -, 17, 14.  Of experts with about one row each (32 of 4096 x 4096, 128 of 1024 x 1024) the first two 84, 105 and 49, 75; with four (8, 32, 64 experts of 2048 x 2048) 21, 15, 16; 79,
@@ -995,11 +1001,11 @@ namespace
     }
     bool evenInput(const r355_linear_backward_args& a, const char* dz, uint32_t lddz)
     {
-        return a.n % 8u == 0u && evenRows(dz, lddz, 2) && evenRows(a.w, a.ldw, 2) && (a.groups == 1u || a.w_stride % 8 == 0);
+        return a.n % 8u == 0u && evenOperand(dz, lddz) && evenOperand(a.w, a.ldw) && (a.groups == 1u || a.w_stride % 8 == 0);
     }
     bool evenWeight(const r355_linear_backward_args& a, const char* dz, uint32_t lddz)
     {
-        return evenRows(dz, lddz, 2) && evenRows(a.x, a.ldx, 2);
+        return evenOperand(dz, lddz) && evenOperand(a.x, a.ldx);
     }
     // Operands to be laid out anew in a workspace, one after the other, and what that takes
     struct Copies
@@ -1041,9 +1047,9 @@ namespace
     {
         Copies         c;
         const uint32_t rows = a.source ? a.x_rows : a.rows;
-        if(a.k % 8u != 0u || !evenRows(a.x, a.ldx, 2))
+        if(a.k % 8u != 0u || !evenOperand(a.x, a.ldx))
             p.a = c.add(Copy{p.a, 0u, 1u, rows, a.k, a.ldx, rows, eights(a.k)}, workspace), p.lda = eights(a.k);
-        if(a.k % 8u != 0u || !evenRows(a.w, a.ldw, 2) || (a.groups > 1u && a.w_stride % 8 != 0))
+        if(a.k % 8u != 0u || !evenOperand(a.w, a.ldw) || (a.groups > 1u && a.w_stride % 8 != 0))
             p.b = c.add(Copy{p.b, p.strideB, a.groups, a.n, a.k, a.ldw, a.n, eights(a.k)}, workspace), p.ldb = eights(a.k), p.strideB = (uint64_t)a.n * eights(a.k) * 2u;
         p.k = eights(a.k);
         if(a.source && (uint64_t)rows * p.lda * 2u > FAR)
@@ -1055,11 +1061,11 @@ namespace
     {
         Copies         c;
         const uint32_t n8 = eights(a.n), k8 = eights(a.k);
-        if((wantX && a.n % 8u != 0u) || !evenRows(dz, lddz, 2))
+        if((wantX && a.n % 8u != 0u) || !evenOperand(dz, lddz))
             px.a = pw.a = c.add(Copy{dz, 0u, 1u, a.rows, a.n, lddz, a.rows, n8}, workspace), px.lda = pw.lda = n8;
-        if(wantX && (a.n % 8u != 0u || !evenRows(a.w, a.ldw, 2) || (a.groups > 1u && a.w_stride % 8 != 0)))
+        if(wantX && (a.n % 8u != 0u || !evenOperand(a.w, a.ldw) || (a.groups > 1u && a.w_stride % 8 != 0)))
             px.b = c.add(Copy{px.b, px.strideB, a.groups, a.n, a.k, a.ldw, n8, k8}, workspace), px.ldb = k8, px.strideB = (uint64_t)n8 * k8 * 2u;
-        if(wantW && !evenRows(a.x, a.ldx, 2))
+        if(wantW && !evenOperand(a.x, a.ldx))
             pw.b = c.add(Copy{pw.b, 0u, 1u, a.rows, a.k, a.ldx, a.rows, k8}, workspace), pw.ldb = k8;
         px.k = n8;
         return c;
