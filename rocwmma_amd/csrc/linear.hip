@@ -236,9 +236,10 @@ namespace
     // straight from global memory; their sums meet in LDS in the order of the waves.  The weights are the first operand: a lane then holds four of them of one row of x.
     // Bound by HBM: two rows of each of 16 experts of 1326 x 6520 50 us, 5.5 TB/s.  (Single pieces in turn: rows that do not begin with a cache line have lines of two waves, 30 rows of 8 experts
     // of 8192 x 4104 167 instead of 162 us; and such lines come twice where they are read nontemporally, 162 instead of 125.)
-    template <typename T, uint32_t RB, uint32_t CB, uint32_t DEPTH>
+    template <typename T>
     __global__ void __launch_bounds__(64 * WAVES, 2) linearFew(LinearParams p)
     {
+        constexpr uint32_t RB = 1u, CB = 1u, DEPTH = 4u; // (written out for one block the loads are scheduled worse: 16 x 16384 x 4096 38.7 us instead of 35.7)
         constexpr uint32_t ROWS = 16u * CB, COLS = 16u * RB, PITCH = COLS + 4u;
         __shared__ __attribute__((aligned(16))) float sums[WAVES * ROWS * PITCH];
         GroupTiles<ROWS> tiles{p};
@@ -772,7 +773,7 @@ namespace
     {
         p.tilesN             = static_cast<uint32_t>(tilesOf(p.n, 16u));
         const uint64_t groups = (mostTiles(p, 16u) * p.tilesN + 7u) / 8u * 8u;
-        hipLaunchKernelGGL((linearFew<T, 1, 1, 4>), dim3(static_cast<uint32_t>(groups)), dim3(64 * WAVES), 0, s, p);
+        hipLaunchKernelGGL(linearFew<T>, dim3(static_cast<uint32_t>(groups)), dim3(64 * WAVES), 0, s, p);
     }
 
     int tooMany(const char* what)
