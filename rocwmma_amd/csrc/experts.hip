@@ -85,7 +85,7 @@ namespace
         return in ? __expf(v - (most == -INFINITY ? 0.0f : most)) : 0.0f;
     }
 
-    // the largest of a token's logits, and the sum of the exponentials
+    // The largest of a token's logits, and the sum of the exponentials.  (For the choice by score plus bias it comes before the keys: 16384 tokens, 8 of 256, 26.4 -> 29.2 us, by sigmoid 28.2.)
     template <uint32_t V>
     __device__ __forceinline__ void ofAll(const RouteParams& p, const float (&x)[V], uint32_t lane, float& most, float& all)
     {
@@ -189,7 +189,8 @@ namespace
         }
     }
 
-    // Weights of the choices, in the lanes that hold them
+    // Weights of the choices, in the lanes that hold them.  (Reciprocals and the logarithm are the hardware's, a step of 32 bits: the weights of 16384 tokens are off by 6.7e-8 of their norm,
+    // torch's in 32 bits by 5.9e-8.)
     template <uint32_t V>
     __device__ __forceinline__ float weightOf(const RouteParams& p, const float (&x)[V], uint32_t lane, float logit)
     {

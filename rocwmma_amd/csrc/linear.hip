@@ -437,7 +437,9 @@ namespace
     }
 
     // ---- The gradient's part element by element: dz, dgate and the bias's gradient, one pass over dy, z and gate.  Bound by HBM: three operands and two results of 4099 x 4096 in bf16 31 us,
-    // 5.4 TB/s.  (Made once and read by both products: in their loads it would be made anew for each tile that a row is part of, and dz would have to lie somewhere for the transposed reads anyway.)
+    // 5.4 TB/s.  (Made once and read by both products: in their loads it would be made anew for each tile that a row is part of, and dz would have to lie somewhere for the transposed reads anyway.  dz is rounded to 16
+    // bits, as the matrix instructions take no more; a product of its f32 value in two parts would take twice as many.  With it dx and dW are off by 0.0023 of their norm in bf16, of which a result's own
+    // rounding is 0.0017.)
     struct GradParams
     {
         const char*    dy;
@@ -963,6 +965,8 @@ namespace
     // -, 10, 15; 24 -, 17, 14.  Of experts with about one row each (32 of 4096 x 4096, 128 of 1024 x 1024) the first two 84, 105 and 49, 75; with four (8, 32, 64 experts of 2048 x 2048) 21, 15, 16; 79,
     // 54, 48 and 143, 105, 95; with twelve 37, 21, 17; 166, 73, 48 and 321, 143, 95: the kernel for few rows reads the weights at 5.7 TB/s, and once more for every 20 rows or so, after 4 us, whatever their
     // lengths; where the tiles' plan takes more, as of few groups, it wins (4 of 1024 x 1024 with four 5.6, 4.9, 6.7; 16 of 1326 x 6520 with two -, 51, 71).
+    // The host knows the average alone.  Rows that meet in fewer groups take less time than rows of all of them, if more than a choice by the rows themselves would: 128 rows over 128 groups of
+    // 2048 x 2048, one each 182, in an eighth of the groups 65, in one 48 (one matrix of as many rows 10); 256 over 64, four each 95, in an eighth 21, in one 43 (9); 2048 over 64 97, 44, 44 (23).
     enum class Kernel
     {
         DOTS,

@@ -6,11 +6,11 @@
 // holds two images of A and three of B, so that loads run two stages ahead (B of the small tiles three).  The buffers go round at run time: the loop is one stage long, and
 // what that costs, an addition for each address of a read, hides behind matrix instructions (six stages unrolled, as the GEMM has them, would be 36 KB of code for each epilogue).
 //
-// Bound by the matrix cores under the power limit where the sum is long and the tiles are whole (bf16 8192^3 726 us, 1.51 PFLOP/s; 4000 x 8192 x 4096 with GELU and two results 207 us, matrix cores
+// Bound by the matrix cores under the power limit where the sum is long and the tiles are whole (bf16 8192^3 706 to 734 us, 1.50 to 1.56 PFLOP/s; 4000 x 8192 x 4096 with GELU and two results 207 us, matrix cores
 // busy 67 % of the CU's cycles, 72 % in the gradients of 4096 x 4096); by the start and end of a tile, some 11 us of the large one, where it is short; by HBM and the loads' latency where
 // a group has few rows of its own weights (16384 rows over 64 groups of 2048 x 2048 203 us, 37 %).
 //
-// Rows are ragged: a workgroup finds its group from the offsets in device memory (Groups).  A tile that has fewer rows reads its last one again, what that gives is not
+// Rows are ragged: a workgroup finds its group from the offsets in device memory (GroupTiles).  A tile that has fewer rows reads its last one again, what that gives is not
 // stored; a sum that ends inside a stage is completed with zeros by loads past the end of their buffer.
 //
 // Compiled once per type.
