@@ -13,7 +13,7 @@ def _on(stream):
 
     if stream is None:
         stream = torch.cuda.default_stream()
-    return torch.cuda.stream(stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(stream))
+    return torch.cuda.stream(stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(getattr(stream, "cuda_stream", stream)))
 
 
 class ExpertLayer:

@@ -45,3 +45,5 @@ def test_streams(monkeypatch):
     monkeypatch.setattr(torch.cuda, "stream", lambda s: s)
     mine = Stream()
     assert expert_layer._on(mine) is mine and isinstance(expert_layer._on(None), Stream) and expert_layer._on(77) == ("external", 77)
+    other = type("Other", (), {"cuda_stream": 78})()  # (as the calls take it)
+    assert expert_layer._on(other) == ("external", 78)
